@@ -197,6 +197,66 @@ int tgbm_metric_score(const char *objective, int n_rows, int trees_per_round, co
 int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_round, const float *d_label,
                               const float *d_raw, float *d_out, void *cuda_stream);
 
+/* ---- operators on the scores of many classes (no counterpart in the reference) ----
+ * All pointers whose names begin with d_ are DEVICE pointers of the caller, on the current device; the kernels are queued on
+ * `cuda_stream` (a cudaStream_t, NULL = default stream) and the calls return without waiting.  Nothing is allocated and nothing is
+ * kept from one call for the next: calls on different streams do not disturb each other, and a call may be captured into a graph.
+ * Arguments are checked before anything is queued: 1 and a message in tgbm_last_error().
+ * Scores are a matrix of n_rows x n_classes in `type`, class k of row n at d_scores[n * row_stride + k * class_stride] (strides in
+ * elements, none negative).  Row stride 1: by class, as tgbm_booster_get_ypred and tgbm_predict_raw lay them out; class stride 1:
+ * by row, as networks do.  Where neither is 1 the operators work as well, more slowly. */
+#define TGBM_F32 0
+#define TGBM_F16 1
+#define TGBM_BF16 2
+#define TGBM_SCORES_MAX_CLASSES (1 << 20)
+#define TGBM_SCORES_MAX_TOP 128
+
+/* Scores as a user's rules change them before classes are chosen.  For class k of row n, with c the number of times it stands in
+ * the row's history:
+ *   z = c > 0 ? (s > 0 ? s / repetition : s * repetition) : s;   z -= c * frequency + (c > 0 ? presence : 0);
+ *   z += d_bias[k];   out = allowed ? z : -infinity
+ * computed in floats and rounded once.  d_out: the same type, strides of its own; d_out = d_scores with the same strides works in
+ * place; otherwise the two must not share memory.
+ * d_bias: n_classes floats, or NULL.
+ * d_allowed: n_masks rows of at least (n_classes + 31) / 32 words, `mask_stride` words apart, class k in bit k & 31 of word k >> 5;
+ * NULL: every class is allowed.  d_allowed_row[n]: the row's mask (outside [0, n_masks): all its classes are allowed); NULL: row n
+ * has mask n.
+ * d_history[d_history_ptr[n] .. d_history_ptr[n + 1]): classes given before, repeated as often as they were, in any order; numbers
+ * outside [0, n_classes) are passed over.  d_history_ptr has n_rows + 1 entries, d_history n_history; NULL: no histories. */
+int tgbm_scores_adjust(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, void *d_out,
+                       long long out_row_stride, long long out_class_stride, const float *d_bias, const unsigned *d_allowed, int n_masks,
+                       long long mask_stride, const int *d_allowed_row, const long long *d_history_ptr, const int *d_history,
+                       long long n_history, float repetition, float frequency, float presence, void *cuda_stream);
+
+/* The `top` largest scores of every row, 1 <= top <= TGBM_SCORES_MAX_TOP: d_values and d_ids are n_rows x top, largest first, of
+ * equal scores the lower class first.  -infinity (masked) and NaN are never chosen; where a row has fewer than `top` other scores
+ * the last entries are -infinity and class -1.  d_lse (n_rows floats, or NULL): log of the sum over ALL classes of
+ * exp(score / temperature), so that value / temperature - lse is the log of a class's share; NaN where a score is. */
+int tgbm_scores_top(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int top,
+                    float temperature, float *d_values, int *d_ids, float *d_lse, void *cuda_stream);
+
+/* Distance of a student's scores s from what is kept of a teacher: per row `top` classes d_ids and their scores d_logits t (type
+ * logits_type; rows ids_stride and logits_stride elements apart).  With T the temperature, p = softmax(s / T):
+ *   q_j = exp(t_j / T - L);  L = d_lse[n], the teacher's log-sum-exp over all classes AT THIS T (what tgbm_scores_top gives), and
+ *   the mass that is not listed, r = max(0, 1 - sum q), lies on the unlisted classes together; d_lse NULL: L = log sum exp(t_j / T)
+ *   over the listed ones, r = 0.
+ *   loss = w (alpha T^2 (sum q_j log(q_j / p_j) + r log(r / p_r)) - (1 - alpha) log softmax(s)_y)
+ * with p_r the student's share of the unlisted classes, w = d_weights[n] (NULL: 1) and y = d_labels[n] (outside [0, n_classes), or
+ * NULL: no such term).  A class number outside [0, n_classes) is passed over, one that stands twice in a row holds the sum; a row
+ * that lists nothing, or only -infinity, has no teacher: its first term is 0.
+ * d_loss: n_rows floats (NULL: not wanted, where there is a gradient).
+ * gives: TGBM_GIVES_LOSS; TGBM_GIVES_GRADIENT: d_grad holds d loss / d s in the type of the scores; TGBM_GIVES_PAIRS: pairs of floats
+ * (gradient, hessian) as a booster takes them, hessian = max(2 w (alpha p (1 - p) + (1 - alpha) p1 (1 - p1)), 1e-16), p1 = softmax(s), each
+ * term where the row has it -- with alpha = 0 the pairs of the objective multi:softmax; the unlisted classes' share of the first term's
+ * second derivative that could make it negative is left out.  Strides of d_grad in elements (pairs). */
+#define TGBM_GIVES_LOSS 0
+#define TGBM_GIVES_GRADIENT 1
+#define TGBM_GIVES_PAIRS 2
+int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int top,
+                        const int *d_ids, long long ids_stride, int logits_type, const void *d_logits, long long logits_stride,
+                        const float *d_lse, const int *d_labels, const float *d_weights, float temperature, float alpha, float *d_loss,
+                        int gives, void *d_grad, long long grad_row_stride, long long grad_class_stride, void *cuda_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -62,6 +62,10 @@ def load() -> C.CDLL:
     lib.tgbm_predict_raw_timed.argtypes = [C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, vp, vp]
     lib.tgbm_metric_score.argtypes = [C.c_char_p, C.c_int, C.c_int, vp, vp, vp, C.c_int, fp]
     lib.tgbm_metric_score_noalloc.argtypes = [C.c_char_p, C.c_int, C.c_int, vp, vp, vp, vp]
+    ll, i32, f32 = C.c_longlong, C.c_int, C.c_float
+    lib.tgbm_scores_adjust.argtypes = [i32, i32, i32, vp, ll, ll, vp, ll, ll, vp, vp, i32, ll, vp, vp, vp, ll, f32, f32, f32, vp]
+    lib.tgbm_scores_top.argtypes = [i32, i32, i32, vp, ll, ll, i32, f32, vp, vp, vp, vp]
+    lib.tgbm_scores_distill.argtypes = [i32, i32, i32, vp, ll, ll, i32, vp, ll, i32, vp, ll, vp, vp, vp, f32, f32, vp, i32, vp, ll, ll, vp]
     lib.sparse_train_scikit.argtypes = [C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float,
                                         C.c_float, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.c_float,
                                         C.c_char_p, ip, C.c_char_p, vp, ip, vp, vp, C.c_int]

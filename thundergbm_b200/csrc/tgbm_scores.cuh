@@ -1,0 +1,246 @@
+// Device code of the operators on scores (tgbm_scores.cu): element types, reductions, the teacher's side of a row.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tgbm_device.cuh"
+#include "tgbm_scores.h"
+
+namespace tgbm {
+
+__device__ __forceinline__ float score_f32(float v) { return v; }
+__device__ __forceinline__ float score_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float score_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T score_from(float v);
+template <> __device__ __forceinline__ float score_from<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half score_from<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 score_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
+
+// 2^x, one instruction; 0 for -inf, flushes results below 2^-126 (a class that far below the row's best adds nothing to a
+// float sum that holds a 1)
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+template <typename V> __device__ __forceinline__ V warp_sum(V v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Place of a score in the order of a row: larger scores first, of equal ones the lower class.  0: not a score that can be
+// chosen (-inf: masked; NaN).  Adding 0 makes one of the two zeros.
+__device__ __forceinline__ unsigned score_key(float v) {
+    const unsigned b = __float_as_uint(__fadd_rn(v, 0.f));
+    return v > minus_inf() ? ((b & 0x80000000u) ? ~b : (b | 0x80000000u)) : 0u;
+}
+__device__ __forceinline__ float key_score(unsigned key) {
+    return key == 0u ? minus_inf() : __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
+}
+
+__device__ __forceinline__ float teacher_logit(const DistillArgs &a, long long n, int e) {
+    const long long at = n * a.logits_stride + e;
+    if (a.logits_type == SCORE_F32) return static_cast<const float *>(a.logits)[at];
+    if (a.logits_type == SCORE_F16) return score_f32(static_cast<const __half *>(a.logits)[at]);
+    return score_f32(static_cast<const __nv_bfloat16 *>(a.logits)[at]);
+}
+
+// ---- the teacher's side of one row -----------------------------------------------------------
+// What a row's listed scores t_j say at temperature T: q_j = exp(t_j / T - L) with L the teacher's log-sum-exp over all classes,
+// or (none given) that of the listed ones; of the mass that is left, `rest`, nothing is known but that it lies on the others.
+// A class that is listed twice holds the sum of both.  Worked in doubles: `rest` and the logarithms are differences of nearly
+// equal numbers, and there are only a few of them per row.
+struct TeacherRow {
+    float q[SCORES_MAX_TOP];   // mass of a listed class; only where id >= 0
+    int id[SCORES_MAX_TOP];    // -1: no class, or one that stands further in front
+    double entropy;            // sum of q log q over the listed classes and the rest
+    float total, rest;         // all mass (0: the row has no teacher), what is not listed
+};
+
+// one warp; entry e = lane + 32 s of the row's list
+__device__ __forceinline__ void read_teacher(TeacherRow &r, const DistillArgs &a, long long n, double inv_t) {
+    const int top = a.top, k = a.k;
+    const int *ids = a.ids + n * a.ids_stride;
+    const float *lse = a.lse ? a.lse + n : nullptr;
+    constexpr int S = SCORES_MAX_TOP / 32;
+    const int lane = threadIdx.x & 31;
+    int id[S];
+    double u[S], q[S], lq[S];
+    float best = minus_inf();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int e = lane + 32 * s;
+        id[s] = -1;
+        float t = minus_inf();
+        if (e < top) {
+            const int i = ids[e];
+            if (i >= 0 && i < k) { id[s] = i; t = teacher_logit(a, n, e); }
+        }
+        u[s] = (double)t * inv_t;
+        best = t != t ? t : best != best ? best : fmaxf(best, t);
+    }
+    const bool broken = __any_sync(0xffffffffu, best != best);
+    best = warp_max(best);
+    const bool none = best == minus_inf() && !broken;   // nothing is listed, or nothing that the teacher thinks possible
+    double L;
+    if (lse) {
+        L = (double)*lse;
+    } else {
+        double sum = 0;
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+            if (s == 0 || 32 * s < top) sum += id[s] >= 0 ? exp(u[s] - (double)best * inv_t) : 0.0;
+        L = (double)best * inv_t + log(warp_sum(sum));
+    }
+    double mass = 0, entropy = 0;
+    int distinct = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        lq[s] = u[s] - L;
+        q[s] = id[s] >= 0 && !none ? exp(lq[s]) : 0.0;
+        if (s > 0 && 32 * s >= top) continue;
+        // an earlier entry of the same class takes this one's mass
+        const unsigned same = __match_any_sync(0xffffffffu, id[s]);
+        const int first = __ffs(same) - 1;
+        if (__any_sync(0xffffffffu, id[s] >= 0 && first != lane)) {
+            double sum = 0;
+            for (int l = 0; l < 32; ++l) {
+                const double v = __shfl_sync(0xffffffffu, q[s], l);
+                if (same >> l & 1) sum += v;
+            }
+            if (id[s] >= 0) {
+                if (first != lane) { id[s] = -1; q[s] = 0; }
+                else if (same != 1u << lane) { q[s] = sum; lq[s] = log(sum); }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < s; ++b) {
+            for (int l = 0; l < 32; ++l) {   // entry l of this segment against all of segment b
+                const int other = __shfl_sync(0xffffffffu, id[s], l);
+                const unsigned hit = __ballot_sync(0xffffffffu, other >= 0 && other == id[b]);
+                if (hit) {
+                    const double v = __shfl_sync(0xffffffffu, q[s], l);
+                    if (hit >> lane & 1) { q[b] += v; lq[b] = log(q[b]); }
+                    if (lane == l) { id[s] = -1; q[s] = 0; }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int e = lane + 32 * s;
+        if (e < top) { r.id[e] = id[s]; r.q[e] = (float)q[s]; }
+        mass += q[s];
+        if (q[s] != 0) entropy += q[s] * lq[s];
+        distinct += id[s] >= 0;
+    }
+    mass = warp_sum(mass);
+    entropy = warp_sum(entropy);
+    distinct = warp_sum(distinct);
+    const double rest = lse && !none && distinct < k && mass < 1 ? 1.0 - mass : 0.0;
+    if (lane == 0) {
+        r.total = none ? 0.f : (float)(mass + rest);
+        r.rest = (float)rest;
+        r.entropy = rest > 0 ? entropy + rest * log(rest) : entropy;
+    }
+}
+
+// ---- the student's side ----------------------------------------------------------------------
+// Scores are taken relative to the largest of their kind, so a sum of exponentials holds a 1 and does not overflow.  "Rest"
+// are the classes summed in the pass over the row -- those that the teacher does not list, or (no bucket for them is needed) all --
+// and `top`, `sum`, `sum1` are those of all classes.  The rest has a reference of its own: a student far from all of it still
+// gets the gradient that says which of them to raise.  Without a score above -inf a reference is 0 and its sums are 0.
+struct StudentRow {
+    float base, rest, rest1;   // largest of the rest; sums of exp((s - base) / T) and exp(s - base)
+    float top, sum, sum1;      // the same of all classes
+};
+__device__ __forceinline__ float row_top(float largest) { return largest == minus_inf() ? 0.f : largest; }
+
+// Factors of a row's gradients.  For class i with shares p (at T) and p1 (at 1):
+//   listed:  g = soft * (total * p - q) + hard * (p1 - [label])
+//   others:  g = soft * (total * p - rest * p / p_rest) + hard * (p1 - [label])
+//   h = max(curve * p (1 - p) + 2 hard * p1 (1 - p1), 1e-16)
+struct DistillRow {
+    float base, c;            // others: e = exp((s - base) / T) = 2^((s - base) c); p = e * to_p, p1 = exp(s - base) * to_p1
+    float to_p, to_p1, to_g;  // soft * (total * p - rest * p / p_rest) = e * to_g
+    float top, inv_sum, inv_sum1;
+    float soft, hard;         // w alpha T, w (1 - alpha)
+    float total, curve;       // the teacher's mass; 2 w alpha where the row has a teacher
+    int label;                // -1: none
+};
+
+constexpr float LOG2E = 1.44269504088896341f;
+constexpr float MIN_HESSIAN = 1e-16f;   // the softmax objective's
+
+__device__ __forceinline__ float2 finish_gh(const DistillRow &d, int i, float g, float p, float p1) {
+    g += d.hard * (i == d.label ? p1 - 1.f : p1);
+    return make_float2(g, fmaxf(d.curve * (p * (1.f - p)) + 2.f * d.hard * (p1 * (1.f - p1)), MIN_HESSIAN));
+}
+template <bool TWO>   // the hard labels need the shares at temperature 1 as well
+__device__ __forceinline__ float2 other_gh(const DistillRow &d, int i, float s) {
+    const float x = __fsub_rn(s, d.base), e = exp2_fast(x * d.c), p = e * d.to_p;
+    return finish_gh(d, i, e * d.to_g, p, TWO ? exp2_fast(x * LOG2E) * d.to_p1 : p);
+}
+template <bool TWO>
+__device__ __forceinline__ float2 listed_gh(const DistillRow &d, int i, float s, float q) {
+    const float x = __fsub_rn(s, d.top), p = exp2_fast(x * d.c) * d.inv_sum;
+    return finish_gh(d, i, d.soft * (d.total * p - q), p, TWO ? exp2_fast(x * LOG2E) * d.inv_sum1 : p);
+}
+
+// label of a row as a class, -1 where it has none
+__device__ __forceinline__ int row_label(const DistillArgs &a, long long n) {
+    if (a.labels) {
+        const int y = a.labels[n];
+        return y >= 0 && y < a.k ? y : -1;
+    }
+    if (a.labels_f) {
+        const float y = a.labels_f[n];
+        return y >= 0.f && y < (float)a.k ? (int)y : -1;
+    }
+    return -1;
+}
+
+__device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const TeacherRow &t, const StudentRow &s, float w, int label) {
+    DistillRow d;
+    const float c = (float)(1.44269504088896341 / (double)a.temperature);
+    const float alpha = t.total == 0.f ? 0.f : a.alpha;
+    const float low = __fsub_rn(s.base, s.top);
+    d.base = s.base; d.top = s.top; d.c = c;
+    d.inv_sum = s.sum == 0.f ? 0.f : 1.f / s.sum;
+    d.inv_sum1 = s.sum1 == 0.f ? 0.f : 1.f / s.sum1;
+    d.to_p = exp2_fast(low * c) * d.inv_sum;
+    d.to_p1 = exp2_fast(low * LOG2E) * d.inv_sum1;
+    d.label = label;
+    d.soft = w * alpha * a.temperature;
+    d.hard = label >= 0 ? w * (1.f - a.alpha) : 0.f;
+    d.total = t.total;
+    d.to_g = d.soft * (t.total * d.to_p - (t.rest > 0.f && s.rest != 0.f ? t.rest / s.rest : 0.f));
+    d.curve = 2.f * w * alpha;
+    return d;
+}
+// listed: sum over the listed classes of q (s - top) / T; mass: of their q
+__device__ __forceinline__ float distill_loss(const DistillArgs &a, const TeacherRow &t, const StudentRow &s, float w, int label,
+                                              double listed, double mass, float label_score) {
+    double loss = 0;
+    const double inv_t = 1.0 / (double)a.temperature;
+    // (a row without a score above -inf: its listed sum or its label's score is -inf already, and the loss infinite)
+    const double log_sum = s.sum == 0.f ? 0.0 : log((double)s.sum), log_sum1 = s.sum1 == 0.f ? 0.0 : log((double)s.sum1);
+    if (t.total != 0.f) {
+        double kl = t.entropy - (listed - mass * log_sum);
+        if (t.rest > 0.f) kl -= (double)t.rest * (((double)s.base - (double)s.top) * inv_t + log((double)s.rest) - log_sum);
+        loss += (double)a.alpha * a.temperature * a.temperature * kl;
+    }
+    if (label >= 0 && a.alpha < 1.f) loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - log_sum1);
+    return (float)((double)w * loss);
+}
+
+}  // namespace tgbm

@@ -1,0 +1,143 @@
+"""Operators on the scores of many classes, on CUDA tensors.
+
+Scores are a tensor of rows x classes (float32, float16 or bfloat16, any strides).  A booster keeps all rows of a class side by side:
+`torch.from_numpy(booster.ypred()).cuda().t()` is such a tensor, no copy is made of it.
+
+    adjust   penalties for classes a row was given before, a bias per class, classes a row may not have
+    top      the largest scores of every row, their classes, the row's log-sum-exp
+    distill  loss on a teacher's largest scores and on hard labels, with its gradient
+
+Results come on the stream that is torch's current one on the scores' device, in the layout of the scores; nothing waits.
+Every function is one call of the C interface (tgbm_scores_* in include/thundergbm.h, which defines the operators); what the
+arguments may not be is refused there or here before anything is queued.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_GIVES = {'loss': 0, 'gradient': 1, 'pairs': 2}
+MAX_TOP = 128
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _scores(t, name='scores'):
+    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _TYPE,
+          f'{name}: a CUDA tensor of rows x classes in float32, float16 or bfloat16')
+    _need(t.size(1) >= 1 and t.size(0) < 2 ** 31, f'{name}: at least one class and fewer than 2^31 rows')
+
+
+def _beside(t, scores, dtype, shape, name):
+    """Address of a contiguous tensor on the scores' device."""
+    if t is None:
+        return None
+    _need(isinstance(t, torch.Tensor) and t.device == scores.device and t.dtype == dtype and t.is_contiguous() and tuple(t.shape) == shape,
+          f'{name}: a contiguous {dtype} tensor of shape {shape} on {scores.device}')
+    return t.data_ptr()
+
+
+def _call(name, scores, *args):
+    lib = _lib.lib()
+    device = scores.device.index
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if torch.cuda.current_device() == device:
+        rc = getattr(lib, name)(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = getattr(lib, name)(*args, stream)
+    _lib.check(rc)
+
+
+def _like(scores, *more, dtype=None):
+    """New memory in the layout of the scores; more: values per cell."""
+    n, k = scores.shape
+    dtype = dtype or scores.dtype
+    if scores.stride(0) < scores.stride(1):
+        out = torch.empty((k, n, *more), dtype=dtype, device=scores.device)
+        return out.transpose(0, 1)
+    return torch.empty((n, k, *more), dtype=dtype, device=scores.device)
+
+
+def adjust(scores, *, out=None, bias=None, allowed=None, allowed_row=None, history=None, repetition=1.0, frequency=0.0, presence=0.0):
+    """Scores after penalties, bias and mask, in their own type; `out=scores` changes them in place.
+
+    bias: float32, one per class.  allowed: int32 words (masks x ceil(classes / 32)), class k in bit k % 32 of word k // 32, bits of
+    classes that may be chosen set; allowed_row: int32, the mask of every row (-1: none), without it row n has mask n.
+    history: (ptr, classes), int64 (rows + 1) and int32: what row n was given before is classes[ptr[n]:ptr[n + 1]]; a class that stands
+    there c > 0 times has its score divided (above 0) or multiplied by `repetition`, less c * frequency + presence."""
+    _scores(scores)
+    n, k = scores.shape
+    if out is None:
+        out = _like(scores)
+    else:
+        _scores(out, 'out')
+        _need(out.shape == scores.shape and out.dtype == scores.dtype and out.device == scores.device, 'out: shape, type and device of the scores')
+    masks = words = 0
+    if allowed is not None:
+        _need(isinstance(allowed, torch.Tensor) and allowed.dim() == 2, 'allowed: masks x words')
+        masks, words = allowed.shape
+        _need(words >= (k + 31) // 32, 'allowed: a bit for every class')
+    else:
+        _need(allowed_row is None, 'allowed_row: there are no masks')
+    given = 0
+    ptr = ids = None
+    if history is not None:
+        ptr, ids = history
+        _need(isinstance(ids, torch.Tensor) and ids.dim() == 1, 'history: (ptr, classes)')
+        given = ids.numel()
+    _call('tgbm_scores_adjust', scores, n, k, _TYPE[scores.dtype], scores.data_ptr(), scores.stride(0), scores.stride(1), out.data_ptr(),
+          out.stride(0), out.stride(1), _beside(bias, scores, torch.float32, (k,), 'bias'),
+          _beside(allowed, scores, torch.int32, (masks, words), 'allowed'), masks, words,
+          _beside(allowed_row, scores, torch.int32, (n,), 'allowed_row'), _beside(ptr, scores, torch.int64, (n + 1,), 'history'),
+          _beside(ids, scores, torch.int32, (given,), 'history'), given, repetition, frequency, presence)
+    return out
+
+
+def top(scores, k, *, temperature=1.0):
+    """(values, classes, lse): the k largest scores of every row (float32, rows x k; largest first, of equal ones the lower class first),
+    their classes (int32) and the log of the sum over all classes of exp(score / temperature).  Masked scores (-inf) and NaN are not
+    chosen: a row that runs out of others ends in -inf and class -1."""
+    _scores(scores)
+    _need(1 <= k <= MAX_TOP, f'k: 1 to {MAX_TOP}')
+    n = scores.size(0)
+    values = torch.empty((n, k), dtype=torch.float32, device=scores.device)
+    ids = torch.empty((n, k), dtype=torch.int32, device=scores.device)
+    lse = torch.empty(n, dtype=torch.float32, device=scores.device)
+    _call('tgbm_scores_top', scores, n, scores.size(1), _TYPE[scores.dtype], scores.data_ptr(), scores.stride(0), scores.stride(1), k,
+          temperature, values.data_ptr(), ids.data_ptr(), lse.data_ptr())
+    return values, ids, lse
+
+
+def distill(scores, ids, logits, *, lse=None, labels=None, weights=None, temperature=1.0, alpha=1.0, gives='gradient'):
+    """(loss, gradient) of a student's scores against a teacher's largest ones.
+
+    ids (int32) and logits (float32, float16 or bfloat16), rows x up to 128: classes and scores that are kept of the teacher, entries of
+    class -1 are none; their rows may be apart (a slice of a longer list).  lse: the teacher's log-sum-exp at this temperature (from
+    `top`); with it the mass that is not listed is compared as one class, without it the listed ones are taken for all.  labels:
+    int32, -1 for none; the loss on them weighs 1 - alpha.  weights: float32, per row.
+    gives: 'loss' (no gradient: None), 'gradient' (rows x classes, type of the scores), 'pairs' (rows x classes x 2, float32:
+    gradient and hessian, what a booster grows trees from)."""
+    _scores(scores)
+    n, k = scores.shape
+    _need(gives in _GIVES, "gives: 'loss', 'gradient' or 'pairs'")
+    for t, name, types in ((ids, 'ids', (torch.int32,)), (logits, 'logits', _TYPE)):
+        _need(isinstance(t, torch.Tensor) and t.device == scores.device and t.dim() == 2 and t.dtype in types and t.size(0) == n,
+              f'{name}: rows x kept classes on {scores.device}')
+        _need(t.size(1) <= 1 or t.stride(1) == 1, f'{name}: the entries of a row have to be side by side')
+    _need(ids.shape == logits.shape, 'ids and logits: one score for every class')
+    loss = torch.empty(n, dtype=torch.float32, device=scores.device)
+    grad = _like(scores, 2, dtype=torch.float32) if gives == 'pairs' else _like(scores) if gives == 'gradient' else None
+    per = 2 if gives == 'pairs' else 1
+    _call('tgbm_scores_distill', scores, n, k, _TYPE[scores.dtype], scores.data_ptr(), scores.stride(0), scores.stride(1), ids.size(1),
+          ids.data_ptr(), ids.stride(0), _TYPE[logits.dtype], logits.data_ptr(), logits.stride(0),
+          _beside(lse, scores, torch.float32, (n,), 'lse'), _beside(labels, scores, torch.int32, (n,), 'labels'),
+          _beside(weights, scores, torch.float32, (n,), 'weights'), temperature, alpha, loss.data_ptr(), _GIVES[gives],
+          None if grad is None else grad.data_ptr(), 0 if grad is None else grad.stride(0) // per,
+          0 if grad is None else grad.stride(1) // per)
+    return loss, grad
