@@ -15,6 +15,7 @@ namespace tgbm {
 namespace {
 
 constexpr int ROW_THREADS = 256;
+constexpr int FEW = 32, FEW_THREADS = 128;   // classes that a thread's registers hold, rows of a block then
 
 template <typename T> struct Scores {
     T *p;
@@ -84,6 +85,104 @@ __global__ void __launch_bounds__(ROW_THREADS) k_adjust(AdjustArgs a, Scores<T> 
 }
 
 // ------------------------------------------------------------------ top
+// A thread per row where there are few classes.  The rows of a block are written together: they lie side by side.
+template <typename T, int KP>
+__global__ void __launch_bounds__(FEW_THREADS) k_top_few(TopArgs a, Scores<T> in) {
+    extern __shared__ float found[];   // FEW_THREADS x top values, then as many classes
+    int *found_id = reinterpret_cast<int *>(found + FEW_THREADS * a.top);
+    const int tid = threadIdx.x;
+    for (long long n0 = (long long)blockIdx.x * FEW_THREADS; n0 < a.n; n0 += (long long)gridDim.x * FEW_THREADS) {
+        const long long n = n0 + tid;
+        if (n < a.n) {
+            float x[KP];
+            float m = minus_inf(), s = 0;
+            unsigned left = 0;
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                x[i] = i < a.k ? in(n, i) : minus_inf();
+                m = fmaxf(m, x[i]);
+                if (x[i] > minus_inf()) left |= 1u << i;
+            }
+            const float top = row_top(m);
+            if (a.lse) {
+#pragma unroll
+                for (int i = 0; i < KP; ++i) s += exp2_fast(__fsub_rn(x[i], top) * a.c);
+                a.lse[n] = (float)((double)top * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
+            }
+            for (int j = 0; j < a.top; ++j) {
+                float v = minus_inf();
+                int id = -1;
+#pragma unroll
+                for (int i = 0; i < KP; ++i)
+                    if ((left >> i & 1) && x[i] > v) { v = x[i]; id = i; }
+                if (id >= 0) left &= ~(1u << id);
+                found[tid * a.top + j] = __fadd_rn(v, 0.f);
+                found_id[tid * a.top + j] = id;
+            }
+        }
+        __syncthreads();
+        const int cells = (int)min((long long)FEW_THREADS, a.n - n0) * a.top;
+        for (int i = tid; i < cells; i += FEW_THREADS) {
+            a.values[n0 * a.top + i] = found[i];
+            a.ids[n0 * a.top + i] = found_id[i];
+        }
+        __syncthreads();
+    }
+}
+
+// A block takes a tile of rows x all classes into shared memory, a warp chooses for one row after the other.  By class: the rows of
+// a class are copied side by side, a cell of row r and class c lies at c * (rows + 1) + r, so that neither the copies nor the
+// reads along a row meet in a bank.  By row: a warp copies its own rows.
+constexpr int TILE_ROW_CLASSES = 1024;   // by row: above, a block takes a row
+constexpr int TILE_WARPS = 8, TILE_THREADS = 32 * TILE_WARPS;
+
+template <typename T, bool BY_CLASS>
+__device__ __forceinline__ void load_tile(float *tile, const Scores<T> &in, long long n0, int rows, int rows_log, int k) {
+    auto copy = [](float *to, const T *from) {
+        if constexpr (sizeof(T) == 4) copy_async4(to, from);
+        else *to = score_f32(*from);
+    };
+    if (BY_CLASS) {
+        const int r = threadIdx.x & ((1 << rows_log) - 1), per = TILE_THREADS >> rows_log;
+        if (r < rows) {
+            const T *p = in.at(n0 + r, 0);
+#pragma unroll 8
+            for (int c = threadIdx.x >> rows_log; c < k; c += per) copy(tile + c * ((1 << rows_log) + 1) + r, p + c * in.cls);
+        }
+    } else {
+        for (int r = threadIdx.x >> 5; r < rows; r += TILE_WARPS) {
+            const T *p = in.at(n0 + r, 0);
+#pragma unroll 8
+            for (int c = threadIdx.x & 31; c < k; c += 32) copy(tile + r * k + c, p + c * in.cls);
+        }
+    }
+}
+
+template <typename T, bool BY_CLASS, int G>
+__global__ void __launch_bounds__(TILE_THREADS) k_top_tile(TopArgs a, Scores<T> in, int rows_log) {
+    extern __shared__ __align__(16) float tile[];
+    __shared__ __align__(16) unsigned room[TILE_WARPS][2 * TOP_ROOM * G];
+    const long long n0 = (long long)blockIdx.x << rows_log;
+    const int rows = (int)min(1ll << rows_log, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    load_tile<T, BY_CLASS>(tile, in, n0, rows, rows_log, a.k);
+    copies_done();
+    if (BY_CLASS) __syncthreads(); else __syncwarp();
+    for (int r = warp; r < rows; r += TILE_WARPS) {
+        const float *z = BY_CLASS ? tile + r : tile + r * a.k;
+        const int step = BY_CLASS ? (1 << rows_log) + 1 : 1;
+        const long long n = n0 + r;
+        if (a.lse) {
+            float m = minus_inf(), s = 0;
+            for (int i = lane; i < a.k; i += 32) m = fmaxf(m, z[i * step]);
+            m = row_top(warp_max(m));
+            for (int i = lane; i < a.k; i += 32) s += exp2_fast(__fsub_rn(z[i * step], m) * a.c);
+            s = warp_sum(s);
+            if (lane == 0) a.lse[n] = (float)((double)m * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
+        }
+        warp_top<G>(z, step, a.k, a.top, room[warp], a.values + n * a.top, a.ids + n * a.top);
+    }
+}
+
 // A block per row: the largest of the keys below the last one chosen, again and again.
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) k_top_any(TopArgs a, Scores<T> in) {
@@ -104,16 +203,15 @@ __global__ void __launch_bounds__(ROW_THREADS) k_top_any(TopArgs a, Scores<T> in
     m = row_top(warp_max(part[lane & (ROW_THREADS / 32 - 1)]));
     __syncthreads();
     if (a.lse) {
-        const float c = (float)(1.44269504088896341 / (double)a.temperature);
         float s = 0;
-        for (int k = threadIdx.x; k < a.k; k += ROW_THREADS) s += exp2_fast(__fsub_rn(in(n, k), m) * c);
+        for (int k = threadIdx.x; k < a.k; k += ROW_THREADS) s += exp2_fast(__fsub_rn(in(n, k), m) * a.c);
         s = warp_sum(s);
         if (lane == 0) part[warp] = s;
         __syncthreads();
         if (threadIdx.x == 0) {
             s = 0;
             for (int w = 0; w < ROW_THREADS / 32; ++w) s += part[w];
-            a.lse[n] = broken ? __int_as_float(0x7fffffff) : (float)((double)m / (double)a.temperature + log((double)s));
+            a.lse[n] = broken ? __int_as_float(0x7fffffff) : (float)((double)m * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
         }
     }
     unsigned long long last = ~0ull;
@@ -143,21 +241,23 @@ __global__ void __launch_bounds__(ROW_THREADS) k_top_any(TopArgs a, Scores<T> in
 template <typename T, bool TWO>
 __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scores<T> in) {
     extern __shared__ unsigned listed_bits[];
-    __shared__ TeacherRow teacher;
+    __shared__ TeacherSide teacher;
+    __shared__ int list_id[SCORES_MAX_TOP];
+    __shared__ float list_q[SCORES_MAX_TOP];
     __shared__ StudentRow student;
     __shared__ DistillRow drow;
     __shared__ float part[3][ROW_THREADS / 32];
     const long long n = blockIdx.x;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, W = ROW_THREADS / 32;
-    const double inv_t = 1.0 / (double)a.temperature;
-    const float c = (float)(1.44269504088896341 / (double)a.temperature);
+    const double inv_t = a.inv_t;
+    const float c = a.c;
     for (int i = threadIdx.x; i < (a.k + 31) / 32; i += ROW_THREADS) listed_bits[i] = 0;
     __syncthreads();
     if (warp == 0) {
-        read_teacher(teacher, a, n, inv_t);
-        __syncwarp();
+        const TeacherSide t = read_teacher(a, n, list_id, list_q);
+        if (lane == 0) teacher = t;
         for (int j = lane; j < a.top; j += 32)
-            if (teacher.id[j] >= 0) atomicOr(&listed_bits[teacher.id[j] >> 5], 1u << (teacher.id[j] & 31));
+            if (list_id[j] >= 0) atomicOr(&listed_bits[list_id[j] >> 5], 1u << (list_id[j] & 31));
     }
     __syncthreads();
     auto is_listed = [&](int k) { return listed_bits[k >> 5] >> (k & 31) & 1; };
@@ -186,17 +286,17 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
         st.base = base; st.rest = s; st.rest1 = s1;
         float top = s > 0.f || s != s ? base : minus_inf();
         for (int j = lane; j < a.top; j += 32)
-            if (teacher.id[j] >= 0) top = fmaxf(top, in(n, teacher.id[j]));
+            if (list_id[j] >= 0) top = fmaxf(top, in(n, list_id[j]));
         st.top = row_top(warp_max(top));
         float l = 0, l1 = 0;
         double ql = 0, mass = 0;
         for (int j = lane; j < a.top; j += 32)
-            if (teacher.id[j] >= 0) {
-                const float z = in(n, teacher.id[j]), x = __fsub_rn(z, st.top);
+            if (list_id[j] >= 0) {
+                const float z = in(n, list_id[j]), x = __fsub_rn(z, st.top);
                 l += exp2_fast(x * c);
                 if (TWO) l1 += exp2_fast(x * LOG2E);
-                if (teacher.q[j] != 0.f) ql += (double)teacher.q[j] * (((double)z - (double)st.top) * inv_t);
-                mass += teacher.q[j];
+                if (list_q[j] != 0.f) ql += (double)list_q[j] * (((double)z - (double)st.top) * inv_t);
+                mass += list_q[j];
             }
         l = warp_sum(l); l1 = warp_sum(l1);
         if (!TWO) l1 = l;
@@ -225,7 +325,179 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
         for (int k = threadIdx.x; k < a.k; k += ROW_THREADS)
             if (!is_listed(k)) put(k, other_gh<TWO>(d, k, in(n, k)));
         for (int j = threadIdx.x; j < a.top; j += ROW_THREADS)
-            if (teacher.id[j] >= 0) put(teacher.id[j], listed_gh<TWO>(d, teacher.id[j], in(n, teacher.id[j]), teacher.q[j]));
+            if (list_id[j] >= 0) put(list_id[j], listed_gh<TWO>(d, list_id[j], in(n, list_id[j]), list_q[j]));
+    }
+    if (a.maxbits) track_max(mg, mh, a.maxbits);
+}
+
+// A thread per row where there are few classes: the row's scores stay in registers, what the teacher says of a class in a
+// column of shared memory (a class that is listed twice holds the sum).  Rows of a class are read side by side.
+
+template <typename T, int KP, bool TWO>
+__global__ void __launch_bounds__(FEW_THREADS) k_distill_few(DistillArgs a, Scores<T> in) {
+    __shared__ float qs[KP][FEW_THREADS];
+    const int tid = threadIdx.x, K = a.k;
+    float mg = 0, mh = 0;
+    for (long long n = (long long)blockIdx.x * FEW_THREADS + tid; n < a.n; n += (long long)gridDim.x * FEW_THREADS) {
+        float x[KP];
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            x[i] = i < K ? in(n, i) : minus_inf();
+            qs[i][tid] = 0.f;
+        }
+        const int *ids = a.ids + n * a.ids_stride;
+        // the teacher
+        TeacherSide t;
+        unsigned listed = 0;
+        float best = minus_inf();
+        bool broken = false;
+        for (int e = 0; e < a.top; ++e) {
+            const int id = ids[e];
+            if (id < 0 || id >= K) continue;
+            const float l = teacher_logit(a, n, e);
+            broken |= l != l;
+            best = fmaxf(best, l);
+            listed |= 1u << id;
+        }
+        const bool none = best == minus_inf() && !broken;
+        double mass = 0;
+        if (none) {
+            listed = 0;
+            t.total = t.rest = 0.f;
+        } else if (a.lse) {
+            const double L = (double)a.lse[n];
+            for (int e = 0; e < a.top; ++e) {
+                const int id = ids[e];
+                if (id < 0 || id >= K) continue;
+                const double q = exp((double)teacher_logit(a, n, e) * a.inv_t - L);
+                mass += q;
+                qs[id][tid] += (float)q;
+            }
+            const double rest = __popc(listed) < K && mass < 1 ? 1.0 - mass : 0.0;
+            t.rest = (float)rest;
+            t.total = (float)(mass + rest);
+        } else {
+            float sum = 0;
+            for (int e = 0; e < a.top; ++e) {
+                const int id = ids[e];
+                if (id >= 0 && id < K) sum += fine_exp(teacher_logit(a, n, e), best, a.c, a.c_low);
+            }
+            const float inv = 1.f / sum;
+            for (int e = 0; e < a.top; ++e) {
+                const int id = ids[e];
+                if (id >= 0 && id < K) qs[id][tid] += fine_exp(teacher_logit(a, n, e), best, a.c, a.c_low) * inv;
+            }
+            t.rest = 0.f;
+            t.total = 1.f;
+            mass = 1;
+        }
+        // the student: the listed classes apart where the rest is a class of its own
+        const unsigned apart = t.rest > 0.f ? listed : 0u;
+        StudentRow s;
+        float m = minus_inf(), mt = minus_inf();
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            mt = fmaxf(mt, x[i]);
+            if (!(apart >> i & 1)) m = fmaxf(m, x[i]);
+        }
+        s.top = row_top(mt);
+        s.base = row_top(m);
+        s.rest = s.rest1 = 0.f;
+        float l = 0, l1 = 0;
+#pragma unroll
+        for (int i = 0; i < KP; ++i)
+            if (!(apart >> i & 1)) {
+                const float d = __fsub_rn(x[i], s.base);
+                s.rest += exp2_fast(d * a.c);
+                if (TWO) s.rest1 += exp2_fast(d * LOG2E);
+            }
+        if (apart) {
+#pragma unroll
+            for (int i = 0; i < KP; ++i)
+                if (apart >> i & 1) {
+                    const float d = __fsub_rn(x[i], s.top);
+                    l += exp2_fast(d * a.c);
+                    if (TWO) l1 += exp2_fast(d * LOG2E);
+                }
+        }
+        const float low = __fsub_rn(s.base, s.top);
+        s.sum = s.rest * exp2_fast(low * a.c) + l;
+        s.sum1 = TWO ? s.rest1 * exp2_fast(low * LOG2E) + l1 : s.sum;
+        const float w = a.weights ? a.weights[n] : 1.f;
+        const int label = row_label(a, n);
+        const DistillRow d = distill_row(a, t, s, w, label);
+        if (a.loss) {
+            double of_listed = 0, of_q = 0;
+            unsigned left = listed;
+            while (left) {
+                const int id = __ffs(left) - 1;
+                left &= left - 1;
+                const float q = qs[id][tid];
+                if (q == 0.f) continue;
+                of_q += (double)q * fine_log(q);
+                of_listed += (double)q * (((double)in(n, id) - (double)s.top) * a.inv_t);
+            }
+            t.entropy = of_q;
+            a.loss[n] = distill_loss(a, t, s, w, label, of_listed, mass, label >= 0 ? in(n, label) : 0.f);
+        }
+        if (a.gives == GIVES_LOSS) continue;
+#pragma unroll
+        for (int i = 0; i < KP; ++i) {
+            if (i >= K) break;
+            const float q = qs[i][tid];
+            const float2 gh = (apart >> i & 1) || apart == 0 ? listed_gh<TWO>(d, i, x[i], q) : other_gh<TWO>(d, i, x[i]);
+            const long long at = n * a.out.row + i * a.out.cls;
+            if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
+            else static_cast<T *>(a.out.data)[at] = score_from<T>(gh.x);
+            mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
+        }
+    }
+    if (a.maxbits) track_max(mg, mh, a.maxbits);
+}
+
+// A tile as in k_top_tile: the teacher's lists are read while the scores are on their way, a warp finds the factors of one row after
+// the other, and the gradients are written the way the scores were read.
+template <typename T, bool BY_CLASS, bool TWO>
+__global__ void __launch_bounds__(TILE_THREADS) k_distill_tile(DistillArgs a, Scores<T> in, int rows_log) {
+    extern __shared__ __align__(16) float tile[];
+    const int R = 1 << rows_log, step = BY_CLASS ? R + 1 : 1;
+    int *list_id = reinterpret_cast<int *>(tile + (size_t)a.k * (BY_CLASS ? R + 1 : R));
+    float *list_q = reinterpret_cast<float *>(list_id + R * a.top);
+    __shared__ TeacherSide side[32];
+    __shared__ DistillRow factors[32];
+    const long long n0 = (long long)blockIdx.x << rows_log;
+    const int rows = (int)min((long long)R, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    load_tile<T, BY_CLASS>(tile, in, n0, rows, rows_log, a.k);
+    for (int r = warp; r < rows; r += TILE_WARPS) {
+        const TeacherSide t = read_teacher(a, n0 + r, list_id + r * a.top, list_q + r * a.top);
+        if (lane == 0) side[r] = t;
+    }
+    copies_done();
+    if (BY_CLASS) __syncthreads(); else __syncwarp();
+    float mg = 0, mh = 0;
+    auto put = [&](const DistillRow &d, int r, int c, float z) {
+        const int e = r * a.top + min(listed_entry(z), a.top - 1);
+        const float2 gh = is_listed_cell(z) ? listed_gh<TWO>(d, c, __int_as_float(list_id[e]), list_q[e]) : other_gh<TWO>(d, c, z);
+        const long long n = n0 + r;
+        const long long at = n * a.out.row + c * a.out.cls;
+        if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
+        else static_cast<T *>(a.out.data)[at] = score_from<T>(gh.x);
+        mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
+    };
+    for (int r = warp; r < rows; r += TILE_WARPS) {
+        float *z = BY_CLASS ? tile + r : tile + r * a.k;
+        const DistillRow d = warp_student<TWO>(a, side[r], n0 + r, z, step, list_id + r * a.top, list_q + r * a.top);
+        if (BY_CLASS) { if (lane == 0) factors[r] = d; }
+        else if (a.gives != GIVES_LOSS)
+            for (int c = lane; c < a.k; c += 32) put(d, r, c, z[c]);
+    }
+    if (BY_CLASS && a.gives != GIVES_LOSS) {
+        __syncthreads();
+        const int r = threadIdx.x & (R - 1), per = TILE_THREADS >> rows_log;
+        if (r < rows) {
+            const DistillRow d = factors[r];
+            for (int c = threadIdx.x >> rows_log; c < a.k; c += per) put(d, r, c, tile[c * step + r]);
+        }
     }
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
@@ -233,6 +505,25 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
 }  // namespace
 
 // ------------------------------------------------------------------ launches
+constexpr int FEW_BLOCKS = 148 * 16;   // at most what the GPU holds at once; the blocks walk the rows
+
+// Rows of a tile, as a power of two from 8 to 32, and its shared memory; 0 bytes: the row is too long for a tile.  Several
+// blocks should fit on an SM, so that one copies while another computes; with few rows the tiles are smaller and there are
+// more of them.  (A row's result does not depend on the tile it is in.)
+constexpr size_t TILE_SHARED = 200 * 1024, TILE_WANTED = 40 * 1024;
+struct Tile {
+    int rows_log = 5;
+    size_t shared = 0;
+};
+Tile tile_of(int n, int k, bool by_class, size_t per_row) {
+    auto shared = [&](int log) { return sizeof(float) * (size_t)k * ((1 << log) + (by_class ? 1 : 0)) + (per_row << log); };
+    Tile t;
+    if (!by_class && k > TILE_ROW_CLASSES) return t;
+    while (t.rows_log > 3 && (shared(t.rows_log) > TILE_WANTED || (n >> t.rows_log) < 2 * 148)) --t.rows_log;
+    if (shared(t.rows_log) <= TILE_SHARED) t.shared = shared(t.rows_log);
+    return t;
+}
+
 void scores_adjust(const AdjustArgs &a, cudaStream_t stream) {
     if (a.n == 0) return;
     const bool by_class = a.in.row < a.in.cls;
@@ -248,20 +539,74 @@ void scores_adjust(const AdjustArgs &a, cudaStream_t stream) {
     TGBM_CUDA(cudaGetLastError());
 }
 
-void scores_top(const TopArgs &a, cudaStream_t stream) {
-    if (a.n == 0) return;
+void scores_top(const TopArgs &given, cudaStream_t stream) {
+    if (given.n == 0) return;
+    TopArgs a = given;
+    a.inv_t = 1.0 / (double)a.temperature;
+    a.c = (float)(1.44269504088896341 * a.inv_t);
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
+        if (a.k <= FEW) {
+            const int blocks = (int)std::min(((long long)a.n + FEW_THREADS - 1) / FEW_THREADS, (long long)FEW_BLOCKS);
+            const size_t smem = (size_t)FEW_THREADS * a.top * 8;
+            auto go = [&](auto kern) {
+                if (smem > 48 * 1024) allow_shared(kern, (size_t)FEW_THREADS * SCORES_MAX_TOP * 8);
+                kern<<<blocks, FEW_THREADS, smem, stream>>>(a, scores_of<T>(a.in));
+            };
+            if (a.k <= 8) go(k_top_few<T, 8>);
+            else if (a.k <= 16) go(k_top_few<T, 16>);
+            else go(k_top_few<T, 32>);
+            return;
+        }
+        const bool by_class = a.in.row < a.in.cls;
+        const Tile tile = tile_of(a.n, a.k, by_class, 0);
+        if (tile.shared) {
+            auto go = [&](auto kern) {
+                if (tile.shared > 30 * 1024) allow_shared(kern, TILE_SHARED);
+                kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, scores_of<T>(a.in), tile.rows_log);
+            };
+            auto groups = [&](auto by) {
+                constexpr bool B = decltype(by)::value;
+                if (a.top <= 32) go(k_top_tile<T, B, 1>);
+                else if (a.top <= 64) go(k_top_tile<T, B, 2>);
+                else go(k_top_tile<T, B, 4>);
+            };
+            by_class ? groups(std::true_type{}) : groups(std::false_type{});
+            return;
+        }
         k_top_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, scores_of<T>(a.in));
     });
     TGBM_CUDA(cudaGetLastError());
 }
 
-void scores_distill(const DistillArgs &a, cudaStream_t stream) {
-    if (a.n == 0) return;
+void scores_distill(const DistillArgs &given, cudaStream_t stream) {
+    if (given.n == 0) return;
+    DistillArgs a = given;
+    a.inv_t = 1.0 / (double)a.temperature;
+    a.c = (float)(1.44269504088896341 * a.inv_t);
+    a.c_low = (float)(1.44269504088896341 * a.inv_t - (double)a.c);
     const bool two = a.alpha < 1.f && a.temperature != 1.f;
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
+        if (a.k <= FEW) {
+            const int blocks = (int)std::min(((long long)a.n + FEW_THREADS - 1) / FEW_THREADS, (long long)FEW_BLOCKS);
+            auto go = [&](auto kern) { kern<<<blocks, FEW_THREADS, 0, stream>>>(a, scores_of<T>(a.in)); };
+            if (a.k <= 8) two ? go(k_distill_few<T, 8, true>) : go(k_distill_few<T, 8, false>);
+            else if (a.k <= 16) two ? go(k_distill_few<T, 16, true>) : go(k_distill_few<T, 16, false>);
+            else two ? go(k_distill_few<T, 32, true>) : go(k_distill_few<T, 32, false>);
+            return;
+        }
+        const bool by_class = a.in.row < a.in.cls;
+        const Tile tile = tile_of(a.n, a.k, by_class, 8 * (size_t)a.top);
+        if (tile.shared) {
+            auto go = [&](auto kern) {
+                if (tile.shared > 40 * 1024) allow_shared(kern, TILE_SHARED);
+                kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, scores_of<T>(a.in), tile.rows_log);
+            };
+            if (by_class) two ? go(k_distill_tile<T, true, true>) : go(k_distill_tile<T, true, false>);
+            else two ? go(k_distill_tile<T, false, true>) : go(k_distill_tile<T, false, false>);
+            return;
+        }
         auto kern = two ? k_distill_any<T, true> : k_distill_any<T, false>;
         constexpr size_t most = SCORES_MAX_CLASSES / 8;
         const size_t smem = sizeof(unsigned) * (size_t)((a.k + 31) / 32);

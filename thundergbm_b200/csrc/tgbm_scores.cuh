@@ -26,6 +26,25 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
+// log of a float sum to about 2^-25, absolutely (logf is off by half a step of its result, which for a sum of many terms is
+// several times that): the exponent is exact, the rest lies in [sqrt(1/2), sqrt(2))
+__device__ __forceinline__ double fine_log(float x) {
+    if (!(x >= 1.17549435e-38f && x <= 3.40282347e38f)) return (double)logf(x);
+    const int b = __float_as_int(x), e = (b - 0x3f3504f3) >> 23;
+    return (double)e * 0.6931471805599453 + (double)logf(__int_as_float(b - (e << 23)));
+}
+
+// exp((x - ref) / T) to a few steps of the result wherever it lies: what x - ref and the product with 1 / T lose is put back.
+// c + c_low = log2(e) / T.
+__device__ __forceinline__ float fine_exp(float x, float ref, float c, float c_low) {
+    const float d = __fsub_rn(x, ref);
+    const float b = __fsub_rn(d, x);
+    const float lost = __fsub_rn(__fsub_rn(x, __fsub_rn(d, b)), __fadd_rn(ref, b));
+    const float y = __fmul_rn(d, c);
+    const float low = __fmaf_rn(d, c, -y) + (d * c_low + lost * c);
+    return fabsf(low) < 1.f ? __fmaf_rn(exp2f(y), low * 0.693147181f, exp2f(y)) : exp2f(y);   // (not for infinities)
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -59,16 +78,16 @@ __device__ __forceinline__ float teacher_logit(const DistillArgs &a, long long n
 // or (none given) that of the listed ones; of the mass that is left, `rest`, nothing is known but that it lies on the others.
 // A class that is listed twice holds the sum of both.  Worked in doubles: `rest` and the logarithms are differences of nearly
 // equal numbers, and there are only a few of them per row.
-struct TeacherRow {
-    float q[SCORES_MAX_TOP];   // mass of a listed class; only where id >= 0
-    int id[SCORES_MAX_TOP];    // -1: no class, or one that stands further in front
-    double entropy;            // sum of q log q over the listed classes and the rest
+struct TeacherSide {
+    double entropy;            // sum of q log q over the listed classes
     float total, rest;         // all mass (0: the row has no teacher), what is not listed
 };
 
-// one warp; entry e = lane + 32 s of the row's list
-__device__ __forceinline__ void read_teacher(TeacherRow &r, const DistillArgs &a, long long n, double inv_t) {
+// One warp; entry e = lane + 32 s of the row's list.  list_id[e]: the class, -1 where it is none or stands further in front;
+// list_q[e]: its mass.
+__device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long long n, int *list_id, float *list_q) {
     const int top = a.top, k = a.k;
+    const double inv_t = a.inv_t;
     const int *ids = a.ids + n * a.ids_stride;
     const float *lse = a.lse ? a.lse + n : nullptr;
     constexpr int S = SCORES_MAX_TOP / 32;
@@ -138,7 +157,7 @@ __device__ __forceinline__ void read_teacher(TeacherRow &r, const DistillArgs &a
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const int e = lane + 32 * s;
-        if (e < top) { r.id[e] = id[s]; r.q[e] = (float)q[s]; }
+        if (e < top) { list_id[e] = id[s]; list_q[e] = (float)q[s]; }
         mass += q[s];
         if (q[s] != 0) entropy += q[s] * lq[s];
         distinct += id[s] >= 0;
@@ -147,11 +166,12 @@ __device__ __forceinline__ void read_teacher(TeacherRow &r, const DistillArgs &a
     entropy = warp_sum(entropy);
     distinct = warp_sum(distinct);
     const double rest = lse && !none && distinct < k && mass < 1 ? 1.0 - mass : 0.0;
-    if (lane == 0) {
-        r.total = none ? 0.f : (float)(mass + rest);
-        r.rest = (float)rest;
-        r.entropy = rest > 0 ? entropy + rest * log(rest) : entropy;
-    }
+    __syncwarp();
+    TeacherSide r;
+    r.total = none ? 0.f : (float)(mass + rest);
+    r.rest = (float)rest;
+    r.entropy = entropy;
+    return r;
 }
 
 // ---- the student's side ----------------------------------------------------------------------
@@ -209,9 +229,9 @@ __device__ __forceinline__ int row_label(const DistillArgs &a, long long n) {
     return -1;
 }
 
-__device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const TeacherRow &t, const StudentRow &s, float w, int label) {
+__device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const TeacherSide &t, const StudentRow &s, float w, int label) {
     DistillRow d;
-    const float c = (float)(1.44269504088896341 / (double)a.temperature);
+    const float c = a.c;
     const float alpha = t.total == 0.f ? 0.f : a.alpha;
     const float low = __fsub_rn(s.base, s.top);
     d.base = s.base; d.top = s.top; d.c = c;
@@ -228,19 +248,192 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Te
     return d;
 }
 // listed: sum over the listed classes of q (s - top) / T; mass: of their q
-__device__ __forceinline__ float distill_loss(const DistillArgs &a, const TeacherRow &t, const StudentRow &s, float w, int label,
+__device__ __forceinline__ float distill_loss(const DistillArgs &a, const TeacherSide &t, const StudentRow &s, float w, int label,
                                               double listed, double mass, float label_score) {
     double loss = 0;
-    const double inv_t = 1.0 / (double)a.temperature;
+    const double inv_t = a.inv_t;
     // (a row without a score above -inf: its listed sum or its label's score is -inf already, and the loss infinite)
-    const double log_sum = s.sum == 0.f ? 0.0 : log((double)s.sum), log_sum1 = s.sum1 == 0.f ? 0.0 : log((double)s.sum1);
+    const double log_sum = s.sum == 0.f ? 0.0 : fine_log(s.sum);
     if (t.total != 0.f) {
         double kl = t.entropy - (listed - mass * log_sum);
-        if (t.rest > 0.f) kl -= (double)t.rest * (((double)s.base - (double)s.top) * inv_t + log((double)s.rest) - log_sum);
+        if (t.rest > 0.f) kl += (double)t.rest * (fine_log(t.rest) - ((double)s.base - (double)s.top) * inv_t - fine_log(s.rest) + log_sum);
         loss += (double)a.alpha * a.temperature * a.temperature * kl;
     }
-    if (label >= 0 && a.alpha < 1.f) loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - log_sum1);
+    if (label >= 0 && a.alpha < 1.f)
+        loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - (s.sum1 == 0.f ? 0.0 : s.sum1 == s.sum ? log_sum : fine_log(s.sum1)));
     return (float)((double)w * loss);
+}
+
+// ---- a row whose scores lie in shared memory, one warp ---------------------------------------
+// asynchronous copy of one float into shared memory
+__device__ __forceinline__ void copy_async4(float *to, const float *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// The `top` largest of k scores z[i * step], in order.  The k-th largest of the maxima of 32 G groups of classes is no more than
+// the k-th largest score, so the scores from there on hold the answer: few more than `top`, unless the large ones lie in few groups.
+// They are collected in class order, and each finds its place by counting those before it.  Rows with too many (more than
+// TOP_ROOM G) choose one after the other.  `room`: TOP_ROOM G keys and as many classes of the warp's own.
+constexpr int TOP_ROOM = 64;
+
+template <int G>
+__device__ __forceinline__ void warp_top(const float *z, int step, int k, int top, unsigned *room, float *values, int *ids) {
+    const int lane = threadIdx.x & 31;
+    unsigned *keys = room;
+    int *place = reinterpret_cast<int *>(room + TOP_ROOM * G);
+    unsigned mx[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) mx[g] = 0;
+    for (int i = lane; i < k;) {
+#pragma unroll
+        for (int g = 0; g < G; ++g, i += 32)
+            if (i < k) mx[g] = max(mx[g], score_key(z[i * step]));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) keys[lane + 32 * g] = mx[g];
+    __syncwarp();
+    // the largest key that at least `top` of the maxima reach
+    unsigned from = 0xffffffffu;
+    {
+        int above[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) above[g] = 0;
+        for (int j = 0; j < 32 * G; j += 4) {
+            const uint4 o = *reinterpret_cast<const uint4 *>(keys + j);
+#pragma unroll
+            for (int g = 0; g < G; ++g) above[g] += (o.x > mx[g]) + (o.y > mx[g]) + (o.z > mx[g]) + (o.w > mx[g]);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+            if (above[g] < top) from = min(from, mx[g]);
+    }
+    from = __reduce_min_sync(0xffffffffu, from);
+    __syncwarp();
+    int m = 0, equal = 0;
+    const unsigned before = (1u << lane) - 1;
+    for (int i0 = 0; i0 < k; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned key = i < k ? score_key(z[i * step]) : 0u;
+        unsigned take = __ballot_sync(0xffffffffu, key > from);
+        const unsigned eq = __ballot_sync(0xffffffffu, key == from && from != 0u);
+        if (eq) {   // of those equal to the border `top` are enough
+            const bool first = (eq >> lane & 1) && equal + __popc(eq & before) < top;
+            take |= __ballot_sync(0xffffffffu, first);
+            equal += __popc(eq);
+        }
+        const int at = m + __popc(take & before);
+        if ((take >> lane & 1) && at < TOP_ROOM * G) { keys[at] = key; place[at] = i; }
+        m += __popc(take);
+    }
+    if (m <= TOP_ROOM * G) {
+        if (lane < 4 && m + lane < TOP_ROOM * G) keys[m + lane] = 0;   // (read four at a time)
+        __syncwarp();
+        for (int c = lane; c < m; c += 32) {
+            const unsigned own = keys[c];
+            int rank = 0;
+            for (int j = 0; j < m; j += 4) {
+                const uint4 o = *reinterpret_cast<const uint4 *>(keys + j);
+                // of equal ones the lower class, which stands in front
+                rank += (o.x >= own + (j >= c)) + (o.y >= own + (j + 1 >= c)) + (o.z >= own + (j + 2 >= c)) + (o.w >= own + (j + 3 >= c));
+            }
+            if (rank < top) { values[rank] = key_score(own); ids[rank] = place[c]; }
+        }
+        for (int j = m + lane; j < top; j += 32) { values[j] = minus_inf(); ids[j] = -1; }
+    } else {
+        unsigned long long last = ~0ull;
+        for (int j = 0; j < top; ++j) {
+            unsigned long long b = 0;
+            for (int i = lane; i < k; i += 32) {
+                const unsigned key = score_key(z[i * step]);
+                const unsigned long long v = (unsigned long long)key << 32 | (unsigned)~i;
+                if (key && v < last && v > b) b = v;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+            last = b;
+            if (lane == 0) { values[j] = key_score((unsigned)(b >> 32)); ids[j] = b ? (int)~(unsigned)b : -1; }
+        }
+    }
+    __syncwarp();
+}
+
+// A cell of a tile that holds the number of its entry in the row's list instead of a score: a NaN of a kind of its own.  (A score
+// that is such a NaN itself leaves its row without a finite sum: whatever entry of the list is taken, the results are NaN.)
+constexpr unsigned LISTED_CELL = 0xffca5000u;
+__device__ __forceinline__ float listed_cell(int entry) { return __uint_as_float(LISTED_CELL | (unsigned)entry); }
+__device__ __forceinline__ bool is_listed_cell(float z) { return (__float_as_uint(z) & 0xffffff80u) == LISTED_CELL; }
+__device__ __forceinline__ int listed_entry(float z) { return (int)(__float_as_uint(z) & 0x7fu); }
+
+// The student's side of the row z[i * step].  The cells of listed classes are marked, and their scores take the place of the class
+// numbers in the list.  Returns the factors of the row's gradients.
+template <bool TWO>
+__device__ __forceinline__ DistillRow warp_student(const DistillArgs &a, const TeacherSide &t, long long n, float *z, int step, int *list_id,
+                                                   const float *list_q) {
+    constexpr int S = SCORES_MAX_TOP / 32;
+    const int lane = threadIdx.x & 31, k = a.k;
+    const int label = row_label(a, n);
+    const float label_score = label >= 0 ? z[label * step] : 0.f, w = a.weights ? a.weights[n] : 1.f;
+    float x[S];
+    float top = minus_inf();
+    __syncwarp();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int e = lane + 32 * s;
+        x[s] = minus_inf();
+        if (e < a.top && list_id[e] >= 0) {
+            float *cell = z + list_id[e] * step;
+            x[s] = *cell;
+            *cell = minus_inf();
+            top = fmaxf(top, x[s]);
+        }
+    }
+    __syncwarp();
+    float m = minus_inf();
+    for (int i = lane; i < k; i += 32) m = fmaxf(m, z[i * step]);
+    m = warp_max(m);
+    StudentRow st;
+    st.base = row_top(m);
+    st.top = row_top(fmaxf(warp_max(top), m));
+    float s0 = 0, s1 = 0;
+    for (int i = lane; i < k; i += 32) {
+        const float d = __fsub_rn(z[i * step], st.base);
+        s0 += exp2_fast(d * a.c);
+        if (TWO) s1 += exp2_fast(d * LOG2E);
+    }
+    st.rest = warp_sum(s0);
+    st.rest1 = TWO ? warp_sum(s1) : st.rest;
+    float l = 0, l1 = 0;
+    double of_listed = 0, mass = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        if (s > 0 && 32 * s >= a.top) continue;
+        const int e = lane + 32 * s;
+        if (e < a.top && list_id[e] >= 0) {
+            const float d = __fsub_rn(x[s], st.top), q = list_q[e];
+            l += exp2_fast(d * a.c);
+            if (TWO) l1 += exp2_fast(d * LOG2E);
+            if (a.loss) {
+                if (q != 0.f) of_listed += (double)q * (((double)x[s] - (double)st.top) * a.inv_t);
+                mass += q;
+            }
+            z[list_id[e] * step] = listed_cell(e);
+            list_id[e] = __float_as_int(x[s]);
+        }
+    }
+    l = warp_sum(l);
+    if (TWO) l1 = warp_sum(l1);
+    const float low = __fsub_rn(st.base, st.top);
+    st.sum = st.rest * exp2_fast(low * a.c) + l;
+    st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + l1 : st.sum;
+    if (a.loss) {
+        of_listed = warp_sum(of_listed);
+        mass = warp_sum(mass);
+        const float loss = distill_loss(a, t, st, w, label, of_listed, mass, label_score);
+        if (lane == 0) a.loss[n] = loss;
+    }
+    __syncwarp();
+    return distill_row(a, t, st, w, label);
 }
 
 }  // namespace tgbm

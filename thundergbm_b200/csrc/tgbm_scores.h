@@ -36,6 +36,8 @@ struct TopArgs {
     int n = 0, k = 0, top = 0;
     ScoreView in;
     float temperature = 1.f;
+    double inv_t = 1;          // filled in by scores_top, scores_distill: 1 / T, and c with exp(x / T) = 2^(x c)
+    float c = 0;
     float *values = nullptr;   // n x top
     int *ids = nullptr;        // n x top
     float *lse = nullptr;      // n, or null
@@ -55,6 +57,8 @@ struct DistillArgs {
     const float *labels_f = nullptr;  // ... the same as floats (the booster's)
     const float *weights = nullptr;
     float temperature = 1.f, alpha = 1.f;
+    double inv_t = 1;
+    float c = 0, c_low = 0;
     int gives = GIVES_LOSS;
     float *loss = nullptr;            // n, or null
     ScoreView out;                    // gradient in the scores' type, or (gradient, hessian) pairs of floats

@@ -18,27 +18,28 @@ import torch
 from . import _lib
 
 _TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_INT = (torch.int32,)
 _GIVES = {'loss': 0, 'gradient': 1, 'pairs': 2}
 MAX_TOP = 128
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
+def _refuse(what):
+    raise ValueError(what)
 
 
 def _scores(t, name='scores'):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _TYPE,
-          f'{name}: a CUDA tensor of rows x classes in float32, float16 or bfloat16')
-    _need(t.size(1) >= 1 and t.size(0) < 2 ** 31, f'{name}: at least one class and fewer than 2^31 rows')
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _TYPE):
+        _refuse(f'{name}: a CUDA tensor of rows x classes in float32, float16 or bfloat16')
+    if not (t.size(1) >= 1 and t.size(0) < 2 ** 31 and t.size(1) < 2 ** 31):
+        _refuse(f'{name}: at least one class and fewer than 2^31 rows')
 
 
 def _beside(t, scores, dtype, shape, name):
     """Address of a contiguous tensor on the scores' device."""
     if t is None:
         return None
-    _need(isinstance(t, torch.Tensor) and t.device == scores.device and t.dtype == dtype and t.is_contiguous() and tuple(t.shape) == shape,
-          f'{name}: a contiguous {dtype} tensor of shape {shape} on {scores.device}')
+    if not (isinstance(t, torch.Tensor) and t.device == scores.device and t.dtype == dtype and t.is_contiguous() and t.shape == shape):
+        _refuse(f'{name}: a contiguous {dtype} tensor of shape {shape} on {scores.device}')
     return t.data_ptr()
 
 
@@ -77,19 +78,23 @@ def adjust(scores, *, out=None, bias=None, allowed=None, allowed_row=None, histo
         out = _like(scores)
     else:
         _scores(out, 'out')
-        _need(out.shape == scores.shape and out.dtype == scores.dtype and out.device == scores.device, 'out: shape, type and device of the scores')
+        if not (out.shape == scores.shape and out.dtype == scores.dtype and out.device == scores.device):
+            _refuse('out: shape, type and device of the scores')
     masks = words = 0
     if allowed is not None:
-        _need(isinstance(allowed, torch.Tensor) and allowed.dim() == 2, 'allowed: masks x words')
+        if not (isinstance(allowed, torch.Tensor) and allowed.dim() == 2):
+            _refuse('allowed: masks x words')
         masks, words = allowed.shape
-        _need(words >= (k + 31) // 32, 'allowed: a bit for every class')
-    else:
-        _need(allowed_row is None, 'allowed_row: there are no masks')
+        if words < (k + 31) // 32:
+            _refuse('allowed: a bit for every class')
+    elif allowed_row is not None:
+        _refuse('allowed_row: there are no masks')
     given = 0
     ptr = ids = None
     if history is not None:
         ptr, ids = history
-        _need(isinstance(ids, torch.Tensor) and ids.dim() == 1, 'history: (ptr, classes)')
+        if not (isinstance(ids, torch.Tensor) and ids.dim() == 1):
+            _refuse('history: (ptr, classes)')
         given = ids.numel()
     _call('tgbm_scores_adjust', scores, n, k, _TYPE[scores.dtype], scores.data_ptr(), scores.stride(0), scores.stride(1), out.data_ptr(),
           out.stride(0), out.stride(1), _beside(bias, scores, torch.float32, (k,), 'bias'),
@@ -104,7 +109,8 @@ def top(scores, k, *, temperature=1.0):
     their classes (int32) and the log of the sum over all classes of exp(score / temperature).  Masked scores (-inf) and NaN are not
     chosen: a row that runs out of others ends in -inf and class -1."""
     _scores(scores)
-    _need(1 <= k <= MAX_TOP, f'k: 1 to {MAX_TOP}')
+    if not 1 <= k <= MAX_TOP:
+        _refuse(f'k: 1 to {MAX_TOP}')
     n = scores.size(0)
     values = torch.empty((n, k), dtype=torch.float32, device=scores.device)
     ids = torch.empty((n, k), dtype=torch.int32, device=scores.device)
@@ -125,12 +131,15 @@ def distill(scores, ids, logits, *, lse=None, labels=None, weights=None, tempera
     gradient and hessian, what a booster grows trees from)."""
     _scores(scores)
     n, k = scores.shape
-    _need(gives in _GIVES, "gives: 'loss', 'gradient' or 'pairs'")
-    for t, name, types in ((ids, 'ids', (torch.int32,)), (logits, 'logits', _TYPE)):
-        _need(isinstance(t, torch.Tensor) and t.device == scores.device and t.dim() == 2 and t.dtype in types and t.size(0) == n,
-              f'{name}: rows x kept classes on {scores.device}')
-        _need(t.size(1) <= 1 or t.stride(1) == 1, f'{name}: the entries of a row have to be side by side')
-    _need(ids.shape == logits.shape, 'ids and logits: one score for every class')
+    if gives not in _GIVES:
+        _refuse("gives: 'loss', 'gradient' or 'pairs'")
+    for t, name, types in ((ids, 'ids', _INT), (logits, 'logits', _TYPE)):
+        if not (isinstance(t, torch.Tensor) and t.device == scores.device and t.dim() == 2 and t.dtype in types and t.size(0) == n):
+            _refuse(f'{name}: rows x kept classes, {", ".join(map(str, types))}, on {scores.device}')
+        if t.stride(1) != 1 and t.size(1) > 1:
+            _refuse(f'{name}: the entries of a row have to be side by side')
+    if ids.shape != logits.shape:
+        _refuse('ids and logits: one score for every class')
     loss = torch.empty(n, dtype=torch.float32, device=scores.device)
     grad = _like(scores, 2, dtype=torch.float32) if gives == 'pairs' else _like(scores) if gives == 'gradient' else None
     per = 2 if gives == 'pairs' else 1
