@@ -8,11 +8,14 @@
 #include <cmath>
 
 #include "../../include/thundergbm.h"
+#include <cooperative_groups.h>
+
 #include "tgbm_kernels.cuh"
 #include "tgbm_scores.cuh"
 
 namespace tgbm {
 namespace {
+namespace cg = cooperative_groups;
 
 constexpr int ROW_THREADS = 256;
 constexpr int FEW = 32, FEW_THREADS = 128;   // classes that a thread's registers hold, rows of a block then
@@ -181,6 +184,271 @@ __global__ void __launch_bounds__(TILE_THREADS) k_top_tile(TopArgs a, Scores<T> 
         }
         warp_top<G>(z, step, a.k, a.top, room[warp], a.values + n * a.top, a.ids + n * a.top);
     }
+}
+
+// A long row: a block takes it, or a cluster of blocks where there are few rows, each a part.  One pass.  From its first packs a
+// block learns a border that at least `top` scores reach (the top-th largest of the maxima of groups of threads); only scores
+// that reach it are kept, in shared memory.  Where that list fills up the border is raised.  At the end the list (about
+// top * k / first packs' scores long) is narrowed down the same way until each entry can count those before it.
+// An entry orders scores and classes at once, so no choice depends on the order of the list.
+constexpr int WIDE_THREADS = 512, WIDE_WARPS = WIDE_THREADS / 32, WIDE_PACKS = 4, WIDE_CLUSTER = 8;
+constexpr int WIDE_ROOM = 2048, WIDE_GROUPS = WIDE_THREADS / 2, WIDE_LAST = 256;
+static_assert(WIDE_GROUPS >= SCORES_MAX_TOP && WIDE_CLUSTER * SCORES_MAX_TOP <= WIDE_ROOM, "");
+typedef unsigned long long Entry;   // score_key << 32 | ~class
+
+struct TopList {
+    Entry e[WIDE_ROOM];
+    Entry group[WIDE_GROUPS];
+    Entry border;              // entries below it cannot be among the `top`
+    int count;
+};
+__device__ __forceinline__ Entry entry_of(float v, int k) { return (Entry)score_key(v) << 32 | (unsigned)~k; }
+constexpr Entry LOWEST_ENTRY = 1ull << 32;   // what is below is no score that can be chosen
+
+// border = the top-th largest of the groups' maxima (every thread has one, those of two neighbours make a group's); all threads
+__device__ __forceinline__ void find_border(TopList &l, Entry mine, int top) {
+    mine = mine < LOWEST_ENTRY ? 0 : mine;
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+    if (!(threadIdx.x & 1)) l.group[threadIdx.x >> 1] = mine;
+    __syncthreads();
+    if (threadIdx.x < WIDE_GROUPS) {
+        const Entry own = l.group[threadIdx.x];
+        int above = 0;
+#pragma unroll 8
+        for (int j = 0; j < WIDE_GROUPS; j += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&l.group[j]);
+            above += (o.x > own) + (o.y > own);
+        }
+        if (own && above == top - 1 && own > l.border) l.border = own;   // (one thread at most: entries differ)
+    }
+    __syncthreads();
+}
+
+// Keeps the entries that reach the border, which is raised to that of their groups first, or (exactly) to the top-th largest entry,
+// found bit by bit; all threads.
+__device__ __noinline__ void narrow(TopList &l, int top, bool exactly) {
+    constexpr int U = WIDE_ROOM / WIDE_THREADS;
+    const int m = l.count;
+    Entry own[U], most = 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int at = threadIdx.x + i * WIDE_THREADS;
+        own[i] = at < m ? l.e[at] : 0;
+        most = max(most, own[i]);
+    }
+    if (exactly) {
+        Entry reached = 0;
+        for (int bit = 63; bit >= 0; --bit) {
+            const Entry trial = reached | 1ull << bit;
+            int reach = 0;
+#pragma unroll
+            for (int i = 0; i < U; ++i) reach += __syncthreads_count(own[i] >= trial);
+            if (reach >= top) reached = trial;
+        }
+        if (threadIdx.x == 0 && reached > l.border) l.border = reached;
+        __syncthreads();
+    } else {
+        find_border(l, most, top);
+    }
+    if (threadIdx.x == 0) l.count = 0;
+    __syncthreads();
+    const Entry border = l.border;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (own[i] >= border) l.e[atomicAdd(&l.count, 1)] = own[i];
+    __syncthreads();
+}
+// (where large entries fall into few groups, the second way leaves no more than `top`, which is within `room`)
+__device__ __forceinline__ void narrow_to(TopList &l, int top, int room) {
+    bool exactly = false;
+    while (l.count > room) {
+        const int before = l.count;
+        narrow(l, top, exactly);
+        exactly = l.count * 2 > before;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(WIDE_THREADS, 2) k_top_wide(TopArgs a, Scores<T> in) {
+    constexpr int V = Pack<T>::V, STEP = WIDE_THREADS * WIDE_PACKS;
+    __shared__ __align__(16) TopList l;
+    __shared__ Entry best[SCORES_MAX_TOP];
+    __shared__ float parts[WIDE_WARPS][2], whole[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long n = blockIdx.x / C;
+    const int per = (a.k + C - 1) / C, lo = min(a.k, rank * per), hi = min(a.k, lo + per);
+    const Part<T> part(in.at(n, 0), lo, hi);
+    const uint4 *body = part.body();
+    uint4 w[WIDE_PACKS], ahead[WIDE_PACKS];
+    auto fetch = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u)
+            if (from + u * WIDE_THREADS + tid < part.packs) ahead[u] = __ldg(body + from + u * WIDE_THREADS + tid);
+    };
+    fetch(0);
+    if (tid == 0) { l.count = 0; l.border = LOWEST_ENTRY; }
+    __syncthreads();
+    Entry border = LOWEST_ENTRY;
+    float border_score = -FLT_MAX;
+    Running<false> run;
+    int last = 0;   // where this thread's last entry went
+    auto push = [&](Entry e) {
+        last = atomicAdd(&l.count, 1);
+        if (last < WIDE_ROOM) l.e[last] = e;
+        return last < WIDE_ROOM;
+    };
+    if (tid < part.head + part.tail) {   // cells of no pack, 2 V - 2 at most
+        const int k = part.single(tid);
+        const float x = score_f32(part.p[k]);
+        run.raise(x, a.c);
+        run.add(x, row_top(run.m), a.c);
+        const Entry e = entry_of(x, lo + k);
+        if (e >= LOWEST_ENTRY) push(e);
+    }
+    __syncthreads();
+    for (int from = 0; from < part.packs; from += STEP) {
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
+        fetch(from + STEP);
+        auto has = [&](int u) { return from + u * WIDE_THREADS + tid < part.packs; };
+        auto each = [&](int u, auto &&f) {   // f(bit of the cell, score, class)
+            Pack<T> p;
+            p.bits = w[u];
+            float v[V];
+            p.unpack(v);
+            const int k = lo + part.head + (from + u * WIDE_THREADS + tid) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) f(u * V + i, v[i], k + i);
+        };
+        auto most = [&] {
+            Entry e = 0;
+#pragma unroll
+            for (int u = 0; u < WIDE_PACKS; ++u)
+                if (has(u)) each(u, [&](int, float x, int k) { e = max(e, entry_of(x, k)); });
+            return e;
+        };
+        if (from == 0 && part.packs * V > WIDE_ROOM / 2) {
+            find_border(l, most(), a.top);
+            border = l.border;
+            if (border > LOWEST_ENTRY) border_score = key_score((unsigned)(border >> 32));
+        }
+        unsigned dropped = 0;
+        last = 0;
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u) {
+            if (!has(u)) break;
+            float largest = minus_inf();
+            each(u, [&](int, float x, int) { largest = fmaxf(largest, x); });
+            run.raise(largest, a.c);
+            const float base = row_top(run.m);
+            each(u, [&](int, float x, int) { run.add(x, base, a.c); });
+            if (largest >= border_score)
+                each(u, [&](int bit, float x, int k) {
+                    if (x >= border_score) {
+                        const Entry e = entry_of(x, k);
+                        if (e >= border && !push(e)) dropped |= 1u << bit;
+                    }
+                });
+        }
+        if (__syncthreads_or(last >= WIDE_ROOM * 3 / 4)) {   // all threads see the same: the list is full, or soon will be
+            if (tid == 0) l.count = min(l.count, WIDE_ROOM);
+            find_border(l, most(), a.top);
+            narrow_to(l, a.top, WIDE_LAST);
+            constexpr int WARP_CELLS = 32 * WIDE_PACKS * V;
+            static_assert(WIDE_LAST + WARP_CELLS <= WIDE_ROOM, "");
+            for (int turn = 0; turn < WIDE_WARPS; ++turn) {
+                const bool full = l.count > WIDE_ROOM - WARP_CELLS;
+                __syncthreads();
+                if (full) narrow_to(l, a.top, WIDE_LAST);
+                border = l.border;
+                if (warp == turn && dropped) {
+#pragma unroll
+                    for (int u = 0; u < WIDE_PACKS; ++u)
+                        if (has(u)) each(u, [&](int bit, float x, int k) {
+                            if ((dropped >> bit & 1) && entry_of(x, k) >= border) push(entry_of(x, k));
+                        });
+                }
+                __syncthreads();
+            }
+            border_score = border > LOWEST_ENTRY ? key_score((unsigned)(border >> 32)) : -FLT_MAX;
+        }
+    }
+    __syncthreads();
+    narrow_to(l, a.top, WIDE_LAST);
+    run.join_warp(a.c);
+    if (lane == 0) { parts[warp][0] = run.m; parts[warp][1] = run.s; }
+    const int m = l.count;
+    if (tid < SCORES_MAX_TOP) best[tid] = 0;
+    if (tid == 0 && (m & 1)) l.e[m] = 0;   // (m < WIDE_ROOM; read in twos)
+    __syncthreads();
+    if (tid < m) {
+        const Entry own = l.e[tid];
+        int before = 0;
+        for (int j = 0; j < m; j += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2 *>(&l.e[j]);
+            before += (o.x > own) + (o.y > own);
+        }
+        if (before < a.top) best[before] = own;
+    }
+    if (warp == 0) {
+        Running<false> all;
+        if (lane < WIDE_WARPS) { all.m = parts[lane][0]; all.s = parts[lane][1]; }
+        all.join_warp(a.c);
+        if (lane == 0) { whole[0] = all.m; whole[1] = all.s; }
+    }
+    auto give = [&](int j, Entry e) {
+        a.values[n * a.top + j] = key_score((unsigned)(e >> 32));
+        a.ids[n * a.top + j] = e ? (int)~(unsigned)e : -1;
+    };
+    auto give_lse = [&](const Running<false> &r) {
+        if (a.lse) a.lse[n] = (float)((double)row_top(r.m) * a.inv_t + (r.s == 0.f ? (double)minus_inf() : fine_log(r.s)));
+    };
+    if (C == 1) {
+        __syncthreads();
+        if (tid < a.top) give(tid, best[tid]);
+        if (tid == WIDE_THREADS - 1) {
+            Running<false> r;
+            r.m = whole[0]; r.s = whole[1];
+            give_lse(r);
+        }
+        return;
+    }
+    cluster.sync();
+    if (rank == 0) {
+        // the parts' lists, each in order: an entry's place is its own plus that among the others
+        for (int i = tid; i < C * a.top; i += WIDE_THREADS) l.e[i] = *cluster.map_shared_rank(&best[i % a.top], i / a.top);
+        __syncthreads();
+        int found = 0;
+        for (int i0 = 0; i0 < C * a.top; i0 += WIDE_THREADS) {
+            const int i = i0 + tid;
+            const Entry own = i < C * a.top ? l.e[i] : 0;
+            if (own) {
+                int before = i % a.top;
+                for (int c = 0; c < C; ++c) {
+                    if (c == i / a.top) continue;
+                    int x = 0, y = a.top;   // entries [0, x) are larger, [y, top) are not
+                    while (x < y) {
+                        const int mid = (x + y) / 2;
+                        if (l.e[c * a.top + mid] > own) x = mid + 1; else y = mid;
+                    }
+                    before += x;
+                }
+                if (before < a.top) give(before, own);
+            }
+            found += __syncthreads_count(own != 0);
+        }
+        if (tid >= found && tid < a.top) give(tid, 0);
+        if (tid == 0) {
+            Running<false> r;
+            for (int c = 0; c < C; ++c) {
+                const float *o = cluster.map_shared_rank(whole, c);
+                r.join(o[0], o[1], 0.f, a.c);
+            }
+            give_lse(r);
+        }
+    }
+    cluster.sync();   // (the others' shared memory is read until here)
 }
 
 // A block per row: the largest of the keys below the last one chosen, again and again.
@@ -502,6 +770,194 @@ __global__ void __launch_bounds__(TILE_THREADS) k_distill_tile(DistillArgs a, Sc
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
+// A long row, taken as in k_top_wide.  The first pass sums up the classes that the teacher does not list, which a bit map marks; the second
+// finds the row in the L2 cache (the launch sees to it that the rows at work fit there) and writes what unlisted classes get; the
+// few cells of listed classes and of the label are written over it.
+template <typename T, bool TWO>
+__global__ void __launch_bounds__(WIDE_THREADS, 2) k_distill_wide(DistillArgs a, Scores<T> in) {
+    constexpr int V = Pack<T>::V;
+    extern __shared__ unsigned bits[];
+    __shared__ int list_id[SCORES_MAX_TOP];
+    __shared__ float list_q[SCORES_MAX_TOP];
+    __shared__ TeacherSide teacher;
+    __shared__ DistillRow factors;
+    __shared__ float parts[WIDE_WARPS][3], whole[3];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long n = blockIdx.x / C;
+    const int per = (a.k + C - 1) / C, lo = min(a.k, rank * per), hi = min(a.k, lo + per);
+    const Part<T> part(in.at(n, 0), lo, hi);
+    const uint4 *body = part.body();
+    uint4 ahead[WIDE_PACKS];
+    auto fetch = [&](int from) {
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u)
+            if (from + u * WIDE_THREADS + tid < part.packs) ahead[u] = __ldg(body + from + u * WIDE_THREADS + tid);
+    };
+    fetch(0);
+    for (int i = tid; i < (per + 31) / 32 + 1; i += WIDE_THREADS) bits[i] = 0;   // (a word more: read in twos)
+    __syncthreads();
+    if (warp == 0) {
+        const TeacherSide t = read_teacher(a, n, list_id, list_q);
+        if (lane == 0) teacher = t;
+        for (int e = lane; e < a.top; e += 32) {
+            const int k = list_id[e] - lo;
+            if (list_id[e] >= lo && k < hi - lo) atomicOr(&bits[k >> 5], 1u << (k & 31));
+        }
+    }
+    __syncthreads();
+    auto listed = [&](int k) { return bits[k >> 5] >> (k & 31) & 1; };   // k: cell of the part
+    Running<TWO> run;
+    if (tid < part.head + part.tail) {
+        const int k = part.single(tid);
+        if (!listed(k)) {
+            const float x = score_f32(part.p[k]);
+            run.raise(x, a.c);
+            run.add(x, row_top(run.m), a.c);
+        }
+    }
+    for (int from = 0; from < part.packs; from += WIDE_THREADS * WIDE_PACKS) {
+        uint4 w[WIDE_PACKS];
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
+        fetch(from + WIDE_THREADS * WIDE_PACKS);
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u) {
+            const int at = from + u * WIDE_THREADS + tid;
+            if (at >= part.packs) break;
+            Pack<T> p;
+            p.bits = w[u];
+            float v[V];
+            p.unpack(v);
+            const int k = part.head + at * V;
+            const unsigned mark = __funnelshift_r(bits[k >> 5], bits[(k >> 5) + 1], k & 31) & ((1u << V) - 1);
+            if (mark) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (mark >> i & 1) v[i] = minus_inf();
+            }
+            float largest = v[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) largest = fmaxf(largest, v[i]);
+            run.raise(largest, a.c);
+            const float base = row_top(run.m);
+#pragma unroll
+            for (int i = 0; i < V; ++i) run.add(v[i], base, a.c);
+        }
+    }
+    run.join_warp(a.c);
+    if (lane == 0) { parts[warp][0] = run.m; parts[warp][1] = run.s; parts[warp][2] = run.s1; }
+    __syncthreads();
+    if (warp == 0) {
+        Running<TWO> all;
+        if (lane < WIDE_WARPS) { all.m = parts[lane][0]; all.s = parts[lane][1]; all.s1 = parts[lane][2]; }
+        all.join_warp(a.c);
+        if (C > 1) {
+            if (lane == 0) { whole[0] = all.m; whole[1] = all.s; whole[2] = all.s1; }
+        }
+        run = all;
+    }
+    if (C > 1) {
+        cluster.sync();
+        if (warp == 0) {
+            run = Running<TWO>();
+            for (int c = 0; c < C; ++c) {
+                const float *o = cluster.map_shared_rank(whole, c);
+                run.join(o[0], o[1], o[2], a.c);
+            }
+        }
+    }
+    const int label = row_label(a, n);
+    if (warp == 0) {
+        const TeacherSide t = teacher;
+        const float w = a.weights ? a.weights[n] : 1.f;
+        StudentRow st;
+        st.base = row_top(run.m); st.rest = run.s; st.rest1 = TWO ? run.s1 : run.s;
+        float top = run.m;
+        for (int e = lane; e < a.top; e += 32)
+            if (list_id[e] >= 0) top = fmaxf(top, in(n, list_id[e]));
+        st.top = row_top(warp_max(top));
+        float s = 0, s1 = 0;
+        double of_listed = 0, mass = 0;
+        for (int e = lane; e < a.top; e += 32)
+            if (list_id[e] >= 0) {
+                const float z = in(n, list_id[e]), d = __fsub_rn(z, st.top), q = list_q[e];
+                s += exp2_fast(d * a.c);
+                if (TWO) s1 += exp2_fast(d * LOG2E);
+                if (q != 0.f) of_listed += (double)q * (((double)z - (double)st.top) * a.inv_t);
+                mass += q;
+            }
+        const float low = __fsub_rn(st.base, st.top);
+        st.sum = st.rest * exp2_fast(low * a.c) + warp_sum(s);
+        st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + warp_sum(s1) : st.sum;
+        of_listed = warp_sum(of_listed);
+        mass = warp_sum(mass);
+        if (lane == 0) {
+            factors = distill_row(a, t, st, w, label);
+            if (a.loss && rank == 0) a.loss[n] = distill_loss(a, t, st, w, label, of_listed, mass, label >= 0 ? in(n, label) : 0.f);
+        }
+    }
+    if (a.gives != GIVES_LOSS) {
+        __syncthreads();
+        DistillRow d = factors;
+        T *out = static_cast<T *>(a.out.data) + n * a.out.row + lo;             // a.out.cls is 1
+        float2 *pairs = static_cast<float2 *>(a.out.data) + n * a.out.row + lo;
+        auto put = [&](int k, float2 gh) {
+            if (a.gives == GIVES_PAIRS) pairs[k] = gh;
+            else out[k] = score_from<T>(gh.x);
+        };
+        d.label = -1;
+        if (tid < part.head + part.tail) {
+            const int k = part.single(tid);
+            put(k, other_gh<TWO>(d, k, score_f32(part.p[k])));
+        }
+        const bool aligned = reinterpret_cast<uintptr_t>(out + part.head) % 16 == 0;
+        fetch(0);
+        for (int from = 0; from < part.packs; from += WIDE_THREADS * WIDE_PACKS) {
+            uint4 w[WIDE_PACKS];
+#pragma unroll
+            for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
+            fetch(from + WIDE_THREADS * WIDE_PACKS);
+#pragma unroll
+            for (int u = 0; u < WIDE_PACKS; ++u) {
+                const int at = from + u * WIDE_THREADS + tid;
+                if (at >= part.packs) break;
+                Pack<T> p;
+                p.bits = w[u];
+                float v[V];
+                p.unpack(v);
+                const int k = part.head + at * V;
+                if (a.gives == GIVES_PAIRS) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) pairs[k + i] = other_gh<TWO>(d, k + i, v[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        const float x = __fsub_rn(v[i], d.base), e = exp2_fast(x * d.c);
+                        v[i] = e * d.to_g;
+                        if (d.hard != 0.f) v[i] += d.hard * (TWO ? exp2_fast(x * LOG2E) * d.to_p1 : e * d.to_p);
+                    }
+                    if (aligned) {
+                        p.pack(v);
+                        __stcs(reinterpret_cast<uint4 *>(out + k), p.bits);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < V; ++i) out[k + i] = score_from<T>(v[i]);
+                    }
+                }
+            }
+        }
+        __syncthreads();   // what follows is written over it
+        d.label = label;
+        for (int e = tid; e < a.top; e += WIDE_THREADS) {
+            const int k = list_id[e] - lo;
+            if (list_id[e] >= lo && k < hi - lo) put(k, listed_gh<TWO>(d, list_id[e], in(n, list_id[e]), list_q[e]));
+        }
+        if (tid == WIDE_THREADS - 1 && label >= lo && label < hi && !listed(label - lo)) put(label - lo, other_gh<TWO>(d, label, in(n, label)));
+    }
+    if (C > 1) cluster.sync();   // (the others' shared memory is read until they are here)
+}
+
 }  // namespace
 
 // ------------------------------------------------------------------ launches
@@ -539,6 +995,28 @@ void scores_adjust(const AdjustArgs &a, cudaStream_t stream) {
     TGBM_CUDA(cudaGetLastError());
 }
 
+// Blocks of a cluster for a long row: one, and more where there are not rows enough for two blocks per SM, or where the rows
+// that are at work at once would not fit into the L2 cache for a second pass (`twice` bytes of a row; 0: there is none).
+// A part is not shorter than what a block takes in one step.
+int blocks_per_row(int n, int k, int size, size_t twice) {
+    constexpr long long SLOTS = 2 * 148;
+    constexpr size_t L2_ROOM = 48u << 20;
+    int c = 1;
+    while (c < WIDE_CLUSTER && k / (2 * c) >= WIDE_THREADS * WIDE_PACKS * 16 / size &&
+           (n * (2ll * c) <= SLOTS || (twice && (size_t)std::min<long long>(n, SLOTS / c) * twice > L2_ROOM))) c *= 2;
+    return c;
+}
+template <typename... P, typename... A>
+void launch_clusters(void (*kernel)(P...), int n, int cluster, size_t smem, cudaStream_t stream, A &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)n * cluster)); cfg.blockDim = dim3(WIDE_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
+    TGBM_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
 void scores_top(const TopArgs &given, cudaStream_t stream) {
     if (given.n == 0) return;
     TopArgs a = given;
@@ -574,6 +1052,10 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
             by_class ? groups(std::true_type{}) : groups(std::false_type{});
             return;
         }
+        if (a.in.cls == 1) {
+            launch_clusters(k_top_wide<T>, a.n, blocks_per_row(a.n, a.k, (int)sizeof(T), 0), 0, stream, a, scores_of<T>(a.in));
+            return;
+        }
         k_top_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, scores_of<T>(a.in));
     });
     TGBM_CUDA(cudaGetLastError());
@@ -605,6 +1087,14 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
             };
             if (by_class) two ? go(k_distill_tile<T, true, true>) : go(k_distill_tile<T, true, false>);
             else two ? go(k_distill_tile<T, false, true>) : go(k_distill_tile<T, false, false>);
+            return;
+        }
+        if (a.in.cls == 1 && (a.gives == GIVES_LOSS || a.out.cls == 1) && !a.maxbits) {
+            const int c = blocks_per_row(a.n, a.k, (int)sizeof(T), a.gives == GIVES_LOSS ? 0 : a.k * sizeof(T));
+            const size_t smem = sizeof(unsigned) * (size_t)(((a.k + c - 1) / c + 31) / 32 + 1);
+            auto kern = two ? k_distill_wide<T, true> : k_distill_wide<T, false>;
+            if (smem > 40 * 1024) allow_shared(kern, SCORES_MAX_CLASSES / 8 + 4);
+            launch_clusters(kern, a.n, c, smem, stream, a, scores_of<T>(a.in));
             return;
         }
         auto kern = two ? k_distill_any<T, true> : k_distill_any<T, false>;

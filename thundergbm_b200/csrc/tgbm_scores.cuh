@@ -3,6 +3,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "tgbm_device.cuh"
 #include "tgbm_scores.h"
 
@@ -435,5 +437,90 @@ __device__ __forceinline__ DistillRow warp_student(const DistillArgs &a, const T
     __syncwarp();
     return distill_row(a, t, st, w, label);
 }
+
+// ---- a long row in global memory, a block or a cluster of blocks -----------------------------
+// 16 bytes of scores
+template <typename T> struct Pack {
+    static constexpr int V = 16 / (int)sizeof(T);
+    uint4 bits;
+    __device__ __forceinline__ void unpack(float (&v)[V]) const {
+        const unsigned w[4] = {bits.x, bits.y, bits.z, bits.w};
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+                v[2 * i] = f.x; v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    __device__ __forceinline__ void pack(const float (&v)[V]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const unsigned *>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<const unsigned *>(&h);
+            }
+        }
+        bits = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// The part [lo, hi) of a row whose cells lie side by side: single cells up to the first 16-byte boundary, packs, single cells.
+template <typename T> struct Part {
+    const T *p;
+    int head, packs, tail;   // cells [0, head), head + V * packs, the rest
+    __device__ __forceinline__ Part(const T *row, int lo, int hi) : p(row + lo) {
+        constexpr int V = Pack<T>::V;
+        const int n = hi - lo;
+        head = min(n, (int)((16 - reinterpret_cast<uintptr_t>(p) % 16) % 16 / sizeof(T)));
+        packs = (n - head) / V;
+        tail = n - head - packs * V;
+    }
+    __device__ __forceinline__ const uint4 *body() const { return reinterpret_cast<const uint4 *>(p + head); }
+    // cell of the i-th single one
+    __device__ __forceinline__ int single(int i) const { return i < head ? i : i + Pack<T>::V * packs; }
+};
+
+// running sum of exponentials relative to the largest score so far
+template <bool TWO> struct Running {
+    float m, s, s1;
+    __device__ __forceinline__ Running() : m(minus_inf()), s(0.f), s1(0.f) {}
+    __device__ __forceinline__ void raise(float to, float c) {
+        if (to > m) {
+            const float d = __fsub_rn(m, to);
+            s *= exp2_fast(d * c);
+            if (TWO) s1 *= exp2_fast(d * LOG2E);
+            m = to;
+        }
+    }
+    __device__ __forceinline__ void add(float x, float base, float c) {   // base = row_top(m)
+        const float d = __fsub_rn(x, base);
+        s += exp2_fast(d * c);
+        if (TWO) s1 += exp2_fast(d * LOG2E);
+    }
+    __device__ __forceinline__ void join(float om, float os, float os1, float c) {   // another one's
+        const float to = fmaxf(m, om);
+        const float a = m == to ? 0.f : __fsub_rn(m, to), b = om == to ? 0.f : __fsub_rn(om, to);
+        s = s * exp2_fast(a * c) + os * exp2_fast(b * c);
+        if (TWO) s1 = s1 * exp2_fast(a * LOG2E) + os1 * exp2_fast(b * LOG2E);
+        m = to;
+    }
+    __device__ __forceinline__ void join_warp(float c) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+            join(__shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), TWO ? __shfl_xor_sync(0xffffffffu, s1, o) : 0.f, c);
+    }
+};
 
 }  // namespace tgbm
