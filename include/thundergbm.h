@@ -122,6 +122,13 @@ TgbmBooster *tgbm_booster_create(int n_rows, const float *val, const int *row_pt
                                  const int *group, int num_group, const TgbmParam *param, TgbmComm *comm);
 /* Booster::boost x n_rounds; queues the work on the booster's stream and returns */
 int tgbm_booster_boost(TgbmBooster *b, int n_rounds);
+/* Objectives multi:softmax and multi:softprob, before the first round: trees are grown on the pairs of tgbm_scores_distill (below) instead of
+ * the hard labels' alone -- per row of this rank `top` classes and scores of a teacher, its log-sum-exp at `temperature` (or NULL), the
+ * labels' part weighing 1 - alpha.  Host arrays n_rows x top, n_rows x top, n_rows; copied.  Classes are positions among the labels
+ * (tgbm_booster_get_labels).  With a communicator every rank calls it.  Metrics stay those of the labels; model files do not change. */
+int tgbm_booster_set_teacher(TgbmBooster *b, int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
+/* that loss on the current scores: its mean over this rank's rows */
+int tgbm_booster_teacher_loss(TgbmBooster *b, double *out);
 int tgbm_booster_sync(TgbmBooster *b);
 /* boost + sync, bracketed by CUDA events on the booster's stream: device time of the n_rounds in ms */
 int tgbm_booster_boost_timed(TgbmBooster *b, int n_rounds, float *elapsed_ms);
@@ -256,6 +263,24 @@ int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_score
                         const int *d_ids, long long ids_stride, int logits_type, const void *d_logits, long long logits_stride,
                         const float *d_lse, const int *d_labels, const float *d_weights, float temperature, float alpha, float *d_loss,
                         int gives, void *d_grad, long long grad_row_stride, long long grad_class_stride, void *cuda_stream);
+
+/* A model's raw scores (as sparse_predict_scikit and dense_predict_scikit compute them, before the objective's transformation) through
+ * tgbm_scores_adjust and tgbm_scores_top, from and to HOST arrays: the `top` best classes of every row under the caller's rules.  For models of
+ * several classes (trees_per_iter >= 2); classes are positions among the model's labels.  rules NULL: none.  values and ids: row_size x
+ * top; lse (or NULL): row_size. */
+typedef struct {
+    const float *bias;            /* one per class, or NULL */
+    const unsigned *allowed;      /* n_masks x (classes + 31) / 32 words, or NULL */
+    int n_masks;
+    const int *allowed_row;       /* mask of every row, or NULL: row n has mask n */
+    const long long *history_ptr; /* row_size + 1, or NULL */
+    const int *history;
+    float repetition, frequency, presence; /* 1, 0, 0: no penalty */
+} TgbmTopRules;
+int tgbm_predict_top(int row_size, float *val, int *row_ptr, int *col_ptr, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                     const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse);
+int tgbm_predict_top_dense(int row_size, int n_cols, void *x, int is_f64, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                           const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse);
 
 #ifdef __cplusplus
 }

@@ -31,6 +31,11 @@ class TgbmProfile(C.Structure):
                                             'kernel_launches', 'hist_rows')]
 
 
+class TgbmTopRules(C.Structure):
+    _fields_ = [('bias', C.c_void_p), ('allowed', C.c_void_p), ('n_masks', C.c_int), ('allowed_row', C.c_void_p), ('history_ptr', C.c_void_p),
+                ('history', C.c_void_p), ('repetition', C.c_float), ('frequency', C.c_float), ('presence', C.c_float)]
+
+
 def load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f'{LIB_PATH} not found: build it first (python -m thundergbm_b200.build)')
@@ -62,6 +67,11 @@ def load() -> C.CDLL:
     lib.tgbm_predict_raw_timed.argtypes = [C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float, vp, vp]
     lib.tgbm_metric_score.argtypes = [C.c_char_p, C.c_int, C.c_int, vp, vp, vp, C.c_int, fp]
     lib.tgbm_metric_score_noalloc.argtypes = [C.c_char_p, C.c_int, C.c_int, vp, vp, vp, vp]
+    lib.tgbm_booster_set_teacher.argtypes = [vp, C.c_int, vp, vp, vp, C.c_float, C.c_float]
+    lib.tgbm_booster_teacher_loss.argtypes = [vp, P(C.c_double)]
+    rules = [vp, C.c_int, C.c_int, C.c_float, P(TgbmTopRules), C.c_int, C.c_float, vp, vp, vp]   # from the model on
+    lib.tgbm_predict_top.argtypes = [C.c_int, vp, vp, vp] + rules
+    lib.tgbm_predict_top_dense.argtypes = [C.c_int, C.c_int, vp, C.c_int] + rules
     ll, i32, f32 = C.c_longlong, C.c_int, C.c_float
     lib.tgbm_scores_adjust.argtypes = [i32, i32, i32, vp, ll, ll, vp, ll, ll, vp, vp, i32, ll, vp, vp, vp, ll, f32, f32, f32, vp]
     lib.tgbm_scores_top.argtypes = [i32, i32, i32, vp, ll, ll, i32, f32, vp, vp, vp, vp]

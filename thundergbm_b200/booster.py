@@ -78,6 +78,25 @@ class Booster:
             raise RuntimeError(self._lib.tgbm_last_error().decode())
         self._keep = None  # the library copied everything it needs
 
+    def set_teacher(self, ids, logits, lse=None, temperature: float = 1.0, alpha: float = 1.0):
+        """Grow trees towards a teacher's largest scores (multi:softmax, multi:softprob; before the first round): `ids` and `logits`
+        rows x up to 128, classes as positions in labels() (-1: none); `lse` the teacher's log-sum-exp at this temperature, with
+        which the mass of the classes that are not listed counts as one class; the loss on the labels weighs 1 - alpha."""
+        n = self.info.n_rows
+        ids, logits = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logits, np.float32)
+        if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[0] != n:
+            raise ValueError('ids and logits: rows x kept classes, one score for every class')
+        lse = None if lse is None else np.ascontiguousarray(lse, np.float32)
+        if lse is not None and lse.shape != (n,):
+            raise ValueError('lse: one per row')
+        _lib.check(self._lib.tgbm_booster_set_teacher(self.handle, ids.shape[1], _ptr(ids), _ptr(logits), _ptr(lse), temperature, alpha))
+
+    def teacher_loss(self) -> float:
+        """Mean over the rows of the loss that set_teacher() describes, on the current scores."""
+        o = C.c_double(0)
+        _lib.check(self._lib.tgbm_booster_teacher_loss(self.handle, C.byref(o)))
+        return o.value
+
     def boost(self, n_rounds: int):
         _lib.check(self._lib.tgbm_booster_boost(self.handle, n_rounds))
 

@@ -22,6 +22,7 @@
 #include "tgbm_small.cuh"
 #include "tgbm_exact.cuh"
 #include "tgbm_rank.cuh"
+#include "tgbm_scores.h"
 
 namespace tgbm {
 
@@ -62,6 +63,14 @@ struct BoosterImpl {
     int n_chunks = 0;
     DevBuf<float> cut_val, y, ypred, metric;
     DevBuf<int> cut_ptr, cut_fid;
+    // a teacher's largest scores of every row (top = 0: none)
+    struct Teacher {
+        int top = 0;
+        float temperature = 1, alpha = 1;
+        DevBuf<int> ids;
+        DevBuf<float> logits, lse;
+    } teacher;
+    DistillArgs distill_args() const;
     DevBuf<float2> gh;
     DevBuf<int2> ghq;
     DevBuf<unsigned> maxbits;
@@ -1138,6 +1147,14 @@ void BoosterImpl::gradient(int round) {
             case REG_LINEAR: case REG_LOGISTIC: case BINARY_LOGISTIC:
                 launch_after(k_grad_pointwise, gb, tb, 0, stream, y.p, ypred.p, N, logistic, gh.p, maxbits.p); break;
             case MULTI_SOFTMAX: case MULTI_SOFTPROB:
+                if (teacher.top) {
+                    DistillArgs a = distill_args();
+                    a.gives = GIVES_PAIRS;
+                    a.out.data = gh.p; a.out.row = 1; a.out.cls = N;
+                    a.maxbits = maxbits.p;
+                    scores_distill(a, stream);
+                    break;
+                }
                 launch_after(k_grad_softmax, gb, tb, 0, stream, y.p, ypred.p, N, K, gh.p, maxbits.p); break;
             case RANK_PAIRWISE: case RANK_NDCG:
                 rank.gradient(rstate.p, p.rank_seed, ypred.p, gh.p, maxbits.p, stream); break;
@@ -1170,6 +1187,62 @@ void BoosterImpl::gradient(int round) {
     else quantize(k_quantize<false>, p.quant_bits);
     ++launches;
     if (comm && comm->active()) comm->allreduce(root_sum.p, 2 * (size_t)K + (f32 ? 2 : 0), Comm::I64, Comm::SUM, stream);
+}
+
+DistillArgs BoosterImpl::distill_args() const {
+    DistillArgs a;
+    a.n = N; a.k = K; a.top = teacher.top;
+    a.in.data = ypred.p; a.in.row = 1; a.in.cls = N;
+    a.ids = teacher.ids.p; a.ids_stride = teacher.top;
+    a.logits = teacher.logits.p; a.logits_stride = teacher.top;
+    a.lse = teacher.lse.p;
+    a.labels_f = y.p;
+    a.temperature = teacher.temperature; a.alpha = teacher.alpha;
+    return a;
+}
+
+void Booster::set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha) {
+    BoosterImpl &m = *impl_;
+    TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "a teacher needs objective multi:softmax or multi:softprob");
+    TGBM_CHECK(m.rounds == 0, "the teacher has to be there before the first round");
+    TGBM_CHECK(top >= 1 && top <= SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(SCORES_MAX_TOP) + "]");
+    TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
+    TGBM_CHECK(alpha >= 0.f && alpha <= 1.f, "alpha outside [0, 1]");
+    TGBM_CHECK((ids && logits) || m.N == 0, "teacher: null pointer");
+    TGBM_CUDA(cudaStreamSynchronize(m.stream));
+    BoosterImpl::Teacher &t = m.teacher;
+    const size_t cells = (size_t)m.N * top;
+    t.top = 0;   // (none, should an allocation fail)
+    t.ids.alloc(cells); t.logits.alloc(cells); t.lse.alloc(lse ? m.N : 0);
+    if (cells) {
+        upload_h2d(t.ids.p, ids, t.ids.bytes(), m.stream, upload_threads());
+        upload_h2d(t.logits.p, logits, t.logits.bytes(), m.stream, upload_threads());
+        if (lse) upload_h2d(t.lse.p, lse, t.lse.bytes(), m.stream, upload_threads());
+        TGBM_CUDA(cudaStreamSynchronize(m.stream));
+    }
+    t.top = top; t.temperature = temperature; t.alpha = alpha;
+}
+
+double Booster::teacher_loss() {
+    BoosterImpl &m = *impl_;
+    TGBM_CHECK(m.teacher.top, "the booster has no teacher");
+    sync();
+    if (m.N == 0) return 0;
+    DevBuf<float> loss;
+    DevBuf<double> partial, sum;
+    loss.alloc(m.N);
+    const int blocks = std::max(1, std::min(ceil_div(m.N, 256), 1024));
+    partial.alloc(blocks); sum.alloc(1);
+    DistillArgs a = m.distill_args();
+    a.loss = loss.p;
+    scores_distill(a, m.stream);
+    k_partial_sums<<<blocks, 256, 0, m.stream>>>(loss.p, m.N, partial.p);
+    k_metric_sum<<<1, 32, 0, m.stream>>>(partial.p, blocks, sum.p);
+    TGBM_CUDA(cudaGetLastError());
+    double total = 0;
+    TGBM_CUDA(cudaMemcpyAsync(&total, sum.p, sizeof(total), cudaMemcpyDeviceToHost, m.stream));
+    TGBM_CUDA(cudaStreamSynchronize(m.stream));
+    return total / m.N;
 }
 
 // Base score (include/thundergbm/objective/regression_obj.h:35-53 and :95-114): gradients at y_pred = 0,

@@ -5,6 +5,7 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <functional>
 #include <memory>
 #include <vector>
 
@@ -41,6 +42,11 @@ public:
     // rounds [done, done+n) ; asynchronous on the booster's stream
     void boost(int n_rounds);
     bool sync();   // waits; fp32 mode: builds the rounds again whose gradients did not fit the integer grid (true: there were some)
+
+    // Multi-class objectives, before the first round: gradients against a teacher's largest scores (tgbm_scores.h), mixed with those
+    // on the labels.  Host arrays of this rank's rows, copied: n x top, n x top, n (or null).
+    void set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
+    double teacher_loss();   // that loss on the current scores, the mean over this rank's rows; syncs
 
     int rounds_done() const;
     int trees_per_round() const;
@@ -88,10 +94,12 @@ struct ModelRef {
     std::vector<const TreeNode *> trees;   // [round * K + class], n_nodes records each
 };
 class PredictPlan;
+// What happens to the raw scores [K][N] on the device instead of predict_transform and the copy to `out`; has to wait for `stream`.
+typedef std::function<void(float *scores, int n, int k, cudaStream_t stream)> ScoreStep;
 std::shared_ptr<PredictPlan> make_predict_plan(const ModelRef &m);
 bool predict_plan_fits(const PredictPlan &plan, int n_rounds, int K);   // ... and is on the current device
 void predict(const DataSet &ds, PredictPlan &plan, float learning_rate, float base_score, int objective, const std::vector<float> &label,
-             float *out, float *kernel_ms = nullptr);
+             float *out, float *kernel_ms = nullptr, const ScoreStep *step = nullptr);
 void predict_release_workspaces() noexcept;
 // ObjectiveFunction::predict_transform on raw scores (in place; may shrink `y`)
 void predict_transform(int objective, int num_class, const std::vector<float> &label, int n_rows, std::vector<float> &y);

@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <chrono>
 #include <climits>
+#include <cmath>
 #include <cstring>
 #include <future>
 #include <map>
@@ -13,6 +14,7 @@
 #include "../../include/thundergbm.h"
 #include "tgbm_booster.h"
 #include "tgbm_device.cuh"
+#include "tgbm_scores.h"
 
 // the opaque C handle is the C++ tree container
 struct Tree : tgbm::Tree {
@@ -305,6 +307,73 @@ void train_scikit(Load &&load, int depth, int n_trees, int n_device, float min_c
     });
 }
 
+// adjust and top on the raw scores of a prediction, from and to host arrays
+template <typename View>
+int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, float learning_rate, const TgbmTopRules *rules, int top, float temperature,
+                float *values, int *ids, float *lse) {
+    return guard([&] {
+        tgbm::DataSet ds;
+        view(ds);
+        TGBM_CHECK(model && *model, "model is null!");
+        TGBM_CHECK(trees_per_iter >= 2, "the largest scores of a row need a model of several classes (multi:softmax, multi:softprob)");
+        TGBM_CHECK(top >= 1 && top <= tgbm::SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(tgbm::SCORES_MAX_TOP) + "]");
+        TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
+        const int n = ds.n_rows, k = trees_per_iter, words = (k + 31) / 32;
+        if (n == 0) return;
+        TGBM_CHECK(values && ids, "values or ids: null pointer");
+        static const TgbmTopRules none{nullptr, nullptr, 0, nullptr, nullptr, nullptr, 1.f, 0.f, 0.f};
+        const TgbmTopRules &r = rules ? *rules : none;
+        TGBM_CHECK(r.repetition > 0.f && std::isfinite(r.repetition) && std::isfinite(r.frequency) && std::isfinite(r.presence),
+                   "penalties have to be finite, the one for repetition positive");
+        TGBM_CHECK(!r.allowed || r.n_masks >= (r.allowed_row ? 1 : n), "fewer masks than rows, and none named for each row");
+        long long given = 0;
+        if (r.history_ptr) {
+            TGBM_CHECK(r.history_ptr[0] >= 0, "history: the first row begins before the list");
+            for (int i = 0; i < n; ++i) TGBM_CHECK(r.history_ptr[i] <= r.history_ptr[i + 1], "history: rows have to follow one another");
+            given = r.history_ptr[n];
+            TGBM_CHECK(r.history || given == 0, "history: null pointer");
+        }
+        const tgbm::ScoreStep step = [&](float *scores, int rows, int classes, cudaStream_t st) {
+            const int threads = tgbm::upload_threads();
+            tgbm::DevBuf<float> d_bias, d_values, d_lse;
+            tgbm::DevBuf<unsigned> d_allowed;
+            tgbm::DevBuf<int> d_row, d_history, d_ids;
+            tgbm::DevBuf<long long> d_ptr;
+            auto up = [&](auto &buf, const auto *src, size_t count) {
+                buf.alloc(count);
+                tgbm::upload_h2d(buf.p, src, buf.bytes(), st, threads);
+            };
+            tgbm::AdjustArgs a;
+            a.n = rows; a.k = classes;
+            a.in.data = scores; a.in.row = 1; a.in.cls = rows;
+            a.out = a.in;
+            if (r.bias) { up(d_bias, r.bias, classes); a.bias = d_bias.p; }
+            if (r.allowed) {
+                up(d_allowed, r.allowed, (size_t)r.n_masks * words);
+                a.allowed = d_allowed.p; a.n_masks = r.n_masks; a.mask_stride = words;
+                if (r.allowed_row) { up(d_row, r.allowed_row, rows); a.allowed_row = d_row.p; }
+            }
+            if (given) {
+                up(d_ptr, r.history_ptr, (size_t)rows + 1);
+                up(d_history, r.history, (size_t)given);
+                a.history_ptr = d_ptr.p; a.history = d_history.p; a.n_history = given;
+                a.repetition = r.repetition; a.frequency = r.frequency; a.presence = r.presence;
+            }
+            if (a.bias || a.allowed || given) tgbm::scores_adjust(a, st);
+            tgbm::TopArgs t;
+            t.n = rows; t.k = classes; t.top = top; t.in = a.in; t.temperature = temperature;
+            d_values.alloc((size_t)rows * top); d_ids.alloc((size_t)rows * top);
+            t.values = d_values.p; t.ids = d_ids.p;
+            if (lse) { d_lse.alloc(rows); t.lse = d_lse.p; }
+            tgbm::scores_top(t, st);
+            tgbm::download_d2h(values, d_values.p, d_values.bytes(), st, threads);
+            tgbm::download_d2h(ids, d_ids.p, d_ids.bytes(), st, threads);
+            if (lse) tgbm::download_d2h(lse, d_lse.p, d_lse.bytes(), st, threads);
+        };
+        tgbm::predict(ds, *plan_of(*model, n_trees, trees_per_iter), learning_rate, 0.f, tgbm::OBJ_UNKNOWN, {}, nullptr, nullptr, &step);
+    });
+}
+
 template <typename View>
 void predict_scikit(View &&view, float *y_pred, ::Tree **model, int n_trees, int trees_per_iter, char *objective, int num_class,
                     float learning_rate, float *group_label, int verbose) {
@@ -387,6 +456,17 @@ void dense_predict_scikit(int row_size, int n_cols, void *x, int is_f64, float *
                           float *group_label, int verbose) {
     predict_scikit([&](tgbm::DataSet &ds) { ds.view_dense(row_size, n_cols, x, is_f64 != 0); }, y_pred, model, n_trees, trees_per_iter,
                    objective, num_class, learning_rate, group_label, verbose);
+}
+
+int tgbm_predict_top(int row_size, float *val, int *row_ptr, int *col_ptr, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                     const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse) {
+    return predict_top([&](tgbm::DataSet &ds) { ds.view_sparse(row_size, val, row_ptr, col_ptr); }, model, n_trees, trees_per_iter, learning_rate,
+                       rules, top, temperature, values, ids, lse);
+}
+int tgbm_predict_top_dense(int row_size, int n_cols, void *x, int is_f64, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                           const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse) {
+    return predict_top([&](tgbm::DataSet &ds) { ds.view_dense(row_size, n_cols, x, is_f64 != 0); }, model, n_trees, trees_per_iter, learning_rate,
+                       rules, top, temperature, values, ids, lse);
 }
 
 void save(char *model_path, char *objective, float learning_rate, int num_class, int n_trees, int trees_per_iter,
@@ -554,6 +634,18 @@ TgbmBooster *tgbm_booster_create(int n_rows, const float *val, const int *row_pt
     return h;
 }
 
+int tgbm_booster_set_teacher(TgbmBooster *b, int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha) {
+    return guard([&] {
+        TGBM_CHECK(b != nullptr, "null booster");
+        b->b->set_teacher(top, ids, logits, lse, temperature, alpha);
+    });
+}
+int tgbm_booster_teacher_loss(TgbmBooster *b, double *out) {
+    return guard([&] {
+        TGBM_CHECK(b && out, "null pointer");
+        *out = b->b->teacher_loss();
+    });
+}
 int tgbm_booster_boost(TgbmBooster *b, int n_rounds) { return guard([&] { b->b->boost(n_rounds); }); }
 int tgbm_booster_sync(TgbmBooster *b) { return guard([&] { b->b->sync(); }); }
 int tgbm_booster_set_profile(TgbmBooster *b, int on) { return guard([&] { b->b->set_profile(on != 0); }); }

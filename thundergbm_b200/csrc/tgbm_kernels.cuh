@@ -934,6 +934,21 @@ static __global__ void k_metric_partial(int objective, const float *__restrict__
         partial[blockIdx.x] = t;
     }
 }
+// sums of floats by blocks of 256 threads, in a fixed order
+static __global__ void k_partial_sums(const float *v, int n, double *partial) {
+    __shared__ double ws[8];
+    double s = 0;
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) s += (double)v[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = 0;
+        for (int w = 0; w < 8; ++w) t += ws[w];
+        partial[blockIdx.x] = t;
+    }
+}
 // one warp: lane l adds partial[l], partial[l+32], ... in that order, then a fixed shuffle tree
 static __global__ void k_metric_sum(const double *__restrict__ partial, int nb, double *__restrict__ out) {
     double t = 0;

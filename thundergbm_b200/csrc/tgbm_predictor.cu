@@ -1057,7 +1057,7 @@ bool predict_plan_fits(const PredictPlan &plan, int n_rounds, int K) {
 constexpr double DIRECT_VISITS = 4e8;
 
 void predict(const DataSet &ds, PredictPlan &plan, float learning_rate, float base_score, int objective, const std::vector<float> &label,
-             float *out, float *kernel_ms) {
+             float *out, float *kernel_ms, const ScoreStep *step) {
     const int N = ds.n_rows, K = plan.K, n_rounds = plan.n_rounds, n_nodes = plan.n_nodes, depth = plan.depth;
     if (N == 0) return;
     if (K > 1) base_score = 0;  // predictor.cu:81-83
@@ -1081,12 +1081,17 @@ void predict(const DataSet &ds, PredictPlan &plan, float learning_rate, float ba
 
     // scores: small ones are written straight into page-locked memory
     DevBuf<float> d_out;
-    float *scores = static_cast<float *>(ws.take(sizeof(float) * (size_t)N * K)), *scores_dev = nullptr;
+    // (not where they are read several times before anything goes back)
+    float *scores = step ? nullptr : static_cast<float *>(ws.take(sizeof(float) * (size_t)N * K)), *scores_dev = nullptr;
     if (scores) scores_dev = static_cast<float *>(ws.device(scores));
     else { d_out.alloc((size_t)N * K); scores_dev = d_out.p; }
     auto finish = [&]() {
         TGBM_CUDA(cudaGetLastError());
         if (kernel_ms) TGBM_CUDA(cudaEventRecord(ev.e1, st));
+        if (step) {
+            (*step)(scores_dev, N, K, st);
+            return;
+        }
         DevBuf<float> d_label;
         if (transforms) {
             const float *labels = nullptr;

@@ -96,7 +96,11 @@ class TGBMModel:
         return (C.c_float * max(len(self._group_label), self.num_class))(*self._group_label)
 
     # -- API ---------------------------------------------------------------------------------------
-    def fit(self, X, y, groups=None):
+    def fit(self, X, y, groups=None, teacher=None):
+        """`teacher` (multi:softmax and multi:softprob, one GPU): the arguments of Booster.set_teacher as a dict -- ids, logits and, if
+        wanted, lse, temperature, alpha; what predict_top() of another model returns is such a teacher's ids, logits and lse."""
+        if teacher is not None:
+            return self._fit_teacher(X, y, teacher)
         self._free()
         dense = self._dense(X)
         if dense is not None:
@@ -134,6 +138,101 @@ class TGBMModel:
         else:
             self._group_label, self._n_labels = None, self._counted(n_labels)
         return self
+
+    def _fit_teacher(self, X, y, teacher):
+        from .booster import Booster
+        from .synth import CsrData
+        if self.objective not in ('multi:softmax', 'multi:softprob'):
+            raise ValueError('a teacher needs objective multi:softmax or multi:softprob')
+        if self.n_gpus != 1:
+            raise ValueError('training from a teacher runs on one GPU')
+        if self.tree_method not in ('auto', 'hist', 'exact'):
+            raise ValueError('unknown tree_method ' + self.tree_method)
+        val, indptr, indices, n = self._csr(X)
+        y = np.ascontiguousarray(y, np.float32)
+        if y.shape[0] != n:
+            raise ValueError('X and y have different numbers of rows')
+        if np.shape(teacher['ids'])[0] != n:
+            raise ValueError('X and the teacher have different numbers of rows')
+        width = int(indices.max(initial=-1)) + 1
+        exact = self.tree_method == 'exact' or (self.tree_method == 'auto' and width > 20000)   # src/thundergbm/trainer.cu:19-23
+        b = Booster(CsrData(n, width, indptr, indices, val, y), depth=self.depth, n_trees=self.n_trees,
+                    min_child_weight=self.min_child_weight, lambda_=self.lambda_tgbm, gamma=self.gamma, max_num_bin=self.max_num_bin,
+                    verbose=self.verbose, column_sampling_rate=self.column_sampling_rate, bagging=int(self.bagging),
+                    learning_rate=self.learning_rate, objective=self.objective, num_class=self.num_class, exact_builder=int(exact))
+        try:
+            b.set_teacher(**teacher)
+            b.boost(self.n_trees)
+            b.sync()
+            model = C.c_void_p(None)
+            _lib.check(self._lib.tgbm_booster_to_model(b.handle, C.byref(model)))
+            info, labels = b.info, b.labels()
+        finally:
+            b.close()
+        self._free()
+        self.model, self.num_class, self.tree_per_iter = model, info.num_class, info.trees_per_round
+        self.group_label = [float(v) for v in labels]
+        return self
+
+    def predict_top(self, X, k=1, bias=None, allowed=None, allowed_row=None, history=None, repetition=1.0, frequency=0.0, presence=0.0,
+                    temperature=1.0):
+        """(classes, scores, lse) of the k best classes of every row, for models of several classes: classes are positions in `group_label`
+        (int32, rows x k; -1 where a row has no more), scores the model's raw ones under the rules given, best first, and
+        scores / temperature - lse the logs of their probabilities.
+
+        bias: one per class (log of the ratio of class priors, say).  allowed: truth values, rows x classes or masks x classes with
+        `allowed_row` naming every row's mask (-1: all classes).  history: per row a list of classes it was given before; one that
+        stands there c > 0 times has its score divided (above 0) or multiplied by `repetition`, less c * frequency + presence."""
+        if self.model is None:
+            raise ValueError('Please train the model first or load model from file!')
+        dense = self._dense(X)
+        if dense is not None:
+            n = X.shape[0]
+        else:
+            val, indptr, indices, n = self._csr(X)
+        classes = self.tree_per_iter
+        rules = _lib.TgbmTopRules(repetition=repetition, frequency=frequency, presence=presence)
+        keep = []
+
+        def field(name, a, dtype, shape, what):
+            a = np.ascontiguousarray(a, dtype)
+            if a.shape != shape:
+                raise ValueError(what)
+            keep.append(a)
+            setattr(rules, name, a.ctypes.data)
+        if bias is not None:
+            field('bias', bias, np.float32, (classes,), 'bias: one per class')
+        if allowed is not None:
+            allowed = np.asarray(allowed)
+            if allowed.ndim != 2 or allowed.shape[1] != classes or (allowed_row is None and allowed.shape[0] != n):
+                raise ValueError('allowed: rows x classes, or masks x classes and allowed_row')
+            masks = allowed.shape[0]
+            bits = np.zeros((masks, (classes + 31) // 32 * 32), bool)
+            bits[:, :classes] = allowed != 0
+            words = np.packbits(bits, axis=1, bitorder='little').view(np.uint32)
+            field('allowed', words, np.uint32, (masks, (classes + 31) // 32), '')
+            rules.n_masks = masks
+            if allowed_row is not None:
+                field('allowed_row', allowed_row, np.int32, (n,), 'allowed_row: one mask per row')
+        elif allowed_row is not None:
+            raise ValueError('allowed_row: there are no masks')
+        if history is not None:
+            if len(history) != n:
+                raise ValueError('history: a list for every row')
+            ptr = np.zeros(n + 1, np.int64)
+            np.cumsum([len(h) for h in history], out=ptr[1:])
+            ids = np.concatenate([np.asarray(h, np.int32).reshape(-1) for h in history]) if n else np.zeros(0, np.int32)
+            field('history_ptr', ptr, np.int64, (n + 1,), '')
+            field('history', ids, np.int32, (int(ptr[-1]),), '')
+        if not 1 <= k <= 128:
+            raise ValueError('k: 1 to 128')
+        values, ids, lse = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
+        rest = (C.byref(self.model), self.n_trees, self.tree_per_iter, self.learning_rate, C.byref(rules), k, temperature, _vp(values), _vp(ids), _vp(lse))
+        if dense is not None:
+            _lib.check(self._lib.tgbm_predict_top_dense(n, X.shape[1], _vp(dense[0]), dense[1], *rest))
+        else:
+            _lib.check(self._lib.tgbm_predict_top(n, _vp(val), _vp(indptr), _vp(indices), *rest))
+        return ids, values, lse
 
     def predict(self, X, groups=None):
         if self.model is None:
