@@ -41,48 +41,217 @@ template <typename F> void by_type(int type, F &&f) {
 // ------------------------------------------------------------------ adjust
 // A block takes a tile of rows x classes.  How often a class stands in the history of its row is counted in shared memory: every
 // entry of the tile's histories that falls into its classes adds one (integers: in any order the same), so a history may be
-// of any length.
+// of any length.  A few instructions per score decide the time, so there are three ways through a tile.
 constexpr int ADJUST_CELLS = 8192;
 
-template <typename T, bool BY_CLASS>
-__global__ void __launch_bounds__(ROW_THREADS) k_adjust(AdjustArgs a, Scores<T> in, Scores<T> out, int tile_rows, int tile_classes) {
-    extern __shared__ int count[];
+// histories of `rows` rows into counts[cell(row, class - k0)]: the rows' entries lie one behind the other, so the block's threads share
+// them evenly, and each finds the row of its entries among the rows' ends
+constexpr int ADJUST_MOST_ROWS = 1024;
+template <int MOST_ROWS, typename C>
+__device__ __forceinline__ void count_histories(const AdjustArgs &a, long long n0, int rows, int k0, int classes, int *count, int cells, C &&cell) {
+    __shared__ long long ends[MOST_ROWS];
+    int4 *zero = reinterpret_cast<int4 *>(count);
+    const long long lo = max(0ll, a.history_ptr[n0]), hi = min(a.n_history, a.history_ptr[n0 + rows]);
+    if (MOST_ROWS > 1)
+        for (int r = threadIdx.x; r < rows; r += ROW_THREADS) ends[r] = a.history_ptr[n0 + r + 1];
+    for (int i = threadIdx.x; i < (cells + 3) / 4; i += ROW_THREADS) zero[i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    constexpr int AHEAD = 4;
+    for (long long h = lo + threadIdx.x; h < hi; h += AHEAD * ROW_THREADS) {
+        int c[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) c[i] = h + i * ROW_THREADS < hi ? a.history[h + i * ROW_THREADS] - k0 : -1;
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (c[i] < 0 || c[i] >= classes) continue;
+            int x = 0, y = MOST_ROWS == 1 ? 0 : rows - 1;   // the first row that ends behind the entry
+            while (x < y) {
+                const int mid = (x + y) / 2;
+                if (ends[mid] > h + i * ROW_THREADS) y = mid; else x = mid + 1;
+            }
+            atomicAdd(&count[cell(x, c[i])], 1);
+        }
+    }
+    __syncthreads();
+}
+// z / r from r's reciprocal, rounded once: the product's error times the reciprocal is put back (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990).  A score that was given before is in almost every warp, so
+// all scores pay for it: a division costs the batch of 50003 x 250 some 10 us more.
+__device__ __forceinline__ float penalised(const AdjustArgs &a, float z, int times) {
+    const float up = __fmul_rn(z, a.repetition), q = __fmul_rn(z, a.inv_repetition);
+    const float error = __fmaf_rn(-q, a.repetition, z);
+    const float down = fabsf(z) >= 1e-30f && fabsf(q) <= FLT_MAX ? __fmaf_rn(error, a.inv_repetition, q) : q;
+    return (z > 0.f ? down : up) - ((float)times * a.frequency + a.presence);
+}
+// the row's mask; null: all classes are allowed
+__device__ __forceinline__ const unsigned *mask_of(const AdjustArgs &a, long long n) {
+    if (!a.allowed) return nullptr;
+    const long long m = a.allowed_row ? (long long)a.allowed_row[n] : n;
+    return m >= 0 && m < a.n_masks ? a.allowed + m * a.mask_stride : nullptr;
+}
+
+// By class: a lane per row, a warp takes neighbouring classes, eight at a time: their scores are read together, and their bits lie in
+// one word of the row's mask.  Class strides are ints here: an address is one instruction.
+// Blocks per SM (4 x 61 registers): 29 us for 50003 x 250 with histories, 40 with 6 blocks and fewer registers.
+constexpr int ADJUST_ROWS = 32, ADJUST_AHEAD = 8, ADJUST_CLASSES = ADJUST_CELLS / ADJUST_ROWS;
+
+template <typename T, bool HISTORY>
+__global__ void __launch_bounds__(ROW_THREADS, 4) k_adjust_class(AdjustArgs a, Scores<T> in, Scores<T> out) {
+    constexpr int A = ADJUST_AHEAD;
+    extern __shared__ __align__(16) int count[];
+    const long long n0 = (long long)blockIdx.x * ADJUST_ROWS;
+    const int k0 = blockIdx.y * ADJUST_CLASSES, classes = min(ADJUST_CLASSES, a.k - k0), rows = (int)min((long long)ADJUST_ROWS, a.n - n0);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, in_cls = (int)in.cls, out_cls = (int)out.cls;
+    const long long n = n0 + min(lane, rows - 1);
+    const int per = (classes + A * ROW_THREADS / 32 - 1) / (A * ROW_THREADS / 32) * A, from = warp * per, to = lane < rows ? min(classes, from + per) : from;
+    const T *src = in.at(n, k0 + from);
+    T *dst = out.at(n, k0 + from);
+    T ahead[A];
+    auto fetch = [&](int left) {
+        if (left >= A) {
+#pragma unroll
+            for (int i = 0; i < A; ++i) ahead[i] = src[(long long)i * in_cls];
+        } else {
+#pragma unroll
+            for (int i = 0; i < A; ++i)
+                if (i < left) ahead[i] = src[(long long)i * in_cls];
+        }
+        src += (long long)A * in_cls;
+    };
+    fetch(to - from);   // on their way while the histories are counted
+    const unsigned *mask = mask_of(a, n);
+    if (HISTORY) count_histories<ADJUST_ROWS>(a, n0, rows, k0, classes, count, classes * ADJUST_ROWS, [](int r, int c) { return c * ADJUST_ROWS + r; });
+    for (int c = from; c < to; c += A) {
+        float z[A];
+        const int k = k0 + c;   // a multiple of 8
+#pragma unroll
+        for (int i = 0; i < A; ++i) z[i] = score_f32(ahead[i]);
+        fetch(to - c - A);
+        const unsigned word = mask ? mask[k >> 5] >> (k & 31) : 0xffffffffu;
+        if (HISTORY) {
+            int times[A];
+#pragma unroll
+            for (int i = 0; i < A; ++i) times[i] = count[min(c + i, classes - 1) * ADJUST_ROWS + lane];
+#pragma unroll
+            for (int i = 0; i < A; ++i)
+                if (times[i]) z[i] = penalised(a, z[i], times[i]);
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < A; ++i) z[i] += a.bias[min(k + i, a.k - 1)];
+        }
+#pragma unroll
+        for (int i = 0; i < A; ++i)
+            if (!(word >> i & 1)) z[i] = minus_inf();
+        if (c + A <= to) {
+#pragma unroll
+            for (int i = 0; i < A; ++i) dst[(long long)i * out_cls] = score_from<T>(z[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < A; ++i)
+                if (c + i < to) dst[(long long)i * out_cls] = score_from<T>(z[i]);
+        }
+        dst += (long long)A * out_cls;
+    }
+}
+
+// By row, long rows whose scores start on 16-byte boundaries: a block takes LONG_CELLS classes of a row, a thread 16 bytes at a
+// time.
+constexpr int LONG_CELLS = 4096;
+
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS, 8) k_adjust_long(AdjustArgs a, Scores<T> in, Scores<T> out) {
+    constexpr int V = Pack<T>::V;
+    extern __shared__ __align__(16) int count[];
+    const long long n = blockIdx.x;
+    const int k0 = blockIdx.y * LONG_CELLS, classes = min(LONG_CELLS, a.k - k0);
+    const T *src = in.at(n, k0);
+    T *dst = out.at(n, k0);
+    constexpr int U = LONG_CELLS / (ROW_THREADS * V);
+    Pack<T> ahead[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {   // all of them on their way while the history is counted
+        const int c = (u * ROW_THREADS + threadIdx.x) * V;
+        if (c + V <= classes) ahead[u].bits = __ldg(reinterpret_cast<const uint4 *>(src + c));
+    }
+    const unsigned *mask = mask_of(a, n);
+    if (a.history_ptr) count_histories<1>(a, n, 1, k0, classes, count, classes, [](int, int c) { return c; });
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int c = (u * ROW_THREADS + threadIdx.x) * V;
+        if (c >= classes) break;
+        const int k = k0 + c;
+        float z[V];
+        Pack<T> p;
+        const bool whole = c + V <= classes;   // else the row's last few
+        if (whole) {
+            p = ahead[u];
+            p.unpack(z);
+        } else {
+            for (int i = 0; i < V; ++i) z[i] = c + i < classes ? score_f32(src[c + i]) : 0.f;
+        }
+        if (a.history_ptr) {
+            int times[V], any = 0;   // (V * 4 bytes of counts; what lies behind the last class is 0 or not used)
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+                const int4 m = *reinterpret_cast<const int4 *>(count + c + i);
+                times[i] = m.x; times[i + 1] = m.y; times[i + 2] = m.z; times[i + 3] = m.w;
+                any |= m.x | m.y | m.z | m.w;
+            }
+            if (any) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (times[i]) z[i] = penalised(a, z[i], times[i]);
+            }
+        }
+        if (a.bias) {
+            if (whole && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
+#pragma unroll
+                for (int i = 0; i < V; i += 4) {
+                    const float4 b = __ldg(reinterpret_cast<const float4 *>(a.bias + k + i));
+                    z[i] += b.x; z[i + 1] += b.y; z[i + 2] += b.z; z[i + 3] += b.w;
+                }
+            } else {
+                for (int i = 0; i < V; ++i)
+                    if (c + i < classes) z[i] += a.bias[k + i];
+            }
+        }
+        if (mask) {
+            const unsigned word = mask[k >> 5] >> (k & 31);   // (k is a multiple of V, and V divides 32)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (!(word >> i & 1)) z[i] = minus_inf();
+        }
+        if (whole) {
+            p.pack(z);
+            *reinterpret_cast<uint4 *>(dst + c) = p.bits;
+        } else {
+            for (int i = 0; i < V; ++i)
+                if (c + i < classes) dst[c + i] = score_from<T>(z[i]);
+        }
+    }
+}
+
+// Anything else by row, in tiles of whole rows (or parts of one): cell i of the tile is class i mod tile_classes; `inverse` is
+// 2^32 / tile_classes rounded up (exact for cells below 2^16), 0 for a tile of one row.
+template <typename T>
+__global__ void __launch_bounds__(ROW_THREADS) k_adjust_tile(AdjustArgs a, Scores<T> in, Scores<T> out, int tile_rows, int tile_classes, unsigned inverse) {
+    extern __shared__ __align__(16) int count[];
     const long long n0 = (long long)blockIdx.x * tile_rows;
     const int k0 = blockIdx.y * tile_classes;
     const int rows = (int)min((long long)tile_rows, a.n - n0), classes = min(tile_classes, a.k - k0);
-    const int cells = tile_rows * tile_classes;
-    auto cell = [&](int r, int c) { return BY_CLASS ? c * tile_rows + r : r * tile_classes + c; };
-    if (a.history_ptr) {
-        for (int i = threadIdx.x; i < cells; i += ROW_THREADS) count[i] = 0;
-        __syncthreads();
-        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-        for (int r = warp; r < rows; r += ROW_THREADS / 32) {
-            const long long lo = max(0ll, a.history_ptr[n0 + r]), hi = min(a.n_history, a.history_ptr[n0 + r + 1]);
-            for (long long h = lo + lane; h < hi; h += 32) {
-                const int c = a.history[h] - k0;
-                if (c >= 0 && c < classes) atomicAdd(&count[cell(r, c)], 1);
-            }
-        }
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < cells; i += ROW_THREADS) {
-        const int r = BY_CLASS ? i % tile_rows : i / tile_classes, c = BY_CLASS ? i / tile_rows : i % tile_classes;
-        if (r >= rows || c >= classes) continue;
+    if (a.history_ptr) count_histories<ADJUST_MOST_ROWS>(a, n0, rows, k0, classes, count, tile_rows * tile_classes, [&](int r, int c) { return r * tile_classes + c; });
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows * tile_classes; i += ROW_THREADS) {
+        const int r = (int)__umulhi((unsigned)i, inverse), c = i - r * tile_classes;
+        if (c >= classes) continue;
         const long long n = n0 + r;
         const int k = k0 + c;
         float z = in(n, k);
-        if (a.history_ptr) {
-            const int m = count[i];
-            if (m) {
-                z = z > 0.f ? z / a.repetition : z * a.repetition;
-                z -= (float)m * a.frequency + a.presence;
-            }
-        }
+        if (a.history_ptr && count[i]) z = penalised(a, z, count[i]);
         if (a.bias) z += a.bias[k];
-        if (a.allowed) {
-            const int m = a.allowed_row ? a.allowed_row[n] : (int)n;
-            if (m >= 0 && m < a.n_masks && !(a.allowed[m * a.mask_stride + (k >> 5)] >> (k & 31) & 1)) z = minus_inf();
-        }
+        const unsigned *mask = mask_of(a, n);
+        if (mask && !(mask[k >> 5] >> (k & 31) & 1)) z = minus_inf();
         *out.at(n, k) = score_from<T>(z);
     }
 }
@@ -980,17 +1149,30 @@ Tile tile_of(int n, int k, bool by_class, size_t per_row) {
     return t;
 }
 
-void scores_adjust(const AdjustArgs &a, cudaStream_t stream) {
-    if (a.n == 0) return;
-    const bool by_class = a.in.row < a.in.cls;
-    const int tile_rows = by_class ? 32 : std::max(1, std::min(a.n, ADJUST_CELLS / std::min(a.k, ADJUST_CELLS)));
-    const int tile_classes = by_class ? ADJUST_CELLS / 32 : std::min(a.k, ADJUST_CELLS);
-    const dim3 grid((unsigned)((a.n + (long long)tile_rows - 1) / tile_rows), (unsigned)((a.k + tile_classes - 1) / tile_classes));
-    const size_t smem = a.history_ptr ? sizeof(int) * (size_t)tile_rows * tile_classes : 0;
+void scores_adjust(const AdjustArgs &given, cudaStream_t stream) {
+    if (given.n == 0) return;
+    AdjustArgs a = given;
+    a.inv_repetition = 1.f / a.repetition;
+    const bool by_class = a.in.row < a.in.cls && a.out.row < a.out.cls && std::max(a.in.cls, a.out.cls) <= INT_MAX / ADJUST_AHEAD;
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
-        if (by_class) k_adjust<T, true><<<grid, ROW_THREADS, smem, stream>>>(a, scores_of<T>(a.in), scores_of<T>(a.out), tile_rows, tile_classes);
-        else k_adjust<T, false><<<grid, ROW_THREADS, smem, stream>>>(a, scores_of<T>(a.in), scores_of<T>(a.out), tile_rows, tile_classes);
+        constexpr int V = Pack<T>::V;
+        const Scores<T> in = scores_of<T>(a.in), out = scores_of<T>(a.out);
+        const size_t counts = a.history_ptr ? sizeof(int) * ADJUST_CELLS : 0;
+        auto parts = [](long long n, int of) { return (unsigned)((n + of - 1) / of); };
+        auto aligned = [&](const Scores<T> &s) { return s.cls == 1 && s.row % V == 0 && reinterpret_cast<uintptr_t>(s.p) % 16 == 0; };
+        if (by_class) {
+            auto kern = counts ? k_adjust_class<T, true> : k_adjust_class<T, false>;
+            kern<<<dim3(parts(a.n, ADJUST_ROWS), parts(a.k, ADJUST_CLASSES)), ROW_THREADS, counts, stream>>>(a, in, out);
+        } else if (a.k >= ROW_THREADS * V / 2 && aligned(in) && aligned(out)) {
+            // (shorter rows leave most of a block without a pack)
+            k_adjust_long<T><<<dim3((unsigned)a.n, parts(a.k, LONG_CELLS)), ROW_THREADS, counts ? sizeof(int) * LONG_CELLS : 0, stream>>>(a, in, out);
+        } else {
+            const int tile_classes = std::max(2, std::min(a.k, ADJUST_CELLS)), tile_rows = std::max(1, std::min(a.n, ADJUST_CELLS / 4 / tile_classes));
+            static_assert(ADJUST_CELLS / 4 / 2 <= ADJUST_MOST_ROWS, "");
+            const unsigned inverse = tile_rows == 1 ? 0u : (unsigned)(((1ull << 32) + tile_classes - 1) / tile_classes);
+            k_adjust_tile<T><<<dim3(parts(a.n, tile_rows), parts(a.k, tile_classes)), ROW_THREADS, counts, stream>>>(a, in, out, tile_rows, tile_classes, inverse);
+        }
     });
     TGBM_CUDA(cudaGetLastError());
 }

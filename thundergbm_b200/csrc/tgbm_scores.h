@@ -29,6 +29,7 @@ struct AdjustArgs {
     const int *history = nullptr;
     long long n_history = 0;
     float repetition = 1.f, frequency = 0.f, presence = 0.f;
+    float inv_repetition = 1.f;          // filled in by scores_adjust
 };
 void scores_adjust(const AdjustArgs &a, cudaStream_t stream);
 
