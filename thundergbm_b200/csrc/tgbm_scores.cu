@@ -304,54 +304,69 @@ __global__ void __launch_bounds__(FEW_THREADS) k_top_few(TopArgs a, Scores<T> in
 
 // A block takes a tile of rows x all classes into shared memory, a warp chooses for one row after the other.  By class: the rows of
 // a class are copied side by side, a cell of row r and class c lies at c * (rows + 1) + r, so that neither the copies nor the
-// reads along a row meet in a bank.  By row: a warp copies its own rows.
+// reads along a row meet in a bank.  By row: a warp copies its own rows.  What a warp does for a row is a few hundred
+// instructions, and they decide the time: the kernels are made for the number of scores per lane (E, see WarpRow).
 constexpr int TILE_ROW_CLASSES = 1024;   // by row: above, a block takes a row
-constexpr int TILE_WARPS = 8, TILE_THREADS = 32 * TILE_WARPS;
+constexpr int TILE_WARPS = 8, TILE_THREADS = 32 * TILE_WARPS, TILE_MOST_ROWS = 32;
 
-template <typename T, bool BY_CLASS>
-__device__ __forceinline__ void load_tile(float *tile, const Scores<T> &in, long long n0, int rows, int rows_log, int k) {
+template <typename T>
+__device__ __noinline__ void load_tile_of(float *tile, const T *p, long long row, long long cls, bool by_class, int rows, int rows_log, int k) {
     auto copy = [](float *to, const T *from) {
         if constexpr (sizeof(T) == 4) copy_async4(to, from);
         else *to = score_f32(*from);
     };
-    if (BY_CLASS) {
-        const int r = threadIdx.x & ((1 << rows_log) - 1), per = TILE_THREADS >> rows_log;
-        if (r < rows) {
-            const T *p = in.at(n0 + r, 0);
+    if (by_class) {
+        const int r = threadIdx.x & ((1 << rows_log) - 1), per = TILE_THREADS >> rows_log, c0 = threadIdx.x >> rows_log;
+        if (r >= rows) return;
+        const T *from = p + r * row + c0 * cls;
+        float *to = tile + c0 * ((1 << rows_log) + 1) + r;
+        const int step = per * ((1 << rows_log) + 1);
 #pragma unroll 8
-            for (int c = threadIdx.x >> rows_log; c < k; c += per) copy(tile + c * ((1 << rows_log) + 1) + r, p + c * in.cls);
-        }
+        for (int c = c0; c < k; c += per, from += per * cls, to += step) copy(to, from);
     } else {
         for (int r = threadIdx.x >> 5; r < rows; r += TILE_WARPS) {
-            const T *p = in.at(n0 + r, 0);
+            const int lane = threadIdx.x & 31;
+            const T *from = p + r * row + lane * cls;
+            float *to = tile + r * k + lane;
 #pragma unroll 8
-            for (int c = threadIdx.x & 31; c < k; c += 32) copy(tile + r * k + c, p + c * in.cls);
+            for (int c = lane; c < k; c += 32, from += 32 * cls, to += 32) copy(to, from);
         }
     }
 }
+__device__ __forceinline__ void load_tile(float *tile, const ScoreView &v, long long n0, bool by_class, int rows, int rows_log, int k) {
+    const long long at = n0 * v.row;
+    if (v.type == SCORE_F32) load_tile_of(tile, static_cast<const float *>(v.data) + at, v.row, v.cls, by_class, rows, rows_log, k);
+    else if (v.type == SCORE_F16) load_tile_of(tile, static_cast<const __half *>(v.data) + at, v.row, v.cls, by_class, rows, rows_log, k);
+    else load_tile_of(tile, static_cast<const __nv_bfloat16 *>(v.data) + at, v.row, v.cls, by_class, rows, rows_log, k);
+}
 
-template <typename T, bool BY_CLASS, int G>
-__global__ void __launch_bounds__(TILE_THREADS) k_top_tile(TopArgs a, Scores<T> in, int rows_log) {
+template <int E, int G>
+__global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : E == 16 ? 3 : 4) k_top_tile(TopArgs a, bool by_class, int rows_log) {
     extern __shared__ __align__(16) float tile[];
     __shared__ __align__(16) unsigned room[TILE_WARPS][2 * TOP_ROOM * G];
+    __shared__ float sums[TILE_MOST_ROWS][2];
     const long long n0 = (long long)blockIdx.x << rows_log;
     const int rows = (int)min(1ll << rows_log, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    load_tile<T, BY_CLASS>(tile, in, n0, rows, rows_log, a.k);
+    load_tile(tile, a.in, n0, by_class, rows, rows_log, a.k);
     copies_done();
-    if (BY_CLASS) __syncthreads(); else __syncwarp();
+    __syncthreads();
     for (int r = warp; r < rows; r += TILE_WARPS) {
-        const float *z = BY_CLASS ? tile + r : tile + r * a.k;
-        const int step = BY_CLASS ? (1 << rows_log) + 1 : 1;
-        const long long n = n0 + r;
+        const WarpRow<E> row(by_class ? tile + r : tile + r * a.k, by_class ? (1 << rows_log) + 1 : 1, a.k);
         if (a.lse) {
             float m = minus_inf(), s = 0;
-            for (int i = lane; i < a.k; i += 32) m = fmaxf(m, z[i * step]);
+            row.each([&](float x, int, int) { m = fmaxf(m, x); });
             m = row_top(warp_max(m));
-            for (int i = lane; i < a.k; i += 32) s += exp2_fast(__fsub_rn(z[i * step], m) * a.c);
+            row.each([&](float x, int, int) { s += exp2_fast(__fsub_rn(x, m) * a.c); });
             s = warp_sum(s);
-            if (lane == 0) a.lse[n] = (float)((double)m * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
+            if (lane == 0) { sums[r][0] = m; sums[r][1] = s; }
         }
-        warp_top<G>(z, step, a.k, a.top, room[warp], a.values + n * a.top, a.ids + n * a.top);
+        const long long n = n0 + r;
+        warp_top<E, G>(row, a.top, room[warp], a.values + n * a.top, a.ids + n * a.top);
+    }
+    __syncthreads();
+    if (a.lse && threadIdx.x < rows) {
+        const float m = sums[threadIdx.x][0], s = sums[threadIdx.x][1];
+        a.lse[n0 + threadIdx.x] = (float)((double)m * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
     }
 }
 
@@ -892,49 +907,74 @@ __global__ void __launch_bounds__(FEW_THREADS) k_distill_few(DistillArgs a, Scor
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
-// A tile as in k_top_tile: the teacher's lists are read while the scores are on their way, a warp finds the factors of one row after
-// the other, and the gradients are written the way the scores were read.
-template <typename T, bool BY_CLASS, bool TWO>
-__global__ void __launch_bounds__(TILE_THREADS) k_distill_tile(DistillArgs a, Scores<T> in, int rows_log) {
+// A tile as in k_top_tile: the teacher's lists are read while the scores are on their way, a warp sums up one row after the other, a
+// lane each finds the rows' losses and the factors of their gradients, and the gradients are written the way the scores were read.
+template <int E, bool TWO, int S>
+__global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(DistillArgs a, bool by_class, int rows_log) {
     extern __shared__ __align__(16) float tile[];
-    const int R = 1 << rows_log, step = BY_CLASS ? R + 1 : 1;
-    int *list_id = reinterpret_cast<int *>(tile + (size_t)a.k * (BY_CLASS ? R + 1 : R));
+    const int R = 1 << rows_log, step = by_class ? R + 1 : 1;
+    int *list_id = reinterpret_cast<int *>(tile + (size_t)a.k * (by_class ? R + 1 : R));
     float *list_q = reinterpret_cast<float *>(list_id + R * a.top);
-    __shared__ TeacherSide side[32];
-    __shared__ DistillRow factors[32];
+    __shared__ RowSums sums[TILE_MOST_ROWS];
+    __shared__ DistillRow factors[TILE_MOST_ROWS];
     const long long n0 = (long long)blockIdx.x << rows_log;
     const int rows = (int)min((long long)R, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    load_tile<T, BY_CLASS>(tile, in, n0, rows, rows_log, a.k);
+    load_tile(tile, a.in, n0, by_class, rows, rows_log, a.k);
     for (int r = warp; r < rows; r += TILE_WARPS) {
-        const TeacherSide t = read_teacher(a, n0 + r, list_id + r * a.top, list_q + r * a.top);
-        if (lane == 0) side[r] = t;
+        const TeacherSide t = read_teacher<S>(a, n0 + r, list_id + r * a.top, list_q + r * a.top);
+        if (lane == 0) sums[r].teacher = t;
     }
     copies_done();
-    if (BY_CLASS) __syncthreads(); else __syncwarp();
-    float mg = 0, mh = 0;
-    auto put = [&](const DistillRow &d, int r, int c, float z) {
-        const int e = r * a.top + min(listed_entry(z), a.top - 1);
-        const float2 gh = is_listed_cell(z) ? listed_gh<TWO>(d, c, __int_as_float(list_id[e]), list_q[e]) : other_gh<TWO>(d, c, z);
-        const long long n = n0 + r;
-        const long long at = n * a.out.row + c * a.out.cls;
-        if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
-        else static_cast<T *>(a.out.data)[at] = score_from<T>(gh.x);
-        mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
-    };
-    for (int r = warp; r < rows; r += TILE_WARPS) {
-        float *z = BY_CLASS ? tile + r : tile + r * a.k;
-        const DistillRow d = warp_student<TWO>(a, side[r], n0 + r, z, step, list_id + r * a.top, list_q + r * a.top);
-        if (BY_CLASS) { if (lane == 0) factors[r] = d; }
-        else if (a.gives != GIVES_LOSS)
-            for (int c = lane; c < a.k; c += 32) put(d, r, c, z[c]);
+    __syncthreads();
+    for (int r = warp; r < rows; r += TILE_WARPS)
+        warp_student<E, TWO, S>(a, n0 + r, by_class ? tile + r : tile + r * a.k, step, list_id + r * a.top, list_q + r * a.top, sums[r]);
+    __syncthreads();
+    if (threadIdx.x < rows) {
+        const RowSums &r = sums[threadIdx.x];
+        const long long n = n0 + threadIdx.x;
+        const StudentRow s = student_of(a, r);
+        const float w = a.weights ? a.weights[n] : 1.f;
+        const int label = row_label(a, n);
+        if (a.gives != GIVES_LOSS) factors[threadIdx.x] = distill_row(a, r.teacher, s, w, label);
+        if (a.loss) a.loss[n] = distill_loss(a, r.teacher, s, w, label, r.of_listed, r.mass, r.label_score);
     }
-    if (BY_CLASS && a.gives != GIVES_LOSS) {
-        __syncthreads();
-        const int r = threadIdx.x & (R - 1), per = TILE_THREADS >> rows_log;
-        if (r < rows) {
-            const DistillRow d = factors[r];
-            for (int c = threadIdx.x >> rows_log; c < a.k; c += per) put(d, r, c, tile[c * step + r]);
+    if (a.gives == GIVES_LOSS) return;
+    __syncthreads();
+    float mg = 0, mh = 0;
+    // cells from `first` on, `per` apart, of row r
+    auto write = [&](int r, const float *z, int first, int per) {
+        const DistillRow d = factors[r];
+        const long long at = (n0 + r) * a.out.row + first * a.out.cls, cls = per * a.out.cls;
+        auto cell = [&](int c) {
+            const float x = z[c * step];
+            const int e = r * a.top + min(listed_entry(x), a.top - 1);
+            const float2 gh = is_listed_cell(x) ? listed_gh<TWO>(d, c, __int_as_float(list_id[e]), list_q[e]) : other_gh<TWO>(d, c, x);
+            mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
+            return gh;
+        };
+        if (a.gives == GIVES_PAIRS) {
+            float2 *to = static_cast<float2 *>(a.out.data) + at;
+#pragma unroll 4
+            for (int c = first; c < a.k; c += per, to += cls) *to = cell(c);
+        } else if (a.out.type == SCORE_F32) {
+            float *to = static_cast<float *>(a.out.data) + at;
+#pragma unroll 4
+            for (int c = first; c < a.k; c += per, to += cls) *to = cell(c).x;
+        } else {
+            const bool half = a.out.type == SCORE_F16;
+            unsigned short *to = static_cast<unsigned short *>(a.out.data) + at;
+#pragma unroll 4
+            for (int c = first; c < a.k; c += per, to += cls) {
+                const float g = cell(c).x;
+                *to = half ? __half_as_ushort(__float2half_rn(g)) : __bfloat16_as_ushort(__float2bfloat16_rn(g));
+            }
         }
+    };
+    if (by_class) {
+        const int r = threadIdx.x & (R - 1);
+        if (r < rows) write(r, tile + r, threadIdx.x >> rows_log, TILE_THREADS >> rows_log);
+    } else {
+        for (int r = warp; r < rows; r += TILE_WARPS) write(r, tile + r * a.k, lane, 32);
     }
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
@@ -1177,6 +1217,15 @@ void scores_adjust(const AdjustArgs &given, cudaStream_t stream) {
     TGBM_CUDA(cudaGetLastError());
 }
 
+// f(E) for the number of scores a lane has of a row (WarpRow)
+template <typename F> void by_lane(int k, F &&f) {
+    if (k <= 128) f(std::integral_constant<int, 4>{});
+    else if (k <= 256) f(std::integral_constant<int, 8>{});
+    else if (k <= 512) f(std::integral_constant<int, 16>{});
+    else if (k <= 1024) f(std::integral_constant<int, 32>{});
+    else f(std::integral_constant<int, 0>{});
+}
+
 // Blocks of a cluster for a long row: one, and more where there are not rows enough for two blocks per SM, or where the rows
 // that are at work at once would not fit into the L2 cache for a second pass (`twice` bytes of a row; 0: there is none).
 // A part is not shorter than what a block takes in one step.
@@ -1221,17 +1270,16 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
         const bool by_class = a.in.row < a.in.cls;
         const Tile tile = tile_of(a.n, a.k, by_class, 0);
         if (tile.shared) {
-            auto go = [&](auto kern) {
-                if (tile.shared > 30 * 1024) allow_shared(kern, TILE_SHARED);
-                kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, scores_of<T>(a.in), tile.rows_log);
-            };
-            auto groups = [&](auto by) {
-                constexpr bool B = decltype(by)::value;
-                if (a.top <= 32) go(k_top_tile<T, B, 1>);
-                else if (a.top <= 64) go(k_top_tile<T, B, 2>);
-                else go(k_top_tile<T, B, 4>);
-            };
-            by_class ? groups(std::true_type{}) : groups(std::false_type{});
+            by_lane(a.k, [&](auto e) {
+                constexpr int E = decltype(e)::value;
+                auto go = [&](auto kern) {
+                    if (tile.shared > 30 * 1024) allow_shared(kern, TILE_SHARED);
+                    kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, by_class, tile.rows_log);
+                };
+                if (a.top <= 32) go(k_top_tile<E, 1>);
+                else if (a.top <= 64) go(k_top_tile<E, 2>);
+                else go(k_top_tile<E, 4>);
+            });
             return;
         }
         if (a.in.cls == 1) {
@@ -1263,12 +1311,15 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
         const bool by_class = a.in.row < a.in.cls;
         const Tile tile = tile_of(a.n, a.k, by_class, 8 * (size_t)a.top);
         if (tile.shared) {
-            auto go = [&](auto kern) {
-                if (tile.shared > 40 * 1024) allow_shared(kern, TILE_SHARED);
-                kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, scores_of<T>(a.in), tile.rows_log);
-            };
-            if (by_class) two ? go(k_distill_tile<T, true, true>) : go(k_distill_tile<T, true, false>);
-            else two ? go(k_distill_tile<T, false, true>) : go(k_distill_tile<T, false, false>);
+            by_lane(a.k, [&](auto e) {
+                constexpr int E = decltype(e)::value;
+                auto go = [&](auto kern) {
+                    if (tile.shared > 40 * 1024) allow_shared(kern, TILE_SHARED);
+                    kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, by_class, tile.rows_log);
+                };
+                if (a.top <= 32) two ? go(k_distill_tile<E, true, 1>) : go(k_distill_tile<E, false, 1>);
+                else two ? go(k_distill_tile<E, true, 4>) : go(k_distill_tile<E, false, 4>);
+            });
             return;
         }
         if (a.in.cls == 1 && (a.gives == GIVES_LOSS || a.out.cls == 1) && !a.maxbits) {

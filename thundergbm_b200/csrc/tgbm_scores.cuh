@@ -87,12 +87,13 @@ struct TeacherSide {
 
 // One warp; entry e = lane + 32 s of the row's list.  list_id[e]: the class, -1 where it is none or stands further in front;
 // list_q[e]: its mass.
+// S: segments of 32 entries that the list may have.
+template <int S = SCORES_MAX_TOP / 32>
 __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long long n, int *list_id, float *list_q) {
     const int top = a.top, k = a.k;
     const double inv_t = a.inv_t;
     const int *ids = a.ids + n * a.ids_stride;
     const float *lse = a.lse ? a.lse + n : nullptr;
-    constexpr int S = SCORES_MAX_TOP / 32;
     const int lane = threadIdx.x & 31;
     int id[S];
     double u[S], q[S], lq[S];
@@ -126,9 +127,10 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
     int distinct = 0;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        lq[s] = u[s] - L;
-        q[s] = id[s] >= 0 && !none ? exp(lq[s]) : 0.0;
+        lq[s] = q[s] = 0;
         if (s > 0 && 32 * s >= top) continue;
+        lq[s] = u[s] - L;
+        if (id[s] >= 0 && !none) q[s] = exp(lq[s]);
         // an earlier entry of the same class takes this one's mass
         const unsigned same = __match_any_sync(0xffffffffu, id[s]);
         const int first = __ffs(same) - 1;
@@ -162,11 +164,10 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
         if (e < top) { list_id[e] = id[s]; list_q[e] = (float)q[s]; }
         mass += q[s];
         if (q[s] != 0) entropy += q[s] * lq[s];
-        distinct += id[s] >= 0;
+        distinct += __popc(__ballot_sync(0xffffffffu, id[s] >= 0));
     }
     mass = warp_sum(mass);
-    entropy = warp_sum(entropy);
-    distinct = warp_sum(distinct);
+    if (a.loss) entropy = warp_sum(entropy);
     const double rest = lse && !none && distinct < k && mass < 1 ? 1.0 - mass : 0.0;
     __syncwarp();
     TeacherSide r;
@@ -204,8 +205,9 @@ constexpr float LOG2E = 1.44269504088896341f;
 constexpr float MIN_HESSIAN = 1e-16f;   // the softmax objective's
 
 __device__ __forceinline__ float2 finish_gh(const DistillRow &d, int i, float g, float p, float p1) {
-    g += d.hard * (i == d.label ? p1 - 1.f : p1);
-    return make_float2(g, fmaxf(d.curve * (p * (1.f - p)) + 2.f * d.hard * (p1 * (1.f - p1)), MIN_HESSIAN));
+    g = __fmaf_rn(d.hard, i == d.label ? p1 - 1.f : p1, g);
+    const float cp = d.curve * p, cp1 = (2.f * d.hard) * p1;
+    return make_float2(g, fmaxf(__fmaf_rn(-cp, p, cp) + __fmaf_rn(-cp1, p1, cp1), MIN_HESSIAN));
 }
 template <bool TWO>   // the hard labels need the shares at temperature 1 as well
 __device__ __forceinline__ float2 other_gh(const DistillRow &d, int i, float s) {
@@ -273,61 +275,89 @@ __device__ __forceinline__ void copy_async4(float *to, const float *from) {
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The `top` largest of k scores z[i * step], in order.  The k-th largest of the maxima of 32 G groups of classes is no more than
-// the k-th largest score, so the scores from there on hold the answer: few more than `top`, unless the large ones lie in few groups.
-// They are collected in class order, and each finds its place by counting those before it.  Rows with too many (more than
-// TOP_ROOM G) choose one after the other.  `room`: TOP_ROOM G keys and as many classes of the warp's own.
+// The row z[i * step], i < k: lane l has the scores l, l + 32, ...  E > 0: at most 32 E scores, in registers; 0: they are read again from
+// shared memory by every pass.  each(f): f(score, class) for all lanes together, -inf behind the last class.
+template <int E> struct WarpRow {
+    const float *z;
+    int step, k;
+    float x[E ? E : 1];
+    __device__ __forceinline__ WarpRow(const float *z_, int step_, int k_) : z(z_), step(step_), k(k_) {
+        if constexpr (E > 0) {
+            const int lane = threadIdx.x & 31;
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = lane + 32 * j < k ? z[(lane + 32 * j) * step] : minus_inf();
+        }
+    }
+    template <typename F> __device__ __forceinline__ void each(F &&f) const {
+        const int lane = threadIdx.x & 31;
+        if constexpr (E > 0) {
+#pragma unroll
+            for (int j = 0; j < E; ++j) f(x[j], lane + 32 * j, j);
+        } else {
+            for (int i = 0; i < k; i += 32) f(i + lane < k ? z[(i + lane) * step] : minus_inf(), i + lane, i / 32);
+        }
+    }
+};
+
+// score_key without its special cases: what cannot be chosen (-inf; NaN is made one) lies below LOWEST_KEY
+constexpr unsigned LOWEST_KEY = 0x00800000u;
+__device__ __forceinline__ unsigned plain_key(float v) {
+    const unsigned b = __float_as_uint(__fadd_rn(fmaxf(v, minus_inf()), 0.f));
+    return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+}
+
+// The `top` largest scores of a row, in order.  A border that at least `top` of the maxima of 32 G groups of classes reach is
+// reached by at least `top` scores, and by few more if few more of the maxima do: it is found by bisection.  The scores from there
+// on are collected in class order, and each finds its place by counting those before it.  Rows with too many (more than
+// TOP_ROOM G: ties, or large scores in few groups) choose one after the other.  `room`: TOP_ROOM G keys and as many classes of
+// the warp's own.
 constexpr int TOP_ROOM = 64;
 
-template <int G>
-__device__ __forceinline__ void warp_top(const float *z, int step, int k, int top, unsigned *room, float *values, int *ids) {
+template <int E, int G>
+__device__ __forceinline__ void warp_top(const WarpRow<E> &row, int top, unsigned *room, float *values, int *ids) {
     const int lane = threadIdx.x & 31;
     unsigned *keys = room;
     int *place = reinterpret_cast<int *>(room + TOP_ROOM * G);
     unsigned mx[G];
 #pragma unroll
     for (int g = 0; g < G; ++g) mx[g] = 0;
-    for (int i = lane; i < k;) {
+    row.each([&](float x, int, int j) {
+        const unsigned key = plain_key(x);
+        if constexpr (E > 0) {
+            mx[j % G] = max(mx[j % G], key);
+        } else {
 #pragma unroll
-        for (int g = 0; g < G; ++g, i += 32)
-            if (i < k) mx[g] = max(mx[g], score_key(z[i * step]));
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) keys[lane + 32 * g] = mx[g];
-    __syncwarp();
-    // the largest key that at least `top` of the maxima reach
-    unsigned from = 0xffffffffu;
-    {
-        int above[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) above[g] = 0;
-        for (int j = 0; j < 32 * G; j += 4) {
-            const uint4 o = *reinterpret_cast<const uint4 *>(keys + j);
-#pragma unroll
-            for (int g = 0; g < G; ++g) above[g] += (o.x > mx[g]) + (o.y > mx[g]) + (o.z > mx[g]) + (o.w > mx[g]);
+            for (int g = 0; g < G; ++g)
+                if (j % G == g) mx[g] = max(mx[g], key);
         }
+    });
+    unsigned low = mx[0], high = mx[0];
 #pragma unroll
-        for (int g = 0; g < G; ++g)
-            if (above[g] < top) from = min(from, mx[g]);
-    }
-    from = __reduce_min_sync(0xffffffffu, from);
-    __syncwarp();
-    int m = 0, equal = 0;
-    const unsigned before = (1u << lane) - 1;
-    for (int i0 = 0; i0 < k; i0 += 32) {
-        const int i = i0 + lane;
-        const unsigned key = i < k ? score_key(z[i * step]) : 0u;
-        unsigned take = __ballot_sync(0xffffffffu, key > from);
-        const unsigned eq = __ballot_sync(0xffffffffu, key == from && from != 0u);
-        if (eq) {   // of those equal to the border `top` are enough
-            const bool first = (eq >> lane & 1) && equal + __popc(eq & before) < top;
-            take |= __ballot_sync(0xffffffffu, first);
-            equal += __popc(eq);
+    for (int g = 1; g < G; ++g) { low = min(low, mx[g]); high = max(high, mx[g]); }
+    low = __reduce_min_sync(0xffffffffu, low);
+    high = __reduce_max_sync(0xffffffffu, high);
+    for (int steps = 0; steps < 12; ++steps) {   // all maxima reach `low` at first; at least `top` always do
+        const unsigned mid = low + (high - low + 1) / 2;
+        if (mid == low) break;
+        int reach = 0;
+#pragma unroll
+        for (int g = 0; g < G; ++g) reach += __popc(__ballot_sync(0xffffffffu, mx[g] >= mid));
+        if (reach >= top) {
+            low = mid;
+            if (reach <= top + 1) break;
+        } else {
+            high = mid - 1;
         }
+    }
+    const unsigned from = max(low, LOWEST_KEY), before = (1u << lane) - 1;
+    int m = 0;
+    row.each([&](float x, int i, int) {
+        const unsigned key = plain_key(x);
+        const unsigned take = __ballot_sync(0xffffffffu, key >= from);
         const int at = m + __popc(take & before);
-        if ((take >> lane & 1) && at < TOP_ROOM * G) { keys[at] = key; place[at] = i; }
+        if (key >= from && at < TOP_ROOM * G) { keys[at] = key; place[at] = i; }
         m += __popc(take);
-    }
+    });
     if (m <= TOP_ROOM * G) {
         if (lane < 4 && m + lane < TOP_ROOM * G) keys[m + lane] = 0;   // (read four at a time)
         __syncwarp();
@@ -336,9 +366,10 @@ __device__ __forceinline__ void warp_top(const float *z, int step, int k, int to
             int rank = 0;
             for (int j = 0; j < m; j += 4) {
                 const uint4 o = *reinterpret_cast<const uint4 *>(keys + j);
-                // of equal ones the lower class, which stands in front
-                rank += (o.x >= own + (j >= c)) + (o.y >= own + (j + 1 >= c)) + (o.z >= own + (j + 2 >= c)) + (o.w >= own + (j + 3 >= c));
+                const unsigned over = own + (j + 4 > c);   // of equal ones the lower class, which stands in front
+                rank += (o.x >= over) + (o.y >= over) + (o.z >= over) + (o.w >= over);
             }
+            for (int j = c & ~3; j < c; ++j) rank += keys[j] == own;
             if (rank < top) { values[rank] = key_score(own); ids[rank] = place[c]; }
         }
         for (int j = m + lane; j < top; j += 32) { values[j] = minus_inf(); ids[j] = -1; }
@@ -346,11 +377,11 @@ __device__ __forceinline__ void warp_top(const float *z, int step, int k, int to
         unsigned long long last = ~0ull;
         for (int j = 0; j < top; ++j) {
             unsigned long long b = 0;
-            for (int i = lane; i < k; i += 32) {
-                const unsigned key = score_key(z[i * step]);
+            row.each([&](float x, int i, int) {
+                const unsigned key = plain_key(x);
                 const unsigned long long v = (unsigned long long)key << 32 | (unsigned)~i;
-                if (key && v < last && v > b) b = v;
-            }
+                if (key >= LOWEST_KEY && v < last && v > b) b = v;
+            });
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
             last = b;
@@ -367,18 +398,35 @@ __device__ __forceinline__ float listed_cell(int entry) { return __uint_as_float
 __device__ __forceinline__ bool is_listed_cell(float z) { return (__float_as_uint(z) & 0xffffff80u) == LISTED_CELL; }
 __device__ __forceinline__ int listed_entry(float z) { return (int)(__float_as_uint(z) & 0x7fu); }
 
-// The student's side of the row z[i * step].  The cells of listed classes are marked, and their scores take the place of the class
-// numbers in the list.  Returns the factors of the row's gradients.
-template <bool TWO>
-__device__ __forceinline__ DistillRow warp_student(const DistillArgs &a, const TeacherSide &t, long long n, float *z, int step, int *list_id,
-                                                   const float *list_q) {
-    constexpr int S = SCORES_MAX_TOP / 32;
+// What one warp finds out about a row.  What follows from it is a few dozen operations per row, which lanes do for a row each.
+struct RowSums {
+    TeacherSide teacher;
+    double of_listed, mass;            // sums over the listed classes of q (s - top) / T, of q
+    float base, rest, rest1, top, l, l1;   // as in StudentRow; l, l1: of the listed classes, relative to `top`
+    float label_score;
+};
+__device__ __forceinline__ StudentRow student_of(const DistillArgs &a, const RowSums &r) {
+    StudentRow s;
+    s.base = r.base; s.rest = r.rest; s.rest1 = r.rest1; s.top = r.top;
+    const float low = __fsub_rn(r.base, r.top);
+    s.sum = r.rest * exp2_fast(low * a.c) + r.l;
+    s.sum1 = r.rest1 * exp2_fast(low * LOG2E) + r.l1;
+    return s;
+}
+
+// The sums of the row z[i * step], by one warp.  The cells of listed classes are marked, and their scores take the place of the class numbers
+// in the list.
+template <int E, bool TWO, int S>
+__device__ __forceinline__ void warp_student(const DistillArgs &a, long long n, float *z, int step, int *list_id, const float *list_q, RowSums &out) {
     const int lane = threadIdx.x & 31, k = a.k;
-    const int label = row_label(a, n);
-    const float label_score = label >= 0 ? z[label * step] : 0.f, w = a.weights ? a.weights[n] : 1.f;
+    float label_score = 0;
+    if (a.loss) {
+        const int label = row_label(a, n);
+        if (label >= 0) label_score = z[label * step];
+        __syncwarp();
+    }
     float x[S];
     float top = minus_inf();
-    __syncwarp();
 #pragma unroll
     for (int s = 0; s < S; ++s) {
         const int e = lane + 32 * s;
@@ -391,32 +439,34 @@ __device__ __forceinline__ DistillRow warp_student(const DistillArgs &a, const T
         }
     }
     __syncwarp();
-    float m = minus_inf();
-    for (int i = lane; i < k; i += 32) m = fmaxf(m, z[i * step]);
-    m = warp_max(m);
-    StudentRow st;
-    st.base = row_top(m);
-    st.top = row_top(fmaxf(warp_max(top), m));
-    float s0 = 0, s1 = 0;
-    for (int i = lane; i < k; i += 32) {
-        const float d = __fsub_rn(z[i * step], st.base);
-        s0 += exp2_fast(d * a.c);
-        if (TWO) s1 += exp2_fast(d * LOG2E);
+    float s0 = 0, s1 = 0, base;
+    {
+        const WarpRow<E> row(z, step, k);
+        float m = minus_inf();
+        row.each([&](float v, int, int) { m = fmaxf(m, v); });
+        m = warp_max(m);
+        base = row_top(m);
+        top = row_top(fmaxf(warp_max(top), m));
+        row.each([&](float v, int, int) {
+            const float d = __fsub_rn(v, base);
+            s0 += exp2_fast(d * a.c);
+            if (TWO) s1 += exp2_fast(d * LOG2E);
+        });
     }
-    st.rest = warp_sum(s0);
-    st.rest1 = TWO ? warp_sum(s1) : st.rest;
+    __syncwarp();
+    s0 = warp_sum(s0);
+    s1 = TWO ? warp_sum(s1) : s0;
     float l = 0, l1 = 0;
     double of_listed = 0, mass = 0;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        if (s > 0 && 32 * s >= a.top) continue;
         const int e = lane + 32 * s;
         if (e < a.top && list_id[e] >= 0) {
-            const float d = __fsub_rn(x[s], st.top), q = list_q[e];
+            const float d = __fsub_rn(x[s], top), q = list_q[e];
             l += exp2_fast(d * a.c);
             if (TWO) l1 += exp2_fast(d * LOG2E);
             if (a.loss) {
-                if (q != 0.f) of_listed += (double)q * (((double)x[s] - (double)st.top) * a.inv_t);
+                if (q != 0.f) of_listed += (double)q * (((double)x[s] - (double)top) * a.inv_t);
                 mass += q;
             }
             z[list_id[e] * step] = listed_cell(e);
@@ -424,18 +474,16 @@ __device__ __forceinline__ DistillRow warp_student(const DistillArgs &a, const T
         }
     }
     l = warp_sum(l);
-    if (TWO) l1 = warp_sum(l1);
-    const float low = __fsub_rn(st.base, st.top);
-    st.sum = st.rest * exp2_fast(low * a.c) + l;
-    st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + l1 : st.sum;
+    l1 = TWO ? warp_sum(l1) : l;
     if (a.loss) {
         of_listed = warp_sum(of_listed);
         mass = warp_sum(mass);
-        const float loss = distill_loss(a, t, st, w, label, of_listed, mass, label_score);
-        if (lane == 0) a.loss[n] = loss;
+    }
+    if (lane == 0) {
+        out.of_listed = of_listed; out.mass = mass; out.base = base; out.rest = s0; out.rest1 = s1; out.top = top; out.l = l; out.l1 = l1;
+        out.label_score = label_score;
     }
     __syncwarp();
-    return distill_row(a, t, st, w, label);
 }
 
 // ---- a long row in global memory, a block or a cluster of blocks -----------------------------
