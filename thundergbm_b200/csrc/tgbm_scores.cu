@@ -371,11 +371,15 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : E == 16 ? 3 : 4) k
 }
 
 // A long row: a block takes it, or a cluster of blocks where there are few rows, each a part.  One pass.  From its first packs a
-// block learns a border that at least `top` scores reach (the top-th largest of the maxima of groups of threads); only scores
-// that reach it are kept, in shared memory.  Where that list fills up the border is raised.  At the end the list (about
-// top * k / first packs' scores long) is narrowed down the same way until each entry can count those before it.
-// An entry orders scores and classes at once, so no choice depends on the order of the list.
-constexpr int WIDE_THREADS = 512, WIDE_WARPS = WIDE_THREADS / 32, WIDE_PACKS = 4, WIDE_CLUSTER = 8;
+// block learns a border that at least `top` scores reach (of the threads' maxima at least `top` do); only scores that reach it are
+// kept, in shared memory, and after some steps the border is raised to what `top` of the kept ones reach: whether one of a warp's
+// 256 scores reaches the border decides how long the warp takes for them.  At the end the list is narrowed down until each
+// entry can count those before it.  Borders are found by bisection, counting across the block.
+// Where the list fills up all the same (ties, or scores that rise along the row), borders order scores and classes at once.
+
+// Four blocks of eight warps per SM: 104 us for 64 of 1024 x 131072 in 16 bits, 111 with two of sixteen, 114 with three, 140 with five (and
+// fewer registers).
+constexpr int WIDE_THREADS = 256, WIDE_BLOCKS = 4, WIDE_WARPS = WIDE_THREADS / 32, WIDE_PACKS = 4, WIDE_CLUSTER = 8;
 constexpr int WIDE_ROOM = 2048, WIDE_GROUPS = WIDE_THREADS / 2, WIDE_LAST = 256;
 static_assert(WIDE_GROUPS >= SCORES_MAX_TOP && WIDE_CLUSTER * SCORES_MAX_TOP <= WIDE_ROOM, "");
 typedef unsigned long long Entry;   // score_key << 32 | ~class
@@ -452,12 +456,108 @@ __device__ __forceinline__ void narrow_to(TopList &l, int top, int room) {
     }
 }
 
+// Raises `low`, a key that at least `top` of what count() counts reach, towards the largest such key until no more than `enough` do;
+// count(key) is the same for all threads.  Returns how many reach it, as far as was counted (`all`: nothing was).
+template <typename F>
+__device__ __forceinline__ int raise_key(unsigned &low, unsigned high, int top, int enough, int all, F &&count) {
+    int reached = all;
+    while (reached > enough && low < high) {
+        const unsigned mid = low + (high - low + 1) / 2;
+        const int c = count(mid);
+        if (c >= top) { low = mid; reached = c; }
+        else high = mid - 1;
+    }
+    return reached;
+}
+// smallest and largest of the threads' keys, for all threads
+__device__ __forceinline__ void key_range(unsigned mine, unsigned (*parts)[2], unsigned &low, unsigned &high) {
+    low = __reduce_min_sync(0xffffffffu, mine);
+    high = __reduce_max_sync(0xffffffffu, mine);
+    if ((threadIdx.x & 31) == 0) { parts[threadIdx.x >> 5][0] = low; parts[threadIdx.x >> 5][1] = high; }
+    __syncthreads();
+    low = __reduce_min_sync(0xffffffffu, parts[threadIdx.x & (WIDE_WARPS - 1)][0]);
+    high = __reduce_max_sync(0xffffffffu, parts[threadIdx.x & (WIDE_WARPS - 1)][1]);
+}
+// The border that `enough` or a few more of the list's entries reach, by their keys; drops the others if asked to.  All threads, with a
+// barrier before; the list is not full.
+__device__ __noinline__ void raise_border(TopList &l, int top, int enough, bool drop, unsigned (*parts)[2]) {
+    constexpr int U = WIDE_ROOM / WIDE_THREADS;
+    const int m = l.count;
+    unsigned key[U], most = 0;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+        const int at = threadIdx.x + i * WIDE_THREADS;
+        key[i] = at < m ? (unsigned)(l.e[at] >> 32) : 0u;
+        most = max(most, key[i]);
+    }
+    unsigned low, high;
+    key_range(most, parts, low, high);
+    low = (unsigned)(l.border >> 32);
+    const int left = raise_key(low, high, top, enough, m, [&](unsigned mid) {
+        int c = 0;
+        for (int i = 0; i < U && i * WIDE_THREADS < m; ++i) c += __syncthreads_count(key[i] >= mid);
+        return c;
+    });
+    if (!drop) {
+        if (threadIdx.x == 0 && (Entry)low << 32 > l.border) l.border = (Entry)low << 32;
+        __syncthreads();
+        return;
+    }
+    if (left == m) return;
+    Entry own[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) own[i] = key[i] >= low && key[i] ? l.e[threadIdx.x + i * WIDE_THREADS] : 0;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        l.count = 0;
+        if ((Entry)low << 32 > l.border) l.border = (Entry)low << 32;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+        if (own[i]) l.e[atomicAdd(&l.count, 1)] = own[i];
+    __syncthreads();
+}
+
+// A step's scores have filled the list: the border is raised to that of the step's own threads' maxima and the list narrowed, then the
+// scores that found no room (`dropped`, the thread's V * WIDE_PACKS cells) are put in, a warp at a time.  The scores are read again: this
+// is rare, and the registers are needed elsewhere.
 template <typename T>
-__global__ void __launch_bounds__(WIDE_THREADS, 2) k_top_wide(TopArgs a, Scores<T> in) {
+__device__ __noinline__ void make_room(TopList &l, int top, const T *cells, int packs, int k0, unsigned dropped) {
+    constexpr int V = Pack<T>::V, WARP_CELLS = 32 * WIDE_PACKS * V;
+    static_assert(WIDE_LAST + WARP_CELLS <= WIDE_ROOM, "");
+    auto each = [&](auto &&f) {
+        for (int u = 0; u < WIDE_PACKS; ++u) {
+            const int at = u * WIDE_THREADS + threadIdx.x;
+            if (at >= packs) break;
+            for (int i = 0; i < V; ++i) f(u * V + i, entry_of(score_f32(cells[at * V + i]), k0 + at * V + i));
+        }
+    };
+    Entry most = 0;
+    each([&](int, Entry e) { most = max(most, e); });
+    if (threadIdx.x == 0) l.count = min(l.count, WIDE_ROOM);
+    find_border(l, most, top);
+    narrow_to(l, top, WIDE_LAST);
+    for (int turn = 0; turn < WIDE_WARPS; ++turn) {
+        const bool full = l.count > WIDE_ROOM - WARP_CELLS;
+        __syncthreads();
+        if (full) narrow_to(l, top, WIDE_LAST);
+        const Entry border = l.border;
+        if ((int)(threadIdx.x >> 5) == turn && dropped)
+            each([&](int bit, Entry e) {
+                if ((dropped >> bit & 1) && e >= border) l.e[atomicAdd(&l.count, 1)] = e;
+            });
+        __syncthreads();
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_top_wide(TopArgs a, Scores<T> in) {
     constexpr int V = Pack<T>::V, STEP = WIDE_THREADS * WIDE_PACKS;
     __shared__ __align__(16) TopList l;
     __shared__ Entry best[SCORES_MAX_TOP];
     __shared__ float parts[WIDE_WARPS][2], whole[2];
+    __shared__ unsigned ranges[WIDE_WARPS][2];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const long long n = blockIdx.x / C;
@@ -505,18 +605,25 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_top_wide(TopArgs a, Scores<
 #pragma unroll
             for (int i = 0; i < V; ++i) f(u * V + i, v[i], k + i);
         };
-        auto most = [&] {
-            Entry e = 0;
+        const int turn = from / STEP;
+        if (turn == 0 && part.packs * V > WIDE_ROOM / 2) {
+            float largest = minus_inf();
 #pragma unroll
             for (int u = 0; u < WIDE_PACKS; ++u)
-                if (has(u)) each(u, [&](int, float x, int k) { e = max(e, entry_of(x, k)); });
-            return e;
-        };
-        if (from == 0 && part.packs * V > WIDE_ROOM / 2) {
-            find_border(l, most(), a.top);
+                if (has(u)) each(u, [&](int, float x, int) { largest = fmaxf(largest, x); });
+            const unsigned mine = score_key(largest);
+            unsigned low, high;
+            key_range(mine, ranges, low, high);
+            low = max(low, (unsigned)(LOWEST_ENTRY >> 32));
+            raise_key(low, high, a.top, a.top + a.top / 8, WIDE_THREADS, [&](unsigned mid) { return __syncthreads_count(mine >= mid); });
+            border = (Entry)low << 32;
+            if (tid == 0) l.border = border;   // (read behind the next barrier)
+        } else if (turn == 1 || turn == 2 || turn == 4) {
+            __syncthreads();
+            raise_border(l, a.top, a.top + a.top / 8, false, ranges);
             border = l.border;
-            if (border > LOWEST_ENTRY) border_score = key_score((unsigned)(border >> 32));
         }
+        if (border > LOWEST_ENTRY) border_score = key_score((unsigned)(border >> 32));
         unsigned dropped = 0;
         last = 0;
 #pragma unroll
@@ -527,38 +634,33 @@ __global__ void __launch_bounds__(WIDE_THREADS, 2) k_top_wide(TopArgs a, Scores<
             run.raise(largest, a.c);
             const float base = row_top(run.m);
             each(u, [&](int, float x, int) { run.add(x, base, a.c); });
-            if (largest >= border_score)
-                each(u, [&](int bit, float x, int k) {
-                    if (x >= border_score) {
-                        const Entry e = entry_of(x, k);
-                        if (e >= border && !push(e)) dropped |= 1u << bit;
-                    }
-                });
+            if (largest >= border_score) {   // few of a lane's V scores, but most often one of some lane's
+                unsigned reach = 0;
+                float v[V];
+                Pack<T> p;
+                p.bits = w[u];
+                p.unpack(v);
+#pragma unroll
+                for (int i = 0; i < V; ++i) reach |= v[i] >= border_score ? 1u << i : 0u;
+                while (reach) {
+                    const int i = __ffs(reach) - 1;
+                    reach &= reach - 1;
+                    float x = v[0];
+#pragma unroll
+                    for (int j = 1; j < V; ++j) x = i == j ? v[j] : x;
+                    const Entry e = entry_of(x, lo + part.head + (from + u * WIDE_THREADS + tid) * V + i);
+                    if (e >= border && !push(e)) dropped |= 1u << (u * V + i);
+                }
+            }
         }
         if (__syncthreads_or(last >= WIDE_ROOM * 3 / 4)) {   // all threads see the same: the list is full, or soon will be
-            if (tid == 0) l.count = min(l.count, WIDE_ROOM);
-            find_border(l, most(), a.top);
-            narrow_to(l, a.top, WIDE_LAST);
-            constexpr int WARP_CELLS = 32 * WIDE_PACKS * V;
-            static_assert(WIDE_LAST + WARP_CELLS <= WIDE_ROOM, "");
-            for (int turn = 0; turn < WIDE_WARPS; ++turn) {
-                const bool full = l.count > WIDE_ROOM - WARP_CELLS;
-                __syncthreads();
-                if (full) narrow_to(l, a.top, WIDE_LAST);
-                border = l.border;
-                if (warp == turn && dropped) {
-#pragma unroll
-                    for (int u = 0; u < WIDE_PACKS; ++u)
-                        if (has(u)) each(u, [&](int bit, float x, int k) {
-                            if ((dropped >> bit & 1) && entry_of(x, k) >= border) push(entry_of(x, k));
-                        });
-                }
-                __syncthreads();
-            }
+            make_room(l, a.top, part.p + part.head + (long long)from * V, part.packs - from, lo + part.head + from * V, dropped);
+            border = l.border;
             border_score = border > LOWEST_ENTRY ? key_score((unsigned)(border >> 32)) : -FLT_MAX;
         }
     }
     __syncthreads();
+    if (l.count > a.top + a.top / 2) raise_border(l, a.top, a.top + a.top / 2, true, ranges);
     narrow_to(l, a.top, WIDE_LAST);
     run.join_warp(a.c);
     if (lane == 0) { parts[warp][0] = run.m; parts[warp][1] = run.s; }
@@ -983,7 +1085,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 // finds the row in the L2 cache (the launch sees to it that the rows at work fit there) and writes what unlisted classes get; the
 // few cells of listed classes and of the label are written over it.
 template <typename T, bool TWO>
-__global__ void __launch_bounds__(WIDE_THREADS, 2) k_distill_wide(DistillArgs a, Scores<T> in) {
+__global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(DistillArgs a, Scores<T> in) {
     constexpr int V = Pack<T>::V;
     extern __shared__ unsigned bits[];
     __shared__ int list_id[SCORES_MAX_TOP];
@@ -1230,7 +1332,7 @@ template <typename F> void by_lane(int k, F &&f) {
 // that are at work at once would not fit into the L2 cache for a second pass (`twice` bytes of a row; 0: there is none).
 // A part is not shorter than what a block takes in one step.
 int blocks_per_row(int n, int k, int size, size_t twice) {
-    constexpr long long SLOTS = 2 * 148;
+    constexpr long long SLOTS = WIDE_BLOCKS * 148;
     constexpr size_t L2_ROOM = 48u << 20;
     int c = 1;
     while (c < WIDE_CLUSTER && k / (2 * c) >= WIDE_THREADS * WIDE_PACKS * 16 / size &&
