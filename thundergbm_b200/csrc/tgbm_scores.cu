@@ -629,17 +629,16 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_top_wide(TopArgs 
 #pragma unroll
         for (int u = 0; u < WIDE_PACKS; ++u) {
             if (!has(u)) break;
-            float largest = minus_inf();
-            each(u, [&](int, float x, int) { largest = fmaxf(largest, x); });
-            run.raise(largest, a.c);
-            const float base = row_top(run.m);
-            each(u, [&](int, float x, int) { run.add(x, base, a.c); });
+            float v[V];
+            Pack<T> p;
+            p.bits = w[u];
+            p.unpack(v);
+            float largest = v[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) largest = fmaxf(largest, v[i]);
+            run.add_pack(v, a.c);
             if (largest >= border_score) {   // few of a lane's V scores, but most often one of some lane's
                 unsigned reach = 0;
-                float v[V];
-                Pack<T> p;
-                p.bits = w[u];
-                p.unpack(v);
 #pragma unroll
                 for (int i = 0; i < V; ++i) reach |= v[i] >= border_score ? 1u << i : 0u;
                 while (reach) {
@@ -1083,15 +1082,18 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 
 // A long row, taken as in k_top_wide.  The first pass sums up the classes that the teacher does not list, which a bit map marks; the second
 // finds the row in the L2 cache (the launch sees to it that the rows at work fit there) and writes what unlisted classes get; the
-// few cells of listed classes and of the label are written over it.
+// few cells of listed classes and of the label are written over it.  (What lies between the passes is one warp's work: done by
+// every warp for itself it took less waiting and more instructions, and the same time.)
 template <typename T, bool TWO>
 __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(DistillArgs a, Scores<T> in) {
-    constexpr int V = Pack<T>::V;
+    constexpr int V = Pack<T>::V, S = SCORES_MAX_TOP / 32;
     extern __shared__ unsigned bits[];
-    __shared__ int list_id[SCORES_MAX_TOP];
-    __shared__ float list_q[SCORES_MAX_TOP];
-    __shared__ TeacherSide teacher;
+    __shared__ int list_id[SCORES_MAX_TOP];   // -1: no class
+    __shared__ float list_t[SCORES_MAX_TOP], list_x[SCORES_MAX_TOP], list_q[SCORES_MAX_TOP];   // the teacher's scores, the student's, masses
     __shared__ DistillRow factors;
+    __shared__ TeacherSide teacher;
+    __shared__ StudentRow student;
+    __shared__ float row_lse, label_score;
     __shared__ float parts[WIDE_WARPS][3], whole[3];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1105,18 +1107,31 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         for (int u = 0; u < WIDE_PACKS; ++u)
             if (from + u * WIDE_THREADS + tid < part.packs) ahead[u] = __ldg(body + from + u * WIDE_THREADS + tid);
     };
+    static_assert(WIDE_THREADS >= SCORES_MAX_TOP, "");
+    // what the row gives besides its scores: read here, where it is waited for together with the lists
+    const int label = row_label(a, n);
+    const float w = a.weights ? a.weights[n] : 1.f;
+    if (tid == WIDE_THREADS - 1) {
+        row_lse = a.lse ? a.lse[n] : 0.f;
+        label_score = label >= 0 ? in(n, label) : 0.f;
+    }
+    int id = -1;
+    if (tid < a.top) {
+        id = a.ids[n * a.ids_stride + tid];
+        if (id < 0 || id >= a.k) id = -1;
+    }
     fetch(0);
     for (int i = tid; i < (per + 31) / 32 + 1; i += WIDE_THREADS) bits[i] = 0;   // (a word more: read in twos)
     __syncthreads();
-    if (warp == 0) {
-        const TeacherSide t = read_teacher(a, n, list_id, list_q);
-        if (lane == 0) teacher = t;
-        for (int e = lane; e < a.top; e += 32) {
-            const int k = list_id[e] - lo;
-            if (list_id[e] >= lo && k < hi - lo) atomicOr(&bits[k >> 5], 1u << (k & 31));
-        }
+    bool repeat = false;   // in this block's part; a class stands in one part
+    if (tid < a.top) {
+        const int k = id - lo;
+        if (id >= lo && k < hi - lo) repeat = atomicOr(&bits[k >> 5], 1u << (k & 31)) >> (k & 31) & 1;
+        list_id[tid] = id;
+        list_t[tid] = teacher_logit(a, n, tid);
+        list_x[tid] = id >= 0 ? in(n, id) : minus_inf();
     }
-    __syncthreads();
+    const bool repeats = __syncthreads_or(repeat) || C > 1;
     auto listed = [&](int k) { return bits[k >> 5] >> (k & 31) & 1; };   // k: cell of the part
     Running<TWO> run;
     if (tid < part.head + part.tail) {
@@ -1147,69 +1162,64 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
                 for (int i = 0; i < V; ++i)
                     if (mark >> i & 1) v[i] = minus_inf();
             }
-            float largest = v[0];
-#pragma unroll
-            for (int i = 1; i < V; ++i) largest = fmaxf(largest, v[i]);
-            run.raise(largest, a.c);
-            const float base = row_top(run.m);
-#pragma unroll
-            for (int i = 0; i < V; ++i) run.add(v[i], base, a.c);
+            run.add_pack(v, a.c);
         }
     }
     run.join_warp(a.c);
     if (lane == 0) { parts[warp][0] = run.m; parts[warp][1] = run.s; parts[warp][2] = run.s1; }
     __syncthreads();
-    if (warp == 0) {
+    {
         Running<TWO> all;
         if (lane < WIDE_WARPS) { all.m = parts[lane][0]; all.s = parts[lane][1]; all.s1 = parts[lane][2]; }
         all.join_warp(a.c);
-        if (C > 1) {
-            if (lane == 0) { whole[0] = all.m; whole[1] = all.s; whole[2] = all.s1; }
-        }
         run = all;
     }
     if (C > 1) {
+        if (tid == 0) { whole[0] = run.m; whole[1] = run.s; whole[2] = run.s1; }
         cluster.sync();
-        if (warp == 0) {
-            run = Running<TWO>();
-            for (int c = 0; c < C; ++c) {
-                const float *o = cluster.map_shared_rank(whole, c);
-                run.join(o[0], o[1], o[2], a.c);
-            }
+        run = Running<TWO>();
+        for (int c = 0; c < C; ++c) {
+            const float *o = cluster.map_shared_rank(whole, c);
+            run.join(o[0], o[1], o[2], a.c);
         }
     }
-    const int label = row_label(a, n);
-    if (warp == 0) {
-        const TeacherSide t = teacher;
-        const float w = a.weights ? a.weights[n] : 1.f;
+    if (warp == 0) {   // the others wait: only what the second pass needs
+        int ids[S];
+        float q[S], t[S], x[S];
+        float top = run.m;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            ids[s] = e < a.top ? list_id[e] : -1;
+            t[s] = e < a.top ? list_t[e] : 0.f;
+            x[s] = e < a.top ? list_x[e] : minus_inf();
+            top = fmaxf(top, x[s]);
+        }
+        const TeacherSide side = teacher_of<S>(a, a.lse ? &row_lse : nullptr, ids, t, q, repeats);
         StudentRow st;
         st.base = row_top(run.m); st.rest = run.s; st.rest1 = TWO ? run.s1 : run.s;
-        float top = run.m;
-        for (int e = lane; e < a.top; e += 32)
-            if (list_id[e] >= 0) top = fmaxf(top, in(n, list_id[e]));
         st.top = row_top(warp_max(top));
-        float s = 0, s1 = 0;
-        double of_listed = 0, mass = 0;
-        for (int e = lane; e < a.top; e += 32)
-            if (list_id[e] >= 0) {
-                const float z = in(n, list_id[e]), d = __fsub_rn(z, st.top), q = list_q[e];
-                s += exp2_fast(d * a.c);
-                if (TWO) s1 += exp2_fast(d * LOG2E);
-                if (q != 0.f) of_listed += (double)q * (((double)z - (double)st.top) * a.inv_t);
-                mass += q;
-            }
+        float s0 = 0, s1 = 0;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            if (e < a.top) { list_id[e] = ids[s]; list_q[e] = q[s]; }
+            if (ids[s] < 0) continue;
+            const float far = __fsub_rn(x[s], st.top);
+            s0 += exp2_fast(far * a.c);
+            if (TWO) s1 += exp2_fast(far * LOG2E);
+        }
         const float low = __fsub_rn(st.base, st.top);
-        st.sum = st.rest * exp2_fast(low * a.c) + warp_sum(s);
+        st.sum = st.rest * exp2_fast(low * a.c) + warp_sum(s0);
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + warp_sum(s1) : st.sum;
-        of_listed = warp_sum(of_listed);
-        mass = warp_sum(mass);
         if (lane == 0) {
-            factors = distill_row(a, t, st, w, label);
-            if (a.loss && rank == 0) a.loss[n] = distill_loss(a, t, st, w, label, of_listed, mass, label >= 0 ? in(n, label) : 0.f);
+            factors = distill_row(a, side, st, w, label);
+            teacher = side;
+            student = st;
         }
     }
+    __syncthreads();
     if (a.gives != GIVES_LOSS) {
-        __syncthreads();
         DistillRow d = factors;
         T *out = static_cast<T *>(a.out.data) + n * a.out.row + lo;             // a.out.cls is 1
         float2 *pairs = static_cast<float2 *>(a.out.data) + n * a.out.row + lo;
@@ -1222,49 +1232,82 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
             const int k = part.single(tid);
             put(k, other_gh<TWO>(d, k, score_f32(part.p[k])));
         }
-        const bool aligned = reinterpret_cast<uintptr_t>(out + part.head) % 16 == 0;
-        fetch(0);
-        for (int from = 0; from < part.packs; from += WIDE_THREADS * WIDE_PACKS) {
-            uint4 w[WIDE_PACKS];
+        // f(scores, cell) for every pack of the thread: a loop of its own for each kind of result, with nothing to decide inside
+        auto sweep = [&](auto &&f) {
+            fetch(0);
+            for (int from = 0; from < part.packs; from += WIDE_THREADS * WIDE_PACKS) {
+                uint4 w[WIDE_PACKS];
 #pragma unroll
-            for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
-            fetch(from + WIDE_THREADS * WIDE_PACKS);
+                for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
+                fetch(from + WIDE_THREADS * WIDE_PACKS);
 #pragma unroll
-            for (int u = 0; u < WIDE_PACKS; ++u) {
-                const int at = from + u * WIDE_THREADS + tid;
-                if (at >= part.packs) break;
-                Pack<T> p;
-                p.bits = w[u];
-                float v[V];
-                p.unpack(v);
-                const int k = part.head + at * V;
-                if (a.gives == GIVES_PAIRS) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) pairs[k + i] = other_gh<TWO>(d, k + i, v[i]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float x = __fsub_rn(v[i], d.base), e = exp2_fast(x * d.c);
-                        v[i] = e * d.to_g;
-                        if (d.hard != 0.f) v[i] += d.hard * (TWO ? exp2_fast(x * LOG2E) * d.to_p1 : e * d.to_p);
-                    }
-                    if (aligned) {
-                        p.pack(v);
-                        __stcs(reinterpret_cast<uint4 *>(out + k), p.bits);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; ++i) out[k + i] = score_from<T>(v[i]);
-                    }
+                for (int u = 0; u < WIDE_PACKS; ++u) {
+                    const int at = from + u * WIDE_THREADS + tid;
+                    if (at >= part.packs) break;
+                    Pack<T> p;
+                    p.bits = w[u];
+                    float v[V];
+                    p.unpack(v);
+                    f(v, part.head + at * V);
                 }
             }
+        };
+        const float2 mb = make_float2(-d.base, -d.base), c2 = make_float2(d.c, d.c), to_g = make_float2(d.to_g, d.to_g);
+        auto gradients = [&](float(&v)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float2 g = mul2(exp_pair(make_float2(v[i], v[i + 1]), mb, c2), to_g);
+                v[i] = g.x; v[i + 1] = g.y;
+            }
+        };
+        auto store = [&](const float(&v)[V], int k) {
+            Pack<T> p;
+            p.pack(v);
+            __stcs(reinterpret_cast<uint4 *>(out + k), p.bits);
+        };
+        const bool aligned = reinterpret_cast<uintptr_t>(out + part.head) % 16 == 0;
+        if (a.gives == GIVES_PAIRS) {
+            sweep([&](float(&v)[V], int k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) pairs[k + i] = other_gh<TWO>(d, k + i, v[i]);
+            });
+        } else if (d.hard == 0.f && aligned) {
+            sweep([&](float(&v)[V], int k) {
+                gradients(v);
+                store(v, k);
+            });
+        } else if (aligned) {
+            sweep([&](float(&v)[V], int k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) v[i] = other_gh<TWO>(d, k + i, v[i]).x;
+                store(v, k);
+            });
+        } else {
+            sweep([&](float(&v)[V], int k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) out[k + i] = score_from<T>(other_gh<TWO>(d, k + i, v[i]).x);
+            });
         }
         __syncthreads();   // what follows is written over it
         d.label = label;
-        for (int e = tid; e < a.top; e += WIDE_THREADS) {
-            const int k = list_id[e] - lo;
-            if (list_id[e] >= lo && k < hi - lo) put(k, listed_gh<TWO>(d, list_id[e], in(n, list_id[e]), list_q[e]));
-        }
-        if (tid == WIDE_THREADS - 1 && label >= lo && label < hi && !listed(label - lo)) put(label - lo, other_gh<TWO>(d, label, in(n, label)));
+        if (warp >= WIDE_WARPS / 2)   // (the first warps have the loss to find)
+            for (int e = tid - WIDE_THREADS / 2; e < a.top; e += WIDE_THREADS / 2) {
+                const int k = list_id[e] - lo;
+                if (list_id[e] >= lo && k < hi - lo) put(k, listed_gh<TWO>(d, list_id[e], list_x[e], list_q[e]));
+            }
+        if (tid == WIDE_THREADS - 1 && label >= lo && label < hi && !listed(label - lo)) put(label - lo, other_gh<TWO>(d, label, label_score));
+    }
+    if (a.loss && rank == 0 && warp == 0) {
+        double of_listed = 0, mass = 0;
+        for (int e = lane; e < a.top; e += 32)
+            if (list_id[e] >= 0) {
+                const double q = (double)list_q[e];
+                if (q != 0) of_listed += q * (((double)list_x[e] - (double)student.top) * a.inv_t);
+                mass += q;
+            }
+        of_listed = warp_sum(of_listed);
+        mass = warp_sum(mass);
+        if (lane == 0) a.loss[n] = distill_loss(a, teacher, student, w, label, of_listed, mass, label_score);
     }
     if (C > 1) cluster.sync();   // (the others' shared memory is read until they are here)
 }

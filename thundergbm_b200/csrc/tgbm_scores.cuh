@@ -47,6 +47,23 @@ __device__ __forceinline__ float fine_exp(float x, float ref, float c, float c_l
     return fabsf(low) < 1.f ? __fmaf_rn(exp2f(y), low * 0.693147181f, exp2f(y)) : exp2f(y);   // (not for infinities)
 }
 
+// two floats in one instruction
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    unsigned long long r, x = *reinterpret_cast<unsigned long long *>(&a), y = *reinterpret_cast<unsigned long long *>(&b);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r, x = *reinterpret_cast<unsigned long long *>(&a), y = *reinterpret_cast<unsigned long long *>(&b);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return *reinterpret_cast<float2 *>(&r);
+}
+// exp((x - base) / T) of two scores; minus_base = (-base, -base), c2 = (c, c)
+__device__ __forceinline__ float2 exp_pair(float2 x, float2 minus_base, float2 c2) {
+    const float2 d = mul2(add2(x, minus_base), c2);
+    return make_float2(exp2_fast(d.x), exp2_fast(d.y));
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -85,30 +102,19 @@ struct TeacherSide {
     float total, rest;         // all mass (0: the row has no teacher), what is not listed
 };
 
-// One warp; entry e = lane + 32 s of the row's list.  list_id[e]: the class, -1 where it is none or stands further in front;
-// list_q[e]: its mass.
-// S: segments of 32 entries that the list may have.
-template <int S = SCORES_MAX_TOP / 32>
-__device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long long n, int *list_id, float *list_q) {
-    const int top = a.top, k = a.k;
+// One warp; entry e = lane + 32 s of the row's list: id[s] a class (-1: none) and t[s] its score become id[s] (-1 also where the class
+// stands further in front, if `repeats` are possible) and the mass q[s].
+template <int S>
+__device__ __forceinline__ TeacherSide teacher_of(const DistillArgs &a, const float *lse, int (&id)[S], const float (&t)[S], float (&mass_of)[S], bool repeats) {
+    const int lane = threadIdx.x & 31, top = a.top;
     const double inv_t = a.inv_t;
-    const int *ids = a.ids + n * a.ids_stride;
-    const float *lse = a.lse ? a.lse + n : nullptr;
-    const int lane = threadIdx.x & 31;
-    int id[S];
     double u[S], q[S], lq[S];
     float best = minus_inf();
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int e = lane + 32 * s;
-        id[s] = -1;
-        float t = minus_inf();
-        if (e < top) {
-            const int i = ids[e];
-            if (i >= 0 && i < k) { id[s] = i; t = teacher_logit(a, n, e); }
-        }
-        u[s] = (double)t * inv_t;
-        best = t != t ? t : best != best ? best : fmaxf(best, t);
+        const float v = id[s] >= 0 ? t[s] : minus_inf();
+        u[s] = (double)v * inv_t;
+        best = v != v ? v : best != best ? best : fmaxf(best, v);
     }
     const bool broken = __any_sync(0xffffffffu, best != best);
     best = warp_max(best);
@@ -131,6 +137,7 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
         if (s > 0 && 32 * s >= top) continue;
         lq[s] = u[s] - L;
         if (id[s] >= 0 && !none) q[s] = exp(lq[s]);
+        if (!repeats) continue;
         // an earlier entry of the same class takes this one's mass
         const unsigned same = __match_any_sync(0xffffffffu, id[s]);
         const int first = __ffs(same) - 1;
@@ -160,20 +167,42 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
     }
 #pragma unroll
     for (int s = 0; s < S; ++s) {
-        const int e = lane + 32 * s;
-        if (e < top) { list_id[e] = id[s]; list_q[e] = (float)q[s]; }
+        mass_of[s] = (float)q[s];
         mass += q[s];
         if (q[s] != 0) entropy += q[s] * lq[s];
         distinct += __popc(__ballot_sync(0xffffffffu, id[s] >= 0));
     }
     mass = warp_sum(mass);
     if (a.loss) entropy = warp_sum(entropy);
-    const double rest = lse && !none && distinct < k && mass < 1 ? 1.0 - mass : 0.0;
-    __syncwarp();
+    const double rest = lse && !none && distinct < a.k && mass < 1 ? 1.0 - mass : 0.0;
     TeacherSide r;
     r.total = none ? 0.f : (float)(mass + rest);
     r.rest = (float)rest;
     r.entropy = entropy;
+    return r;
+}
+
+// The same from the row's list in global memory.  list_id[e], list_q[e]: what becomes of entry e.  S: segments of 32 entries that the
+// list may have.
+template <int S = SCORES_MAX_TOP / 32>
+__device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long long n, int *list_id, float *list_q) {
+    const int lane = threadIdx.x & 31;
+    const int *ids = a.ids + n * a.ids_stride;
+    int id[S];
+    float t[S], q[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int e = lane + 32 * s, i = e < a.top ? ids[e] : -1;
+        id[s] = i >= 0 && i < a.k ? i : -1;
+        t[s] = e < a.top ? teacher_logit(a, n, e) : 0.f;
+    }
+    const TeacherSide r = teacher_of<S>(a, a.lse ? a.lse + n : nullptr, id, t, q, true);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+        const int e = lane + 32 * s;
+        if (e < a.top) { list_id[e] = id[s]; list_q[e] = q[s]; }
+    }
+    __syncwarp();
     return r;
 }
 
@@ -556,6 +585,26 @@ template <bool TWO> struct Running {
         const float d = __fsub_rn(x, base);
         s += exp2_fast(d * c);
         if (TWO) s1 += exp2_fast(d * LOG2E);
+    }
+    template <int V> __device__ __forceinline__ void add_pack(const float (&v)[V], float c) {
+        float largest = v[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) largest = fmaxf(largest, v[i]);
+        raise(largest, c);
+        const float base = -row_top(m);
+        const float2 mb = make_float2(base, base), c2 = make_float2(c, c), one = make_float2(LOG2E, LOG2E);
+        float2 sum = make_float2(0.f, 0.f), sum1 = sum;
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 d = add2(make_float2(v[i], v[i + 1]), mb), x = mul2(d, c2);
+            sum = add2(sum, make_float2(exp2_fast(x.x), exp2_fast(x.y)));
+            if (TWO) {
+                const float2 x1 = mul2(d, one);
+                sum1 = add2(sum1, make_float2(exp2_fast(x1.x), exp2_fast(x1.y)));
+            }
+        }
+        s += __fadd_rn(sum.x, sum.y);
+        if (TWO) s1 += __fadd_rn(sum1.x, sum1.y);
     }
     __device__ __forceinline__ void join(float om, float os, float os1, float c) {   // another one's
         const float to = fmaxf(m, om);
