@@ -268,12 +268,11 @@ __global__ void __launch_bounds__(FEW_THREADS) k_top_few(TopArgs a, Scores<T> in
         if (n < a.n) {
             float x[KP];
             float m = minus_inf(), s = 0;
-            unsigned left = 0;
+            const T *row = in.at(n, 0);
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-                x[i] = i < a.k ? in(n, i) : minus_inf();
+                x[i] = i < a.k ? score_f32(row[(long long)i * (int)in.cls]) : minus_inf();
                 m = fmaxf(m, x[i]);
-                if (x[i] > minus_inf()) left |= 1u << i;
             }
             const float top = row_top(m);
             if (a.lse) {
@@ -281,15 +280,38 @@ __global__ void __launch_bounds__(FEW_THREADS) k_top_few(TopArgs a, Scores<T> in
                 for (int i = 0; i < KP; ++i) s += exp2_fast(__fsub_rn(x[i], top) * a.c);
                 a.lse[n] = (float)((double)top * a.inv_t + (s == 0.f ? (double)minus_inf() : fine_log(s)));
             }
-            for (int j = 0; j < a.top; ++j) {
-                float v = minus_inf();
-                int id = -1;
+            float *values = found + tid * a.top;
+            int *ids = found_id + tid * a.top;
+            if (KP == 8) {   // every score counts those before it: 28 comparisons
+                int rank[KP];
+#pragma unroll
+                for (int i = 0; i < KP; ++i) { x[i] = fmaxf(x[i], minus_inf()); rank[i] = i; }
 #pragma unroll
                 for (int i = 0; i < KP; ++i)
-                    if ((left >> i & 1) && x[i] > v) { v = x[i]; id = i; }
-                if (id >= 0) left &= ~(1u << id);
-                found[tid * a.top + j] = __fadd_rn(v, 0.f);
-                found_id[tid * a.top + j] = id;
+#pragma unroll
+                    for (int j = i + 1; j < KP; ++j) {
+                        const int after = x[j] > x[i];
+                        rank[i] += after;
+                        rank[j] -= after;
+                    }
+#pragma unroll
+                for (int i = 0; i < KP; ++i)
+                    if (rank[i] < a.top) { values[rank[i]] = __fadd_rn(x[i], 0.f); ids[rank[i]] = x[i] > minus_inf() ? i : -1; }
+                for (int j = KP; j < a.top; ++j) { values[j] = minus_inf(); ids[j] = -1; }
+            } else {
+                unsigned left = 0;
+#pragma unroll
+                for (int i = 0; i < KP; ++i) left |= x[i] > minus_inf() ? 1u << i : 0u;
+                for (int j = 0; j < a.top; ++j) {
+                    float v = minus_inf();
+                    int id = -1;
+#pragma unroll
+                    for (int i = 0; i < KP; ++i)
+                        if ((left >> i & 1) && x[i] > v) { v = x[i]; id = i; }
+                    if (id >= 0) left &= ~(1u << id);
+                    values[j] = __fadd_rn(v, 0.f);
+                    ids[j] = id;
+                }
             }
         }
         __syncthreads();
@@ -883,125 +905,168 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
-// A thread per row where there are few classes: the row's scores stay in registers, what the teacher says of a class in a
-// column of shared memory (a class that is listed twice holds the sum).  Rows of a class are read side by side.
-
+// A thread per row where there are few classes: the row's scores and exponentials stay in registers, what the teacher says of a class
+// in a column of shared memory (a class that is listed twice holds the sum).  Rows of a class are read side by side.  Instructions
+// decide the time, some 500 per row of 7 classes: what is only needed for repeats, or for a rest, is branched around.
 template <typename T, int KP, bool TWO>
-__global__ void __launch_bounds__(FEW_THREADS) k_distill_few(DistillArgs a, Scores<T> in) {
+__global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k_distill_few(DistillArgs a, Scores<T> in) {
+    constexpr int ENTRIES = 4;   // entries of a list that stay in registers
+    constexpr bool KEEP = KP <= 16;   // ... and exponentials
     __shared__ float qs[KP][FEW_THREADS];
-    const int tid = threadIdx.x, K = a.k;
+    const int tid = threadIdx.x, K = a.k, in_cls = (int)in.cls, out_cls = (int)a.out.cls;
+    const float inv_t = (float)a.inv_t;
     float mg = 0, mh = 0;
     for (long long n = (long long)blockIdx.x * FEW_THREADS + tid; n < a.n; n += (long long)gridDim.x * FEW_THREADS) {
         float x[KP];
+        const T *row = in.at(n, 0);
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
-            x[i] = i < K ? in(n, i) : minus_inf();
+            x[i] = i < K ? score_f32(row[(long long)i * in_cls]) : minus_inf();
             qs[i][tid] = 0.f;
         }
-        const int *ids = a.ids + n * a.ids_stride;
         // the teacher
+        const int *ids = a.ids + n * a.ids_stride;
+        int id4[ENTRIES];
+        float t4[ENTRIES];
+#pragma unroll
+        for (int e = 0; e < ENTRIES; ++e) {
+            id4[e] = e < a.top ? ids[e] : -1;
+            t4[e] = e < a.top ? teacher_logit(a, n, e) : 0.f;
+        }
+        auto each_entry = [&](auto &&f) {   // f(class, score)
+#pragma unroll
+            for (int e = 0; e < ENTRIES; ++e)
+                if ((unsigned)id4[e] < (unsigned)K) f(id4[e], t4[e]);
+            for (int e = ENTRIES; e < a.top; ++e) {
+                const int id = ids[e];
+                if ((unsigned)id < (unsigned)K) f(id, teacher_logit(a, n, e));
+            }
+        };
         TeacherSide t;
-        unsigned listed = 0;
+        unsigned listed = 0, repeats = 0;
         float best = minus_inf();
         bool broken = false;
-        for (int e = 0; e < a.top; ++e) {
-            const int id = ids[e];
-            if (id < 0 || id >= K) continue;
-            const float l = teacher_logit(a, n, e);
+        each_entry([&](int id, float l) {
             broken |= l != l;
             best = fmaxf(best, l);
+            repeats |= listed & 1u << id;
             listed |= 1u << id;
-        }
+        });
         const bool none = best == minus_inf() && !broken;
-        double mass = 0;
+        double mass = 0, entropy = 0;
+        float q_scale = 1.f;   // q = qs * q_scale
+        t.rest = 0.f;
+        t.total = none ? 0.f : 1.f;
         if (none) {
             listed = 0;
-            t.total = t.rest = 0.f;
         } else if (a.lse) {
             const double L = (double)a.lse[n];
-            for (int e = 0; e < a.top; ++e) {
-                const int id = ids[e];
-                if (id < 0 || id >= K) continue;
-                const double q = exp((double)teacher_logit(a, n, e) * a.inv_t - L);
+            each_entry([&](int id, float l) {
+                const double lq = (double)l * a.inv_t - L, q = exp(lq);
                 mass += q;
+                if (q > 0) entropy += q * lq;
                 qs[id][tid] += (float)q;
-            }
+            });
             const double rest = __popc(listed) < K && mass < 1 ? 1.0 - mass : 0.0;
             t.rest = (float)rest;
             t.total = (float)(mass + rest);
         } else {
-            float sum = 0;
-            for (int e = 0; e < a.top; ++e) {
-                const int id = ids[e];
-                if (id >= 0 && id < K) sum += fine_exp(teacher_logit(a, n, e), best, a.c, a.c_low);
-            }
-            const float inv = 1.f / sum;
-            for (int e = 0; e < a.top; ++e) {
-                const int id = ids[e];
-                if (id >= 0 && id < K) qs[id][tid] += fine_exp(teacher_logit(a, n, e), best, a.c, a.c_low) * inv;
-            }
-            t.rest = 0.f;
-            t.total = 1.f;
+            float sum = 0, far = 0;
+            each_entry([&](int id, float l) {
+                const float e = fine_exp(l, best, a.c, a.c_low);
+                sum += e;
+                if (e > 0.f) far = __fmaf_rn(e, __fsub_rn(l, best) * inv_t, far);
+                qs[id][tid] += e;
+            });
+            q_scale = fast_inverse(sum);
             mass = 1;
+            if (a.loss) entropy = (double)(far * q_scale) - fine_log(sum);
+        }
+        if (repeats && a.loss && !none) {   // a class's share of the entropy is that of the sum
+            entropy = 0;
+            for (unsigned left = listed; left; left &= left - 1) {
+                const float q = qs[__ffs(left) - 1][tid] * q_scale;
+                if (q != 0.f) entropy += (double)q * log((double)q);
+            }
         }
         // the student: the listed classes apart where the rest is a class of its own
         const unsigned apart = t.rest > 0.f ? listed : 0u;
         StudentRow s;
         float m = minus_inf(), mt = minus_inf();
 #pragma unroll
-        for (int i = 0; i < KP; ++i) {
-            mt = fmaxf(mt, x[i]);
-            if (!(apart >> i & 1)) m = fmaxf(m, x[i]);
+        for (int i = 0; i < KP; ++i) mt = fmaxf(mt, x[i]);
+        m = mt;
+        if (apart) {
+            m = minus_inf();
+#pragma unroll
+            for (int i = 0; i < KP; ++i)
+                if (!(apart >> i & 1)) m = fmaxf(m, x[i]);
         }
         s.top = row_top(mt);
         s.base = row_top(m);
         s.rest = s.rest1 = 0.f;
-        float l = 0, l1 = 0;
+        float l = 0, l1 = 0, e[KEEP ? KP : 1], e1[KEEP && TWO ? KP : 1];
+        if (!apart) {
 #pragma unroll
-        for (int i = 0; i < KP; ++i)
-            if (!(apart >> i & 1)) {
-                const float d = __fsub_rn(x[i], s.base);
-                s.rest += exp2_fast(d * a.c);
-                if (TWO) s.rest1 += exp2_fast(d * LOG2E);
+            for (int i = 0; i < KP; ++i) {
+                const float d = __fsub_rn(x[i], s.base), v = exp2_fast(d * a.c), v1 = TWO ? exp2_fast(d * LOG2E) : 0.f;
+                s.rest += v;
+                if (TWO) s.rest1 += v1;
+                if (KEEP) e[i] = v;
+                if (KEEP && TWO) e1[i] = v1;
             }
-        if (apart) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < KP; ++i)
-                if (apart >> i & 1) {
-                    const float d = __fsub_rn(x[i], s.top);
-                    l += exp2_fast(d * a.c);
-                    if (TWO) l1 += exp2_fast(d * LOG2E);
-                }
+            for (int i = 0; i < KP; ++i) {   // (relative to the largest of its kind, as in StudentRow)
+                const bool of_rest = !(apart >> i & 1);
+                const float d = __fsub_rn(x[i], of_rest ? s.base : s.top), v = exp2_fast(d * a.c), v1 = TWO ? exp2_fast(d * LOG2E) : 0.f;
+                if (of_rest) { s.rest += v; s.rest1 += v1; } else { l += v; l1 += v1; }
+                if (KEEP) e[i] = v;
+                if (KEEP && TWO) e1[i] = v1;
+            }
         }
         const float low = __fsub_rn(s.base, s.top);
-        s.sum = s.rest * exp2_fast(low * a.c) + l;
-        s.sum1 = TWO ? s.rest1 * exp2_fast(low * LOG2E) + l1 : s.sum;
+        s.sum = apart ? s.rest * exp2_fast(low * a.c) + l : s.rest;
+        s.sum1 = !TWO ? s.sum : apart ? s.rest1 * exp2_fast(low * LOG2E) + l1 : s.rest1;
         const float w = a.weights ? a.weights[n] : 1.f;
         const int label = row_label(a, n);
         const DistillRow d = distill_row(a, t, s, w, label);
+        double of_listed = 0;
+        float label_score = 0;
         if (a.loss) {
-            double of_listed = 0, of_q = 0;
-            unsigned left = listed;
-            while (left) {
-                const int id = __ffs(left) - 1;
-                left &= left - 1;
-                const float q = qs[id][tid];
-                if (q == 0.f) continue;
-                of_q += (double)q * fine_log(q);
-                of_listed += (double)q * (((double)in(n, id) - (double)s.top) * a.inv_t);
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                if (i == label) label_score = x[i];
+                if (listed >> i & 1) {
+                    const float q = qs[i][tid] * q_scale;
+                    if (q != 0.f) of_listed += (double)(q * inv_t) * ((double)x[i] - (double)s.top);
+                }
             }
-            t.entropy = of_q;
-            a.loss[n] = distill_loss(a, t, s, w, label, of_listed, mass, label >= 0 ? in(n, label) : 0.f);
+            t.entropy = entropy;
+            a.loss[n] = distill_loss(a, t, s, w, label, of_listed, mass, label_score);
         }
         if (a.gives == GIVES_LOSS) continue;
+        const long long at = n * a.out.row;
+        float2 *pairs = static_cast<float2 *>(a.out.data) + at;
+        T *grads = static_cast<T *>(a.out.data) + at;
 #pragma unroll
         for (int i = 0; i < KP; ++i) {
             if (i >= K) break;
-            const float q = qs[i][tid];
-            const float2 gh = (apart >> i & 1) || apart == 0 ? listed_gh<TWO>(d, i, x[i], q) : other_gh<TWO>(d, i, x[i]);
-            const long long at = n * a.out.row + i * a.out.cls;
-            if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
-            else static_cast<T *>(a.out.data)[at] = score_from<T>(gh.x);
+            const bool as_listed = apart == 0 || (apart >> i & 1);   // (a class that is not listed has q = 0)
+            float v, v1 = 0.f;
+            if (KEEP) {
+                v = e[i];
+                if (TWO) v1 = e1[i];
+            } else {
+                const float far = __fsub_rn(x[i], as_listed ? s.top : s.base);
+                v = exp2_fast(far * a.c);
+                if (TWO) v1 = exp2_fast(far * LOG2E);
+            }
+            const float p = v * (as_listed ? d.inv_sum : d.to_p), p1 = TWO ? v1 * (as_listed ? d.inv_sum1 : d.to_p1) : p;
+            const float g = as_listed ? d.soft * __fmaf_rn(d.total, p, -(qs[i][tid] * q_scale)) : v * d.to_g;
+            const float2 gh = finish_gh(d, i, g, p, p1);
+            if (a.gives == GIVES_PAIRS) pairs[(long long)i * out_cls] = gh;
+            else grads[(long long)i * out_cls] = score_from<T>(gh.x);
             mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
         }
     }
@@ -1338,7 +1403,7 @@ void scores_adjust(const AdjustArgs &given, cudaStream_t stream) {
     if (given.n == 0) return;
     AdjustArgs a = given;
     a.inv_repetition = 1.f / a.repetition;
-    const bool by_class = a.in.row < a.in.cls && a.out.row < a.out.cls && std::max(a.in.cls, a.out.cls) <= INT_MAX / ADJUST_AHEAD;
+    const bool by_class = a.in.row < a.in.cls && a.out.row < a.out.cls && std::max(a.in.cls, a.out.cls) <= INT_MAX;
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
         constexpr int V = Pack<T>::V;
@@ -1400,7 +1465,7 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
     a.c = (float)(1.44269504088896341 * a.inv_t);
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
-        if (a.k <= FEW) {
+        if (a.k <= FEW && a.in.cls <= INT_MAX) {   // (an address is one instruction then)
             const int blocks = (int)std::min(((long long)a.n + FEW_THREADS - 1) / FEW_THREADS, (long long)FEW_BLOCKS);
             const size_t smem = (size_t)FEW_THREADS * a.top * 8;
             auto go = [&](auto kern) {
@@ -1445,7 +1510,7 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
     const bool two = a.alpha < 1.f && a.temperature != 1.f;
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
-        if (a.k <= FEW) {
+        if (a.k <= FEW && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
             const int blocks = (int)std::min(((long long)a.n + FEW_THREADS - 1) / FEW_THREADS, (long long)FEW_BLOCKS);
             auto go = [&](auto kern) { kern<<<blocks, FEW_THREADS, 0, stream>>>(a, scores_of<T>(a.in)); };
             if (a.k <= 8) two ? go(k_distill_few<T, 8, true>) : go(k_distill_few<T, 8, false>);

@@ -47,6 +47,13 @@ __device__ __forceinline__ float fine_exp(float x, float ref, float c, float c_l
     return fabsf(low) < 1.f ? __fmaf_rn(exp2f(y), low * 0.693147181f, exp2f(y)) : exp2f(y);   // (not for infinities)
 }
 
+// 1 / x to one step, for normal x
+__device__ __forceinline__ float fast_inverse(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // two floats in one instruction
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     unsigned long long r, x = *reinterpret_cast<unsigned long long *>(&a), y = *reinterpret_cast<unsigned long long *>(&b);
@@ -268,15 +275,15 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Te
     const float alpha = t.total == 0.f ? 0.f : a.alpha;
     const float low = __fsub_rn(s.base, s.top);
     d.base = s.base; d.top = s.top; d.c = c;
-    d.inv_sum = s.sum == 0.f ? 0.f : 1.f / s.sum;
-    d.inv_sum1 = s.sum1 == 0.f ? 0.f : 1.f / s.sum1;
+    d.inv_sum = s.sum == 0.f ? 0.f : fast_inverse(s.sum);
+    d.inv_sum1 = s.sum1 == 0.f ? 0.f : fast_inverse(s.sum1);
     d.to_p = exp2_fast(low * c) * d.inv_sum;
     d.to_p1 = exp2_fast(low * LOG2E) * d.inv_sum1;
     d.label = label;
     d.soft = w * alpha * a.temperature;
     d.hard = label >= 0 ? w * (1.f - a.alpha) : 0.f;
     d.total = t.total;
-    d.to_g = d.soft * (t.total * d.to_p - (t.rest > 0.f && s.rest != 0.f ? t.rest / s.rest : 0.f));
+    d.to_g = d.soft * (t.total * d.to_p - (t.rest > 0.f && s.rest != 0.f ? t.rest * fast_inverse(s.rest) : 0.f));
     d.curve = 2.f * w * alpha;
     return d;
 }
