@@ -864,18 +864,17 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
             if (list_id[j] >= 0) top = fmaxf(top, in(n, list_id[j]));
         st.top = row_top(warp_max(top));
         float l = 0, l1 = 0;
-        double ql = 0, mass = 0;
+        double ql = 0;
         for (int j = lane; j < a.top; j += 32)
             if (list_id[j] >= 0) {
                 const float z = in(n, list_id[j]), x = __fsub_rn(z, st.top);
                 l += exp2_fast(x * c);
                 if (TWO) l1 += exp2_fast(x * LOG2E);
                 if (list_q[j] != 0.f) ql += (double)list_q[j] * (((double)z - (double)st.top) * inv_t);
-                mass += list_q[j];
             }
         l = warp_sum(l); l1 = warp_sum(l1);
         if (!TWO) l1 = l;
-        ql = warp_sum(ql); mass = warp_sum(mass);
+        ql = warp_sum(ql);
         const float low = __fsub_rn(base, st.top);
         st.sum = s * exp2_fast(low * c) + l;
         st.sum1 = TWO ? s1 * exp2_fast(low * LOG2E) + l1 : st.sum;
@@ -884,7 +883,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
             const int label = row_label(a, n);
             student = st;
             drow = distill_row(a, teacher, st, w, label);
-            if (a.loss) a.loss[n] = distill_loss(a, teacher, st, w, label, ql, mass, label >= 0 ? in(n, label) : 0.f);
+            if (a.loss) a.loss[n] = distill_loss(a, teacher, st, w, label, ql, label >= 0 ? in(n, label) : 0.f);
         }
     }
     __syncthreads();
@@ -1043,7 +1042,8 @@ __global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k
                 }
             }
             t.entropy = entropy;
-            a.loss[n] = distill_loss(a, t, s, w, label, of_listed, mass, label_score);
+            t.mass = mass;
+            a.loss[n] = distill_loss(a, t, s, w, label, of_listed, label_score);
         }
         if (a.gives == GIVES_LOSS) continue;
         const long long at = n * a.out.row;
@@ -1074,13 +1074,15 @@ __global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k
 }
 
 // A tile as in k_top_tile: the teacher's lists are read while the scores are on their way, a warp sums up one row after the other, a
-// lane each finds the rows' losses and the factors of their gradients, and the gradients are written the way the scores were read.
+// lane each finds the rows' losses and the factors of their gradients, and the gradients of unlisted classes are written the way the
+// scores were read.  The cells of listed classes and labels, a few per row, are written over them: to tell them apart in that pass
+// took half of its instructions.
 template <int E, bool TWO, int S>
 __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(DistillArgs a, bool by_class, int rows_log) {
     extern __shared__ __align__(16) float tile[];
     const int R = 1 << rows_log, step = by_class ? R + 1 : 1;
     int *list_id = reinterpret_cast<int *>(tile + (size_t)a.k * (by_class ? R + 1 : R));
-    float *list_q = reinterpret_cast<float *>(list_id + R * a.top);
+    float *list_q = reinterpret_cast<float *>(list_id + R * a.top), *list_x = list_q + R * a.top;
     __shared__ RowSums sums[TILE_MOST_ROWS];
     __shared__ DistillRow factors[TILE_MOST_ROWS];
     const long long n0 = (long long)blockIdx.x << rows_log;
@@ -1093,7 +1095,8 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
     copies_done();
     __syncthreads();
     for (int r = warp; r < rows; r += TILE_WARPS)
-        warp_student<E, TWO, S>(a, n0 + r, by_class ? tile + r : tile + r * a.k, step, list_id + r * a.top, list_q + r * a.top, sums[r]);
+        warp_student<E, TWO, S>(a, n0 + r, by_class ? tile + r : tile + r * a.k, step, list_id + r * a.top, list_q + r * a.top,
+                                  list_x + r * a.top, sums[r]);
     __syncthreads();
     if (threadIdx.x < rows) {
         const RowSums &r = sums[threadIdx.x];
@@ -1102,45 +1105,66 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
         const float w = a.weights ? a.weights[n] : 1.f;
         const int label = row_label(a, n);
         if (a.gives != GIVES_LOSS) factors[threadIdx.x] = distill_row(a, r.teacher, s, w, label);
-        if (a.loss) a.loss[n] = distill_loss(a, r.teacher, s, w, label, r.of_listed, r.mass, r.label_score);
+        if (a.loss) a.loss[n] = distill_loss(a, r.teacher, s, w, label, r.of_listed, r.label_score);
     }
     if (a.gives == GIVES_LOSS) return;
     __syncthreads();
     float mg = 0, mh = 0;
+    const int cls = (int)a.out.cls;   // (the launch sees to it)
+    const bool track = a.maxbits != nullptr;
+    auto note = [&](float2 gh) {
+        if (track) { mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y); }
+        return gh;
+    };
     // cells from `first` on, `per` apart, of row r
     auto write = [&](int r, const float *z, int first, int per) {
-        const DistillRow d = factors[r];
-        const long long at = (n0 + r) * a.out.row + first * a.out.cls, cls = per * a.out.cls;
-        auto cell = [&](int c) {
-            const float x = z[c * step];
-            const int e = r * a.top + min(listed_entry(x), a.top - 1);
-            const float2 gh = is_listed_cell(x) ? listed_gh<TWO>(d, c, __int_as_float(list_id[e]), list_q[e]) : other_gh<TWO>(d, c, x);
-            mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y);
-            return gh;
-        };
+        DistillRow d = factors[r];
+        d.label = -1;
+        const long long at = (n0 + r) * a.out.row + (long long)first * cls, apart = (long long)per * cls;
+        const float *from = z + first * step;
+        const int cells = (a.k - first + per - 1) / per, next = per * step;
         if (a.gives == GIVES_PAIRS) {
             float2 *to = static_cast<float2 *>(a.out.data) + at;
 #pragma unroll 4
-            for (int c = first; c < a.k; c += per, to += cls) *to = cell(c);
+            for (int c = 0; c < cells; ++c, from += next, to += apart) *to = note(other_gh<TWO>(d, 0, *from));
         } else if (a.out.type == SCORE_F32) {
             float *to = static_cast<float *>(a.out.data) + at;
 #pragma unroll 4
-            for (int c = first; c < a.k; c += per, to += cls) *to = cell(c).x;
+            for (int c = 0; c < cells; ++c, from += next, to += apart) *to = note(other_gh<TWO>(d, 0, *from)).x;
         } else {
             const bool half = a.out.type == SCORE_F16;
             unsigned short *to = static_cast<unsigned short *>(a.out.data) + at;
 #pragma unroll 4
-            for (int c = first; c < a.k; c += per, to += cls) {
-                const float g = cell(c).x;
+            for (int c = 0; c < cells; ++c, from += next, to += apart) {
+                const float g = note(other_gh<TWO>(d, 0, *from)).x;
                 *to = half ? __half_as_ushort(__float2half_rn(g)) : __bfloat16_as_ushort(__float2bfloat16_rn(g));
             }
         }
     };
+    auto put = [&](int r, int c, float2 gh) {
+        note(gh);
+        const long long at = (n0 + r) * a.out.row + (long long)c * cls;
+        if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
+        else if (a.out.type == SCORE_F32) static_cast<float *>(a.out.data)[at] = gh.x;
+        else static_cast<unsigned short *>(a.out.data)[at] = a.out.type == SCORE_F16 ? __half_as_ushort(__float2half_rn(gh.x)) : __bfloat16_as_ushort(__float2bfloat16_rn(gh.x));
+    };
     if (by_class) {
-        const int r = threadIdx.x & (R - 1);
-        if (r < rows) write(r, tile + r, threadIdx.x >> rows_log, TILE_THREADS >> rows_log);
+        const int r = threadIdx.x & (R - 1), c = threadIdx.x >> rows_log;
+        if (r < rows && c < a.k) write(r, tile + r, c, TILE_THREADS >> rows_log);
     } else {
         for (int r = warp; r < rows; r += TILE_WARPS) write(r, tile + r * a.k, lane, 32);
+    }
+    __syncthreads();   // what follows is written over it
+    // an entry of a list each, then the labels that are not listed
+    for (int i = threadIdx.x; i < rows * a.top; i += TILE_THREADS) {
+        const int c = list_id[i], r = i / a.top;
+        if (c >= 0) put(r, c, listed_gh<TWO>(factors[r], c, list_x[i], list_q[i]));
+    }
+    if (threadIdx.x < rows && factors[threadIdx.x].label >= 0) {
+        const int r = threadIdx.x, c = factors[r].label;
+        int e = 0;
+        while (e < a.top && list_id[r * a.top + e] != c) ++e;
+        if (e == a.top) put(r, c, other_gh<TWO>(factors[r], c, by_class ? tile[c * step + r] : tile[r * a.k + c]));
     }
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
@@ -1363,16 +1387,11 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         if (tid == WIDE_THREADS - 1 && label >= lo && label < hi && !listed(label - lo)) put(label - lo, other_gh<TWO>(d, label, label_score));
     }
     if (a.loss && rank == 0 && warp == 0) {
-        double of_listed = 0, mass = 0;
+        double of_listed = 0;
         for (int e = lane; e < a.top; e += 32)
-            if (list_id[e] >= 0) {
-                const double q = (double)list_q[e];
-                if (q != 0) of_listed += q * (((double)list_x[e] - (double)student.top) * a.inv_t);
-                mass += q;
-            }
+            if (list_id[e] >= 0 && list_q[e] != 0.f) of_listed += (double)list_q[e] * (((double)list_x[e] - (double)student.top) * a.inv_t);
         of_listed = warp_sum(of_listed);
-        mass = warp_sum(mass);
-        if (lane == 0) a.loss[n] = distill_loss(a, teacher, student, w, label, of_listed, mass, label_score);
+        if (lane == 0) a.loss[n] = distill_loss(a, teacher, student, w, label, of_listed, label_score);
     }
     if (C > 1) cluster.sync();   // (the others' shared memory is read until they are here)
 }
@@ -1385,7 +1404,7 @@ constexpr int FEW_BLOCKS = 148 * 16;   // at most what the GPU holds at once; th
 // Rows of a tile, as a power of two from 8 to 32, and its shared memory; 0 bytes: the row is too long for a tile.  Several
 // blocks should fit on an SM, so that one copies while another computes; with few rows the tiles are smaller and there are
 // more of them.  (A row's result does not depend on the tile it is in.)
-constexpr size_t TILE_SHARED = 200 * 1024, TILE_WANTED = 40 * 1024;
+constexpr size_t TILE_SHARED = 190 * 1024, TILE_WANTED = 40 * 1024;
 struct Tile {
     int rows_log = 5;
     size_t shared = 0;
@@ -1483,12 +1502,13 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
             by_lane(a.k, [&](auto e) {
                 constexpr int E = decltype(e)::value;
                 auto go = [&](auto kern) {
-                    if (tile.shared > 30 * 1024) allow_shared(kern, TILE_SHARED);
+                    if (tile.shared > 12 * 1024) allow_shared(kern, TILE_SHARED);   // (beside up to 33 KB of its own)
                     kern<<<(int)(((long long)a.n + (1 << tile.rows_log) - 1) >> tile.rows_log), TILE_THREADS, tile.shared, stream>>>(a, by_class, tile.rows_log);
                 };
-                if (a.top <= 32) go(k_top_tile<E, 1>);
-                else if (a.top <= 64) go(k_top_tile<E, 2>);
-                else go(k_top_tile<E, 4>);
+                if (a.top <= 20) go(k_top_tile<E, 1>);
+                else if (a.top <= 40) go(k_top_tile<E, 2>);
+                else if (a.top <= 80) go(k_top_tile<E, 4>);
+                else go(k_top_tile<E, 8>);
             });
             return;
         }
@@ -1519,8 +1539,8 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
             return;
         }
         const bool by_class = a.in.row < a.in.cls;
-        const Tile tile = tile_of(a.n, a.k, by_class, 8 * (size_t)a.top);
-        if (tile.shared) {
+        const Tile tile = tile_of(a.n, a.k, by_class, 12 * (size_t)a.top);
+        if (tile.shared && (a.gives == GIVES_LOSS || a.out.cls <= INT_MAX)) {
             by_lane(a.k, [&](auto e) {
                 constexpr int E = decltype(e)::value;
                 auto go = [&](auto kern) {
