@@ -1084,19 +1084,43 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
     int *list_id = reinterpret_cast<int *>(tile + (size_t)a.k * (by_class ? R + 1 : R));
     float *list_q = reinterpret_cast<float *>(list_id + R * a.top), *list_x = list_q + R * a.top;
     __shared__ RowSums sums[TILE_MOST_ROWS];
+    __shared__ float lse[TILE_MOST_ROWS];
     __shared__ DistillRow factors[TILE_MOST_ROWS];
     const long long n0 = (long long)blockIdx.x << rows_log;
     const int rows = (int)min((long long)R, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     load_tile(tile, a.in, n0, by_class, rows, rows_log, a.k);
-    for (int r = warp; r < rows; r += TILE_WARPS) {
-        const TeacherSide t = read_teacher<S>(a, n0 + r, list_id + r * a.top, list_q + r * a.top);
-        if (lane == 0) sums[r].teacher = t;
-    }
+    // the lists of this warp's rows: classes to list_id, the teacher's scores to list_x for now
+    for (int r = warp; r < rows; r += TILE_WARPS)
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            if (e >= a.top) continue;
+            copy_async4(reinterpret_cast<float *>(list_id + r * a.top + e), reinterpret_cast<const float *>(a.ids + (n0 + r) * a.ids_stride + e));
+            if (a.logits_type == SCORE_F32) copy_async4(list_x + r * a.top + e, static_cast<const float *>(a.logits) + (n0 + r) * a.logits_stride + e);
+            else list_x[r * a.top + e] = teacher_logit(a, n0 + r, e);
+        }
+    if (threadIdx.x < rows) lse[threadIdx.x] = a.lse ? a.lse[n0 + threadIdx.x] : 0.f;
     copies_done();
     __syncthreads();
-    for (int r = warp; r < rows; r += TILE_WARPS)
-        warp_student<E, TWO, S>(a, n0 + r, by_class ? tile + r : tile + r * a.k, step, list_id + r * a.top, list_q + r * a.top,
-                                  list_x + r * a.top, sums[r]);
+    for (int r = warp; r < rows; r += TILE_WARPS) {
+        int id[S];
+        float t[S], q[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s, i = e < a.top ? list_id[r * a.top + e] : -1;
+            id[s] = i >= 0 && i < a.k ? i : -1;
+            t[s] = e < a.top ? list_x[r * a.top + e] : 0.f;
+        }
+        const TeacherSide side = teacher_of<S>(a, a.lse ? lse + r : nullptr, id, t, q, true);
+        if (lane == 0) sums[r].teacher = side;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            if (e < a.top) { list_id[r * a.top + e] = id[s]; list_q[r * a.top + e] = q[s]; }
+        }
+        __syncwarp();
+        warp_student<E, TWO, S>(a, n0 + r, by_class ? tile + r : tile + r * a.k, step, list_id + r * a.top, list_q + r * a.top, list_x + r * a.top, sums[r]);
+    }
     __syncthreads();
     if (threadIdx.x < rows) {
         const RowSums &r = sums[threadIdx.x];
