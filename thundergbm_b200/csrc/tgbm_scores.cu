@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) k_adjust_class(AdjustArgs a, S
 constexpr int LONG_CELLS = 4096;
 
 template <typename T>
-__global__ void __launch_bounds__(ROW_THREADS, 8) k_adjust_long(AdjustArgs a, Scores<T> in, Scores<T> out) {
+__global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 8 : 6) k_adjust_long(AdjustArgs a, Scores<T> in, Scores<T> out) {
     constexpr int V = Pack<T>::V;
     extern __shared__ __align__(16) int count[];
     const long long n = blockIdx.x;
@@ -378,8 +378,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : E == 16 ? 3 : 4) k
             float m = minus_inf(), s = 0;
             row.each([&](float x, int, int) { m = fmaxf(m, x); });
             m = row_top(warp_max(m));
-            row.each([&](float x, int, int) { s += exp2_fast(__fsub_rn(x, m) * a.c); });
-            s = warp_sum(s);
+            s = warp_sum(row.exps(m, a.c));
             if (lane == 0) { sums[r][0] = m; sums[r][1] = s; }
         }
         const long long n = n0 + r;
@@ -637,12 +636,12 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_top_wide(TopArgs 
             unsigned low, high;
             key_range(mine, ranges, low, high);
             low = max(low, (unsigned)(LOWEST_ENTRY >> 32));
-            raise_key(low, high, a.top, a.top + a.top / 8, WIDE_THREADS, [&](unsigned mid) { return __syncthreads_count(mine >= mid); });
+            raise_key(low, high, a.top, a.top + a.top / 4, WIDE_THREADS, [&](unsigned mid) { return __syncthreads_count(mine >= mid); });
             border = (Entry)low << 32;
             if (tid == 0) l.border = border;   // (read behind the next barrier)
-        } else if (turn == 1 || turn == 2 || turn == 4) {
+        } else if (turn == 3 || turn == 7) {   // (never: 123 us for 64 of 1024 x 131072; behind 1, 2, 4 and 8 steps: 101; like this: 98)
             __syncthreads();
-            raise_border(l, a.top, a.top + a.top / 8, false, ranges);
+            raise_border(l, a.top, a.top + a.top / 4, false, ranges);
             border = l.border;
         }
         if (border > LOWEST_ENTRY) border_score = key_score((unsigned)(border >> 32));
@@ -681,7 +680,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_top_wide(TopArgs 
         }
     }
     __syncthreads();
-    if (l.count > a.top + a.top / 2) raise_border(l, a.top, a.top + a.top / 2, true, ranges);
+    if (l.count > WIDE_LAST) raise_border(l, a.top, WIDE_LAST, true, ranges);
     narrow_to(l, a.top, WIDE_LAST);
     run.join_warp(a.c);
     if (lane == 0) { parts[warp][0] = run.m; parts[warp][1] = run.s; }
@@ -1180,8 +1179,9 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
     }
     __syncthreads();   // what follows is written over it
     // an entry of a list each, then the labels that are not listed
+    const float inv_top = 1.f / (float)a.top;
     for (int i = threadIdx.x; i < rows * a.top; i += TILE_THREADS) {
-        const int c = list_id[i], r = i / a.top;
+        const int c = list_id[i], r = (int)(((float)i + 0.5f) * inv_top);   // i / top: half a cell is far more than the product is off
         if (c >= 0) put(r, c, listed_gh<TWO>(factors[r], c, list_x[i], list_q[i]));
     }
     if (threadIdx.x < rows && factors[threadIdx.x].label >= 0) {

@@ -18,6 +18,7 @@ template <> __device__ __forceinline__ float score_from<float>(float v) { return
 template <> __device__ __forceinline__ __half score_from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 score_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+constexpr float LOG2E = 1.44269504088896341f;
 __device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
 
 // 2^x, one instruction; 0 for -inf, flushes results below 2^-126 (a class that far below the row's best adds nothing to a
@@ -238,7 +239,6 @@ struct DistillRow {
     int label;                // -1: none
 };
 
-constexpr float LOG2E = 1.44269504088896341f;
 constexpr float MIN_HESSIAN = 1e-16f;   // the softmax objective's
 
 __device__ __forceinline__ float2 finish_gh(const DistillRow &d, int i, float g, float p, float p1) {
@@ -323,6 +323,20 @@ template <int E> struct WarpRow {
             const int lane = threadIdx.x & 31;
 #pragma unroll
             for (int j = 0; j < E; ++j) x[j] = lane + 32 * j < k ? z[(lane + 32 * j) * step] : minus_inf();
+        }
+    }
+    // sum of exp((x - base) / T), c as in exp_pair
+    __device__ __forceinline__ float exps(float base, float c) const {
+        if constexpr (E > 0) {
+            const float2 mb = make_float2(-base, -base), c2 = make_float2(c, c);
+            float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < E; j += 2) s = add2(s, exp_pair(make_float2(x[j], x[j + 1]), mb, c2));
+            return __fadd_rn(s.x, s.y);
+        } else {
+            float s = 0;
+            each([&](float v, int, int) { s += exp2_fast(__fsub_rn(v, base) * c); });
+            return s;
         }
     }
     template <typename F> __device__ __forceinline__ void each(F &&f) const {
@@ -492,11 +506,8 @@ __device__ __forceinline__ void warp_student(const DistillArgs &a, long long n, 
         m = warp_max(m);
         base = row_top(m);
         top = row_top(fmaxf(warp_max(top), m));
-        row.each([&](float v, int, int) {
-            const float d = __fsub_rn(v, base);
-            s0 += exp2_fast(d * a.c);
-            if (TWO) s1 += exp2_fast(d * LOG2E);
-        });
+        s0 = row.exps(base, a.c);
+        if (TWO) s1 = row.exps(base, LOG2E);
     }
     __syncwarp();
     s0 = warp_sum(s0);
