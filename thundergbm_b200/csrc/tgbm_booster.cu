@@ -1192,7 +1192,7 @@ void BoosterImpl::gradient(int round) {
 DistillArgs BoosterImpl::distill_args() const {
     DistillArgs a;
     a.n = N; a.k = K; a.top = teacher.top;
-    a.in.data = ypred.p; a.in.row = 1; a.in.cls = N;
+    a.in.data = ypred.p; a.in.row = 1; a.in.cls = N; a.in.one_by_class = N == 1;
     a.ids = teacher.ids.p; a.ids_stride = teacher.top;
     a.logits = teacher.logits.p; a.logits_stride = teacher.top;
     a.lse = teacher.lse.p;

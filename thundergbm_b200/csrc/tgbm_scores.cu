@@ -1193,6 +1193,248 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
+// By class, up to 1024 classes: a lane per row and E neighbouring classes per warp, whose scores stay in registers from the first read to
+// the gradients.  Rows are read and written side by side, and nothing is reduced within a warp: the warps of a block exchange a maximum
+// and sums per row.  What the lists say is worked out by as many threads per row as there are warps.  (A warp per row from a tile in
+// shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them.)
+// The cells of listed classes and labels are written over what they get with the others.
+constexpr int CLASS_ROWS = 32;
+
+struct ListSums {   // of a row's list
+    TeacherSide teacher;
+    double of_listed;      // sum of q (s - top) / T
+    float top, l, l1;      // largest of the listed scores, sums of exponentials relative to it
+    int repeats;           // a class stands in it twice
+};
+
+template <typename T, int E, int W, bool TWO>
+__global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ? 2 : 1) k_distill_class(DistillArgs a, Scores<T> in) {
+    constexpr int THREADS = 32 * W;
+    extern __shared__ float lists[];
+    __shared__ unsigned bits[W][CLASS_ROWS];
+    __shared__ float part[3][W][CLASS_ROWS];
+    __shared__ ListSums of_list[CLASS_ROWS];
+    __shared__ DistillRow factors[CLASS_ROWS];
+    int *list_id = reinterpret_cast<int *>(lists);               // CLASS_ROWS x top: -1 for none
+    float *list_q = lists + CLASS_ROWS * a.top, *list_x = list_q + CLASS_ROWS * a.top;   // (first the teacher's scores, then masses)
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.k, in_cls = (int)in.cls, out_cls = (int)a.out.cls;
+    const long long n0 = (long long)blockIdx.x * CLASS_ROWS;
+    const int rows = (int)min((long long)CLASS_ROWS, a.n - n0), k0 = warp * E;
+    const long long n = n0 + min(lane, rows - 1);
+    float x[E];
+    {
+        const T *from = in.at(n, k0);
+        T raw[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (k0 + j < K) raw[j] = from[(long long)j * in_cls];
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = k0 + j < K ? score_f32(raw[j]) : minus_inf();
+    }
+    bits[warp][lane] = 0;
+    if (tid < CLASS_ROWS) of_list[tid].repeats = 0;
+    __syncthreads();
+    const float inv_top = 1.f / (float)a.top;
+    auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * inv_top); };   // i / top: half a cell is far more than the product is off
+    for (int i = tid; i < rows * a.top; i += THREADS) {
+        const int r = row_of(i), e = i - r * a.top;
+        int id = a.ids[(n0 + r) * a.ids_stride + e];
+        if (id < 0 || id >= K) id = -1;
+        list_id[i] = id;
+        list_q[i] = teacher_logit(a, n0 + r, e);
+        if (id >= 0) {
+            const unsigned bit = 1u << (id % E);
+            if (atomicOr(&bits[id / E][r], bit) & bit) of_list[r].repeats = 1;
+            list_x[i] = in(n0 + r, id);
+        }
+    }
+    __syncthreads();
+    {   // unlisted scores
+        const unsigned listed = bits[warp][lane];
+        float m = minus_inf();
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            if (listed >> j & 1) x[j] = minus_inf();
+            m = fmaxf(m, x[j]);
+        }
+        part[0][warp][lane] = m;
+    }
+    // the lists: W threads per row, each every W-th entry (all lanes of a warp, whether their row is there or not)
+    {
+        const int r = min(tid / W, rows - 1), first = tid % W, top = tid / W < rows ? a.top : 0;
+        int *id = list_id + r * a.top;
+        float *q = list_q + r * a.top;
+        const float *xs = list_x + r * a.top;
+        auto sum = [&](auto v) {
+#pragma unroll
+            for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            return v;
+        };
+        auto largest = [&](float v) {
+#pragma unroll
+            for (int o = W / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+            return v;
+        };
+        const bool repeats = of_list[r].repeats;
+        if (__any_sync(0xffffffffu, repeats)) {   // rare: of a class's entries only the first counts as a class, -2 - its number marks the others
+            if (repeats && first == 0)
+                for (int e = 1; e < top; ++e)
+                    for (int b = 0; b < e && id[e] >= 0; ++b)
+                        if (id[b] == id[e]) id[e] = -2 - b;
+            __syncwarp();
+        }
+        float best = minus_inf(), highest = minus_inf();
+        int distinct = 0, broken = 0;
+        for (int e = first; e < top; e += W)
+            if (id[e] != -1) {
+                best = fmaxf(best, q[e]);
+                broken |= q[e] != q[e];
+                highest = fmaxf(highest, xs[e]);
+                distinct += id[e] >= 0;
+            }
+        best = largest(best);
+        highest = largest(highest);
+        broken = sum(broken);
+        distinct = sum(distinct);
+        const float ref = row_top(highest);
+        const bool none = best == minus_inf() && !broken;
+        double L = 0;
+        if (a.lse) {
+            L = (double)a.lse[n0 + r];
+        } else {
+            double all = 0;
+            for (int e = first; e < top; e += W)
+                if (id[e] != -1) all += exp(((double)q[e] - (double)best) * a.inv_t);
+            L = (double)best * a.inv_t + log(sum(all));
+        }
+        double mass = 0, entropy = 0, of_listed = 0;
+        float l = 0, l1 = 0;
+        for (int e = first; e < top; e += W)
+            if (id[e] != -1) {
+                const double lq = (double)q[e] * a.inv_t - L, v = none ? 0.0 : exp(lq);
+                const float far = __fsub_rn(xs[e], ref);
+                mass += v;
+                if (v != 0) {
+                    entropy += v * lq;
+                    of_listed += v * (((double)xs[e] - (double)ref) * a.inv_t);
+                }
+                if (id[e] >= 0) {
+                    l += exp2_fast(far * a.c);
+                    if (TWO) l1 += exp2_fast(far * LOG2E);
+                }
+                q[e] = (float)v;
+            }
+        mass = sum(mass);
+        l = sum(l);
+        l1 = TWO ? sum(l1) : l;
+        if (a.loss) { entropy = sum(entropy); of_listed = sum(of_listed); }
+        if (__any_sync(0xffffffffu, repeats)) {
+            __syncwarp();
+            if (repeats && first == 0) {
+                for (int e = 1; e < top; ++e)
+                    if (id[e] <= -2) q[-2 - id[e]] += q[e];
+                entropy = 0;
+                for (int e = 0; e < top; ++e)
+                    if (id[e] >= 0 && q[e] != 0.f) entropy += (double)q[e] * log((double)q[e]);
+            }
+        }
+        const double rest = a.lse && !none && distinct < K && mass < 1 ? 1.0 - mass : 0.0;
+        if (first == 0 && tid / W < rows) {
+            ListSums &o = of_list[r];
+            o.teacher.mass = mass; o.teacher.entropy = entropy;
+            o.teacher.total = none ? 0.f : (float)(mass + rest);
+            o.teacher.rest = (float)rest;
+            o.of_listed = of_listed; o.top = highest; o.l = l; o.l1 = l1;
+        }
+    }
+    __syncthreads();
+    float base = part[0][0][lane];
+#pragma unroll
+    for (int w = 1; w < W; ++w) base = fmaxf(base, part[0][w][lane]);
+    const float largest_rest = base;
+    base = row_top(base);
+    {
+        const float2 mb = make_float2(-base, -base), c2 = make_float2(a.c, a.c), one = make_float2(LOG2E, LOG2E);
+        float2 s = make_float2(0.f, 0.f), s1 = s;
+#pragma unroll
+        for (int j = 0; j < E; j += 2) {
+            const float2 d = add2(make_float2(x[j], x[j + 1]), mb), v = mul2(d, c2);
+            s = add2(s, make_float2(exp2_fast(v.x), exp2_fast(v.y)));
+            if (TWO) {
+                const float2 v1 = mul2(d, one);
+                s1 = add2(s1, make_float2(exp2_fast(v1.x), exp2_fast(v1.y)));
+            }
+        }
+        part[1][warp][lane] = __fadd_rn(s.x, s.y);
+        if (TWO) part[2][warp][lane] = __fadd_rn(s1.x, s1.y);
+    }
+    __syncthreads();
+    if (warp == 0 && lane < rows) {
+        const ListSums &o = of_list[lane];
+        const int label = row_label(a, n);
+        const float w = a.weights ? a.weights[n] : 1.f;
+        StudentRow st;
+        st.base = base;
+        st.rest = st.rest1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            st.rest += part[1][i][lane];
+            if (TWO) st.rest1 += part[2][i][lane];
+        }
+        if (!TWO) st.rest1 = st.rest;
+        st.top = row_top(fmaxf(largest_rest, o.top));
+        if (st.rest == 0.f) st.base = st.top;
+        const float low = __fsub_rn(st.base, st.top), high = o.top == minus_inf() ? 0.f : __fsub_rn(o.top, st.top);
+        st.sum = st.rest * exp2_fast(low * a.c) + o.l * exp2_fast(high * a.c);
+        st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + o.l1 * exp2_fast(high * LOG2E) : st.sum;
+        factors[lane] = distill_row(a, o.teacher, st, w, label);
+        if (a.loss)
+            a.loss[n] = distill_loss(a, o.teacher, st, w, label, o.of_listed + (o.teacher.mass != 0 ? o.teacher.mass * ((double)high * a.inv_t) : 0.0),
+                                     label >= 0 ? in(n, label) : 0.f);
+    }
+    if (a.gives == GIVES_LOSS) return;
+    __syncthreads();
+    float mg = 0, mh = 0;
+    const bool track = a.maxbits != nullptr;
+    auto put = [&](int r, int c, float2 gh) {
+        if (track) { mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y); }
+        const long long at = (n0 + r) * a.out.row + (long long)c * out_cls;
+        if (a.gives == GIVES_PAIRS) static_cast<float2 *>(a.out.data)[at] = gh;
+        else static_cast<T *>(a.out.data)[at] = score_from<T>(gh.x);
+    };
+    if (lane < rows) {
+        DistillRow d = factors[lane];
+        d.label = -1;
+        if (a.gives == GIVES_PAIRS) {
+            float2 *to = static_cast<float2 *>(a.out.data) + n * a.out.row + (long long)k0 * out_cls;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (k0 + j >= K) break;
+                const float2 gh = other_gh<TWO>(d, 0, x[j]);
+                if (track) { mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y); }
+                to[(long long)j * out_cls] = gh;
+            }
+        } else {
+            T *to = static_cast<T *>(a.out.data) + n * a.out.row + (long long)k0 * out_cls;
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                if (k0 + j >= K) break;
+                to[(long long)j * out_cls] = score_from<T>(other_gh<TWO>(d, 0, x[j]).x);
+            }
+        }
+    }
+    __syncthreads();   // what follows is written over it: an entry of a list each, then the labels that are not listed
+    for (int i = tid; i < rows * a.top; i += THREADS) {
+        const int c = list_id[i], r = row_of(i);
+        if (c >= 0) put(r, c, listed_gh<TWO>(factors[r], c, list_x[i], list_q[i]));
+    }
+    if (tid < rows) {
+        const int c = factors[tid].label;
+        if (c >= 0 && !(bits[c / E][tid] >> (c % E) & 1)) put(tid, c, other_gh<TWO>(factors[tid], c, in(n, c)));
+    }
+    if (a.maxbits) track_max(mg, mh, a.maxbits);
+}
+
 // A long row, taken as in k_top_wide.  The first pass sums up the classes that the teacher does not list, which a bit map marks; the second
 // finds the row in the L2 cache (the launch sees to it that the rows at work fit there) and writes what unlisted classes get; the
 // few cells of listed classes and of the label are written over it.  (What lies between the passes is one warp's work: done by
@@ -1562,7 +1804,21 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
             else two ? go(k_distill_few<T, 32, true>) : go(k_distill_few<T, 32, false>);
             return;
         }
-        const bool by_class = a.in.row < a.in.cls;
+        const bool by_class = a.in.row < a.in.cls || a.in.one_by_class;
+        if (by_class && a.k <= 1024 && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
+            const size_t smem = 12 * (size_t)CLASS_ROWS * a.top;
+            const unsigned blocks = (unsigned)(((long long)a.n + CLASS_ROWS - 1) / CLASS_ROWS);
+            auto go = [&](auto kern, int warps) {
+                if (smem > 16 * 1024) allow_shared(kern, 12 * (size_t)CLASS_ROWS * SCORES_MAX_TOP);
+                kern<<<blocks, 32 * warps, smem, stream>>>(a, scores_of<T>(a.in));
+            };
+            if (a.k <= 64) two ? go(k_distill_class<T, 8, 8, true>, 8) : go(k_distill_class<T, 8, 8, false>, 8);
+            else if (a.k <= 128) two ? go(k_distill_class<T, 16, 8, true>, 8) : go(k_distill_class<T, 16, 8, false>, 8);
+            else if (a.k <= 256) two ? go(k_distill_class<T, 32, 8, true>, 8) : go(k_distill_class<T, 32, 8, false>, 8);
+            else if (a.k <= 512) two ? go(k_distill_class<T, 32, 16, true>, 16) : go(k_distill_class<T, 32, 16, false>, 16);
+            else two ? go(k_distill_class<T, 32, 32, true>, 32) : go(k_distill_class<T, 32, 32, false>, 32);
+            return;
+        }
         const Tile tile = tile_of(a.n, a.k, by_class, 12 * (size_t)a.top);
         if (tile.shared && (a.gives == GIVES_LOSS || a.out.cls <= INT_MAX)) {
             by_lane(a.k, [&](auto e) {
@@ -1606,6 +1862,7 @@ ScoreView view_of(const char *what, const void *data, int type, int n, int k, lo
     TGBM_CHECK(type >= SCORE_F32 && type <= SCORE_BF16, w + ": unknown type");
     TGBM_CHECK(data != nullptr, w + ": null pointer");
     TGBM_CHECK(reinterpret_cast<uintptr_t>(data) % size_of(type) == 0, w + ": not aligned for its type");
+    const bool one_by_class = n == 1 && row == cls;
     if (n == 1) row = k == 1 ? 1 : cls * k;   // a stride that no step takes
     if (k == 1) cls = row * n;
     TGBM_CHECK(row >= 0 && cls >= 0, w + ": negative stride");
@@ -1613,7 +1870,7 @@ ScoreView view_of(const char *what, const void *data, int type, int n, int k, lo
     TGBM_CHECK(row <= most / n && cls <= most / k, w + ": stride too large");
     if (written) TGBM_CHECK((row >= 1 && cls > (n - 1) * row) || (cls >= 1 && row > (k - 1) * cls), w + ": strides under which cells share memory");
     ScoreView v;
-    v.data = const_cast<void *>(data); v.type = type; v.row = row; v.cls = cls;
+    v.data = const_cast<void *>(data); v.type = type; v.row = row; v.cls = cls; v.one_by_class = one_by_class;
     return v;
 }
 
