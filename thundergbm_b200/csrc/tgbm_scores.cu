@@ -1196,7 +1196,8 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 // By class, up to 1024 classes: a lane per row and E neighbouring classes per warp, whose scores stay in registers from the first read to
 // the gradients.  Rows are read and written side by side, and nothing is reduced within a warp: the warps of a block exchange a maximum
 // and sums per row.  What the lists say is worked out by as many threads per row as there are warps.  (A warp per row from a tile in
-// shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them.)
+// shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them; these are 49, with
+// three blocks per SM instead of four 53, with five (and fewer registers) 68, with sixteen warps of half the classes each 59.)
 // The cells of listed classes and labels are written over what they get with the others.
 constexpr int CLASS_ROWS = 32;
 
@@ -1208,13 +1209,16 @@ struct ListSums {   // of a row's list
 };
 
 template <typename T, int E, int W, bool TWO>
-__global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ? 2 : 1) k_distill_class(DistillArgs a, Scores<T> in) {
+__global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distill_class(DistillArgs a, Scores<T> in) {
     constexpr int THREADS = 32 * W;
     extern __shared__ float lists[];
     __shared__ unsigned bits[W][CLASS_ROWS];
     __shared__ float part[3][W][CLASS_ROWS];
     __shared__ ListSums of_list[CLASS_ROWS];
     __shared__ DistillRow factors[CLASS_ROWS];
+    __shared__ StudentRow students[CLASS_ROWS];
+    __shared__ int labels[CLASS_ROWS];
+    __shared__ float lse[CLASS_ROWS], weights[CLASS_ROWS], label_scores[CLASS_ROWS];
     int *list_id = reinterpret_cast<int *>(lists);               // CLASS_ROWS x top: -1 for none
     float *list_q = lists + CLASS_ROWS * a.top, *list_x = list_q + CLASS_ROWS * a.top;   // (first the teacher's scores, then masses)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, K = a.k, in_cls = (int)in.cls, out_cls = (int)a.out.cls;
@@ -1232,7 +1236,14 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ?
         for (int j = 0; j < E; ++j) x[j] = k0 + j < K ? score_f32(raw[j]) : minus_inf();
     }
     bits[warp][lane] = 0;
-    if (tid < CLASS_ROWS) of_list[tid].repeats = 0;
+    if (tid >= THREADS - CLASS_ROWS) {   // (what the rows give besides, read while the scores are on their way)
+        const int label = row_label(a, n);
+        of_list[lane].repeats = 0;
+        labels[lane] = label;
+        lse[lane] = a.lse ? a.lse[n] : 0.f;
+        weights[lane] = a.weights ? a.weights[n] : 1.f;
+        label_scores[lane] = label >= 0 ? in(n, label) : 0.f;
+    }
     __syncthreads();
     const float inv_top = 1.f / (float)a.top;
     auto row_of = [&](int i) { return (int)(((float)i + 0.5f) * inv_top); };   // i / top: half a cell is far more than the product is off
@@ -1300,7 +1311,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ?
         const bool none = best == minus_inf() && !broken;
         double L = 0;
         if (a.lse) {
-            L = (double)a.lse[n0 + r];
+            L = (double)lse[r];
         } else {
             double all = 0;
             for (int e = first; e < top; e += W)
@@ -1369,10 +1380,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ?
         if (TWO) part[2][warp][lane] = __fadd_rn(s1.x, s1.y);
     }
     __syncthreads();
-    if (warp == 0 && lane < rows) {
-        const ListSums &o = of_list[lane];
-        const int label = row_label(a, n);
-        const float w = a.weights ? a.weights[n] : 1.f;
+    if (warp == 0) {
+        const ListSums &o = of_list[min(lane, rows - 1)];
         StudentRow st;
         st.base = base;
         st.rest = st.rest1 = 0.f;
@@ -1387,13 +1396,17 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ?
         const float low = __fsub_rn(st.base, st.top), high = o.top == minus_inf() ? 0.f : __fsub_rn(o.top, st.top);
         st.sum = st.rest * exp2_fast(low * a.c) + o.l * exp2_fast(high * a.c);
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + o.l1 * exp2_fast(high * LOG2E) : st.sum;
-        factors[lane] = distill_row(a, o.teacher, st, w, label);
-        if (a.loss)
-            a.loss[n] = distill_loss(a, o.teacher, st, w, label, o.of_listed + (o.teacher.mass != 0 ? o.teacher.mass * ((double)high * a.inv_t) : 0.0),
-                                     label >= 0 ? in(n, label) : 0.f);
+        factors[lane] = distill_row(a, o.teacher, st, weights[lane], labels[lane]);
+        students[lane] = st;
+    }
+    __syncthreads();
+    if (a.loss && warp == W - 1 && lane < rows) {   // (the others go on)
+        const ListSums &o = of_list[lane];
+        const float high = o.top == minus_inf() ? 0.f : __fsub_rn(o.top, students[lane].top);
+        a.loss[n] = distill_loss(a, o.teacher, students[lane], weights[lane], labels[lane],
+                                 o.of_listed + (o.teacher.mass != 0 ? o.teacher.mass * ((double)high * a.inv_t) : 0.0), label_scores[lane]);
     }
     if (a.gives == GIVES_LOSS) return;
-    __syncthreads();
     float mg = 0, mh = 0;
     const bool track = a.maxbits != nullptr;
     auto put = [&](int r, int c, float2 gh) {
@@ -1429,8 +1442,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? (E == 32 ? 3 : 4) : W == 16 ?
         if (c >= 0) put(r, c, listed_gh<TWO>(factors[r], c, list_x[i], list_q[i]));
     }
     if (tid < rows) {
-        const int c = factors[tid].label;
-        if (c >= 0 && !(bits[c / E][tid] >> (c % E) & 1)) put(tid, c, other_gh<TWO>(factors[tid], c, in(n, c)));
+        const int c = labels[tid];
+        if (c >= 0 && !(bits[c / E][tid] >> (c % E) & 1)) put(tid, c, other_gh<TWO>(factors[tid], c, label_scores[tid]));
     }
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
