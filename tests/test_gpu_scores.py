@@ -433,3 +433,19 @@ def test_refusals(ops):
     wide = torch.randn(8, 80, device='cuda')
     want = wide[:, :40] + 1
     assert torch.equal(scores.adjust(wide[:, :40], out=wide[:, 40:], bias=torch.ones(40, device='cuda')), want)
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 6, 6), ('class', 6, 90), ('row', 6, 6), ('row', 6, 400), ('row', 6, 9001), ('any', 6, 50), ('class', 6, 5000), ('class', 6, 9001)])
+def test_distill_where_all_that_is_left_is_far_below_zero(ops, layout, n, k):
+    """Nothing but a few listed scores is above -inf, and they lie hundreds below 0 (or above): shares are those of the same scores moved
+    to 0."""
+    r = np.random.default_rng(k)
+    z = _make(r, n, k)
+    ids, logits, lse = _teacher(r, z, 4, 1.0)
+    for i, by in enumerate((-300, -90, 300, -3000, 0)):
+        z[i] = np.where(np.isin(np.arange(k), ids[i]), z[i] + by, -np.inf)
+    t = _tensor(ops[0], z.astype(np.float32), 'f32', layout)
+    labels = ids[:, 1].copy()
+    for T in (1.0, 1.5):
+        for use_lse in (True, False):
+            _check_distill(ops, t, 'f32', ids, logits, 'f32', lse if use_lse else None, labels, None, T, 0.5, (T, use_lse))

@@ -862,6 +862,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
         for (int j = lane; j < a.top; j += 32)
             if (list_id[j] >= 0) top = fmaxf(top, in(n, list_id[j]));
         st.top = row_top(warp_max(top));
+        st.base = reference_of(st.base, st.rest, st.top);
         float l = 0, l1 = 0;
         double ql = 0;
         for (int j = lane; j < a.top; j += 32)
@@ -874,7 +875,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
         l = warp_sum(l); l1 = warp_sum(l1);
         if (!TWO) l1 = l;
         ql = warp_sum(ql);
-        const float low = __fsub_rn(base, st.top);
+        const float low = __fsub_rn(st.base, st.top);
         st.sum = s * exp2_fast(low * c) + l;
         st.sum1 = TWO ? s1 * exp2_fast(low * LOG2E) + l1 : st.sum;
         if (lane == 0) {
@@ -1023,6 +1024,7 @@ __global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k
                 if (KEEP && TWO) e1[i] = v1;
             }
         }
+        s.base = reference_of(s.base, s.rest, s.top);
         const float low = __fsub_rn(s.base, s.top);
         s.sum = apart ? s.rest * exp2_fast(low * a.c) + l : s.rest;
         s.sum1 = !TWO ? s.sum : apart ? s.rest1 * exp2_fast(low * LOG2E) + l1 : s.rest1;
@@ -1392,7 +1394,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
         }
         if (!TWO) st.rest1 = st.rest;
         st.top = row_top(fmaxf(largest_rest, o.top));
-        if (st.rest == 0.f) st.base = st.top;
+        st.base = reference_of(st.base, st.rest, st.top);
         const float low = __fsub_rn(st.base, st.top), high = o.top == minus_inf() ? 0.f : __fsub_rn(o.top, st.top);
         st.sum = st.rest * exp2_fast(low * a.c) + o.l * exp2_fast(high * a.c);
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + o.l1 * exp2_fast(high * LOG2E) : st.sum;
@@ -1567,6 +1569,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         StudentRow st;
         st.base = row_top(run.m); st.rest = run.s; st.rest1 = TWO ? run.s1 : run.s;
         st.top = row_top(warp_max(top));
+        st.base = reference_of(st.base, st.rest, st.top);
         float s0 = 0, s1 = 0;
 #pragma unroll
         for (int s = 0; s < S; ++s) {

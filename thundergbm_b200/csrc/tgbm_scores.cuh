@@ -219,11 +219,14 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
 // Scores are taken relative to the largest of their kind, so a sum of exponentials holds a 1 and does not overflow.  "Rest"
 // are the classes summed in the pass over the row -- those that the teacher does not list, or (no bucket for them is needed) all --
 // and `top`, `sum`, `sum1` are those of all classes.  The rest has a reference of its own: a student far from all of it still
-// gets the gradient that says which of them to raise.  Without a score above -inf a reference is 0 and its sums are 0.
+// gets the gradient that says which of them to raise.  Without a score above -inf in the whole row references are 0.
 struct StudentRow {
     float base, rest, rest1;   // largest of the rest; sums of exp((s - base) / T) and exp(s - base)
     float top, sum, sum1;      // the same of all classes
 };
+// Without a score above -inf the rest has the reference of all classes: its sums are 0 there as anywhere, and what brings them from
+// one reference to the other is 1, not infinite.
+__device__ __forceinline__ float reference_of(float base, float rest, float top) { return rest == 0.f ? top : base; }
 __device__ __forceinline__ float row_top(float largest) { return largest == minus_inf() ? 0.f : largest; }
 
 // Factors of a row's gradients.  For class i with shares p (at T) and p1 (at 1):
@@ -466,8 +469,9 @@ struct RowSums {
 };
 __device__ __forceinline__ StudentRow student_of(const DistillArgs &a, const RowSums &r) {
     StudentRow s;
-    s.base = r.base; s.rest = r.rest; s.rest1 = r.rest1; s.top = r.top;
-    const float low = __fsub_rn(r.base, r.top);
+    s.rest = r.rest; s.rest1 = r.rest1; s.top = r.top;
+    s.base = reference_of(r.base, r.rest, r.top);
+    const float low = __fsub_rn(s.base, r.top);
     s.sum = r.rest * exp2_fast(low * a.c) + r.l;
     s.sum1 = r.rest1 * exp2_fast(low * LOG2E) + r.l1;
     return s;
