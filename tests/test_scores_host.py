@@ -42,6 +42,8 @@ NAN, INF = float('nan'), float('inf')
     (_distill, dict(ids=None), 'null'), (_distill, dict(logits=None), 'null'), (_distill, dict(ids_stride=-1), 'negative'), (_distill, dict(gives=0, loss=None), 'loss'),
     (_distill, dict(g=None), 'null'), (_distill, dict(gives=2, g=P + 65540), 'aligned'), (_distill, dict(g=P), 'share'), (_distill, dict(grs=1, gcs=1), 'share'),
     (_distill, dict(gives=2, g=P + 8), 'share'),
+    (_adjust, dict(bias=P + 2), 'aligned'), (_adjust, dict(ptr=P + 4, ids=P, given=5), 'aligned'), (_top, dict(v=P + 1), 'aligned'), (_distill, dict(ids=P + 2), 'aligned'),
+    (_distill, dict(lt=0, logits=P + 2), 'aligned'), (_distill, dict(loss=P + 3), 'aligned'),
 ])
 def test_refused(lib, call, args, says):
     assert call(lib, **args) == 1

@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 8 : 6) k_adjust_
 #pragma unroll
     for (int u = 0; u < U; ++u) {   // all of them on their way while the history is counted
         const int c = (u * ROW_THREADS + threadIdx.x) * V;
-        if (c + V <= classes) ahead[u].bits = __ldg(reinterpret_cast<const uint4 *>(src + c));
+        if (c + V <= classes) ahead[u].bits = *reinterpret_cast<const uint4 *>(src + c);   // (may be the memory that is written)
     }
     const unsigned *mask = mask_of(a, n);
     if (a.history_ptr) count_histories<1>(a, n, 1, k0, classes, count, classes, [](int, int c) { return c; });
@@ -1906,6 +1906,9 @@ bool share_memory(const ScoreView &a, int a_size, const ScoreView &b, int b_size
     return (in < width && over < lines) || (line - in < width && over + 1 < lines);
 }
 
+void check_pointer(const char *what, const void *p, size_t size) {
+    TGBM_CHECK(reinterpret_cast<uintptr_t>(p) % size == 0, std::string(what) + ": not aligned for its type");
+}
 void check_shape(int n, int k) {
     TGBM_CHECK(n >= 0, "negative number of rows");
     TGBM_CHECK(k >= 1 && k <= TGBM_SCORES_MAX_CLASSES, "number of classes outside [1, " + std::to_string(TGBM_SCORES_MAX_CLASSES) + "]");
@@ -1947,6 +1950,8 @@ int tgbm_scores_adjust(int n_rows, int n_classes, int type, const void *d_scores
         a.out = view_of("out", d_out, type, n_rows, n_classes, out_row_stride, out_class_stride, true);
         const bool in_place = a.in.data == a.out.data && a.in.row == a.out.row && a.in.cls == a.out.cls;
         TGBM_CHECK(in_place || !share_memory(a.in, size_of(type), a.out, size_of(type), n_rows, n_classes), "scores and out share memory but are not the same");
+        check_pointer("bias", d_bias, 4); check_pointer("masks", d_allowed, 4); check_pointer("rows' masks", d_allowed_row, 4);
+        check_pointer("history", d_history_ptr, 8); check_pointer("history", d_history, 4);
         a.bias = d_bias;
         if (d_allowed) {
             TGBM_CHECK(d_allowed_row || n_masks >= n_rows, "fewer masks than rows, and none named for each row");
@@ -1972,6 +1977,7 @@ int tgbm_scores_top(int n_rows, int n_classes, int type, const void *d_scores, l
         a.n = n_rows; a.k = n_classes; a.top = top; a.temperature = temperature;
         a.in = view_of("scores", d_scores, type, n_rows, n_classes, row_stride, class_stride, false);
         TGBM_CHECK(d_values && d_ids, "values or ids: null pointer");
+        check_pointer("values", d_values, 4); check_pointer("ids", d_ids, 4); check_pointer("lse", d_lse, 4);
         a.values = d_values; a.ids = d_ids; a.lse = d_lse;
         scores_top(a, static_cast<cudaStream_t>(cuda_stream));
     });
@@ -1994,6 +2000,8 @@ int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_score
         a.n = n_rows; a.k = n_classes; a.top = top;
         a.in = view_of("scores", d_scores, type, n_rows, n_classes, row_stride, class_stride, false);
         TGBM_CHECK(d_ids && d_logits, "ids or logits: null pointer");
+        check_pointer("ids", d_ids, 4); check_pointer("logits", d_logits, size_of(logits_type)); check_pointer("lse", d_lse, 4);
+        check_pointer("labels", d_labels, 4); check_pointer("weights", d_weights, 4); check_pointer("loss", d_loss, 4);
         a.ids = d_ids; a.ids_stride = ids_stride; a.logits = d_logits; a.logits_type = logits_type; a.logits_stride = logits_stride;
         a.lse = d_lse; a.labels = d_labels; a.weights = d_weights;
         a.temperature = temperature; a.alpha = alpha; a.gives = gives; a.loss = d_loss;
