@@ -155,19 +155,20 @@ __global__ void __launch_bounds__(ROW_THREADS, 4) k_adjust_class(AdjustArgs a, S
     }
 }
 
-// By row, long rows whose scores start on 16-byte boundaries: a block takes LONG_CELLS classes of a row, a thread 16 bytes at a
-// time.
+// By row, long rows: a block takes LONG_CELLS classes of a row, a thread 16 bytes at a time.  The pieces begin at the row's first 16-byte
+// boundary; up to V - 1 cells in front of it go with the first piece, one by one.  EVEN: every row begins at one (256 x 131072 in 16 bits
+// 49 us so, 54 without saying so; 256 x 131071 68 us).
 constexpr int LONG_CELLS = 4096;
 
-template <typename T>
+template <typename T, bool EVEN>
 __global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 8 : 6) k_adjust_long(AdjustArgs a, Scores<T> in, Scores<T> out) {
-    constexpr int V = Pack<T>::V;
-    extern __shared__ __align__(16) int count[];
+    constexpr int V = Pack<T>::V, U = LONG_CELLS / (ROW_THREADS * V);
+    extern __shared__ __align__(16) int count[];   // LONG_CELLS, then V for the cells in front
     const long long n = blockIdx.x;
-    const int k0 = blockIdx.y * LONG_CELLS, classes = min(LONG_CELLS, a.k - k0);
+    const int head = EVEN ? 0 : min(a.k, (int)((16 - reinterpret_cast<uintptr_t>(in.at(n, 0)) % 16) % 16 / sizeof(T)));
+    const int k0 = head + blockIdx.y * LONG_CELLS, classes = max(0, min(LONG_CELLS, a.k - k0)), front = !EVEN && blockIdx.y == 0 ? head : 0;
     const T *src = in.at(n, k0);
     T *dst = out.at(n, k0);
-    constexpr int U = LONG_CELLS / (ROW_THREADS * V);
     Pack<T> ahead[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {   // all of them on their way while the history is counted
@@ -175,23 +176,33 @@ __global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 8 : 6) k_adjust_
         if (c + V <= classes) ahead[u].bits = *reinterpret_cast<const uint4 *>(src + c);   // (may be the memory that is written)
     }
     const unsigned *mask = mask_of(a, n);
-    if (a.history_ptr) count_histories<1>(a, n, 1, k0, classes, count, classes, [](int, int c) { return c; });
+    if (a.history_ptr)
+        count_histories<1>(a, n, 1, k0 - front, classes + front, count, EVEN ? classes : LONG_CELLS + V,
+                           [&](int, int c) { return EVEN ? c : c < front ? LONG_CELLS + c : c - front; });
+    // one cell at a time: in front of the first boundary (c < 0), behind the last
+    auto single = [&](int c, int times) {
+        const int k = k0 + c;
+        float z = score_f32(src[c]);
+        if (times) z = penalised(a, z, times);
+        if (a.bias) z += a.bias[k];
+        if (mask && !(mask[k >> 5] >> (k & 31) & 1)) z = minus_inf();
+        dst[c] = score_from<T>(z);
+    };
+    if (!EVEN && (int)threadIdx.x < front) single((int)threadIdx.x - head, a.history_ptr ? count[LONG_CELLS + threadIdx.x] : 0);
+    const bool even_bias = (reinterpret_cast<uintptr_t>(a.bias + k0) & 15) == 0;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int c = (u * ROW_THREADS + threadIdx.x) * V;
         if (c >= classes) break;
+        if (c + V > classes) {   // the row's last few
+            for (int i = c; i < classes; ++i) single(i, a.history_ptr ? count[i] : 0);
+            break;
+        }
         const int k = k0 + c;
         float z[V];
-        Pack<T> p;
-        const bool whole = c + V <= classes;   // else the row's last few
-        if (whole) {
-            p = ahead[u];
-            p.unpack(z);
-        } else {
-            for (int i = 0; i < V; ++i) z[i] = c + i < classes ? score_f32(src[c + i]) : 0.f;
-        }
+        ahead[u].unpack(z);
         if (a.history_ptr) {
-            int times[V], any = 0;   // (V * 4 bytes of counts; what lies behind the last class is 0 or not used)
+            int times[V], any = 0;
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
                 const int4 m = *reinterpret_cast<const int4 *>(count + c + i);
@@ -205,30 +216,26 @@ __global__ void __launch_bounds__(ROW_THREADS, sizeof(T) == 2 ? 8 : 6) k_adjust_
             }
         }
         if (a.bias) {
-            if (whole && (reinterpret_cast<uintptr_t>(a.bias) & 15) == 0) {
+            if (even_bias) {
 #pragma unroll
                 for (int i = 0; i < V; i += 4) {
                     const float4 b = __ldg(reinterpret_cast<const float4 *>(a.bias + k + i));
                     z[i] += b.x; z[i + 1] += b.y; z[i + 2] += b.z; z[i + 3] += b.w;
                 }
             } else {
-                for (int i = 0; i < V; ++i)
-                    if (c + i < classes) z[i] += a.bias[k + i];
+#pragma unroll
+                for (int i = 0; i < V; ++i) z[i] += __ldg(a.bias + k + i);
             }
         }
-        if (mask) {
-            const unsigned word = mask[k >> 5] >> (k & 31);   // (k is a multiple of V, and V divides 32)
+        if (mask) {   // V bits, of two words where they do not lie in one
+            const unsigned word = EVEN ? mask[k >> 5] >> (k & 31) : __funnelshift_r(mask[k >> 5], mask[(k + V - 1) >> 5], k & 31);
 #pragma unroll
             for (int i = 0; i < V; ++i)
                 if (!(word >> i & 1)) z[i] = minus_inf();
         }
-        if (whole) {
-            p.pack(z);
-            *reinterpret_cast<uint4 *>(dst + c) = p.bits;
-        } else {
-            for (int i = 0; i < V; ++i)
-                if (c + i < classes) dst[c + i] = score_from<T>(z[i]);
-        }
+        Pack<T> p;
+        p.pack(z);
+        *reinterpret_cast<uint4 *>(dst + c) = p.bits;
     }
 }
 
@@ -241,6 +248,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_adjust_tile(AdjustArgs a, Score
     const int k0 = blockIdx.y * tile_classes;
     const int rows = (int)min((long long)tile_rows, a.n - n0), classes = min(tile_classes, a.k - k0);
     if (a.history_ptr) count_histories<ADJUST_MOST_ROWS>(a, n0, rows, k0, classes, count, tile_rows * tile_classes, [&](int r, int c) { return r * tile_classes + c; });
+    const unsigned *first_mask = mask_of(a, n0);
 #pragma unroll 4
     for (int i = threadIdx.x; i < rows * tile_classes; i += ROW_THREADS) {
         const int r = (int)__umulhi((unsigned)i, inverse), c = i - r * tile_classes;
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_adjust_tile(AdjustArgs a, Score
         float z = in(n, k);
         if (a.history_ptr && count[i]) z = penalised(a, z, count[i]);
         if (a.bias) z += a.bias[k];
-        const unsigned *mask = mask_of(a, n);
+        const unsigned *mask = tile_rows == 1 ? first_mask : mask_of(a, n);
         if (mask && !(mask[k >> 5] >> (k & 31) & 1)) z = minus_inf();
         *out.at(n, k) = score_from<T>(z);
     }
@@ -298,17 +306,24 @@ __global__ void __launch_bounds__(FEW_THREADS) k_top_few(TopArgs a, Scores<T> in
                 for (int i = 0; i < KP; ++i)
                     if (rank[i] < a.top) { values[rank[i]] = __fadd_rn(x[i], 0.f); ids[rank[i]] = x[i] > minus_inf() ? i : -1; }
                 for (int j = KP; j < a.top; ++j) { values[j] = minus_inf(); ids[j] = -1; }
-            } else {
-                unsigned left = 0;
-#pragma unroll
-                for (int i = 0; i < KP; ++i) left |= x[i] > minus_inf() ? 1u << i : 0u;
+            } else {   // one after the other; a score that is taken becomes -inf
                 for (int j = 0; j < a.top; ++j) {
                     float v = minus_inf();
                     int id = -1;
 #pragma unroll
-                    for (int i = 0; i < KP; ++i)
-                        if ((left >> i & 1) && x[i] > v) { v = x[i]; id = i; }
-                    if (id >= 0) left &= ~(1u << id);
+                    for (int b = 0; b < KP; b += 16) {
+                        if (b >= a.k) break;
+#pragma unroll
+                        for (int i = b; i < b + 16; ++i)
+                            if (x[i] > v) { v = x[i]; id = i; }
+                    }
+#pragma unroll
+                    for (int b = 0; b < KP; b += 16) {
+                        if (b >= a.k) break;
+#pragma unroll
+                        for (int i = b; i < b + 16; ++i)
+                            if (i == id) x[i] = minus_inf();
+                    }
                     values[j] = __fadd_rn(v, 0.f);
                     ids[j] = id;
                 }
@@ -1711,15 +1726,21 @@ void scores_adjust(const AdjustArgs &given, cudaStream_t stream) {
         const Scores<T> in = scores_of<T>(a.in), out = scores_of<T>(a.out);
         const size_t counts = a.history_ptr ? sizeof(int) * ADJUST_CELLS : 0;
         auto parts = [](long long n, int of) { return (unsigned)((n + of - 1) / of); };
-        auto aligned = [&](const Scores<T> &s) { return s.cls == 1 && s.row % V == 0 && reinterpret_cast<uintptr_t>(s.p) % 16 == 0; };
+        // (the boundaries of a row of scores are those of its results)
+        const bool together = in.cls == 1 && out.cls == 1 && (reinterpret_cast<uintptr_t>(in.p) - reinterpret_cast<uintptr_t>(out.p)) % 16 == 0 &&
+                              (in.row - out.row) % V == 0;
         if (by_class) {
             auto kern = counts ? k_adjust_class<T, true> : k_adjust_class<T, false>;
             kern<<<dim3(parts(a.n, ADJUST_ROWS), parts(a.k, ADJUST_CLASSES)), ROW_THREADS, counts, stream>>>(a, in, out);
-        } else if (a.k >= ROW_THREADS * V / 2 && aligned(in) && aligned(out)) {
+        } else if (a.k >= ROW_THREADS * V / 2 && together) {
             // (shorter rows leave most of a block without a pack)
-            k_adjust_long<T><<<dim3((unsigned)a.n, parts(a.k, LONG_CELLS)), ROW_THREADS, counts ? sizeof(int) * LONG_CELLS : 0, stream>>>(a, in, out);
+            const bool even = reinterpret_cast<uintptr_t>(in.p) % 16 == 0 && in.row % V == 0;
+            auto kern = even ? k_adjust_long<T, true> : k_adjust_long<T, false>;
+            kern<<<dim3((unsigned)a.n, parts(a.k, LONG_CELLS)), ROW_THREADS, counts ? sizeof(int) * (LONG_CELLS + V) : 0, stream>>>(a, in, out);
         } else {
-            const int tile_classes = std::max(2, std::min(a.k, ADJUST_CELLS)), tile_rows = std::max(1, std::min(a.n, ADJUST_CELLS / 4 / tile_classes));
+            int tile_classes = std::max(2, std::min(a.k, ADJUST_CELLS));
+            while (tile_classes > 1024 && (long long)a.n * parts(a.k, tile_classes) < 4 * 148) tile_classes /= 2;   // (8 x 40210: 24 us in 40 blocks)
+            const int tile_rows = std::max(1, std::min(a.n, ADJUST_CELLS / 4 / tile_classes));
             static_assert(ADJUST_CELLS / 4 / 2 <= ADJUST_MOST_ROWS, "");
             const unsigned inverse = tile_rows == 1 ? 0u : (unsigned)(((1ull << 32) + tile_classes - 1) / tile_classes);
             k_adjust_tile<T><<<dim3(parts(a.n, tile_rows), parts(a.k, tile_classes)), ROW_THREADS, counts, stream>>>(a, in, out, tile_rows, tile_classes, inverse);
@@ -1766,7 +1787,8 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
     a.c = (float)(1.44269504088896341 * a.inv_t);
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
-        if (a.k <= FEW && a.in.cls <= INT_MAX) {   // (an address is one instruction then)
+        // (a pick of 64 takes some 300 instructions per thread, a warp from a tile some 500 per row: 12 of 37 took 121 us there for 246388 rows)
+        if ((a.k <= FEW || (a.k <= 2 * FEW && a.top <= 20)) && a.in.cls <= INT_MAX) {   // (an address is one instruction then)
             const int blocks = (int)std::min(((long long)a.n + FEW_THREADS - 1) / FEW_THREADS, (long long)FEW_BLOCKS);
             const size_t smem = (size_t)FEW_THREADS * a.top * 8;
             auto go = [&](auto kern) {
@@ -1775,7 +1797,8 @@ void scores_top(const TopArgs &given, cudaStream_t stream) {
             };
             if (a.k <= 8) go(k_top_few<T, 8>);
             else if (a.k <= 16) go(k_top_few<T, 16>);
-            else go(k_top_few<T, 32>);
+            else if (a.k <= 32) go(k_top_few<T, 32>);
+            else go(k_top_few<T, 64>);
             return;
         }
         const bool by_class = a.in.row < a.in.cls;
