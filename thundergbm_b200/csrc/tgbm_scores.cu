@@ -1467,8 +1467,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
 
 // A long row, taken as in k_top_wide.  The first pass sums up the classes that the teacher does not list, which a bit map marks; the second
 // finds the row in the L2 cache (the launch sees to it that the rows at work fit there) and writes what unlisted classes get; the
-// few cells of listed classes and of the label are written over it.  (What lies between the passes is one warp's work: done by
-// every warp for itself it took less waiting and more instructions, and the same time.)
+// few cells of listed classes and of the label are written over it.  (What lies between the passes is one warp's work, and the
+// others wait for it: what the list says is worked out beside the first pass.)
 template <typename T, bool TWO>
 __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(DistillArgs a, Scores<T> in) {
     constexpr int V = Pack<T>::V, S = SCORES_MAX_TOP / 32;
@@ -1492,6 +1492,18 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         for (int u = 0; u < WIDE_PACKS; ++u)
             if (from + u * WIDE_THREADS + tid < part.packs) ahead[u] = __ldg(body + from + u * WIDE_THREADS + tid);
     };
+    // First pass: a warp takes 32 * WIDE_PACKS neighbouring packs at a time.  The last one works out what the list says meanwhile and
+    // comes in `late` turns behind the others.
+    constexpr int TURN = 32 * WIDE_PACKS;
+    const int turns = (part.packs + TURN - 1) / TURN, late = turns >= 40 ? 2 : turns >= 16 ? 1 : 0;
+    auto first_of = [&](int i) { return (i < late ? i * (WIDE_WARPS - 1) + warp : i * WIDE_WARPS - late + warp) * TURN + lane; };
+    auto fetch_turn = [&](int i) {
+        const int from = first_of(i);
+#pragma unroll
+        for (int u = 0; u < WIDE_PACKS; ++u)
+            if (from + 32 * u < part.packs) ahead[u] = __ldg(body + from + 32 * u);
+    };
+    const int first_turn = warp == WIDE_WARPS - 1 ? late : 0;
     static_assert(WIDE_THREADS >= SCORES_MAX_TOP, "");
     // what the row gives besides its scores: read here, where it is waited for together with the lists
     const int label = row_label(a, n);
@@ -1505,7 +1517,7 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         id = a.ids[n * a.ids_stride + tid];
         if (id < 0 || id >= a.k) id = -1;
     }
-    fetch(0);
+    fetch_turn(first_turn);
     for (int i = tid; i < (per + 31) / 32 + 1; i += WIDE_THREADS) bits[i] = 0;   // (a word more: read in twos)
     __syncthreads();
     bool repeat = false;   // in this block's part; a class stands in one part
@@ -1527,14 +1539,32 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
             run.add(x, row_top(run.m), a.c);
         }
     }
-    for (int from = 0; from < part.packs; from += WIDE_THREADS * WIDE_PACKS) {
+    if (warp == WIDE_WARPS - 1) {
+        int ids[S];
+        float t[S], q[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            ids[s] = e < a.top ? list_id[e] : -1;
+            t[s] = e < a.top ? list_t[e] : 0.f;
+        }
+        const TeacherSide side = teacher_of<S>(a, a.lse ? &row_lse : nullptr, ids, t, q, repeats);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+            const int e = lane + 32 * s;
+            if (e < a.top) { list_id[e] = ids[s]; list_q[e] = q[s]; }
+        }
+        if (lane == 0) teacher = side;
+    }
+    for (int i = first_turn; first_of(i) - lane < part.packs; ++i) {
         uint4 w[WIDE_PACKS];
 #pragma unroll
         for (int u = 0; u < WIDE_PACKS; ++u) w[u] = ahead[u];
-        fetch(from + WIDE_THREADS * WIDE_PACKS);
+        const int from = first_of(i);
+        fetch_turn(i + 1);
 #pragma unroll
         for (int u = 0; u < WIDE_PACKS; ++u) {
-            const int at = from + u * WIDE_THREADS + tid;
+            const int at = from + 32 * u;
             if (at >= part.packs) break;
             Pack<T> p;
             p.bits = w[u];
@@ -1544,8 +1574,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
             const unsigned mark = __funnelshift_r(bits[k >> 5], bits[(k >> 5) + 1], k & 31) & ((1u << V) - 1);
             if (mark) {
 #pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (mark >> i & 1) v[i] = minus_inf();
+                for (int c = 0; c < V; ++c)
+                    if (mark >> c & 1) v[c] = minus_inf();
             }
             run.add_pack(v, a.c);
         }
@@ -1569,29 +1599,17 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         }
     }
     if (warp == 0) {   // the others wait: only what the second pass needs
-        int ids[S];
-        float q[S], t[S], x[S];
         float top = run.m;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int e = lane + 32 * s;
-            ids[s] = e < a.top ? list_id[e] : -1;
-            t[s] = e < a.top ? list_t[e] : 0.f;
-            x[s] = e < a.top ? list_x[e] : minus_inf();
-            top = fmaxf(top, x[s]);
-        }
-        const TeacherSide side = teacher_of<S>(a, a.lse ? &row_lse : nullptr, ids, t, q, repeats);
+        for (int e = lane; e < a.top; e += 32) top = fmaxf(top, list_x[e]);
+        const TeacherSide side = teacher;
         StudentRow st;
         st.base = row_top(run.m); st.rest = run.s; st.rest1 = TWO ? run.s1 : run.s;
         st.top = row_top(warp_max(top));
         st.base = reference_of(st.base, st.rest, st.top);
         float s0 = 0, s1 = 0;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-            const int e = lane + 32 * s;
-            if (e < a.top) { list_id[e] = ids[s]; list_q[e] = q[s]; }
-            if (ids[s] < 0) continue;
-            const float far = __fsub_rn(x[s], st.top);
+        for (int e = lane; e < a.top; e += 32) {
+            if (list_id[e] < 0) continue;
+            const float far = __fsub_rn(list_x[e], st.top);
             s0 += exp2_fast(far * a.c);
             if (TWO) s1 += exp2_fast(far * LOG2E);
         }
@@ -1600,7 +1618,6 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + warp_sum(s1) : st.sum;
         if (lane == 0) {
             factors = distill_row(a, side, st, w, label);
-            teacher = side;
             student = st;
         }
     }
