@@ -9,6 +9,9 @@ of it, which drops explicit zeros (they become missing values), and predict() do
 started from (src/thundergbm/scikit_tgbm.cpp:87-90).  A NumPy matrix goes to dense_train_scikit / dense_predict_scikit
 as it is, and its CSR is made on the GPU: on the host the conversion took most of a call (260 ms of fit() and again of
 predict() for 400009 x 28 values, against 20 ms of training on the GPU).
+
+Beyond the reference: fit(teacher=) grows trees towards another model's largest scores (through Booster, from a CSR), and predict_top()
+gives the best classes of every row under rules.
 """
 from __future__ import annotations
 
