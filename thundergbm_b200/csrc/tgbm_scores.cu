@@ -1670,9 +1670,18 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
         };
         const bool aligned = reinterpret_cast<uintptr_t>(out + part.head) % 16 == 0;
         if (a.gives == GIVES_PAIRS) {
+            const bool twos = reinterpret_cast<uintptr_t>(pairs + part.head) % 16 == 0;
             sweep([&](float(&v)[V], int k) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) pairs[k + i] = other_gh<TWO>(d, k + i, v[i]);
+                for (int i = 0; i < V; i += 2) {
+                    const float2 x = other_gh<TWO>(d, k + i, v[i]), y = other_gh<TWO>(d, k + i + 1, v[i + 1]);
+                    if (twos) {
+                        __stcs(reinterpret_cast<float4 *>(pairs + k + i), make_float4(x.x, x.y, y.x, y.y));
+                    } else {
+                        pairs[k + i] = x;
+                        pairs[k + i + 1] = y;
+                    }
+                }
             });
         } else if (d.hard == 0.f && aligned) {
             sweep([&](float(&v)[V], int k) {
@@ -1780,7 +1789,7 @@ template <typename F> void by_lane(int k, F &&f) {
 // A part is not shorter than what a block takes in one step.
 int blocks_per_row(int n, int k, int size, size_t twice) {
     constexpr long long SLOTS = WIDE_BLOCKS * 148;
-    constexpr size_t L2_ROOM = 48u << 20;
+    constexpr size_t L2_ROOM = 80u << 20;   // (2048 x 65536 in 16 bits: 121 us; with half of that, and clusters of two, 135)
     int c = 1;
     while (c < WIDE_CLUSTER && k / (2 * c) >= WIDE_THREADS * WIDE_PACKS * 16 / size &&
            (n * (2ll * c) <= SLOTS || (twice && (size_t)std::min<long long>(n, SLOTS / c) * twice > L2_ROOM))) c *= 2;
