@@ -449,3 +449,22 @@ def test_distill_where_all_that_is_left_is_far_below_zero(ops, layout, n, k):
     for T in (1.0, 1.5):
         for use_lse in (True, False):
             _check_distill(ops, t, 'f32', ids, logits, 'f32', lse if use_lse else None, labels, None, T, 0.5, (T, use_lse))
+
+
+@pytest.mark.parametrize('kind', TYPES)
+@pytest.mark.parametrize('m', [1, 20, 64, 74, 128])
+def test_top_of_the_lowest_numbers_among_masked_ones(ops, kind, m):
+    """Long rows with nothing but the type's lowest value here and there, each in another thread's hands."""
+    torch, scores = ops
+    low = float(torch.finfo(_type(torch, kind)).min)
+    z = np.full((3, 9001), -np.inf)
+    step = 16 // (4 if kind == 'f32' else 2)
+    z[0, : 75 * step: step] = low
+    z[1, : 75 * step: step] = low
+    z[1, 5000] = low / 2
+    z[2, ::7] = low
+    t = _tensor(torch, z, kind, 'row')
+    values, ids, lse, off = ref.top(_given(t), m)
+    got = scores.top(t, m)
+    assert np.array_equal(got[1].cpu().numpy(), ids) and np.array_equal(got[0].cpu().numpy(), values)
+    _close(got[2].cpu().numpy(), lse, off, kind)

@@ -427,7 +427,7 @@ struct TopList {
     int count;
 };
 __device__ __forceinline__ Entry entry_of(float v, int k) { return (Entry)score_key(v) << 32 | (unsigned)~k; }
-constexpr Entry LOWEST_ENTRY = 1ull << 32;   // what is below is no score that can be chosen
+constexpr Entry LOWEST_ENTRY = (Entry)LOWEST_KEY << 32;   // what is below is no score that can be chosen
 
 // border = the top-th largest of the groups' maxima (every thread has one, those of two neighbours make a group's); all threads
 __device__ __forceinline__ void find_border(TopList &l, Entry mine, int top) {
