@@ -238,7 +238,7 @@ int tgbm_scores_adjust(int n_rows, int n_classes, int type, const void *d_scores
 /* The `top` largest scores of every row, 1 <= top <= TGBM_SCORES_MAX_TOP: d_values and d_ids are n_rows x top, largest first, of
  * equal scores the lower class first.  -infinity (masked) and NaN are never chosen; where a row has fewer than `top` other scores
  * the last entries are -infinity and class -1.  d_lse (n_rows floats, or NULL): log of the sum over ALL classes of
- * exp(score / temperature), so that value / temperature - lse is the log of a class's share; NaN where a score is. */
+ * exp(score / temperature), so that value / temperature - lse is the log of a class's share; NaN where a score is NaN or +infinity. */
 int tgbm_scores_top(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int top,
                     float temperature, float *d_values, int *d_ids, float *d_lse, void *cuda_stream);
 

@@ -7,9 +7,9 @@
 #include <climits>
 #include <cmath>
 
-#include "../../include/thundergbm.h"
 #include <cooperative_groups.h>
 
+#include "../../include/thundergbm.h"
 #include "tgbm_kernels.cuh"
 #include "tgbm_scores.cuh"
 
@@ -41,7 +41,7 @@ template <typename F> void by_type(int type, F &&f) {
 // ------------------------------------------------------------------ adjust
 // A block takes a tile of rows x classes.  How often a class stands in the history of its row is counted in shared memory: every
 // entry of the tile's histories that falls into its classes adds one (integers: in any order the same), so a history may be
-// of any length.  A few instructions per score decide the time, so there are three ways through a tile.
+// of any length.  A few instructions per score decide the time, so there are three ways through the scores.
 constexpr int ADJUST_CELLS = 8192;
 
 // histories of `rows` rows into counts[cell(row, class - k0)]: the rows' entries lie one behind the other, so the block's threads share
@@ -75,8 +75,8 @@ __device__ __forceinline__ void count_histories(const AdjustArgs &a, long long n
     __syncthreads();
 }
 // z / r from r's reciprocal, rounded once: the product's error times the reciprocal is put back (P. Markstein, "Computation of
-// elementary functions on the IBM RISC System/6000 processor", 1990).  A score that was given before is in almost every warp, so
-// all scores pay for it: a division costs the batch of 50003 x 250 some 10 us more.
+// elementary functions on the IBM RISC System/6000 processor", 1990), except where that error is no float.  A score that was given
+// before is in almost every warp, so all scores pay for it: divisions cost the batch of 50003 x 250 4 us more.
 __device__ __forceinline__ float penalised(const AdjustArgs &a, float z, int times) {
     const float up = __fmul_rn(z, a.repetition), q = __fmul_rn(z, a.inv_repetition);
     const float error = __fmaf_rn(-q, a.repetition, z);
@@ -1784,7 +1784,7 @@ template <typename F> void by_lane(int k, F &&f) {
     else f(std::integral_constant<int, 0>{});
 }
 
-// Blocks of a cluster for a long row: one, and more where there are not rows enough for two blocks per SM, or where the rows
+// Blocks of a cluster for a long row: one, and more where there are not rows enough for WIDE_BLOCKS blocks per SM, or where the rows
 // that are at work at once would not fit into the L2 cache for a second pass (`twice` bytes of a row; 0: there is none).
 // A part is not shorter than what a block takes in one step.
 int blocks_per_row(int n, int k, int size, size_t twice) {
