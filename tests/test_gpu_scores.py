@@ -468,3 +468,28 @@ def test_top_of_the_lowest_numbers_among_masked_ones(ops, kind, m):
     got = scores.top(t, m)
     assert np.array_equal(got[1].cpu().numpy(), ids) and np.array_equal(got[0].cpu().numpy(), values)
     _close(got[2].cpu().numpy(), lse, off, kind)
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 40, 90), ('row', 40, 90), ('class', 12, 900), ('row', 12, 9001), ('any', 12, 50)])
+def test_loss_where_nearly_all_mass_is_left_to_the_rest(ops, layout, n, k):
+    """At a high temperature the listed classes hold little on both sides, and nearly the same: what is left of the loss is of second order
+    in the difference of the two.  An error e of the sum over the unlisted classes moves it by (their difference) e; the
+    logarithms of the shares of the rest, and the listed terms, are off by a few steps of the listed mass times what multiplies it."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = r.standard_normal((n, k)) * 1.5
+    T = 6.0
+    ids, logits, lse = _teacher(r, z, 3, T)
+    t = _tensor(torch, z, 'f32', layout)
+    dev = lambda x: torch.from_numpy(x).cuda()   # noqa: E731
+    loss, _ = scores.distill(t, dev(ids), dev(logits), lse=dev(lse), temperature=T, gives='loss')
+    s = _given(t).astype(np.float64) / T
+    want = ref.distill(_given(t), ids, logits, lse, None, None, T, 1.0)['loss']
+    p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    ps = np.take_along_axis(p, ids, 1).sum(1)
+    q = np.exp(logits.astype(np.float64) / T - lse[:, None].astype(np.float64))
+    far = np.abs(np.log(q)).max(1) + np.abs(np.log(np.take_along_axis(p, ids, 1))).max(1)
+    off = T * T * (np.abs(q.sum(1) - ps) * ref.sum_error(3, k) + 8 * ref.U * (q.sum(1) + ps) * (1 + far)) + ref.U * np.abs(want)
+    assert (off < 2e-4 * T * T).all()
+    _close(loss.cpu().numpy(), want, off, k)

@@ -891,6 +891,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
         if (!TWO) l1 = l;
         ql = warp_sum(ql);
         const float low = __fsub_rn(st.base, st.top);
+        st.l = l;
         st.sum = s * exp2_fast(low * c) + l;
         st.sum1 = TWO ? s1 * exp2_fast(low * LOG2E) + l1 : st.sum;
         if (lane == 0) {
@@ -1041,6 +1042,7 @@ __global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k
         }
         s.base = reference_of(s.base, s.rest, s.top);
         const float low = __fsub_rn(s.base, s.top);
+        s.l = l;
         s.sum = apart ? s.rest * exp2_fast(low * a.c) + l : s.rest;
         s.sum1 = !TWO ? s.sum : apart ? s.rest1 * exp2_fast(low * LOG2E) + l1 : s.rest1;
         const float w = a.weights ? a.weights[n] : 1.f;
@@ -1411,7 +1413,8 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
         st.top = row_top(fmaxf(largest_rest, o.top));
         st.base = reference_of(st.base, st.rest, st.top);
         const float low = __fsub_rn(st.base, st.top), high = o.top == minus_inf() ? 0.f : __fsub_rn(o.top, st.top);
-        st.sum = st.rest * exp2_fast(low * a.c) + o.l * exp2_fast(high * a.c);
+        st.l = o.l * exp2_fast(high * a.c);
+        st.sum = st.rest * exp2_fast(low * a.c) + st.l;
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + o.l1 * exp2_fast(high * LOG2E) : st.sum;
         factors[lane] = distill_row(a, o.teacher, st, weights[lane], labels[lane]);
         students[lane] = st;
@@ -1614,7 +1617,8 @@ __global__ void __launch_bounds__(WIDE_THREADS, WIDE_BLOCKS) k_distill_wide(Dist
             if (TWO) s1 += exp2_fast(far * LOG2E);
         }
         const float low = __fsub_rn(st.base, st.top);
-        st.sum = st.rest * exp2_fast(low * a.c) + warp_sum(s0);
+        st.l = warp_sum(s0);
+        st.sum = st.rest * exp2_fast(low * a.c) + st.l;
         st.sum1 = TWO ? st.rest1 * exp2_fast(low * LOG2E) + warp_sum(s1) : st.sum;
         if (lane == 0) {
             factors = distill_row(a, side, st, w, label);

@@ -223,6 +223,7 @@ __device__ __forceinline__ TeacherSide read_teacher(const DistillArgs &a, long l
 struct StudentRow {
     float base, rest, rest1;   // largest of the rest; sums of exp((s - base) / T) and exp(s - base)
     float top, sum, sum1;      // the same of all classes
+    float l;                   // sum of exp((s - top) / T) over the classes that are not of the rest
 };
 // Without a score above -inf the rest has the reference of all classes: its sums are 0 there as anywhere, and what brings them from
 // one reference to the other is 1, not infinite.
@@ -295,16 +296,30 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs &a, const Te
 __device__ __forceinline__ float distill_loss(const DistillArgs &a, const TeacherSide &t, const StudentRow &s, float w, int label,
                                               double listed, float label_score) {
     double loss = 0;
-    const double inv_t = a.inv_t;
     // (a row without a score above -inf: its listed sum or its label's score is -inf already, and the loss infinite)
-    const double log_sum = s.sum == 0.f ? 0.0 : fine_log(s.sum);
+    double log_sum = s.sum == 0.f ? 0.0 : fine_log(s.sum);
     if (t.total != 0.f) {
-        double kl = t.entropy - (listed - t.mass * log_sum);
-        if (t.rest > 0.f) kl += (double)t.rest * (fine_log(t.rest) - ((double)s.base - (double)s.top) * inv_t - fine_log(s.rest) + log_sum);
+        double kl = 0;
+        if (t.rest > 0.f) {
+            // The rest's term and those of the listed classes take most of each other away where both sides leave nearly all mass, and
+            // nearly the same, to the rest: its logarithms are those of 1 - mass and 1 / (1 + ratio), not of their roundings.
+            const double low = ((double)s.base - (double)s.top) * a.inv_t;
+            const float ratio = s.l * exp2f(-__fsub_rn(s.base, s.top) * a.c) / s.rest;   // listed to unlisted sum
+            double share;   // log of the rest's share
+            if (ratio < 1.f) {
+                const double more = log1p((double)ratio);
+                share = -more;
+                log_sum = low + fine_log(s.rest) + more;
+            } else {
+                share = low + fine_log(s.rest) - log_sum;
+            }
+            kl = (1.0 - t.mass) * (log1p(-t.mass) - share);
+        }
+        kl += t.entropy - (listed - t.mass * log_sum);
         loss += (double)a.alpha * a.temperature * a.temperature * kl;
     }
     if (label >= 0 && a.alpha < 1.f)
-        loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - (s.sum1 == 0.f ? 0.0 : s.sum1 == s.sum ? log_sum : fine_log(s.sum1)));
+        loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - (s.sum1 == 0.f ? 0.0 : fine_log(s.sum1)));
     return (float)((double)w * loss);
 }
 
@@ -469,7 +484,7 @@ struct RowSums {
 };
 __device__ __forceinline__ StudentRow student_of(const DistillArgs &a, const RowSums &r) {
     StudentRow s;
-    s.rest = r.rest; s.rest1 = r.rest1; s.top = r.top;
+    s.rest = r.rest; s.rest1 = r.rest1; s.top = r.top; s.l = r.l;
     s.base = reference_of(r.base, r.rest, r.top);
     const float low = __fsub_rn(s.base, r.top);
     s.sum = r.rest * exp2_fast(low * a.c) + r.l;
