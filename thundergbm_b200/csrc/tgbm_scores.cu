@@ -577,7 +577,10 @@ __device__ __noinline__ void make_room(TopList &l, int top, const T *cells, int 
     for (int turn = 0; turn < WIDE_WARPS; ++turn) {
         const bool full = l.count > WIDE_ROOM - WARP_CELLS;
         __syncthreads();
-        if (full) narrow_to(l, top, WIDE_LAST);
+        if (full) {
+            narrow_to(l, top, WIDE_LAST);
+            __syncthreads();   // (its last step reads the count, which the warp below raises)
+        }
         const Entry border = l.border;
         if ((int)(threadIdx.x >> 5) == turn && dropped)
             each([&](int bit, Entry e) {
