@@ -1107,6 +1107,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
     __shared__ RowSums sums[TILE_MOST_ROWS];
     __shared__ float lse[TILE_MOST_ROWS];
     __shared__ DistillRow factors[TILE_MOST_ROWS];
+    __shared__ float label_scores[TILE_MOST_ROWS];
     const long long n0 = (long long)blockIdx.x << rows_log;
     const int rows = (int)min((long long)R, a.n - n0), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     load_tile(tile, a.in, n0, by_class, rows, rows_log, a.k);
@@ -1149,7 +1150,14 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
         const StudentRow s = student_of(a, r);
         const float w = a.weights ? a.weights[n] : 1.f;
         const int label = row_label(a, n);
-        if (a.gives != GIVES_LOSS) factors[threadIdx.x] = distill_row(a, r.teacher, s, w, label);
+        if (a.gives != GIVES_LOSS) {
+            factors[threadIdx.x] = distill_row(a, r.teacher, s, w, label);
+            if (label >= 0) {   // (as the listed classes' cells are: in the pass it gets, and notes, nothing)
+                float *cell = by_class ? tile + label * step + threadIdx.x : tile + threadIdx.x * a.k + label;
+                label_scores[threadIdx.x] = *cell;
+                *cell = minus_inf();
+            }
+        }
         if (a.loss) a.loss[n] = distill_loss(a, r.teacher, s, w, label, r.of_listed, r.label_score);
     }
     if (a.gives == GIVES_LOSS) return;
@@ -1210,7 +1218,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
         const int r = threadIdx.x, c = factors[r].label;
         int e = 0;
         while (e < a.top && list_id[r * a.top + e] != c) ++e;
-        if (e == a.top) put(r, c, other_gh<TWO>(factors[r], c, by_class ? tile[c * step + r] : tile[r * a.k + c]));
+        if (e == a.top) put(r, c, other_gh<TWO>(factors[r], c, label_scores[r]));
     }
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
@@ -1440,6 +1448,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
     };
     if (lane < rows) {
         DistillRow d = factors[lane];
+        const int own = d.label - k0;   // (what its cell gets here is not what it keeps: it is noted then)
         d.label = -1;
         if (a.gives == GIVES_PAIRS) {
             float2 *to = static_cast<float2 *>(a.out.data) + n * a.out.row + (long long)k0 * out_cls;
@@ -1447,7 +1456,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
             for (int j = 0; j < E; ++j) {
                 if (k0 + j >= K) break;
                 const float2 gh = other_gh<TWO>(d, 0, x[j]);
-                if (track) { mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y); }
+                if (track && j != own) { mg = fmaxf(mg, fabsf(gh.x)); mh = fmaxf(mh, gh.y); }
                 to[(long long)j * out_cls] = gh;
             }
         } else {
