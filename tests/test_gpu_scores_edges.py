@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import scores_ref as ref
-from test_gpu_scores import _close, _given, _tensor, ops  # noqa: F401
+from test_gpu_scores import _close, _given, _make, _teacher, _tensor, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -29,3 +29,47 @@ def test_top_of_long_rising_rows(ops, order, kind):
             got = [x.cpu().numpy() for x in scores.top(one.repeat(n, 1), m)]
             assert (got[1] == ids).all() and (got[0] == values).all(), (m, n)
             _close(got[2], lse.repeat(n), off[0], (order, m, n))
+
+
+LAYOUTS = [('class', 12, 6), ('class', 12, 90), ('row', 12, 6), ('row', 12, 400), ('row', 12, 9001), ('any', 12, 50), ('class', 12, 2000), ('any', 3, 20000)]
+
+
+@pytest.mark.parametrize('layout,n,k', LAYOUTS)
+def test_terms_that_weigh_nothing(ops, layout, n, k):
+    """A distance that is infinite counts for nothing where alpha is 0, and neither does a whole row of weight 0: the loss is that of the
+    labels, or 0.  Gradients and pairs likewise."""
+    torch, scores = ops
+    r = np.random.default_rng(n + k)
+    z = _make(r, n, k)
+    ids, logits, lse = _teacher(r, z, 4, 1.0)
+    ids[:, 3] = (ids[:, 2] + 1) % k   # (a class may stand there twice)
+    labels = ids[:, 1].copy()
+    for i in range(0, n, 3):
+        z[i, ids[i, 0]] = -np.inf                                                 # a listed class is masked
+    for i in range(1, n, 3):
+        z[i] = np.where(np.isin(np.arange(k), ids[i]), z[i], -np.inf)             # ... or all that are not listed
+    z[n - 1] = -np.inf                                                            # ... or all
+    t = _tensor(torch, z, 'f32', layout)
+    dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()   # noqa: E731
+    weights = r.random(n).astype(np.float32) + 0.5
+    weights[::2] = 0
+    weights[n - 1] = 0
+    for T in (1.0, 1.7):
+        for use_lse in (True, False):
+            L = lse if use_lse else None
+            # alpha = 0 (the row without any score has no finite label term either: left to its weight)
+            want = ref.distill(_given(t), np.full_like(ids, -1), logits, L, labels, None, T, 0.0)
+            for gives in ('loss', 'gradient', 'pairs'):
+                loss, g = scores.distill(t, dev(ids), dev(logits), lse=dev(L), labels=dev(labels), temperature=T, alpha=0.0, gives=gives)
+                _close(loss.cpu().numpy(), want['loss'], want['loss_off'], (T, use_lse, gives))
+            assert np.isfinite(want['loss'][:n - 1]).all() and np.isinf(want['loss'][n - 1])
+            _close(g[..., 0].cpu().numpy(), want['g'], want['g_off'], (T, use_lse))
+            # weights of 0
+            one = ref.distill(_given(t), ids, logits, L, labels, None, T, 0.6)
+            want = ref.distill(_given(t), ids, logits, L, labels, weights, T, 0.6)
+            assert np.isinf(one['loss'][weights == 0]).any()
+            for gives in ('loss', 'gradient', 'pairs'):
+                loss, g = scores.distill(t, dev(ids), dev(logits), lse=dev(L), labels=dev(labels), weights=dev(weights), temperature=T, alpha=0.6, gives=gives)
+                _close(loss.cpu().numpy(), np.where(weights == 0, 0.0, want['loss']), np.where(weights == 0, 0.0, want['loss_off']), (T, use_lse, gives))
+            _close(g[..., 0].cpu().numpy(), want['g'], want['g_off'], (T, use_lse))
+            assert bool((g[..., 0][dev(weights == 0)] == 0).all())

@@ -316,11 +316,11 @@ __device__ __forceinline__ float distill_loss(const DistillArgs &a, const Teache
             kl = (1.0 - t.mass) * (log1p(-t.mass) - share);
         }
         kl += t.entropy - (listed - t.mass * log_sum);
-        loss += (double)a.alpha * a.temperature * a.temperature * kl;
+        if (a.alpha > 0.f) loss = (double)a.alpha * a.temperature * a.temperature * kl;   // (it may be infinite)
     }
     if (label >= 0 && a.alpha < 1.f)
         loss -= (1.0 - (double)a.alpha) * ((double)label_score - (double)s.top - (s.sum1 == 0.f ? 0.0 : fine_log(s.sum1)));
-    return (float)((double)w * loss);
+    return w == 0.f ? 0.f : (float)((double)w * loss);
 }
 
 // ---- a row whose scores lie in shared memory, one warp ---------------------------------------
