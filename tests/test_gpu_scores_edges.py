@@ -73,3 +73,15 @@ def test_terms_that_weigh_nothing(ops, layout, n, k):
                 _close(loss.cpu().numpy(), np.where(weights == 0, 0.0, want['loss']), np.where(weights == 0, 0.0, want['loss_off']), (T, use_lse, gives))
             _close(g[..., 0].cpu().numpy(), want['g'], want['g_off'], (T, use_lse))
             assert bool((g[..., 0][dev(weights == 0)] == 0).all())
+
+
+def test_a_set_of_no_masks_is_refused(ops):
+    torch, scores = ops
+    z = torch.randn(4, 70, device='cuda')
+    none = torch.zeros(0, 3, dtype=torch.int32, device='cuda')
+    row = torch.zeros(4, dtype=torch.int32, device='cuda')
+    for bad in (dict(allowed=none), dict(allowed=none, allowed_row=row), dict(allowed=torch.zeros(3, 3, dtype=torch.int32, device='cuda'))):
+        with pytest.raises(ValueError, match='allowed'):
+            scores.adjust(z, **bad)
+    assert scores.adjust(z[:0], allowed=none).shape == (0, 70) and scores.adjust(z[:0], allowed=none, allowed_row=row[:0]).shape == (0, 70)
+    assert bool((scores.adjust(z, allowed=torch.zeros(1, 3, dtype=torch.int32, device='cuda'), allowed_row=row) == -float('inf')).all())

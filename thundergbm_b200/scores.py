@@ -89,6 +89,8 @@ def adjust(scores, *, out=None, bias=None, allowed=None, allowed_row=None, histo
         masks, words = allowed.shape
         if words < (k + 31) // 32:
             _refuse('allowed: a bit for every class')
+        if n and masks < (n if allowed_row is None else 1):   # (no masks have no address, which means that all classes are allowed)
+            _refuse('allowed: fewer masks than rows, and none named for each row')
         mask_ptr = _beside(allowed, device, torch.int32, (masks, words), 'allowed')
         if allowed_row is not None:
             row_ptr = _beside(allowed_row, device, torch.int32, (n,), 'allowed_row')
