@@ -85,3 +85,27 @@ def test_a_set_of_no_masks_is_refused(ops):
             scores.adjust(z, **bad)
     assert scores.adjust(z[:0], allowed=none).shape == (0, 70) and scores.adjust(z[:0], allowed=none, allowed_row=row[:0]).shape == (0, 70)
     assert bool((scores.adjust(z, allowed=torch.zeros(1, 3, dtype=torch.int32, device='cuda'), allowed_row=row) == -float('inf')).all())
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('k', [6, 45, 250, 1000, 1024])
+def test_a_slice_of_one_row_is_that_row(ops, kind, k):
+    """One row taken out of a matrix by class, as a view and as a copy of its own, gets the bits that it has among the others."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = _tensor(torch, _make(r, 70, k), kind, 'class+')
+    v, i, lse = scores.top(_tensor(torch, _make(r, 70, k), 'f32', 'row'), min(k, 9), temperature=1.5)
+    y = torch.from_numpy(r.integers(-1, k, 70).astype(np.int32)).cuda()
+    bias, given = torch.randn(k, device='cuda'), torch.arange(71, device='cuda')
+    top, adjusted = scores.top(z, 5, temperature=1.5), scores.adjust(z, bias=bias, history=(given, y), presence=0.3, repetition=1.2)
+    for gives in ('loss', 'gradient', 'pairs'):
+        par = dict(temperature=1.5, alpha=0.6, gives=gives)
+        whole = scores.distill(z, i, v, lse=lse, labels=y, **par)
+        for n in (0, 31, 32, 69):
+            one = slice(n, n + 1)
+            for part in (z[one], z[one].t().contiguous().t()):
+                got = scores.distill(part, i[one], v[one], lse=lse[one], labels=y[one], **par)
+                assert torch.equal(got[0], whole[0][one]) and (gives == 'loss' or torch.equal(got[1], whole[1][one])), (gives, n, part.stride())
+                assert all(torch.equal(a, b[one]) for a, b in zip(scores.top(part, 5, temperature=1.5), top))
+                got = scores.adjust(part, bias=bias, history=(given[:2], y[one]), presence=0.3, repetition=1.2)
+                assert torch.equal(got, adjusted[one])

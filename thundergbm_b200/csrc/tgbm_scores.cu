@@ -1229,7 +1229,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 // shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them; these are 49, with
 // three blocks per SM instead of four 53, with five (and fewer registers) 68, with sixteen warps of half the classes each 59.)
 // The cells of listed classes and labels are written over what they get with the others.
-constexpr int CLASS_ROWS = 32;
+constexpr int CLASS_ROWS = 32, CLASS_MOST = 1024;
 
 struct ListSums {   // of a row's list
     TeacherSide teacher;
@@ -1886,7 +1886,7 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
             return;
         }
         const bool by_class = a.in.row < a.in.cls || a.in.one_by_class;
-        if (by_class && a.k <= 1024 && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
+        if (by_class && a.k <= CLASS_MOST && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
             const size_t smem = 12 * (size_t)CLASS_ROWS * a.top;
             const unsigned blocks = (unsigned)(((long long)a.n + CLASS_ROWS - 1) / CLASS_ROWS);
             auto go = [&](auto kern, int warps) {
@@ -1943,7 +1943,8 @@ ScoreView view_of(const char *what, const void *data, int type, int n, int k, lo
     TGBM_CHECK(type >= SCORE_F32 && type <= SCORE_BF16, w + ": unknown type");
     TGBM_CHECK(data != nullptr, w + ": null pointer");
     TGBM_CHECK(reinterpret_cast<uintptr_t>(data) % size_of(type) == 0, w + ": not aligned for its type");
-    const bool one_by_class = n == 1 && row == cls;
+    // (beyond CLASS_MOST only where nothing else tells the layout: a slice of one such row is left to the kernels for any stride)
+    const bool one_by_class = n == 1 && row >= 1 && (row == cls || (row < cls && k <= CLASS_MOST));
     if (n == 1) row = k == 1 ? 1 : cls * k;   // a stride that no step takes
     if (k == 1) cls = row * n;
     TGBM_CHECK(row >= 0 && cls >= 0, w + ": negative stride");

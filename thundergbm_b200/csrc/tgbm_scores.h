@@ -15,7 +15,7 @@ struct ScoreView {
     void *data = nullptr;
     int type = SCORE_F32;
     long long row = 0, cls = 0;
-    bool one_by_class = false;   // a single row of a matrix that is laid out by class: computed as its neighbours would be
+    bool one_by_class = false;   // a single row of a matrix that is laid out by class: distill computes it, up to 1024 classes, as its neighbours
 };
 
 struct AdjustArgs {
