@@ -125,9 +125,10 @@ int tgbm_booster_boost(TgbmBooster *b, int n_rounds);
 /* Objectives multi:softmax and multi:softprob, before the first round: trees are grown on the pairs of tgbm_scores_distill (below) instead of
  * the hard labels' alone -- per row of this rank `top` classes and scores of a teacher, its log-sum-exp at `temperature` (or NULL), the
  * labels' part weighing 1 - alpha.  Host arrays n_rows x top, n_rows x top, n_rows; copied.  Classes are positions among the labels
- * (tgbm_booster_get_labels).  With a communicator every rank calls it.  Metrics stay those of the labels; model files do not change. */
+ * (tgbm_booster_get_labels).  With a communicator every rank calls it, with the same temperature and alpha and all with lse or none; where
+ * one rank's call is refused, all are, and what was set before stays.  Metrics stay those of the labels; model files do not change. */
 int tgbm_booster_set_teacher(TgbmBooster *b, int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
-/* that loss on the current scores: its mean over this rank's rows */
+/* that loss on the current scores: its mean over this rank's rows (waits as tgbm_booster_sync does; with a communicator every rank calls it) */
 int tgbm_booster_teacher_loss(TgbmBooster *b, double *out);
 int tgbm_booster_sync(TgbmBooster *b);
 /* boost + sync, bracketed by CUDA events on the booster's stream: device time of the n_rounds in ms */

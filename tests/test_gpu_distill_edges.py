@@ -47,3 +47,111 @@ def test_the_grid_of_a_round_is_as_fine_as_its_gradients(gpu, classes, per_class
     assert largest < 2.0 ** -6
     _check_roots(b.trees()[1], want, n, 18)
     b.close()
+
+
+def _teacher_of(n, classes, seed):
+    r = np.random.default_rng(seed)
+    logits = r.standard_normal((n, classes)) * 2
+    ids = np.argsort(-logits, axis=1)[:, :3].astype(np.int32)
+    return ids, np.take_along_axis(logits, ids, 1).astype(np.float32), np.log(np.exp(logits / 2).sum(1)).astype(np.float32)
+
+
+def _rows(n, classes, seed):
+    from thundergbm_b200.synth import dense_to_csr
+    r = np.random.default_rng(seed)
+    y = r.integers(0, classes, n)
+    y[:classes] = np.arange(classes)
+    return dense_to_csr(r.integers(1, 30, (n, 5)).astype(np.float32), y.astype(np.float32))
+
+
+def test_a_refused_teacher_leaves_the_one_before(gpu):
+    from thundergbm_b200.booster import Booster
+    d, t = _rows(1500, 4, 1), _teacher_of(1500, 4, 2)
+    par = dict(objective='multi:softprob', num_class=4, depth=4, n_trees=3, hist_mode='exact')
+    a, b = Booster(d, **par), Booster(d, **par)
+    for x in (a, b):
+        x.set_teacher(*t, 2.0, 0.6)
+    for bad in (dict(alpha=2.0), dict(temperature=0.0)):
+        with pytest.raises(RuntimeError):
+            a.set_teacher(*_teacher_of(1500, 4, 3), **bad)
+    with pytest.raises(ValueError):
+        a.set_teacher(t[0][:5], t[1], t[2])
+    assert a.teacher_loss() == b.teacher_loss()
+    a.boost(3)
+    b.boost(3)
+    assert a.trees().tobytes() == b.trees().tobytes()
+    other = _teacher_of(1500, 4, 3)
+    c, d2 = Booster(d, **par), Booster(d, **par)
+    c.set_teacher(*t, 2.0, 0.6)
+    c.set_teacher(other[0], other[1], None, 1.0, 0.9)     # (another one takes its place)
+    d2.set_teacher(other[0], other[1], None, 1.0, 0.9)
+    c.boost(3)
+    d2.boost(3)
+    assert c.trees().tobytes() == d2.trees().tobytes()
+
+
+def _rank(rank, world, port, q):
+    import os
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for p in (root, os.path.join(root, 'tests')):
+        sys.path.insert(0, p)
+    import torch
+    import torch.distributed as dist
+    from thundergbm_b200.booster import Booster, Comm
+    os.environ['MASTER_ADDR'] = '127.0.0.1'
+    os.environ['MASTER_PORT'] = str(port)
+    os.environ.setdefault('NCCL_NVLS_ENABLE', '0')
+    os.environ['TGBM_COMM_TIMEOUT_S'] = '60'
+    torch.cuda.set_device(rank)
+    dist.init_process_group('gloo', rank=rank, world_size=world)
+    uid = [Comm.unique_id() if rank == 0 else None]
+    dist.broadcast_object_list(uid, src=0)
+    comm = Comm(uid[0], rank, world)
+    d, t = _rows(3000, 4, 1), _teacher_of(3000, 4, 2)
+    lo, hi = 3000 * rank // world, 3000 * (rank + 1) // world
+    b = Booster(d.rows(lo, hi), comm=comm, objective='multi:softprob', num_class=4, depth=4, n_trees=3, hist_mode='exact')
+    mine = tuple(x[lo:hi] for x in t)
+    refused = []
+    for bad in (dict(alpha=2.0), dict(temperature=3.0), dict(lse=None), dict(ids=mine[0][:5])):   # of rank 1 alone
+        args = dict(ids=mine[0], logits=mine[1], lse=mine[2], temperature=2.0, alpha=0.6)
+        if rank == 1:
+            args.update(bad)
+        try:
+            b.set_teacher(**args)
+            refused.append(False)
+        except (ValueError, RuntimeError):
+            refused.append(True)
+    b.set_teacher(*mine, 2.0, 0.6)
+    b.boost(3)
+    q.put((rank, refused, b.trees().tobytes()))
+    b.close()
+    comm.close()
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_ranks_take_a_teacher_together(gpu):
+    """What one rank refuses, or says something else for, no rank takes; what they take grows the trees of one GPU.  Skipped on one GPU."""
+    import os
+    import torch
+    import torch.multiprocessing as mp
+    if torch.cuda.device_count() < 2:
+        pytest.skip('needs 2 GPUs')
+    from thundergbm_b200.booster import Booster
+    b = Booster(_rows(3000, 4, 1), objective='multi:softprob', num_class=4, depth=4, n_trees=3, hist_mode='exact')
+    b.set_teacher(*_teacher_of(3000, 4, 2), 2.0, 0.6)
+    b.boost(3)
+    want = b.trees().tobytes()
+    b.close()
+    ctx = mp.get_context('spawn')
+    q = ctx.Queue()
+    port = 28600 + os.getpid() % 1000
+    procs = [ctx.Process(target=_rank, args=(r, 2, port, q)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = [q.get(timeout=300) for _ in procs]
+    for p in procs:
+        p.join(timeout=120)
+    for rank, refused, trees in res:
+        assert refused == [True] * 4 and trees == want, rank

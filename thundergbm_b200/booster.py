@@ -83,12 +83,18 @@ class Booster:
         rows x up to 128, classes as positions in labels() (-1: none); `lse` the teacher's log-sum-exp at this temperature, with
         which the mass of the classes that are not listed counts as one class; the loss on the labels weighs 1 - alpha."""
         n = self.info.n_rows
-        ids, logits = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logits, np.float32)
-        if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[0] != n:
-            raise ValueError('ids and logits: rows x kept classes, one score for every class')
-        lse = None if lse is None else np.ascontiguousarray(lse, np.float32)
-        if lse is not None and lse.shape != (n,):
-            raise ValueError('lse: one per row')
+        try:
+            ids, logits = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logits, np.float32)
+            if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[0] != n:
+                raise ValueError('ids and logits: rows x kept classes, one score for every class')
+            lse = None if lse is None else np.ascontiguousarray(lse, np.float32)
+            if lse is not None and lse.shape != (n,):
+                raise ValueError('lse: one per row')
+            temperature, alpha = float(temperature), float(alpha)
+        except Exception:
+            # the other ranks of a communicator wait for this one to say that it has no teacher to take
+            self._lib.tgbm_booster_set_teacher(self.handle, 0, None, None, None, 1.0, 1.0)
+            raise
         _lib.check(self._lib.tgbm_booster_set_teacher(self.handle, ids.shape[1], _ptr(ids), _ptr(logits), _ptr(lse), temperature, alpha))
 
     def teacher_loss(self) -> float:

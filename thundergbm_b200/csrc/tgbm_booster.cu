@@ -1203,24 +1203,54 @@ DistillArgs BoosterImpl::distill_args() const {
 
 void Booster::set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha) {
     BoosterImpl &m = *impl_;
-    TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "a teacher needs objective multi:softmax or multi:softprob");
-    TGBM_CHECK(m.rounds == 0, "the teacher has to be there before the first round");
-    TGBM_CHECK(top >= 1 && top <= SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(SCORES_MAX_TOP) + "]");
-    TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
-    TGBM_CHECK(alpha >= 0.f && alpha <= 1.f, "alpha outside [0, 1]");
-    TGBM_CHECK((ids && logits) || m.N == 0, "teacher: null pointer");
-    TGBM_CUDA(cudaStreamSynchronize(m.stream));
-    BoosterImpl::Teacher &t = m.teacher;
-    const size_t cells = (size_t)m.N * top;
-    t.top = 0;   // (none, should an allocation fail)
-    t.ids.alloc(cells); t.logits.alloc(cells); t.lse.alloc(lse ? m.N : 0);
-    if (cells) {
-        upload_h2d(t.ids.p, ids, t.ids.bytes(), m.stream, upload_threads());
-        upload_h2d(t.logits.p, logits, t.logits.bytes(), m.stream, upload_threads());
-        if (lse) upload_h2d(t.lse.p, lse, t.lse.bytes(), m.stream, upload_threads());
+    const bool multi = m.comm && m.comm->active();
+    BoosterImpl::Teacher next;
+    DevBuf<unsigned> said;
+    unsigned words[6] = {};
+    std::string local_err;   // see Booster::init: ranks take a teacher together or not at all
+    try {
+        TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "a teacher needs objective multi:softmax or multi:softprob");
+        TGBM_CHECK(m.rounds == 0, "the teacher has to be there before the first round");
+        TGBM_CHECK(top >= 1 && top <= SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(SCORES_MAX_TOP) + "]");
+        TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
+        TGBM_CHECK(alpha >= 0.f && alpha <= 1.f, "alpha outside [0, 1]");
+        TGBM_CHECK((ids && logits) || m.N == 0, "teacher: null pointer");
+        const size_t cells = (size_t)m.N * top;
+        next.ids.alloc(cells); next.logits.alloc(cells); next.lse.alloc(lse ? m.N : 0);
+        if (cells) {
+            upload_h2d(next.ids.p, ids, next.ids.bytes(), m.stream, upload_threads());
+            upload_h2d(next.logits.p, logits, next.logits.bytes(), m.stream, upload_threads());
+            if (lse) upload_h2d(next.lse.p, lse, next.lse.bytes(), m.stream, upload_threads());
+        }
+        if (multi) said.alloc(6);
         TGBM_CUDA(cudaStreamSynchronize(m.stream));
+        next.top = top; next.temperature = temperature; next.alpha = alpha;
+    } catch (const std::exception &e) {
+        local_err = e.what();
     }
-    t.top = top; t.temperature = temperature; t.alpha = alpha;
+    if (multi) {
+        m.comm->agree(local_err, "taking its teacher", m.stream);
+        // Ranks with rows have to mean the same objective: of a number and of its complement the largest over the ranks are each
+        // other's complement only if all of them said the same.
+        if (m.N) {
+            const float same[3] = {temperature, alpha, lse ? 1.f : 0.f};
+            for (int i = 0; i < 3; ++i) {
+                memcpy(&words[2 * i], &same[i], sizeof(float));
+                words[2 * i + 1] = ~words[2 * i];
+            }
+        }
+        TGBM_CUDA(cudaMemcpyAsync(said.p, words, sizeof(words), cudaMemcpyHostToDevice, m.stream));
+        m.comm->allreduce(said.p, 6, Comm::U32, Comm::MAX, m.stream);
+        TGBM_CUDA(cudaMemcpyAsync(words, said.p, sizeof(words), cudaMemcpyDeviceToHost, m.stream));
+        m.comm->wait(m.stream);
+        for (int i = 0; i < 3 && words[0]; ++i)   // (0: no rank has rows; a temperature is none)
+            TGBM_CHECK(words[2 * i] == ~words[2 * i + 1], "the ranks' teachers differ in temperature, alpha or whether the log-sum-exp is given");
+    } else if (!local_err.empty()) {
+        throw Error(local_err);
+    }
+    BoosterImpl::Teacher &t = m.teacher;
+    t.ids.take(next.ids); t.logits.take(next.logits); t.lse.take(next.lse);
+    t.top = next.top; t.temperature = next.temperature; t.alpha = next.alpha;
 }
 
 double Booster::teacher_loss() {

@@ -44,7 +44,8 @@ public:
     bool sync();   // waits; fp32 mode: builds the rounds again whose gradients did not fit the integer grid (true: there were some)
 
     // Multi-class objectives, before the first round: gradients against a teacher's largest scores (tgbm_scores.h), mixed with those
-    // on the labels.  Host arrays of this rank's rows, copied: n x top, n x top, n (or null).
+    // on the labels.  Host arrays of this rank's rows, copied: n x top, n x top, n (or null).  All ranks call it; what one of them
+    // refuses, or says another temperature for, none takes: they throw and keep what they had.
     void set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
     double teacher_loss();   // that loss on the current scores, the mean over this rank's rows; syncs
 
