@@ -23,6 +23,18 @@ def _ptr(a):
     return None if a is None else a.ctypes.data_as(C.c_void_p)
 
 
+def class_numbers(a):
+    """Numbers of classes (or masks) as int32: whole numbers of any type, of which those that int32 does not hold become -1, no class."""
+    a = np.asarray(a)
+    if a.dtype == np.int32 or a.size == 0:
+        return np.ascontiguousarray(a, np.int32)
+    if a.dtype.kind not in 'biuf' or (a.dtype.kind == 'f' and not (np.floor(a) == a).all()):
+        raise ValueError('class numbers have to be whole numbers')
+    out = np.full(a.shape, -1, np.int32)
+    np.copyto(out, a, casting='unsafe', where=(a >= 0) & (a <= 2 ** 31 - 1))
+    return out
+
+
 class Comm:
     """NCCL communicator of one rank.  `unique_id()` on rank 0, then every rank constructs Comm(id, rank, world)."""
 
@@ -84,7 +96,7 @@ class Booster:
         which the mass of the classes that are not listed counts as one class; the loss on the labels weighs 1 - alpha."""
         n = self.info.n_rows
         try:
-            ids, logits = np.ascontiguousarray(ids, np.int32), np.ascontiguousarray(logits, np.float32)
+            ids, logits = class_numbers(ids), np.ascontiguousarray(logits, np.float32)
             if ids.ndim != 2 or ids.shape != logits.shape or ids.shape[0] != n:
                 raise ValueError('ids and logits: rows x kept classes, one score for every class')
             lse = None if lse is None else np.ascontiguousarray(lse, np.float32)

@@ -21,6 +21,7 @@ import numpy as np
 import scipy.sparse as sp
 
 from . import _lib
+from .booster import class_numbers
 
 _LABELLED = ('binary:logistic', 'multi:softmax', 'multi:softprob')  # objectives that group their labels
 
@@ -216,7 +217,7 @@ class TGBMModel:
             field('allowed', words, np.uint32, (masks, (classes + 31) // 32), '')
             rules.n_masks = masks
             if allowed_row is not None:
-                field('allowed_row', allowed_row, np.int32, (n,), 'allowed_row: one mask per row')
+                field('allowed_row', class_numbers(allowed_row), np.int32, (n,), 'allowed_row: one mask per row')
         elif allowed_row is not None:
             raise ValueError('allowed_row: there are no masks')
         if history is not None:
@@ -224,7 +225,7 @@ class TGBMModel:
                 raise ValueError('history: a list for every row')
             ptr = np.zeros(n + 1, np.int64)
             np.cumsum([len(h) for h in history], out=ptr[1:])
-            ids = np.concatenate([np.asarray(h, np.int32).reshape(-1) for h in history]) if n else np.zeros(0, np.int32)
+            ids = class_numbers(np.concatenate([np.asarray(h).reshape(-1) for h in history if len(h)] or [np.zeros(0, np.int32)]))
             field('history_ptr', ptr, np.int64, (n + 1,), '')
             field('history', ids, np.int32, (int(ptr[-1]),), '')
         if not 1 <= k <= 128:
