@@ -223,7 +223,7 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * the row's history:
  *   z = c > 0 ? (s > 0 ? s / repetition : s * repetition) : s;   z -= c * frequency + (c > 0 ? presence : 0);
  *   z += d_bias[k];   out = allowed ? z : -infinity
- * computed in floats and rounded once.  d_out: the same type, strides of its own; d_out = d_scores with the same strides works in
+ * computed in floats and rounded once (repetition > 0, and a float holds 1 / repetition).  d_out: the same type, strides of its own; d_out = d_scores with the same strides works in
  * place; otherwise the two must not share memory.
  * d_bias: n_classes floats, or NULL.
  * d_allowed: n_masks rows of at least (n_classes + 31) / 32 words, `mask_stride` words apart, class k in bit k & 31 of word k >> 5;

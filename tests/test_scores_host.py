@@ -54,3 +54,10 @@ def test_refused(lib, call, args, says):
 def test_no_rows_is_nothing_to_do(lib, call):
     assert call(lib, n=0, z=None) == 0
     assert lib.tgbm_last_error() == b''
+
+
+@pytest.mark.parametrize('r', [1e-40, 2.9e-39, 1e-45])
+def test_a_repetition_penalty_without_a_reciprocal_is_refused(lib, r):
+    """Scores are divided through the penalty's reciprocal, which a float has to hold: 1e-5 / 1e-40 is one, 1 / 1e-40 is not."""
+    assert _adjust(lib, r=r) == 1
+    assert 'repetition' in lib.tgbm_last_error().decode()

@@ -323,8 +323,8 @@ int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, fl
         TGBM_CHECK(values && ids, "values or ids: null pointer");
         static const TgbmTopRules none{nullptr, nullptr, 0, nullptr, nullptr, nullptr, 1.f, 0.f, 0.f};
         const TgbmTopRules &r = rules ? *rules : none;
-        TGBM_CHECK(r.repetition > 0.f && std::isfinite(r.repetition) && std::isfinite(r.frequency) && std::isfinite(r.presence),
-                   "penalties have to be finite, the one for repetition positive");
+        TGBM_CHECK(r.repetition > 0.f && std::isfinite(r.repetition) && std::isfinite(1.f / r.repetition) && std::isfinite(r.frequency) && std::isfinite(r.presence),
+                   "penalties have to be finite, the one for repetition positive with a finite reciprocal");
         TGBM_CHECK(!r.allowed || r.n_masks >= (r.allowed_row ? 1 : n), "fewer masks than rows, and none named for each row");
         long long given = 0;
         if (r.history_ptr) {

@@ -2002,7 +2002,8 @@ int tgbm_scores_adjust(int n_rows, int n_classes, int type, const void *d_scores
                        long long n_history, float repetition, float frequency, float presence, void *cuda_stream) {
     return scores_call([&] {
         check_shape(n_rows, n_classes);
-        TGBM_CHECK(repetition > 0.f && repetition <= FLT_MAX, "the repetition penalty has to be a positive number");
+        TGBM_CHECK(repetition > 0.f && repetition <= FLT_MAX && 1.f / repetition <= FLT_MAX,
+                   "the repetition penalty has to be a positive number whose reciprocal is one");
         TGBM_CHECK(std::isfinite(frequency) && std::isfinite(presence), "penalties have to be finite");
         TGBM_CHECK(n_history >= 0, "negative length of the histories");
         if (d_allowed) {
