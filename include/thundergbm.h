@@ -209,7 +209,9 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * All pointers whose names begin with d_ are DEVICE pointers of the caller, on the current device; the kernels are queued on
  * `cuda_stream` (a cudaStream_t, NULL = default stream) and the calls return without waiting.  Nothing is allocated and nothing is
  * kept from one call for the next: calls on different streams do not disturb each other, and a call may be captured into a graph.
- * Arguments are checked before anything is queued: 1 and a message in tgbm_last_error().
+ * Arguments are checked before anything is queued: 1 and a message in tgbm_last_error().  No result may share memory with what is read
+ * or with another result, except where it is said to work (adjust refuses it, and distill for scores and gradient; the rest is the caller's
+ * to see to).
  * Scores are a matrix of n_rows x n_classes in `type`, class k of row n at d_scores[n * row_stride + k * class_stride] (strides in
  * elements, none negative).  Row stride 1: by class, as tgbm_booster_get_ypred and tgbm_predict_raw lay them out; class stride 1:
  * by row, as networks do.  Where neither is 1 the operators work as well, more slowly. */
@@ -223,8 +225,9 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * the row's history:
  *   z = c > 0 ? (s > 0 ? s / repetition : s * repetition) : s;   z -= c * frequency + (c > 0 ? presence : 0);
  *   z += d_bias[k];   out = allowed ? z : -infinity
- * computed in floats and rounded once (repetition > 0, and a float holds 1 / repetition).  d_out: the same type, strides of its own; d_out = d_scores with the same strides works in
- * place; otherwise the two must not share memory.
+ * computed in floats and rounded once (repetition > 0, and a float holds 1 / repetition).  d_out: the same type, strides of its own;
+ * d_out = d_scores with the same strides works in place; otherwise the two must not share memory (and where their lines interleave
+ * with gaps between the cells of a line, the call is refused although they do not).
  * d_bias: n_classes floats, or NULL.
  * d_allowed: n_masks rows of at least (n_classes + 31) / 32 words, `mask_stride` words apart, class k in bit k & 31 of word k >> 5;
  * NULL: every class is allowed.  d_allowed_row[n]: the row's mask (outside [0, n_masks): all its classes are allowed); NULL: row n

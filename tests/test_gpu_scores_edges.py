@@ -109,3 +109,34 @@ def test_a_slice_of_one_row_is_that_row(ops, kind, k):
                 assert all(torch.equal(a, b[one]) for a, b in zip(scores.top(part, 5, temperature=1.5), top))
                 got = scores.adjust(part, bias=bias, history=(given[:2], y[one]), presence=0.3, repetition=1.2)
                 assert torch.equal(got, adjusted[one])
+
+
+def test_results_beside_what_is_read(ops):
+    """In place with a row of the scores as the bias is refused; what lies in the gaps of a matrix, or shares its lines, is not."""
+    torch, scores = ops
+    z = torch.randn(6, 40, device='cuda')
+    before = z.clone()
+    for bias in (z[0], z[5]):
+        with pytest.raises(RuntimeError, match='share memory'):
+            scores.adjust(z, out=z, bias=bias)
+    with pytest.raises(RuntimeError, match='share memory'):
+        scores.adjust(z, out=z, history=(torch.arange(7, device='cuda'), z[2, :6].view(torch.int32)))
+    assert torch.equal(z, before)
+    assert torch.equal(scores.adjust(z, bias=z[3]), z + z[3])
+    # records of scores, a bias and room, one behind the other
+    rec = torch.randn(6, 100, device='cuda')
+    want = rec[:, :40] + rec[2, 40:80]
+    scores.adjust(rec[:, :40], out=rec[:, :40], bias=rec[2, 40:80])
+    assert torch.equal(rec[:, :40], want)
+    by_class = torch.randn(40, 100, device='cuda')
+    part, bias = by_class[:, :30].t(), by_class[7, 40:80]
+    want = part + bias
+    assert torch.equal(scores.adjust(part, out=part, bias=bias), want)
+    column = rec[:, 41:42]
+    want = column + rec[1, 50:51]
+    assert torch.equal(scores.adjust(column, out=column, bias=rec[1, 50:51]), want)
+    one = by_class[:, 3:4].t()
+    want = one + bias
+    assert torch.equal(scores.adjust(one, out=one, bias=bias), want)
+    with pytest.raises(RuntimeError, match='share memory'):
+        scores.adjust(part, out=part, bias=by_class[7, 20:60])

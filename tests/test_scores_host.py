@@ -61,3 +61,18 @@ def test_a_repetition_penalty_without_a_reciprocal_is_refused(lib, r):
     """Scores are divided through the penalty's reciprocal, which a float has to hold: 1e-5 / 1e-40 is one, 1 / 1e-40 is not."""
     assert _adjust(lib, r=r) == 1
     assert 'repetition' in lib.tgbm_last_error().decode()
+
+
+FAR = 1 << 30
+
+
+@pytest.mark.parametrize('call,args', [
+    # out is 4 x 40 floats, 640 bytes, at P + 65536; what is read begins or ends inside
+    (_adjust, dict(bias=P + 65536)), (_adjust, dict(bias=P + 65536 - 156)), (_adjust, dict(bias=P + 65536 + 636)),
+    (_adjust, dict(allowed=P + 65536 - 28, masks=4, words=2)), (_adjust, dict(allowed=FAR, masks=4, words=2, row=P + 65536 + 600)),
+    (_adjust, dict(ptr=P + 65536 - 32, ids=FAR, given=5)), (_adjust, dict(ptr=FAR, ids=P + 65536 - 16, given=5)),
+    (_adjust, dict(out=P, bias=P + 160)),   # in place, with a row of the scores as a bias
+])
+def test_results_over_what_is_read_are_refused(lib, call, args):
+    assert call(lib, **args) == 1
+    assert 'share memory' in lib.tgbm_last_error().decode()

@@ -1972,6 +1972,16 @@ bool share_memory(const ScoreView &a, int a_size, const ScoreView &b, int b_size
     return (in < width && over < lines) || (line - in < width && over + 1 < lines);
 }
 
+// Does [p, p + bytes) hold cells of the matrix?  (Where neither stride is 1 the gaps within a line count as cells.)
+bool lies_in(const ScoreView &v, int size, int n, int k, const void *p, long long bytes) {
+    if (!p || bytes <= 0) return false;
+    const bool by_row = n > 1 && (k == 1 || v.cls <= v.row);
+    const long long lines = by_row ? n : k, apart = size * (by_row ? v.row : v.cls), width = size * (by_row ? (k - 1) * v.cls + 1 : (n - 1) * v.row + 1);
+    const long long lo = (long long)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(v.data)), hi = lo + bytes;
+    if (hi <= 0 || lo >= (lines - 1) * apart + width) return false;
+    return lo < width || ((lo - width) / apart + 1) * apart < hi;   // (the first line that ends behind `lo`)
+}
+
 void check_pointer(const char *what, const void *p, size_t size) {
     TGBM_CHECK(reinterpret_cast<uintptr_t>(p) % size == 0, std::string(what) + ": not aligned for its type");
 }
@@ -2029,6 +2039,14 @@ int tgbm_scores_adjust(int n_rows, int n_classes, int type, const void *d_scores
             a.history_ptr = d_history_ptr; a.history = d_history; a.n_history = n_history;
         }
         a.repetition = repetition; a.frequency = frequency; a.presence = presence;
+        auto read = [&](const char *what, const void *p, long long bytes) {
+            TGBM_CHECK(!lies_in(a.out, size_of(type), n_rows, n_classes, p, bytes), std::string("out and ") + what + " share memory");
+        };
+        read("bias", a.bias, 4ll * n_classes);
+        if (n_masks == 1 || mask_stride == (n_classes + 31) / 32) read("masks", a.allowed, 4 * (long long)n_masks * ((n_classes + 31) / 32));
+        read("rows' masks", a.allowed_row, 4ll * n_rows);
+        read("histories", a.history_ptr, 8ll * n_rows + 8);
+        read("histories", a.history, 4 * a.n_history);
         scores_adjust(a, static_cast<cudaStream_t>(cuda_stream));
     });
 }
