@@ -140,3 +140,37 @@ def test_results_beside_what_is_read(ops):
     assert torch.equal(scores.adjust(one, out=one, bias=bias), want)
     with pytest.raises(RuntimeError, match='share memory'):
         scores.adjust(part, out=part, bias=by_class[7, 20:60])
+
+
+def test_results_in_place_and_autograd(ops):
+    """The operators are not recorded by autograd: a tensor that a recorded operation keeps for its backward pass is known to have
+    changed, and one that takes part itself is refused as a place for results."""
+    torch, scores = ops
+    x = torch.randn(4, 30, device='cuda', requires_grad=True)
+    bias = torch.ones(30, device='cuda')
+    y = x.exp()               # (the backward pass reads y)
+    for out in (x, y):
+        with pytest.raises(ValueError, match='autograd'):
+            scores.adjust(out, out=out, bias=bias)
+    y.sum().backward()
+    y = x.exp()
+    scores.adjust(y.detach(), out=y.detach(), bias=bias)
+    with pytest.raises(RuntimeError, match='modified'):
+        y.sum().backward()
+    with torch.no_grad():
+        want = x + 1
+        scores.adjust(x, out=x, bias=bias)
+        assert torch.equal(x, want) and x.requires_grad
+    with torch.inference_mode():
+        z = torch.randn(4, 30, device='cuda')
+        want = z + 1
+        assert torch.equal(scores.adjust(z, out=z, bias=bias), want)
+    # results require no gradient, whatever the scores do; distill's gradient is what backward() takes
+    w = torch.randn(30, 30, device='cuda', requires_grad=True)
+    student = torch.randn(4, 30, device='cuda') @ w
+    v, i, lse = scores.top(student, 3)
+    assert not v.requires_grad and not lse.requires_grad and not scores.adjust(student, bias=bias).requires_grad
+    loss, grad = scores.distill(student, i, v + 1, temperature=2.0)
+    assert not loss.requires_grad
+    student.backward(grad)
+    assert w.grad is not None and bool(w.grad.abs().sum() > 0)

@@ -8,6 +8,7 @@ Scores are a tensor of rows x classes (float32, float16 or bfloat16, any strides
     distill  loss on a teacher's largest scores and on hard labels, with its gradient
 
 Results come on the stream that is torch's current one on the scores' device, in the layout of the scores; nothing waits.
+Autograd does not record them: results require no gradient, also where the scores do (distill returns its gradient).
 Every function is one call of the C interface (tgbm_scores_* in include/thundergbm.h, which defines the operators); what the
 arguments may not be is refused there or here before anything is queued.
 """
@@ -72,13 +73,16 @@ def adjust(scores, *, out=None, bias=None, allowed=None, allowed_row=None, histo
     history: (ptr, classes), int64 (rows + 1) and int32: what row n was given before is classes[ptr[n]:ptr[n + 1]]; a class that stands
     there c > 0 times has its score divided (above 0) or multiplied by `repetition`, less c * frequency + presence."""
     n, k, kind, device = _scores(scores)
-    if out is None:
+    made = out is None
+    if made:
         out, o0, o1 = _like(scores, n, k)
     else:
         _scores(out, 'out')
         o0, o1 = out.stride()
         if not (out.shape == scores.shape and out.dtype == scores.dtype and out.device == scores.device):
             _refuse('out: shape, type and device of the scores')
+        if out.requires_grad and torch.is_grad_enabled():
+            _refuse('out: takes part in autograd, which does not see what is written here')
     masks = words = given = 0
     mask_ptr = row_ptr = bias_ptr = ptr = ids = None
     if bias is not None:
@@ -106,6 +110,8 @@ def adjust(scores, *, out=None, bias=None, allowed=None, allowed_row=None, histo
     s = scores.stride()
     _call(_lib.lib().tgbm_scores_adjust, device, n, k, kind, scores.data_ptr(), s[0], s[1], out.data_ptr(), o0, o1, bias_ptr, mask_ptr, masks, words,
           row_ptr, ptr, ids, given, repetition, frequency, presence)
+    if not made:
+        torch.autograd.graph.increment_version(out)   # (for operations that keep it for their backward pass)
     return out
 
 
