@@ -155,3 +155,70 @@ def test_ranks_take_a_teacher_together(gpu):
         p.join(timeout=120)
     for rank, refused, trees in res:
         assert refused == [True] * 4 and trees == want, rank
+
+
+@pytest.mark.parametrize('classes,n,top,with_lse', [(1100, 1300, 40, True), (1100, 1300, 3, False), (5600, 5600, 5, True)])
+def test_boosters_of_more_than_a_thousand_classes(gpu, classes, n, top, with_lse):
+    """Tiles and, of still more classes, a block per row: roots hold the sums of the definition, in the first round and in the second."""
+    from thundergbm_b200.booster import Booster
+    r = np.random.default_rng(classes + top)
+    d = _rows(n, classes, classes)
+    y = d.y.astype(np.int32)
+    ids = np.stack([r.permutation(classes)[:top] for _ in range(n)]).astype(np.int32)
+    ids[::3, 0] = y[::3]
+    logits = (r.standard_normal((n, top)) * 2).astype(np.float32)
+    lse = (np.log(np.exp(logits.astype(np.float64) / 1.5).sum(1)) + r.uniform(0.01, 2.0, n)).astype(np.float32) if with_lse else None
+    b = Booster(d, objective='multi:softprob', num_class=classes, depth=1, n_trees=2, learning_rate=1.0, hist_mode='exact')
+    b.set_teacher(ids, logits, lse, 1.5, 0.7)
+    for stop in (0, 1):
+        s = b.ypred().T.copy() if stop else np.zeros((n, classes), np.float32)
+        want = ref.distill(s, ids, logits, lse, y, None, 1.5, 0.7)
+        loss = b.teacher_loss()
+        assert abs(loss - want['loss'].mean()) <= want['loss_off'].mean() + 2.0 ** -40 * abs(want['loss']).sum()
+        b.boost(1)
+        _check_roots(b.trees()[stop], want, n, 18)
+    b.close()
+
+
+@pytest.mark.parametrize('n,classes', [(1, 5), (300, 5), (300, 40)])
+def test_entries_of_predict_top_under_rules(gpu, n, classes):
+    """Every entry that comes back, class by class: the score is the class's under the rules, the classes are those with the largest ones,
+    and a row that runs out of allowed classes ends in -1."""
+    from thundergbm_b200.thundergbm import TGBMClassifier
+    r = np.random.default_rng(classes + n)
+    d = _rows(1200, classes, classes)
+    x = np.zeros((1200, 5), np.float32)
+    x[np.repeat(np.arange(1200), np.diff(d.row_ptr)), d.col] = d.val
+    m = TGBMClassifier(depth=4, n_trees=5, learning_rate=0.4, objective='multi:softprob', verbose=0)
+    m.fit(x, d.y)
+    rows = x[:n]
+    s = np.zeros((n, classes), np.float32)
+    all_ids, all_values, _ = m.predict_top(rows, classes)
+    assert (np.sort(all_ids, 1) == np.arange(classes)).all()
+    np.put_along_axis(s, all_ids, all_values, 1)
+    bias = r.standard_normal(classes).astype(np.float32)
+    allowed = r.random((4, classes)) < 0.5
+    allowed[0] = False
+    allowed[0, classes // 2] = True
+    allowed[1] = False
+    row = r.integers(-1, 4, n)
+    past = [r.integers(0, classes, r.integers(0, 6)).tolist() for _ in range(n)]
+    ptr = np.concatenate([[0], np.cumsum([len(h) for h in past])])
+    flat = np.array([c for h in past for c in h], np.int32)
+    par = dict(repetition=1.2, frequency=0.1, presence=0.3)
+    k = 4
+    ids, values, lse = m.predict_top(rows, k, bias=bias, allowed=allowed, allowed_row=row, history=past, temperature=1.5, **par)
+    want, off = ref.adjust(s, bias, allowed, row, (ptr, flat), **par)
+    off = off + ref.U * np.abs(np.where(np.isfinite(want), want, 0)) * (1 + 2.0 ** -18)   # (rounded once more, to the float that is kept)
+    for i in range(n):
+        can = int((want[i] > -np.inf).sum())
+        got = ids[i][:min(k, can)]
+        assert (ids[i][can:] == -1).all() and (values[i][can:] == -np.inf).all()
+        assert len(set(got.tolist())) == got.size and (got >= 0).all() and (got < classes).all()
+        assert (np.abs(values[i][:got.size] - want[i][got]) <= off[i][got]).all()
+        assert (np.diff(values[i][:got.size]) <= 0).all()
+        rest = np.setdiff1d(np.flatnonzero(want[i] > -np.inf), got)
+        if rest.size:   # none that was left out is larger than the last one by more than both may be off
+            assert (want[i][rest] - off[i][rest] <= want[i][got[-1]] + off[i][got[-1]]).all()
+        if can == 0:
+            assert lse[i] == -np.inf
