@@ -76,3 +76,11 @@ FAR = 1 << 30
 def test_results_over_what_is_read_are_refused(lib, call, args):
     assert call(lib, **args) == 1
     assert 'share memory' in lib.tgbm_last_error().decode()
+
+
+@pytest.mark.parametrize('call', [_top, _distill])
+@pytest.mark.parametrize('T', [3e-39, 4.2e-39])
+def test_temperatures_whose_exponents_no_float_holds_are_refused(lib, call, T):
+    """exp(x / T) is 2^(x log2(e) / T): a float has to hold log2(e) / T, not only 1 / T."""
+    assert call(lib, T=T, **({'logits': P + 4096} if call is _distill else {})) == 1
+    assert 'temperature' in lib.tgbm_last_error().decode()

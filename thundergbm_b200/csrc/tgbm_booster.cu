@@ -1212,7 +1212,7 @@ void Booster::set_teacher(int top, const int *ids, const float *logits, const fl
         TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "a teacher needs objective multi:softmax or multi:softprob");
         TGBM_CHECK(m.rounds == 0, "the teacher has to be there before the first round");
         TGBM_CHECK(top >= 1 && top <= SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(SCORES_MAX_TOP) + "]");
-        TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
+        TGBM_CHECK(temperature_fits(temperature), "the temperature has to be a positive number");
         TGBM_CHECK(alpha >= 0.f && alpha <= 1.f, "alpha outside [0, 1]");
         TGBM_CHECK((ids && logits) || m.N == 0, "teacher: null pointer");
         const size_t cells = (size_t)m.N * top;

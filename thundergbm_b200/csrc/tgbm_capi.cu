@@ -317,7 +317,7 @@ int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, fl
         TGBM_CHECK(model && *model, "model is null!");
         TGBM_CHECK(trees_per_iter >= 2, "the largest scores of a row need a model of several classes (multi:softmax, multi:softprob)");
         TGBM_CHECK(top >= 1 && top <= tgbm::SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(tgbm::SCORES_MAX_TOP) + "]");
-        TGBM_CHECK(temperature > 0.f && std::isfinite(temperature) && std::isfinite(1.f / temperature), "the temperature has to be a positive number");
+        TGBM_CHECK(tgbm::temperature_fits(temperature), "the temperature has to be a positive number");
         const int n = ds.n_rows, k = trees_per_iter, words = (k + 31) / 32;
         if (n == 0) return;
         TGBM_CHECK(values && ids, "values or ids: null pointer");

@@ -1989,7 +1989,7 @@ void check_shape(int n, int k) {
     TGBM_CHECK(n >= 0, "negative number of rows");
     TGBM_CHECK(k >= 1 && k <= TGBM_SCORES_MAX_CLASSES, "number of classes outside [1, " + std::to_string(TGBM_SCORES_MAX_CLASSES) + "]");
 }
-void check_temperature(float t) { TGBM_CHECK(t > 0.f && t <= FLT_MAX && 1.0 / (double)t <= FLT_MAX, "the temperature has to be a positive number"); }
+void check_temperature(float t) { TGBM_CHECK(temperature_fits(t), "the temperature has to be a positive number"); }
 void check_list(int top) { TGBM_CHECK(top >= 1 && top <= TGBM_SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(TGBM_SCORES_MAX_TOP) + "]"); }
 
 template <typename F> int scores_call(F &&f) {

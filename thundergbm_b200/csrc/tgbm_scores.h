@@ -3,12 +3,17 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include <cfloat>
+
 namespace tgbm {
 
 enum ScoreType { SCORE_F32 = 0, SCORE_F16 = 1, SCORE_BF16 = 2 };
 enum DistillGives { GIVES_LOSS = 0, GIVES_GRADIENT = 1, GIVES_PAIRS = 2 };
 
 constexpr int SCORES_MAX_CLASSES = 1 << 20, SCORES_MAX_TOP = 128;
+
+// exp(x / t) is computed as 2^(x log2(e) / t), with the factor in a float
+inline bool temperature_fits(float t) { return t > 0.f && t <= FLT_MAX && 1.44269504088896341 / (double)t <= (double)FLT_MAX; }
 
 // rows x classes, class k of row n at data[n * row + k * cls]
 struct ScoreView {
