@@ -174,3 +174,39 @@ def test_results_in_place_and_autograd(ops):
     assert not loss.requires_grad
     student.backward(grad)
     assert w.grad is not None and bool(w.grad.abs().sum() > 0)
+
+
+@pytest.mark.parametrize('layout', ['row', 'row+', 'class', 'any'])
+def test_as_many_classes_as_there_may_be(ops, layout):
+    """2^20 classes, the last ones among the chosen, listed, masked and given ones."""
+    torch, scores = ops
+    n, k = 2, 1 << 20
+    r = np.random.default_rng(5)
+    z = r.standard_normal((n, k))
+    z[:, k - 1] = 9.0
+    z[1, k - 2] = 9.0
+    z[0, :3] = [8.0, -np.inf, 7.5]
+    t = _tensor(torch, z, 'f32', layout)
+    dev = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()   # noqa: E731
+    values, ids, lse, off = ref.top(_given(t), 4, 1.5)
+    got = scores.top(t, 4, temperature=1.5)
+    assert np.array_equal(got[1].cpu().numpy(), ids) and np.array_equal(got[0].cpu().numpy(), values)
+    _close(got[2].cpu().numpy(), lse, off, 'lse')
+    past = (np.array([0, 2, 3]), np.array([k - 1, k - 1, 0], np.int32))
+    bias, allowed = r.standard_normal(k).astype(np.float32), np.ones((1, k), bool)
+    allowed[0, [5, k - 2]] = False
+    want, off = ref.adjust(_given(t), bias, allowed, np.zeros(n, np.int32), past, repetition=1.5, frequency=0.25, presence=0.5)
+    got = scores.adjust(t, bias=dev(bias), allowed=dev(np.packbits(allowed, axis=1, bitorder='little').view(np.int32)),
+                        allowed_row=dev(np.zeros(n, np.int32)), history=(dev(past[0]), dev(past[1])), repetition=1.5, frequency=0.25, presence=0.5)
+    _close(_given(got), want, off + ref.U * np.abs(np.where(np.isfinite(want), want, 0)), 'adjust')
+    ids = np.array([[k - 1, 0, 77], [k - 2, k - 1, 3]], np.int32)
+    logits = r.standard_normal((n, 3)).astype(np.float32) + 8
+    lse = np.array([9.5, 10.0], np.float32)
+    y = np.array([k - 1, 4], np.int32)
+    want = ref.distill(_given(t), ids, logits, lse, y, None, 1.5, 0.6)
+    loss, pairs = scores.distill(t, dev(ids), dev(logits), lse=dev(lse), labels=dev(y), temperature=1.5, alpha=0.6, gives='pairs')
+    _close(loss.cpu().numpy(), want['loss'], want['loss_off'], 'loss')
+    _close(pairs[..., 0].cpu().numpy(), want['g'], want['g_off'], 'g')
+    _close(pairs[..., 1].cpu().numpy(), want['h'], want['h_off'], 'h')
+    loss, grad = scores.distill(t, dev(ids), dev(logits), lse=dev(lse), labels=dev(y), temperature=1.5, alpha=0.6)
+    _close(_given(grad), want['g'], want['g_off'], 'gradient')
