@@ -255,7 +255,7 @@ int tgbm_scores_top(int n_rows, int n_classes, int type, const void *d_scores, l
  * with p_r the student's share of the unlisted classes, w = d_weights[n] (NULL: 1) and y = d_labels[n] (outside [0, n_classes), or
  * NULL: no such term).  A class number outside [0, n_classes) is passed over, one that stands twice in a row holds the sum; a row
  * that lists nothing, or only -infinity, has no teacher: its first term is 0.  What weighs 0 (a term by alpha, a row by w) counts for
- * nothing, also where it is infinite.
+ * nothing, also where it is infinite, and so does a class to which the teacher gives less than a float holds (e^-103 of its mass).
  * d_loss: n_rows floats (NULL: not wanted, where there is a gradient).
  * gives: TGBM_GIVES_LOSS; TGBM_GIVES_GRADIENT: d_grad holds d loss / d s in the type of the scores; TGBM_GIVES_PAIRS: pairs of floats
  * (gradient, hessian) as a booster takes them, hessian = max(2 w (alpha p (1 - p) + (1 - alpha) p1 (1 - p1)), 1e-16), p1 = softmax(s), each

@@ -210,3 +210,24 @@ def test_as_many_classes_as_there_may_be(ops, layout):
     _close(pairs[..., 1].cpu().numpy(), want['h'], want['h_off'], 'h')
     loss, grad = scores.distill(t, dev(ids), dev(logits), lse=dev(lse), labels=dev(y), temperature=1.5, alpha=0.6)
     _close(_given(grad), want['g'], want['g_off'], 'gradient')
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 12, 20), ('class', 12, 90), ('class', 12, 1000), ('row', 12, 400), ('row', 12, 9001), ('any', 12, 50), ('class', 12, 2000), ('any', 3, 20000)])
+def test_masses_that_no_float_holds_are_none(ops, layout, n, k):
+    """A class to which the teacher gives e^-200 of its mass (a float holds e^-103) counts as if it had none, also where the student masks
+    it: the distance stays finite, however the scores are laid out."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = _make(r, n, k)
+    ids, logits, lse = _teacher(r, z, 5, 1.0)
+    logits[:, 4] = logits[:, 0] - 200
+    z[np.arange(n), ids[:, 4]] = -np.inf
+    t = _tensor(torch, z, 'f32', layout)
+    without = ids.copy()
+    without[:, 4] = -1
+    dev = lambda x: None if x is None else torch.from_numpy(np.ascontiguousarray(x)).cuda()   # noqa: E731
+    for L in (lse, None):
+        want = ref.distill(_given(t), without, logits, L, None, None, 1.0, 1.0)
+        loss, _ = scores.distill(t, dev(ids), dev(logits), lse=dev(L), gives='loss')
+        assert np.isfinite(want['loss']).all()
+        _close(loss.cpu().numpy(), want['loss'], want['loss_off'], L is None)

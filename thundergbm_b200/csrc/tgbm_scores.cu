@@ -1355,7 +1355,7 @@ __global__ void __launch_bounds__(32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_distil
                 const double lq = (double)q[e] * a.inv_t - L, v = none ? 0.0 : exp(lq);
                 const float far = __fsub_rn(xs[e], ref);
                 mass += v;
-                if (v != 0) {
+                if ((float)v != 0.f) {   // (what a float does not hold is no mass, as in the other kernels)
                     entropy += v * lq;
                     of_listed += v * (((double)xs[e] - (double)ref) * a.inv_t);
                 }
