@@ -92,7 +92,7 @@ __device__ __forceinline__ const unsigned *mask_of(const AdjustArgs &a, long lon
 
 // By class: a lane per row, a warp takes neighbouring classes, eight at a time: their scores are read together, and their bits lie in
 // one word of the row's mask.  Class strides are ints here: an address is one instruction.
-// Blocks per SM (4 x 61 registers): 29 us for 50003 x 250 with histories, 40 with 6 blocks and fewer registers.
+// Blocks per SM (4 x 61 registers): 31 us for 50003 x 250 with histories, 40 with 6 blocks and fewer registers.
 constexpr int ADJUST_ROWS = 32, ADJUST_AHEAD = 8, ADJUST_CLASSES = ADJUST_CELLS / ADJUST_ROWS;
 
 template <typename T, bool HISTORY>
@@ -413,8 +413,8 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : E == 16 ? 3 : 4) k
 // entry can count those before it.  Borders are found by bisection, counting across the block.
 // Where the list fills up all the same (ties, or scores that rise along the row), borders order scores and classes at once.
 
-// Four blocks of eight warps per SM: 104 us for 64 of 1024 x 131072 in 16 bits, 111 with two of sixteen, 114 with three, 140 with five (and
-// fewer registers).
+// Four blocks of eight warps per SM: 98 us for 64 of 1024 x 131072 in 16 bits, 107 with three, 137 with five (and fewer registers: with
+// four the compiler spills 20 bytes a thread of the 16-bit kernel, 96 of the other).  k_distill_wide, 2048 x 65536 in 16 bits: 123, 119, 140.
 constexpr int WIDE_THREADS = 256, WIDE_BLOCKS = 4, WIDE_WARPS = WIDE_THREADS / 32, WIDE_PACKS = 4, WIDE_CLUSTER = 8;
 constexpr int WIDE_ROOM = 2048, WIDE_GROUPS = WIDE_THREADS / 2, WIDE_LAST = 256;
 static_assert(WIDE_GROUPS >= SCORES_MAX_TOP && WIDE_CLUSTER * SCORES_MAX_TOP <= WIDE_ROOM, "");
@@ -925,7 +925,8 @@ __global__ void __launch_bounds__(ROW_THREADS) k_distill_any(DistillArgs a, Scor
 
 // A thread per row where there are few classes: the row's scores and exponentials stay in registers, what the teacher says of a class
 // in a column of shared memory (a class that is listed twice holds the sum).  Rows of a class are read side by side.  Instructions
-// decide the time, some 500 per row of 7 classes: what is only needed for repeats, or for a rest, is branched around.
+// decide the time, some 1130 per 32 rows of 7 classes: what is only needed for repeats, or for a rest, is branched around.  (Eight blocks
+// per SM for up to 8 classes; with two temperatures the compiler spills 44 bytes a thread then.)
 template <typename T, int KP, bool TWO>
 __global__ void __launch_bounds__(FEW_THREADS, KP == 8 ? 8 : KP == 16 ? 5 : 4) k_distill_few(DistillArgs a, Scores<T> in) {
     constexpr int ENTRIES = 4;   // entries of a list that stay in registers
@@ -1226,8 +1227,9 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 // By class, up to 1024 classes: a lane per row and E neighbouring classes per warp, whose scores stay in registers from the first read to
 // the gradients.  Rows are read and written side by side, and nothing is reduced within a warp: the warps of a block exchange a maximum
 // and sums per row.  What the lists say is worked out by as many threads per row as there are warps.  (A warp per row from a tile in
-// shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them; these are 49, with
-// three blocks per SM instead of four 53, with five (and fewer registers) 68, with sixteen warps of half the classes each 59.)
+// shared memory took 985 instructions per row of 250 classes, and they decided its time: 65 us for 50003 of them; these are 52, with
+// three blocks per SM instead of four 54, with five (and fewer registers) 68.  With four the compiler spills 24 to 44 bytes a thread where a
+// warp has 32 classes.)
 // The cells of listed classes and labels are written over what they get with the others.
 constexpr int CLASS_ROWS = 32, CLASS_MOST = 1024;
 
@@ -1805,7 +1807,7 @@ template <typename F> void by_lane(int k, F &&f) {
 // A part is not shorter than what a block takes in one step.
 int blocks_per_row(int n, int k, int size, size_t twice) {
     constexpr long long SLOTS = WIDE_BLOCKS * 148;
-    constexpr size_t L2_ROOM = 80u << 20;   // (2048 x 65536 in 16 bits: 121 us; with half of that, and clusters of two, 135)
+    constexpr size_t L2_ROOM = 80u << 20;   // (2048 x 65536 in 16 bits: 123 us; with half of that, and clusters of two, 139)
     int c = 1;
     while (c < WIDE_CLUSTER && k / (2 * c) >= WIDE_THREADS * WIDE_PACKS * 16 / size &&
            (n * (2ll * c) <= SLOTS || (twice && (size_t)std::min<long long>(n, SLOTS / c) * twice > L2_ROOM))) c *= 2;

@@ -7,6 +7,8 @@ Scores are a tensor of rows x classes (float32, float16 or bfloat16, any strides
     top      the largest scores of every row, their classes, the row's log-sum-exp
     distill  loss on a teacher's largest scores and on hard labels, with its gradient
 
+(top and distill take several times as long by class above some 5000 classes, or where neither rows nor classes lie side by side.)
+
 Results come on the stream that is torch's current one on the scores' device, in the layout of the scores; nothing waits.
 Autograd does not record them: results require no gradient, also where the scores do (distill returns its gradient).
 Every function is one call of the C interface (tgbm_scores_* in include/thundergbm.h, which defines the operators); what the

@@ -102,7 +102,8 @@ class TGBMModel:
     # -- API ---------------------------------------------------------------------------------------
     def fit(self, X, y, groups=None, teacher=None):
         """`teacher` (multi:softmax and multi:softprob, one GPU): the arguments of Booster.set_teacher as a dict -- ids, logits and, if
-        wanted, lse, temperature, alpha; what predict_top() of another model returns is such a teacher's ids, logits and lse."""
+        wanted, lse, temperature, alpha; what predict_top() of another model returns is such a teacher's ids, logits and lse.
+        `groups` are those of ranking objectives; the others, and so training from a teacher, do not look at them."""
         if teacher is not None:
             return self._fit_teacher(X, y, teacher)
         self._free()
