@@ -210,8 +210,8 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * `cuda_stream` (a cudaStream_t, NULL = default stream) and the calls return without waiting.  Nothing is allocated and nothing is
  * kept from one call for the next: calls on different streams do not disturb each other, and a call may be captured into a graph.
  * Arguments are checked before anything is queued: 1 and a message in tgbm_last_error().  No result may share memory with what is read
- * or with another result, except where it is said to work (adjust refuses it, and distill for scores and gradient; the rest is the caller's
- * to see to).
+ * or with another result, except where it is said to work (adjust and norm refuse it for what they read, distill, feedback and norm_backward for scores
+ * and gradients; the rest is the caller's to see to).
  * Scores are a matrix of n_rows x n_classes in `type`, class k of row n at d_scores[n * row_stride + k * class_stride] (strides in
  * elements, none negative).  Row stride 1: by class, as tgbm_booster_get_ypred and tgbm_predict_raw lay them out; class stride 1:
  * by row, as networks do.  Where neither is 1 the operators work as well, more slowly, and so do top and distill by class above some 5000
@@ -269,6 +269,59 @@ int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_score
                         const int *d_ids, long long ids_stride, int logits_type, const void *d_logits, long long logits_stride,
                         const float *d_lse, const int *d_labels, const float *d_weights, float temperature, float alpha, float *d_loss,
                         int gives, void *d_grad, long long grad_row_stride, long long grad_class_stride, void *cuda_stream);
+
+/* Classes drawn from the scores s of every row, one for each of `draws` given random numbers u (1 to TGBM_SCORES_MAX_DRAWS per row; d_uniform is
+ * n_rows x draws of uniform_type TGBM_F32 or TGBM_F64, in [0, 1): numbers outside are taken as the nearest inside, NaN as 0).
+ *   w_k = exp((s_k - max s) / temperature) for every class whose score is above -infinity
+ *   A: classes with w_k >= min_p that are among the top_k largest scores (of equal ones the lower class first; 0: all)
+ *   B: the shortest beginning of A, largest first, whose mass is at least top_p of A's (never empty; top_p 1: all of A)
+ *   a draw is the first class k of B in class order up to which B's mass goes beyond u times B's whole mass
+ * d_classes: n_rows x draws.  d_logs (or NULL): log of the drawn class's share of B's mass; d_all_logs (or NULL): of all classes' mass.
+ * temperature 0: the largest score (the lower class of equal ones), both logs 0.  A row without a score above -infinity gives class -1 and
+ * logs of -infinity, one that holds NaN or +infinity class -1 and NaN.
+ * Each of the four limits holds for all rows, or (where d_temperature, d_top_k, d_top_p, d_min_p is not NULL) is read per row: a temperature
+ * that is negative or no finite number gives class -1 and NaN, top_k below 1, top_p above 1 or NaN and min_p below 0 or NaN limit
+ * nothing.  Masses are sums of doubles. */
+#define TGBM_F64 3
+#define TGBM_SCORES_MAX_DRAWS 128
+int tgbm_scores_sample(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int draws,
+                       int uniform_type, const void *d_uniform, float temperature, const float *d_temperature, int top_k, const int *d_top_k,
+                       float top_p, const float *d_top_p, float min_p, const float *d_min_p, int *d_classes, float *d_logs, float *d_all_logs,
+                       void *cuda_stream);
+
+/* Loss on classes that were drawn, `draws` per row, and on the gains that followed: with T the temperature, p = softmax(s / T),
+ *   l = log p[class];  r = exp(l - d_old) (d_old NULL: 1, as if drawn now);  held r: r within [1 - clip_low, 1 + clip_high]
+ *   loss = w (mean over the row's draws that count of (-min(r gain, held r gain) + kl (exp(x) - x - 1)) - entropy H)
+ * with x = d_reference - l, H = -sum p log p and w = d_weights[n] (NULL: 1).  d_classes, d_gains, d_old, d_reference and d_logs are n_rows x draws.
+ * A draw counts unless its class lies outside [0, n_classes) or its score is -infinity; a row without one has loss 0 and no gradient.  What
+ * weighs 0 (a gain, kl, entropy, a row by w) counts for nothing.  clip_low 1 and clip_high infinity: r is not held.  kl above 0 needs d_reference.
+ * d_loss: n_rows floats, or NULL; d_logs (or NULL): l, -infinity where the draw does not count.
+ * gives: as for tgbm_scores_distill; pairs have hessian = max(2 w / T^2 (mean |d loss of a draw / d l| + entropy) p (1 - p), 1e-16). */
+int tgbm_scores_feedback(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int draws,
+                         const int *d_classes, const float *d_gains, const float *d_old, const float *d_reference, const float *d_weights,
+                         float temperature, float clip_low, float clip_high, float kl, float entropy, float *d_loss, float *d_logs, int gives,
+                         void *d_grad, long long grad_row_stride, long long grad_class_stride, void *cuda_stream);
+
+/* Every row at mean 0 and variance 1 over its classes, then a gain and a bias per class:
+ *   out_k = (s_k - mean) rstd gain_k + bias_k,  rstd = 1 / sqrt(variance + eps)
+ * over the classes whose score is not -infinity; those stay -infinity.  A row without another class has mean 0 and rstd 0.  d_out: the type
+ * of the scores, strides of its own; d_out = d_scores with the same strides works in place, otherwise the two must not share memory.
+ * d_gain, d_bias: n_classes floats, NULL: 1, 0.  d_mean, d_rstd: n_rows floats, or NULL.  eps > 0. */
+int tgbm_scores_norm(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, void *d_out,
+                     long long out_row_stride, long long out_class_stride, const float *d_gain, const float *d_bias, float eps, float *d_mean,
+                     float *d_rstd, void *cuda_stream);
+
+/* The way back: with x_k = (s_k - mean) rstd and g the gradient of out (`d_grad`, the type of the scores), a_k = g_k gain_k,
+ *   d_out_k = rstd (a_k - mean(a) - x_k mean(a x));  d_grad_gain_k = sum over rows of g_k x_k;  d_grad_bias_k = sum over rows of g_k
+ * means over the classes that the row may have; where a score is -infinity g is not looked at and d_out is 0.  d_mean, d_rstd: from
+ * tgbm_scores_norm.  d_grad_gain and d_grad_bias: n_classes floats, both or both NULL; where they are wanted, d_work is memory of at least
+ * tgbm_scores_norm_work(n_rows, n_classes) bytes, aligned to 16, of which nothing is kept.  Sums are made in the same order every time.
+ * d_out may not share memory with d_grad or d_scores. */
+long long tgbm_scores_norm_work(int n_rows, int n_classes);
+int tgbm_scores_norm_backward(int n_rows, int n_classes, int type, const void *d_grad, long long grad_row_stride, long long grad_class_stride,
+                              const void *d_scores, long long row_stride, long long class_stride, const float *d_mean, const float *d_rstd,
+                              const float *d_gain, void *d_out, long long out_row_stride, long long out_class_stride, float *d_grad_gain,
+                              float *d_grad_bias, void *d_work, long long work_bytes, void *cuda_stream);
 
 /* A model's raw scores (as sparse_predict_scikit and dense_predict_scikit compute them, before the objective's transformation) through
  * tgbm_scores_adjust and tgbm_scores_top, from and to HOST arrays: the `top` best classes of every row under the caller's rules.  For models of

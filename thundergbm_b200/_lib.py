@@ -76,6 +76,11 @@ def load() -> C.CDLL:
     lib.tgbm_scores_adjust.argtypes = [i32, i32, i32, vp, ll, ll, vp, ll, ll, vp, vp, i32, ll, vp, vp, vp, ll, f32, f32, f32, vp]
     lib.tgbm_scores_top.argtypes = [i32, i32, i32, vp, ll, ll, i32, f32, vp, vp, vp, vp]
     lib.tgbm_scores_distill.argtypes = [i32, i32, i32, vp, ll, ll, i32, vp, ll, i32, vp, ll, vp, vp, vp, f32, f32, vp, i32, vp, ll, ll, vp]
+    lib.tgbm_scores_sample.argtypes = [i32, i32, i32, vp, ll, ll, i32, i32, vp, f32, vp, i32, vp, f32, vp, f32, vp, vp, vp, vp, vp]
+    lib.tgbm_scores_feedback.argtypes = [i32, i32, i32, vp, ll, ll, i32, vp, vp, vp, vp, vp, f32, f32, f32, f32, f32, vp, vp, i32, vp, ll, ll, vp]
+    lib.tgbm_scores_norm.argtypes = [i32, i32, i32, vp, ll, ll, vp, ll, ll, vp, vp, f32, vp, vp, vp]
+    lib.tgbm_scores_norm_work.argtypes, lib.tgbm_scores_norm_work.restype = [i32, i32], ll
+    lib.tgbm_scores_norm_backward.argtypes = [i32, i32, i32, vp, ll, ll, vp, ll, ll, vp, vp, vp, vp, ll, ll, vp, vp, vp, ll, vp]
     lib.sparse_train_scikit.argtypes = [C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_int, C.c_float, C.c_float,
                                         C.c_float, C.c_int, C.c_int, C.c_float, C.c_int, C.c_int, C.c_float,
                                         C.c_char_p, ip, C.c_char_p, vp, ip, vp, vp, C.c_int]

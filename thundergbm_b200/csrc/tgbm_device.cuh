@@ -96,6 +96,32 @@ inline void allow_shared(void (*kernel)(P...), size_t most) {
     TGBM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
 }
 
+// ------------------------------------------------------------------ objectives
+// block-wide maximum of |g| and h, then one atomic pair per block (every thread of the block must call it)
+__device__ inline void track_max(float ag, float h, unsigned *maxbits) {
+    // non-negative floats order like their bit patterns
+    __shared__ unsigned smax[2][32];
+    unsigned a = __float_as_uint(ag), b = __float_as_uint(h);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
+    if (lane == 0) { smax[0][warp] = a; smax[1][warp] = b; }
+    __syncthreads();
+    if (warp == 0) {
+        a = lane < nw ? smax[0][lane] : 0u;
+        b = lane < nw ? smax[1][lane] : 0u;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+            b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+        }
+        if (lane == 0) { atomicMax(maxbits, a); atomicMax(maxbits + 1, b); }
+    }
+}
+
 // ---- portable expf ------------------------------------------------------------------------
 // Cody-Waite reduction and a degree-5 polynomial written with explicit IEEE fp32 operations
 // only, so that a host restatement of the same lines gives the same bits.  Replaces expf in

@@ -447,32 +447,6 @@ static __global__ void k_map_labels(float *__restrict__ y, int n, const float *_
     }
 }
 
-// ------------------------------------------------------------------ objectives
-// block-wide maximum of |g| and h, then one atomic pair per block (every thread of the block must call it)
-__device__ inline void track_max(float ag, float h, unsigned *maxbits) {
-    // non-negative floats order like their bit patterns
-    __shared__ unsigned smax[2][32];
-    unsigned a = __float_as_uint(ag), b = __float_as_uint(h);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-        b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-    }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = (blockDim.x + 31) >> 5;
-    if (lane == 0) { smax[0][warp] = a; smax[1][warp] = b; }
-    __syncthreads();
-    if (warp == 0) {
-        a = lane < nw ? smax[0][lane] : 0u;
-        b = lane < nw ? smax[1][lane] : 0u;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-            b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-        }
-        if (lane == 0) { atomicMax(maxbits, a); atomicMax(maxbits + 1, b); }
-    }
-}
-
 // SquareLoss / LogisticLoss gradients (include/thundergbm/objective/regression_obj.h:129-154)
 __device__ __forceinline__ float2 pointwise_gh(int logistic, float y, float yp) {
     if (logistic) {

@@ -12,6 +12,7 @@
 #include "../../include/thundergbm.h"
 #include "tgbm_kernels.cuh"
 #include "tgbm_scores.cuh"
+#include "tgbm_scores_check.h"
 
 namespace tgbm {
 namespace {
@@ -19,24 +20,6 @@ namespace cg = cooperative_groups;
 
 constexpr int ROW_THREADS = 256;
 constexpr int FEW = 32, FEW_THREADS = 128;   // classes that a thread's registers hold, rows of a block then
-
-template <typename T> struct Scores {
-    T *p;
-    long long row, cls;
-    __device__ __forceinline__ T *at(long long n, long long k) const { return p + n * row + k * cls; }
-    __device__ __forceinline__ float operator()(long long n, long long k) const { return score_f32(*at(n, k)); }
-};
-template <typename T> Scores<T> scores_of(const ScoreView &v) { return Scores<T>{static_cast<T *>(v.data), v.row, v.cls}; }
-
-// f<T>() for the element type
-template <typename F> void by_type(int type, F &&f) {
-    switch (type) {
-    case SCORE_F32: f(float{}); break;
-    case SCORE_F16: f(__half{}); break;
-    case SCORE_BF16: f(__nv_bfloat16{}); break;
-    default: throw Error("unknown type of scores");
-    }
-}
 
 // ------------------------------------------------------------------ adjust
 // A block takes a tile of rows x classes.  How often a class stands in the history of its row is counted in shared memory: every
@@ -1231,7 +1214,7 @@ __global__ void __launch_bounds__(TILE_THREADS, E == 32 ? 2 : 4) k_distill_tile(
 // three blocks per SM instead of four 54, with five (and fewer registers) 68.  With four the compiler spills 24 to 44 bytes a thread where a
 // warp has 32 classes.)
 // The cells of listed classes and labels are written over what they get with the others.
-constexpr int CLASS_ROWS = 32, CLASS_MOST = 1024;
+constexpr int CLASS_ROWS = 32;
 
 struct ListSums {   // of a row's list
     TeacherSide teacher;
@@ -1888,7 +1871,7 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
             return;
         }
         const bool by_class = a.in.row < a.in.cls || a.in.one_by_class;
-        if (by_class && a.k <= CLASS_MOST && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
+        if (by_class && a.k <= SCORES_CLASS_MOST && std::max(a.in.cls, a.out.cls) <= INT_MAX) {
             const size_t smem = 12 * (size_t)CLASS_ROWS * a.top;
             const unsigned blocks = (unsigned)(((long long)a.n + CLASS_ROWS - 1) / CLASS_ROWS);
             auto go = [&](auto kern, int warps) {
@@ -1935,76 +1918,7 @@ void scores_distill(const DistillArgs &given, cudaStream_t stream) {
 }  // namespace tgbm
 
 // ------------------------------------------------------------------ C entries
-namespace {
 using namespace tgbm;
-
-int size_of(int type) { return type == SCORE_F32 ? 4 : 2; }
-
-ScoreView view_of(const char *what, const void *data, int type, int n, int k, long long row, long long cls, bool written) {
-    const std::string w(what);
-    TGBM_CHECK(type >= SCORE_F32 && type <= SCORE_BF16, w + ": unknown type");
-    TGBM_CHECK(data != nullptr, w + ": null pointer");
-    TGBM_CHECK(reinterpret_cast<uintptr_t>(data) % size_of(type) == 0, w + ": not aligned for its type");
-    // (beyond CLASS_MOST only where nothing else tells the layout: a slice of one such row is left to the kernels for any stride)
-    const bool one_by_class = n == 1 && row >= 1 && (row == cls || (row < cls && k <= CLASS_MOST));
-    if (n == 1) row = k == 1 ? 1 : cls * k;   // a stride that no step takes
-    if (k == 1) cls = row * n;
-    TGBM_CHECK(row >= 0 && cls >= 0, w + ": negative stride");
-    const long long most = LLONG_MAX / 16;
-    TGBM_CHECK(row <= most / n && cls <= most / k, w + ": stride too large");
-    if (written) TGBM_CHECK((row >= 1 && cls > (n - 1) * row) || (cls >= 1 && row > (k - 1) * cls), w + ": strides under which cells share memory");
-    ScoreView v;
-    v.data = const_cast<void *>(data); v.type = type; v.row = row; v.cls = cls; v.one_by_class = one_by_class;
-    return v;
-}
-
-// whether two matrices of n x k share memory (true also where that is not easily told)
-bool share_memory(const ScoreView &a, int a_size, const ScoreView &b, int b_size, int n, int k) {
-    auto end = [&](const ScoreView &v, int size) { return reinterpret_cast<uintptr_t>(v.data) + size * (uintptr_t)((n - 1) * v.row + (k - 1) * v.cls + 1); };
-    const uintptr_t pa = reinterpret_cast<uintptr_t>(a.data), pb = reinterpret_cast<uintptr_t>(b.data);
-    if (end(a, a_size) <= pb || end(b, b_size) <= pa) return false;
-    if (a_size != b_size || a.row != b.row || a.cls != b.cls || (pa > pb ? pa - pb : pb - pa) % a_size) return true;
-    // parts of one larger matrix, side by side: `d` cells apart are `over` lines and `in` cells
-    const long long d = (long long)((pa > pb ? pa - pb : pb - pa) / a_size);
-    const bool by_row = a.cls <= a.row;
-    const long long line = by_row ? a.row : a.cls, step = by_row ? a.cls : a.row;
-    const long long lines = by_row ? n : k, cells = by_row ? k : n;
-    if (line <= 0) return true;
-    const long long over = d / line, in = d % line, width = (cells - 1) * step + 1;
-    return (in < width && over < lines) || (line - in < width && over + 1 < lines);
-}
-
-// Does [p, p + bytes) hold cells of the matrix?  (Where neither stride is 1 the gaps within a line count as cells.)
-bool lies_in(const ScoreView &v, int size, int n, int k, const void *p, long long bytes) {
-    if (!p || bytes <= 0) return false;
-    const bool by_row = n > 1 && (k == 1 || v.cls <= v.row);
-    const long long lines = by_row ? n : k, apart = size * (by_row ? v.row : v.cls), width = size * (by_row ? (k - 1) * v.cls + 1 : (n - 1) * v.row + 1);
-    const long long lo = (long long)(reinterpret_cast<uintptr_t>(p) - reinterpret_cast<uintptr_t>(v.data)), hi = lo + bytes;
-    if (hi <= 0 || lo >= (lines - 1) * apart + width) return false;
-    return lo < width || ((lo - width) / apart + 1) * apart < hi;   // (the first line that ends behind `lo`)
-}
-
-void check_pointer(const char *what, const void *p, size_t size) {
-    TGBM_CHECK(reinterpret_cast<uintptr_t>(p) % size == 0, std::string(what) + ": not aligned for its type");
-}
-void check_shape(int n, int k) {
-    TGBM_CHECK(n >= 0, "negative number of rows");
-    TGBM_CHECK(k >= 1 && k <= TGBM_SCORES_MAX_CLASSES, "number of classes outside [1, " + std::to_string(TGBM_SCORES_MAX_CLASSES) + "]");
-}
-void check_temperature(float t) { TGBM_CHECK(temperature_fits(t), "the temperature has to be a positive number"); }
-void check_list(int top) { TGBM_CHECK(top >= 1 && top <= TGBM_SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(TGBM_SCORES_MAX_TOP) + "]"); }
-
-template <typename F> int scores_call(F &&f) {
-    try {
-        set_last_error("");
-        f();
-        return 0;
-    } catch (const std::exception &e) {
-        set_last_error(e.what());
-        return 1;
-    }
-}
-}  // namespace
 
 extern "C" {
 

@@ -18,6 +18,24 @@ template <> __device__ __forceinline__ float score_from<float>(float v) { return
 template <> __device__ __forceinline__ __half score_from<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 score_from<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+template <typename T> struct Scores {
+    T *p;
+    long long row, cls;
+    __device__ __forceinline__ T *at(long long n, long long k) const { return p + n * row + k * cls; }
+    __device__ __forceinline__ float operator()(long long n, long long k) const { return score_f32(*at(n, k)); }
+};
+template <typename T> Scores<T> scores_of(const ScoreView &v) { return Scores<T>{static_cast<T *>(v.data), v.row, v.cls}; }
+
+// f<T>() for the element type
+template <typename F> inline void by_type(int type, F &&f) {
+    switch (type) {
+    case SCORE_F32: f(float{}); break;
+    case SCORE_F16: f(__half{}); break;
+    case SCORE_BF16: f(__nv_bfloat16{}); break;
+    default: throw Error("unknown type of scores");
+    }
+}
+
 constexpr float LOG2E = 1.44269504088896341f;
 __device__ __forceinline__ float minus_inf() { return __int_as_float(0xff800000); }
 
