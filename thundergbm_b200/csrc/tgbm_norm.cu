@@ -4,24 +4,27 @@
 #include <climits>
 #include <cmath>
 
+#include <cooperative_groups.h>
+
 #include "../../include/thundergbm.h"
 #include "tgbm_scores.cuh"
 #include "tgbm_scores_check.h"
 
 namespace tgbm {
 namespace {
+namespace cg = cooperative_groups;
 
 constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32;
 
 // sum over the block, the same in all threads and every time; `parts`: one per warp
-template <typename V> __device__ __forceinline__ V block_sum(V v, V *parts) {
+template <int W = ROW_WARPS, typename V> __device__ __forceinline__ V block_sum(V v, V *parts) {
     v = warp_sum(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
     __syncthreads();
     V s = parts[0];
 #pragma unroll
-    for (int i = 1; i < ROW_WARPS; ++i) s += parts[i];
+    for (int i = 1; i < W; ++i) s += parts[i];
     return s;
 }
 
@@ -88,6 +91,428 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_backward_any(NormBackwardA
     }
 }
 
+// ---- by class: a lane has a row, the W warps of a block (W = 1: each for itself) share its classes, E in a row each ---------------
+// Scores stay in registers from the read to the write.
+__device__ __forceinline__ bool there(float x) { return x != minus_inf(); }
+
+// Sums of two numbers over the warps that share a lane's row, the same order in every warp; `turn` alternates, so that nothing is written over
+// that is still read.  From 16 warps on a warp adds for a row or two what all of them have, for all of them.
+template <int W> struct Shared {
+    float2 v[2][W > 1 ? W : 1][33];
+    float2 sum[2][32];
+};
+template <int W> __device__ __forceinline__ float2 over_warps(Shared<W> &sh, int turn, float2 v) {
+    if constexpr (W > 1) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        sh.v[turn][warp][lane] = v;
+        __syncthreads();
+        if constexpr (W <= 8) {
+            v = sh.v[turn][0][lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v = add2(v, sh.v[turn][w][lane]);
+        } else {
+#pragma unroll
+            for (int r = warp; r < 32; r += W) {
+                float2 u = sh.v[turn][lane & (W - 1)][r];
+#pragma unroll
+                for (int o = W / 2; o > 0; o >>= 1) u = add2(u, make_float2(__shfl_xor_sync(0xffffffffu, u.x, o), __shfl_xor_sync(0xffffffffu, u.y, o)));
+                if (lane == 0) sh.sum[turn][r] = u;
+            }
+            __syncthreads();
+            v = sh.sum[turn][lane];
+        }
+    }
+    return v;
+}
+// Scores k0, k0 + 1, ... of a lane's row, -inf behind the last class; what steps along the classes is one instruction per address.
+template <int E, typename T> __device__ __forceinline__ void read_classes(const T *from, int cls, int here, float none, float (&x)[E]) {
+    T raw[E];
+    if (here >= E) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) raw[j] = from[(long long)j * cls];
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) raw[j] = j < here ? from[(long long)j * cls] : score_from<T>(none);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) x[j] = score_f32(raw[j]);
+}
+template <int E, typename T, typename F> __device__ __forceinline__ void write_classes(T *to, int cls, int here, F &&value) {
+    if (here >= E) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) to[(long long)j * cls] = score_from<T>(value(j));
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (j < here) to[(long long)j * cls] = score_from<T>(value(j));
+    }
+}
+
+template <typename T, int E, int W, bool WEIGHTS>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_norm_class(NormArgs a, Scores<T> in, Scores<T> out) {
+    __shared__ Shared<W> sh;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k0 = W == 1 ? 0 : warp * E, here = a.k - k0;
+    const long long n0 = W == 1 ? (blockIdx.x * 4ll + warp) * 32 + lane : blockIdx.x * 32ll + lane, n = min(n0, a.n - 1ll);
+    float x[E];
+    read_classes<E>(in.at(n, k0), (int)in.cls, here, minus_inf(), x);
+    float s = 0, c = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (there(x[j])) { s += x[j]; c += 1.f; }
+    const float2 first = over_warps(sh, 0, make_float2(s, c));
+    const float inv = 1.f / fmaxf(first.y, 1.f), mean = first.x * inv;
+    float q = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const float d = __fsub_rn(x[j], mean);
+        if (there(x[j])) q = __fmaf_rn(d, d, q);
+    }
+    q = over_warps(sh, 1, make_float2(q, 0.f)).x;
+    const float rstd = first.y != 0.f ? 1.f / sqrtf(q * inv + a.eps) : 0.f;
+    if (n0 != n) return;
+    if (k0 == 0) {
+        if (a.mean) a.mean[n] = mean;
+        if (a.rstd) a.rstd[n] = rstd;
+    }
+    const float by = first.y != 0.f ? rstd : 1.f;   // (-inf stays what it is)
+    const float *gain = a.gain ? a.gain + k0 : nullptr, *bias = a.bias ? a.bias + k0 : nullptr;
+    write_classes<E>(out.at(n, k0), (int)out.cls, here, [&](int j) {
+        const float y = __fsub_rn(x[j], mean) * by;
+        if (!WEIGHTS) return y;
+        return there(x[j]) ? __fmaf_rn(y, gain ? __ldg(gain + j) : 1.f, bias ? __ldg(bias + j) : 0.f) : x[j];
+    });
+}
+
+// ---- by row, up to 1024 classes: L lanes have a row, E classes each, L apart -----------------------------------------
+template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v) {
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <typename T, int L, int E>
+__global__ void __launch_bounds__(ROW_THREADS) k_norm_row(NormArgs a, Scores<T> in, Scores<T> out) {
+    constexpr int R = ROW_THREADS / L;
+    const int l = threadIdx.x & (L - 1), K = a.k;
+    const long long n0 = blockIdx.x * (long long)R + threadIdx.x / L, n = min(n0, a.n - 1ll);
+    float x[E];
+    {
+        const T *from = in.at(n, l);
+        T raw[E];
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (l + j * L < K) raw[j] = from[(long long)j * L * in.cls];
+#pragma unroll
+        for (int j = 0; j < E; ++j) x[j] = l + j * L < K ? score_f32(raw[j]) : minus_inf();
+    }
+    float s = 0;
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (there(x[j])) { s += x[j]; ++c; }
+    s = lanes_sum<L>(s); c = lanes_sum<L>(c);
+    const float inv = 1.f / (float)max(c, 1), mean = s * inv;
+    float q = 0;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+        const float d = __fsub_rn(x[j], mean);
+        if (there(x[j])) q = __fmaf_rn(d, d, q);
+    }
+    q = lanes_sum<L>(q);
+    const float rstd = c ? 1.f / sqrtf(q * inv + a.eps) : 0.f;
+    if (n0 != n) return;
+    if (l == 0) {
+        if (a.mean) a.mean[n] = mean;
+        if (a.rstd) a.rstd[n] = rstd;
+    }
+    T *to = out.at(n, l);
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (l + j * L < K) {
+            const float y = __fsub_rn(x[j], mean) * rstd;
+            to[(long long)j * L * out.cls] = score_from<T>(!there(x[j]) ? x[j] : __fmaf_rn(y, a.gain ? a.gain[l + j * L] : 1.f, a.bias ? a.bias[l + j * L] : 0.f));
+        }
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// ---- long rows: a block, or a cluster of blocks, each with a part of the row in its registers -------------------------------
+// A thread's scores: packs of 16 bytes, TH packs apart (EVEN: rows, gains and results all begin on such boundaries), or single ones, TH apart.
+constexpr int LONG_CLUSTER = 8;
+
+template <typename T, int TH, int P, bool EVEN> struct Hold {
+    static constexpr int V = EVEN ? Pack<T>::V : 1, E = P * V;
+    static constexpr int CELLS = TH * E;   // of a block
+    static __device__ __forceinline__ int first(int u) { return (u * TH + (int)threadIdx.x) * V; }
+    Pack<T> w[EVEN ? P : 1];
+    T one[EVEN ? 1 : P];
+    __device__ __forceinline__ void read(const T *p, int cells) {   // cells: of the part (EVEN: whole packs)
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+            if (cells == CELLS || first(u) < cells) {
+                if constexpr (EVEN) w[u].bits = __ldg(reinterpret_cast<const uint4 *>(p + first(u)));
+                else one[u] = p[first(u)];
+            }
+    }
+    __device__ __forceinline__ void get(int u, float (&v)[V]) const {
+        if constexpr (EVEN) w[u].unpack(v);
+        else v[0] = score_f32(one[u]);
+    }
+    // cells h to h + Q of pack u
+    template <int Q> __device__ __forceinline__ void get_some(int u, int h, float (&v)[Q]) const {
+        if constexpr (!EVEN) v[0] = score_f32(one[u]);
+        else if constexpr (Q == V) w[u].unpack(v);
+        else {
+            float all[V];
+            w[u].unpack(all);
+#pragma unroll
+            for (int i = 0; i < Q; ++i) v[i] = all[h + i];
+        }
+    }
+    template <int Q> __device__ __forceinline__ void set_some(int u, int h, const float (&v)[Q]) {
+        if constexpr (!EVEN) one[u] = score_from<T>(v[0]);
+        else if constexpr (Q == V) w[u].pack(v);
+        else {
+            Pack<T> some;
+            float all[V] = {};
+#pragma unroll
+            for (int i = 0; i < Q; ++i) all[i] = v[i];
+            some.pack(all);
+            if (h == 0) { w[u].bits.x = some.bits.x; w[u].bits.y = some.bits.y; }
+            else { w[u].bits.z = some.bits.x; w[u].bits.w = some.bits.y; }
+        }
+    }
+    __device__ __forceinline__ void write(T *p, int u) const {
+        if constexpr (EVEN) *reinterpret_cast<uint4 *>(p + first(u)) = w[u].bits;
+        else p[first(u)] = one[u];
+    }
+};
+template <int V> __device__ __forceinline__ void read_floats(const float *p, float none, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = p ? __ldg(p) : none;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 f = p ? __ldg(reinterpret_cast<const float4 *>(p + i)) : make_float4(none, none, none, none);
+            v[i] = f.x; v[i + 1] = f.y; v[i + 2] = f.z; v[i + 3] = f.w;
+        }
+    }
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    unsigned long long r, x = *reinterpret_cast<unsigned long long *>(&a), y = *reinterpret_cast<unsigned long long *>(&b), z = *reinterpret_cast<unsigned long long *>(&c);
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
+
+// Sums of M numbers over a warp (M a power of two up to 32): lanes exchange half of what they hold until each holds one.  Lane l has the sum
+// of number l / (32 / M).
+template <int M> __device__ __forceinline__ float sums_spread(float (&v)[M]) {
+    const int lane = threadIdx.x & 31;
+    int o = 16;
+#pragma unroll
+    for (int m = M; m > 1; m >>= 1, o >>= 1) {
+        const bool upper = lane & o;
+#pragma unroll
+        for (int i = 0; i < m / 2; ++i) {
+            const float give = upper ? v[i] : v[i + m / 2], keep = upper ? v[i + m / 2] : v[i];
+            v[i] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
+    }
+    for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    return v[0];
+}
+// sums of M numbers over a block of TH threads, the same in all of them; all threads, with two barriers
+template <int TH, int M> struct LongSums {
+    float part[TH / 32][M], sum[M];
+};
+template <int TH, int M> __device__ __forceinline__ void long_sums(LongSums<TH, M> &sh, float (&v)[M]) {
+    constexpr int W = TH / 32, PER = 32 / M;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float s = sums_spread<M>(v);
+    if (lane % PER == 0) sh.part[warp][lane / PER] = s;
+    __syncthreads();
+    if (warp < M) {
+        const float t = lanes_sum<W>(sh.part[lane & (W - 1)][warp]);
+        if (lane == 0) sh.sum[warp] = t;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int m = 0; m < M; ++m) v[m] = sh.sum[m];
+}
+
+// R rows at a time: gains and biases are read once for all of them (for one row of 16-bit scores they are four times its bytes, from the L2 cache),
+// and barriers and exchanges are shared.  A row whose sum is finite holds no -inf, so only the others look at every score whether it is there.
+template <int TH, int R> struct LongShared {
+    LongSums<TH, R> sum, square;
+    float part[TH / 32], moments[R][3], of_row[R][2];
+};
+template <typename T, int TH, int P, int R, bool EVEN, bool FULL>
+__device__ __forceinline__ void norm_long(const NormArgs &a, const Scores<T> &in, const Scores<T> &out, LongShared<TH, R> &sh) {
+    typedef Hold<T, TH, P, EVEN> H;
+    constexpr int V = H::V;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const long long n0 = (long long)(blockIdx.x / C) * R;
+    const int lo = rank * H::CELLS, cells = FULL ? H::CELLS : min(a.k - lo, H::CELLS), rows = (int)min((long long)R, a.n - n0);   // (no block is without a cell)
+    H x[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) x[r].read(in.at(n0 + min(r, rows - 1), lo), cells);
+    auto each = [&](int r, auto &&f) {
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+            if (FULL || H::first(u) < cells) {
+                float v[V];
+                x[r].get(u, v);
+                f(v);
+            }
+    };
+    float mean[R], square[R], count[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        float2 s = make_float2(0.f, 0.f);
+        each(r, [&](const float (&v)[V]) {
+            if constexpr (V == 1) s.x += v[0];
+            else {
+#pragma unroll
+                for (int i = 0; i < V; i += 2) s = add2(s, make_float2(v[i], v[i + 1]));
+            }
+        });
+        mean[r] = s.x + s.y;
+    }
+    long_sums<TH>(sh.sum, mean);
+    bool masked = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        count[r] = (float)cells;
+        masked |= !finite(mean[r]);
+    }
+    if (masked) {   // (the same in all threads)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (finite(mean[r])) continue;
+            float s = 0, c = 0;
+            each(r, [&](const float (&v)[V]) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (there(v[i])) { s += v[i]; c += 1.f; }
+            });
+            mean[r] = block_sum<TH / 32>(s, sh.part);
+            count[r] = block_sum<TH / 32>(c, sh.part);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        mean[r] *= 1.f / fmaxf(count[r], 1.f);
+        const float2 m = make_float2(-mean[r], -mean[r]);
+        float2 s = make_float2(0.f, 0.f);
+        if (!masked) {
+            each(r, [&](const float (&v)[V]) {
+                if constexpr (V == 1) {
+                    const float d = __fsub_rn(v[0], mean[r]);
+                    s.x = __fmaf_rn(d, d, s.x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) {
+                        const float2 d = add2(make_float2(v[i], v[i + 1]), m);
+                        s = fma2(d, d, s);
+                    }
+                }
+            });
+        } else {
+            each(r, [&](const float (&v)[V]) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float d = __fsub_rn(v[i], mean[r]);
+                    if (there(v[i])) s.x = __fmaf_rn(d, d, s.x);
+                }
+            });
+        }
+        square[r] = s.x + s.y;
+    }
+    {   // of the parts' counts, means and squares those of the row; a warp per row
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const float s = sums_spread<R>(square);
+        if (lane % (32 / R) == 0) sh.square.part[warp][lane / (32 / R)] = s;
+        __syncthreads();
+        if (warp < R) {
+            const float t = lanes_sum<TH / 32>(sh.square.part[lane & (TH / 32 - 1)][warp]);
+            if (lane == 0) {
+                float m = mean[0], c = count[0];
+#pragma unroll
+                for (int r = 1; r < R; ++r)
+                    if (warp == r) { m = mean[r]; c = count[r]; }
+                sh.moments[warp][0] = c; sh.moments[warp][1] = m; sh.moments[warp][2] = t;
+            }
+            __syncwarp();
+        }
+        if (C > 1) cluster.sync();
+        if (warp < R) {
+            float c = 0, m = 0, q = 0;
+            if (lane < C) {
+                const float *o = C > 1 ? cluster.map_shared_rank(sh.moments[warp], lane) : sh.moments[warp];
+                c = o[0]; m = o[1]; q = o[2];
+            }
+            const float all = lanes_sum<LONG_CLUSTER>(c), whole = lanes_sum<LONG_CLUSTER>(c * m) / fmaxf(all, 1.f), d = __fsub_rn(m, whole);
+            const float sum = lanes_sum<LONG_CLUSTER>(c == 0.f ? 0.f : __fmaf_rn(c * d, d, q));
+            if (lane == 0) {
+                const float by = all != 0.f ? 1.f / sqrtf(sum / all + a.eps) : 0.f;
+                sh.of_row[warp][0] = whole; sh.of_row[warp][1] = by;
+                if (rank == 0 && warp < rows) {
+                    if (a.mean) a.mean[n0 + warp] = whole;
+                    if (a.rstd) a.rstd[n0 + warp] = by;
+                }
+            }
+        }
+        if (C > 1) cluster_arrive();
+        __syncthreads();
+    }
+    float rstd[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) { mean[r] = sh.of_row[r][0]; rstd[r] = sh.of_row[r][1]; }
+#pragma unroll
+    for (int u = 0; u < P; ++u)
+        if (FULL || H::first(u) < cells) {
+            constexpr int Q = V < 4 ? V : 4;   // (four at a time: fewer registers)
+#pragma unroll
+            for (int h = 0; h < V; h += Q) {
+                float g[Q], b[Q];
+                read_floats<Q>(a.gain ? a.gain + lo + H::first(u) + h : nullptr, 1.f, g);
+                read_floats<Q>(a.bias ? a.bias + lo + H::first(u) + h : nullptr, 0.f, b);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    float f[Q];
+                    x[r].get_some(u, h, f);
+                    if (V == 1 || masked) {
+#pragma unroll
+                        for (int i = 0; i < Q; ++i)
+                            if (there(f[i])) f[i] = __fmaf_rn(__fsub_rn(f[i], mean[r]) * rstd[r], g[i], b[i]);
+                    } else {
+                        const float2 m = make_float2(-mean[r], -mean[r]), by = make_float2(rstd[r], rstd[r]);
+#pragma unroll
+                        for (int i = 0; i + 1 < Q; i += 2) {
+                            const float2 y = fma2(mul2(add2(make_float2(f[i], f[i + 1]), m), by), make_float2(g[i], g[i + 1]), make_float2(b[i], b[i + 1]));
+                            f[i] = y.x; f[i + 1] = y.y;
+                        }
+                    }
+                    x[r].set_some(u, h, f);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (r < rows) x[r].write(out.at(n0 + r, lo), u);
+        }
+    if (C > 1) cluster_wait();   // (no block leaves while another may still read its moments)
+}
+template <typename T, int TH, int P, int R, bool EVEN>
+__global__ void __launch_bounds__(TH, 1024 / TH) k_norm_long(NormArgs a, Scores<T> in, Scores<T> out) {
+    __shared__ LongShared<TH, R> sh;
+    const int C = (int)cg::this_cluster().num_blocks();
+    if (a.k == C * Hold<T, TH, P, EVEN>::CELLS) norm_long<T, TH, P, R, EVEN, true>(a, in, out, sh);
+    else norm_long<T, TH, P, R, EVEN, false>(a, in, out, sh);
+}
+
 // Gradients of gain and bias: a block sums a share of the rows for 32 classes, the shares are added in order afterwards.
 constexpr int SHARES = 296;
 inline int shares_of(int n, int k) { return (int)std::max(1ll, std::min<long long>({(long long)SHARES, (n + 31ll) / 32, (1ll << 23) / k + 1})); }
@@ -125,11 +550,95 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_weights_join(NormBackwardA
 }
 }  // namespace
 
+// f(E, W) for kernels by class: E classes of each of W warps
+template <typename F> void by_class_sizes(int k, F &&f) {
+    using std::integral_constant;
+    if (k <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    else if (k <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    else if (k <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    else if (k <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (k <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (k <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (k <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+}
+// f(L, E) for kernels by row: E classes of each of L lanes
+template <typename F> void by_row_sizes(int k, F &&f) {
+    using std::integral_constant;
+    if (k <= 4) f(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    else if (k <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    else if (k <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    else if (k <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    else if (k <= 64) f(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+    else if (k <= 128) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    else if (k <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (k <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+}
+constexpr int ROW_MOST = 1024;   // classes of a row that a warp's registers hold
+
+bool on_16(const void *p, long long row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
+
+template <typename... P, typename... A>
+void launch_long(void (*kernel)(P...), long long rows, int cluster, int threads, cudaStream_t stream, A &&...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = cluster; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
+    TGBM_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
+}
+
 void scores_norm(const NormArgs &a, cudaStream_t stream) {
     if (a.n == 0) return;
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
-        k_norm_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, scores_of<T>(a.in), scores_of<T>(a.out));
+        const Scores<T> in = scores_of<T>(a.in), out = scores_of<T>(a.out);
+        const bool by_class = (in.row < in.cls && out.row < out.cls) || a.in.one_by_class;
+        if (by_class && a.k <= SCORES_CLASS_MOST && std::max(in.cls, out.cls) <= INT_MAX) {
+            by_class_sizes(a.k, [&](auto e, auto w) {
+                constexpr int E = decltype(e)::value, W = decltype(w)::value;
+                const long long rows = W == 1 ? 128 : 32;
+                auto kern = a.gain || a.bias ? k_norm_class<T, E, W, true> : k_norm_class<T, E, W, false>;
+                kern<<<(unsigned)((a.n + rows - 1) / rows), W == 1 ? 128 : 32 * W, 0, stream>>>(a, in, out);
+            });
+            return;
+        }
+        if (a.k <= ROW_MOST) {
+            by_row_sizes(a.k, [&](auto l, auto e) {
+                constexpr int L = decltype(l)::value, E = decltype(e)::value;
+                const long long rows = ROW_THREADS / L;
+                k_norm_row<T, L, E><<<(unsigned)((a.n + rows - 1) / rows), ROW_THREADS, 0, stream>>>(a, in, out);
+            });
+            return;
+        }
+        if (in.cls == 1 && out.cls == 1) {
+            const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T)) && on_16(out.p, out.row, sizeof(T)) && on_16(a.gain, 0, 4) && on_16(a.bias, 0, 4);
+            bool done = false;
+            // Parts of a row that 512 threads hold, and several rows at a time where the rows are many: the smaller parts first, which need more blocks
+            // for a row (at most LONG_CLUSTER) and hold more rows.
+            auto go = [&](auto p, auto rows, auto ev) {
+                constexpr bool EVEN = decltype(ev)::value;
+                constexpr int TH = 512, P = decltype(p)::value, R = decltype(rows)::value;
+                const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
+                if (done || c > LONG_CLUSTER || (R > 1 && (long long)a.n * c < 2 * 148 * R)) return;
+                launch_long(k_norm_long<T, TH, P, R, EVEN>, (a.n + R - 1) / R, c, TH, stream, a, in, out);
+                done = true;
+            };
+            using std::integral_constant;
+            auto all = [&](auto ev) {
+                constexpr int S = decltype(ev)::value ? 2 : 8;   // packs of a quarter of what a thread holds
+                go(integral_constant<int, S>{}, integral_constant<int, 4>{}, ev);
+                go(integral_constant<int, S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 2 * S>{}, integral_constant<int, 2>{}, ev);
+                go(integral_constant<int, 2 * S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 4 * S>{}, integral_constant<int, 1>{}, ev);
+            };
+            even ? all(std::true_type{}) : all(std::false_type{});
+            if (done) return;
+        }
+        k_norm_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, in, out);
     });
     TGBM_CUDA(cudaGetLastError());
 }
