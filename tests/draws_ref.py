@@ -11,13 +11,14 @@ def _per_row(v, n, none):
 
 
 def sample(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
-    """(classes, logs, all_logs, bound on the error of both): masses are doubles, good to 2^-33, and the logs are rounded once"""
+    """(classes, logs, all_logs, bounds on the errors of both): what a draw is left to has its mass in doubles, good to 2^-33, and logs are
+    rounded once; the mass of all classes may be a sum of floats (the relative error of that is the error of its log)"""
     z = z.astype(np.float64)
     n, k = z.shape
     u2 = u.reshape(n, -1).astype(np.float64)
     T, K, P, M = _per_row(temperature, n, 1.0), _per_row(top_k, n, 0), _per_row(top_p, n, 1.0), _per_row(min_p, n, 0.0)
     ids = np.full(u2.shape, -1, np.int32)
-    logs, every = np.full(u2.shape, np.nan), np.full(u2.shape, np.nan)
+    logs, every, off = np.full(u2.shape, np.nan), np.full(u2.shape, np.nan), np.zeros(u2.shape)
     for i in range(n):
         s = z[i]
         if not np.isfinite(T[i]) or T[i] < 0 or np.isnan(s).any() or s.max() == np.inf:
@@ -29,6 +30,7 @@ def sample(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
             ids[i], logs[i], every[i] = np.argmax(s), 0, 0
             continue
         w = np.where(s > -np.inf, np.exp((s - s.max()) / T[i]), 0)
+        off[i] = sum_error((w * np.where(w > 0, (s.max() - s) / T[i], 0)).sum() / w.sum(), k)
         order = np.argsort(-s, kind='stable')
         order = order[s[order] > -np.inf]
         if M[i] > 0:
@@ -46,9 +48,9 @@ def sample(z, u, temperature=1.0, top_k=None, top_p=None, min_p=None):
             v = v if v > 0 else 0.0
             c = min(np.searchsorted(upto, v * upto[-1], side='right'), last)
             ids[i, d], logs[i, d], every[i, d] = c, np.log(w[c] / upto[-1]), np.log(w[c] / w.sum())
-    bound = 2.0 ** -32 + U * SLACK * np.fmax(np.abs(np.where(np.isfinite(logs), logs, 0)), np.abs(np.where(np.isfinite(every), every, 0)))
+    size = lambda v: U * SLACK * np.abs(np.where(np.isfinite(v), v, 0))   # noqa: E731
     shape = u.shape
-    return ids.reshape(shape), logs.reshape(shape), every.reshape(shape), bound.reshape(shape)
+    return ids.reshape(shape), logs.reshape(shape), every.reshape(shape), (2.0 ** -32 + size(logs)).reshape(shape), (off * SLACK + size(every)).reshape(shape)
 
 
 def feedback(s, classes, gains, old=None, reference=None, weights=None, temperature=1.0, clip=None, kl=0.0, entropy=0.0):

@@ -36,10 +36,10 @@ def _check_sample(ops, t, u, limits, what):
     got = scores.sample(t, _dev(torch, u), **given)
     assert torch.equal(t.nan_to_num(nan=9.0), before.nan_to_num(nan=9.0))
     assert got[0].dtype == torch.int32 and got[1].dtype == got[2].dtype == torch.float32 and all(x.shape == u.shape for x in got)
-    ids, logs, every, off = ref.sample(_given(t), u, **limits)
+    ids, logs, every, off, all_off = ref.sample(_given(t), u, **limits)
     assert np.array_equal(got[0].cpu().numpy(), ids), what
     _close(got[1].cpu().numpy(), logs, off, what + ('logs',))
-    _close(got[2].cpu().numpy(), every, off, what + ('all logs',))
+    _close(got[2].cpu().numpy(), every, all_off, what + ('all logs',))
     return ids
 
 
@@ -113,10 +113,10 @@ def test_sample_of_unusual_numbers(ops, kind, layout, n, k):
                 for (name, v), none in zip(limits.items(), (1.0, 0.0, 0) if 'top_p' in limits else (np.nan,) * 3)}
         given = {name: _dev(torch, v) if isinstance(v, np.ndarray) else v for name, v in limits.items()}
         got = ops[1].sample(t, _dev(torch, u), **given)
-        ids, logs, every, off = ref.sample(_given(t), u, **want)
+        ids, logs, every, off, all_off = ref.sample(_given(t), u, **want)
         assert np.array_equal(got[0].cpu().numpy(), ids), limits
         _close(got[1].cpu().numpy(), logs, off, limits)
-        _close(got[2].cpu().numpy(), every, off, limits)
+        _close(got[2].cpu().numpy(), every, all_off, limits)
 
 
 def test_sample_draws_what_it_says(ops):
