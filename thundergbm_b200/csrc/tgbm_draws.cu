@@ -6,12 +6,16 @@
 #include <climits>
 #include <cmath>
 
+#include <cooperative_groups.h>
+
 #include "../../include/thundergbm.h"
 #include "tgbm_scores.cuh"
 #include "tgbm_scores_check.h"
+#include "tgbm_scores_long.cuh"
 
 namespace tgbm {
 namespace {
+namespace cg = cooperative_groups;
 
 constexpr int ROW_THREADS = 256, ROW_WARPS = ROW_THREADS / 32;
 
@@ -278,21 +282,6 @@ template <int W> struct ListShared {
     unsigned short k[MOST][APART];
     int size[32];
 };
-template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-template <int L> __device__ __forceinline__ float lanes_min(float v) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-template <int L> __device__ __forceinline__ float lanes_max(float v) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 template <int W> struct Over {   // `turn` alternates, so that one barrier is enough
     ClassShared<W> &sh;
     int turn = 0;
@@ -799,6 +788,494 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
     }
 }
 
+// ---- long rows: a cluster of up to 8 blocks (or one) holds the row in its registers -------------------------------------------
+// Classes stand in the order block, u, thread, place in the pack (Hold); a segment is what a warp has of one u, 32 packs side by side.
+//
+// Limits: as above the scores that can be left are those from a border on, which is raised by bisection over the registers while more than
+// LONG_WANT reach it.  They go into a list in the first block, in class order, and that block alone goes on: every entry counts the larger ones,
+// which is its place in descending order; prefix sums in that order tell where top_p ends, prefix sums in class order which class a random number
+// falls on.  Rows where more than LONG_LIST are left, and rows without limits, take their draws from sums per segment.
+constexpr int LONG_LIST = 1024, LONG_WANT = 384;
+
+template <int W, int S> struct LongRow {
+    Powers powers;
+    double sums[W], slot_sum[2], sum, front;          // of the warps, of this block (read by the others), of the row, of the blocks in front
+    float lows[W], highs[W], slot_low[2], slot_high[2], low, high;
+    int counts[W], slot_count[2], count, front_count;
+    double segment[S];                                // of a segment, then of all in front of it
+    int segment_count[S];
+    int tie;
+    float x[LONG_LIST];
+    int k[LONG_LIST];
+    double w[LONG_LIST], upto[LONG_LIST];
+};
+
+template <typename T, int TH, int P, bool EVEN>
+__global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) {
+    typedef Hold<T, TH, P, EVEN> H;
+    constexpr int V = H::V, W = TH / 32, S = P * W;
+    __shared__ __align__(16) LongRow<W, S> sh;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long n = blockIdx.x / C;
+    const int lo = rank * H::CELLS, cells = min(a.k - lo, H::CELLS);
+    H hold;
+    hold.read(in.at(n, lo), cells);
+    if (warp == 0) sh.powers.fill();
+    const Limits l = limits_of(a, n);
+    // f(score, class - lo) in class order within u; -inf behind the last class
+    auto each_of = [&](int u, auto &&f) {
+        float v[V];
+        if (H::first(u) < cells) hold.get(u, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) f(H::first(u) < cells ? v[i] : minus_inf(), H::first(u) + i);
+    };
+    auto each = [&](auto &&f) {
+#pragma unroll
+        for (int u = 0; u < P; ++u) each_of(u, f);
+    };
+    // of all threads of all blocks, the same everywhere; front, front_count: of the blocks in front of this one
+    int turn = 0;
+    double front = 0;
+    int front_count = 0;
+    auto total = [&](double &sum, float &low, float &high, int &count) {
+        sum = warp_sum(sum); low = lanes_min<32>(low); high = lanes_max<32>(high); count = warp_sum(count);
+        if (lane == 0) { sh.sums[warp] = sum; sh.lows[warp] = low; sh.highs[warp] = high; sh.counts[warp] = count; }
+        __syncthreads();
+        if (warp == 0) {
+            sum = lanes_sum<W>(sh.sums[lane & (W - 1)]); count = lanes_sum<W>(sh.counts[lane & (W - 1)]);
+            low = lanes_min<W>(sh.lows[lane & (W - 1)]); high = lanes_max<W>(sh.highs[lane & (W - 1)]);
+            if (lane == 0) { sh.slot_sum[turn] = sum; sh.slot_low[turn] = low; sh.slot_high[turn] = high; sh.slot_count[turn] = count; }
+        }
+        if (C > 1) cluster.sync();
+        if (warp == 0) {
+            double before = 0, its = sum;
+            int before_count = 0, its_count = count;
+            if (C > 1) {
+                const LongRow<W, S> *o = cluster.map_shared_rank(&sh, lane < C ? lane : 0);
+                its = o->slot_sum[turn]; its_count = o->slot_count[turn]; low = o->slot_low[turn]; high = o->slot_high[turn];
+                low = lanes_min<LONG_CLUSTER>(low); high = lanes_max<LONG_CLUSTER>(high);
+                sum = 0; count = 0;
+                for (int b = 0; b < C; ++b) {   // one after the other: where one block's part ends the next one's begins
+                    if (b == rank) { before = sum; before_count = count; }
+                    sum += __shfl_sync(0xffffffffu, its, b);
+                    count += __shfl_sync(0xffffffffu, its_count, b);
+                }
+            }
+            if (lane == 0) { sh.sum = sum; sh.low = low; sh.high = high; sh.count = count; sh.front = before; sh.front_count = before_count; }
+        }
+        __syncthreads();
+        sum = sh.sum; low = sh.low; high = sh.high; count = sh.count; front = sh.front; front_count = sh.front_count;
+        turn ^= 1;
+    };
+    // sums of the segments become those of all segments in front; returns the block's
+    auto prefix = [&](auto *of) {
+        auto before = of[0] - of[0];
+        __syncthreads();
+        if (warp == 0) {
+            for (int s = 0; s < S; s += 32) {
+                const auto own = s + lane < S ? of[s + lane] : before - before;
+                auto upto = own;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const auto v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                if (s + lane < S) of[s + lane] = before + (upto - own);
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        __syncthreads();
+    };
+    float top = minus_inf(), low = -minus_inf(), none = 0;
+    double sum = 0;
+    int count = 0;
+    each([&](float x, int) {
+        top = fmaxf(top, x);
+        low = fminf(low, x > minus_inf() ? x : low);
+        count |= x != x;
+    });
+    total(sum, low, top, count);
+    const bool bad = l.broken || count || top == -minus_inf();
+    if (bad || top == minus_inf()) {   // (the same for all blocks; none reads another's memory any more than it did before the last barrier)
+        const float v = bad ? __int_as_float(0x7fffffff) : minus_inf();
+        if (rank == 0)
+            for (int d = tid; d < a.draws; d += TH) put_draw(a, n * a.draws + d, -1, v, v);
+        if (C > 1) cluster.sync();
+        return;
+    }
+    const Exponent weight(l);
+    auto weight_of = [&](float v) { return weight(sh.powers, v, top); };
+    const int top_k = l.greedy ? 1 : l.top_k;
+    const bool by_count = top_k < a.k, by_mass = l.top_p < 1 && !l.greedy, by_share = l.min_p > 0 && !l.greedy;
+    const float lowest_of_all = low;
+    double all = 0;
+    // what is left: larger than `at`, or equal to it and a class up to `last`
+    float at = minus_inf();
+    int last = a.k;
+    auto left = [&](float x, int k) { return x > at || (x == at && x > minus_inf() && lo + k <= last); };
+    // masses of segments, of what is left
+    auto segments = [&] {
+        double s[P], mine = 0;
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+            s[u] = 0;
+            each_of(u, [&](float x, int k) { s[u] += left(x, k) ? weight_of(x) : 0.0; });
+        }
+        constexpr int PER = 32 / P;
+        mine = sums_spread<P>(s);
+        if (lane % PER == 0) {
+            sh.segment[lane / PER * W + warp] = mine;
+            sh.segment_count[lane / PER * W + warp] = mine > 0;
+        }
+        mine = lane % PER == 0 ? mine : 0.0;
+        float f0 = 0, f1 = 0;
+        int c0 = 0;
+        total(mine, f0, f1, c0);
+        prefix(sh.segment);
+        return mine;
+    };
+    double mass = 0;
+    bool listed = false;
+    if (by_count || by_mass || by_share) {
+        if (!by_count && !by_share) {
+            each([&](float x, int) { all += weight_of(x); });
+        } else {
+            const float c = (float)(l.inv_t * 1.4426950408889634);
+            float part = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                float s = 0;
+                each_of(u, [&](float x, int) { s += exp2_fast(__fsub_rn(x, top) * c); });
+                part += s;
+            }
+            all = (double)part;
+        }
+        float f0 = 0, f1 = 0;
+        count = 0;
+        total(all, f0, f1, count);
+        if (l.greedy) all = 1.0;
+        // the border, rounded down as in k_sample_limited; what lies 750 T below the largest score has no mass in any case
+        const float t = (float)(1.0 / l.inv_t);
+        float down = -750.f * t;
+        if (by_share) down = logf((float)l.min_p) * t;
+        else if (by_mass && !by_count) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
+        low = __fadd_rn(top, down) - (fabsf(down) + t + fabsf(top)) * 2e-6f;
+        if (l.greedy) low = top;
+        if (!(low <= top)) low = lowest_of_all;
+        low = fmaxf(low, lowest_of_all);
+        count = 0;
+        each([&](float x, int) { count += x >= low; });
+        total(sum, f0, f1, count);
+        float high = top;
+        bool narrowing = count > LONG_WANT && (by_count ? top_k <= LONG_LIST : by_mass && !by_share);
+        const double enough = by_count ? (double)top_k : l.top_p * all * (1 + 1e-9);
+        const int want = max(LONG_WANT, by_count ? top_k : 0);
+        while (narrowing && count > want && low < high) {
+            const float mid = middle(low, high);
+            float up = -minus_inf(), below = minus_inf();
+            int reach = 0;
+            sum = 0;
+            each([&](float x, int) {
+                if (x >= mid) {
+                    ++reach;
+                    up = fminf(up, x);
+                    if (!by_count) sum += weight_of(x);
+                } else if (x >= low) {
+                    below = fmaxf(below, x);
+                }
+            });
+            total(sum, up, below, reach);
+            if ((by_count ? (double)reach : sum) >= enough) { low = up; count = reach; }
+            else high = below;
+        }
+        listed = count <= LONG_LIST;
+        if (listed) {
+            // into the first block's list, in class order
+            auto counted = [&](int u) {
+                int c = 0;
+                each_of(u, [&](float x, int) { c += x >= low; });
+                return c;
+            };
+            int mine = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const int c = counted(u);
+                mine += c;
+                const int s = __reduce_add_sync(0xffffffffu, c);
+                if (lane == 0) sh.segment_count[u * W + warp] = s;
+            }
+            total(sum, f0, f1, mine);
+            prefix(sh.segment_count);
+            LongRow<W, S> *to = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const int c = counted(u);
+                if (!__any_sync(0xffffffffu, c)) continue;
+                int upto = c;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                int place = front_count + sh.segment_count[u * W + warp] + upto - c;
+                each_of(u, [&](float x, int k) {
+                    if (x >= low) { to->x[place] = x; to->k[place] = lo + k; ++place; }
+                });
+            }
+            if (C > 1) cluster.sync();
+            else __syncthreads();
+            if (rank != 0) return;
+        } else {
+            // over all scores
+            if (by_share) {
+                float lightest = -minus_inf();
+                each([&](float x, int) {
+                    if (x >= low && weight_of(x) >= l.min_p) lightest = fminf(lightest, x);
+                });
+                count = 0;
+                total(sum, lightest, f1, count);
+                at = lightest;
+            } else {
+                at = lowest_of_all;
+            }
+            auto together = [&](double &s, float &up, float &below) {
+                int c = 0;
+                total(s, up, below, c);
+            };
+            // the first r of the scores that equal `at`
+            auto cut_ties = [&](int r) {
+                int mine = 0;
+#pragma unroll
+                for (int u = 0; u < P; ++u) {
+                    int c = 0;
+                    each_of(u, [&](float x, int k) { c += x == at && lo + k <= last; });
+                    mine += c;
+                    const int s = __reduce_add_sync(0xffffffffu, c);
+                    if (lane == 0) sh.segment_count[u * W + warp] = s;
+                }
+                total(sum, f0, f1, mine);
+                prefix(sh.segment_count);
+#pragma unroll
+                for (int u = 0; u < P; ++u) {
+                    int c = 0;
+                    each_of(u, [&](float x, int k) { c += x == at && lo + k <= last; });
+                    int upto = c;
+#pragma unroll
+                    for (int o = 1; o < 32; o *= 2) {
+                        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                        if (lane >= o) upto += v;
+                    }
+                    int seen = front_count + sh.segment_count[u * W + warp] + upto - c;
+                    each_of(u, [&](float x, int k) {
+                        if (x == at && lo + k <= last && ++seen == r)
+                            for (int b = 0; b < C; ++b) (C > 1 ? cluster.map_shared_rank(&sh, b) : &sh)->tie = lo + k;
+                    });
+                }
+                if (C > 1) cluster.sync();
+                else __syncthreads();
+                last = sh.tie;
+            };
+            auto measured = [&](bool masses) {
+                return [&, masses](auto &&f) {
+                    each([&](float x, int k) {
+                        if (left(x, k)) f(x, masses ? weight_of(x) : 1.0);
+                    });
+                };
+            };
+            auto settle = [&](bool masses, double target) {
+                const float found = reached(true, target, at, top, measured(masses), together);
+                double above = 0;
+                int ties = 0;
+                measured(masses)([&](float x, double m) {
+                    if (x > found) above += m;
+                    ties += x == found;
+                });
+                total(above, f0, f1, ties);
+                const int r = masses ? ties_left(target, above, weight_of(found), ties) : (int)(target - above);
+                if (found > at) { at = found; last = a.k; }
+                if (r < ties) cut_ties(r);
+            };
+            if (by_count) {
+                count = 0;
+                each([&](float x, int k) { count += left(x, k); });
+                total(sum, f0, f1, count);
+                if (top_k < count) settle(false, (double)top_k);
+            }
+            if (by_mass) {
+                sum = 0;
+                measured(true)([&](float, double m) { sum += m; });
+                count = 0;
+                total(sum, f0, f1, count);
+                settle(true, l.top_p * sum);
+            }
+            mass = segments();
+        }
+    } else {
+        mass = all = segments();
+    }
+    auto put = [&](long long i, int cls, float score, double log_mass, double log_all) {
+        const double lw = ((double)score - (double)top) * l.inv_t;
+        put_draw(a, i, cls, (float)(lw - log_mass), (float)(lw - log_all));
+    };
+    if (!listed) {
+        // this block's draws: those that fall into [front, front + its mass), and where nothing is left behind it also what rounding leaves there
+        const double log_mass = log(mass), log_all = log(all), own_end = front + sh.slot_sum[turn ^ 1];   // (the last total was of the masses)
+        bool behind = false;
+        for (int b = rank + 1; b < C; ++b) behind |= cluster.map_shared_rank(&sh, b)->slot_sum[turn ^ 1] > 0;
+        const bool some = own_end > front;
+        for (int d = warp; d < a.draws; d += W) {
+            const long long i = n * a.draws + d;
+            const double target = uniform_of(a, i) * mass;
+            if (!(some && front <= target && (own_end > target || !behind))) continue;
+            // the last segment that begins at or before the target; the one in front of it (or behind) where it is empty
+            int from = 0, to = S;
+            while (to - from > 1) {
+                const int mid = (from + to) / 2;
+                if (front + sh.segment[mid] <= target) from = mid;
+                else to = mid;
+            }
+            while (from > 0 && !sh.segment_count[from]) --from;
+            while (from < S - 1 && !sh.segment_count[from]) ++from;
+            const int cell = ((from / W) * TH + (from % W) * 32 + lane) * V;
+            float x[V];
+            double w[V], own = 0;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                x[j] = cell < cells ? in(n, lo + cell + j) : minus_inf();
+                w[j] = left(x[j], cell + j) ? weight_of(x[j]) : 0.0;
+                own += w[j];
+            }
+            double upto = own;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const double v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            double before = front + sh.segment[from] + (upto - own);
+            const unsigned has = __ballot_sync(0xffffffffu, own > 0), hit = __ballot_sync(0xffffffffu, own > 0 && before + own > target);
+            const int src = hit ? __ffs(hit) - 1 : 31 - __clz(has);
+            if (lane == src) {
+                int cls = 0;
+                float s = 0;
+                bool found = false;
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (!found && w[j] > 0) {
+                        before += w[j];
+                        cls = lo + cell + j;
+                        s = x[j];
+                        found = before > target;
+                    }
+                put(i, cls, s, log_mass, log_all);
+            }
+        }
+        if (C > 1) cluster.sync();   // (others look at this block's sums)
+        return;
+    }
+    // ---- the list: `count` entries, in class order
+    constexpr int Q = LONG_LIST / TH;
+    const int size = count;
+    // exclusive prefix of the threads' sums
+    auto scan = [&](double own, double &whole) {
+        double upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh.sums[warp] = upto;
+        __syncthreads();
+        double before = 0;
+        whole = 0;
+        for (int v = 0; v < W; ++v) {
+            if (v == warp) before = whole;
+            whole += sh.sums[v];
+        }
+        return before + (upto - own);
+    };
+    int place[Q], heavy = 0;
+    double mine[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int i = q * TH + tid;
+        place[q] = size;
+        mine[q] = 0;
+        if (i < size) {
+            const float x = sh.x[i];
+            mine[q] = weight_of(x);
+            heavy += mine[q] >= l.min_p;
+            int larger = 0;
+            for (int j = 0; j < i; ++j) larger += sh.x[j] >= x;
+            for (int j = i + 1; j < size; ++j) larger += sh.x[j] > x;
+            place[q] = larger;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (place[q] < size) sh.w[place[q]] = mine[q];
+    heavy = warp_sum(heavy);
+    if (lane == 0) sh.counts[warp] = heavy;
+    __syncthreads();
+    heavy = 0;
+    for (int v = 0; v < W; ++v) heavy += sh.counts[v];
+    int keep = min(heavy, top_k);   // in descending order
+    if (by_mass) {
+        // entry i Q + q in descending order: prefix sums
+        double s = 0, whole;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) s += tid * Q + q < keep ? sh.w[tid * Q + q] : 0.0;
+        double upto = scan(s, whole);
+        const double target = l.top_p * (by_count || by_share ? whole : all);
+        int before = 0;   // entries in front of which the target is not reached
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (tid * Q + q < keep) {
+                before += tid * Q + q == 0 || upto < target;
+                upto += sh.w[tid * Q + q];
+            }
+        before = warp_sum(before);
+        __syncthreads();
+        if (lane == 0) sh.counts[warp] = before;
+        __syncthreads();
+        keep = 0;
+        for (int v = 0; v < W; ++v) keep += sh.counts[v];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (q * TH + tid < size) sh.w[q * TH + tid] = place[q] < keep ? mine[q] : 0.0;   // in class order now
+    __syncthreads();
+    {
+        double s = 0;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) s += tid * Q + q < size ? sh.w[tid * Q + q] : 0.0;
+        double upto = scan(s, mass);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (tid * Q + q < size) {
+                upto += sh.w[tid * Q + q];
+                sh.upto[tid * Q + q] = upto;
+            }
+    }
+    __syncthreads();
+    mass = sh.upto[size - 1];
+    for (int d = tid; d < a.draws; d += TH) {
+        const long long i = n * a.draws + d;
+        const double target = uniform_of(a, i) * mass;
+        int from = 0, to = size - 1;   // the first entry beyond the target, or the last that is left
+        while (from < to) {
+            const int mid = (from + to) / 2;
+            if (sh.upto[mid] > target || sh.upto[mid] >= mass) to = mid;
+            else from = mid + 1;
+        }
+        while (from > 0 && !(sh.w[from] > 0)) --from;   // (prefix sums by different threads are not rounded alike)
+        put(i, sh.k[from], sh.x[from], log(mass), log(all));
+    }
+}
+
 // ------------------------------------------------------------------ feedback
 // A row's sums, relative to its largest score: sum of e = exp((s - top) / T) and of e (s - top).  What follows from them and the draws:
 //   g_i = p_i (by_d (s_i - top) + flat) + [draws of i],  h_i = max(curve p_i (1 - p_i), 1e-16),  p_i = e_i to_p
@@ -978,7 +1455,7 @@ void scores_sample(const SampleArgs &a, cudaStream_t stream) {
             });
             return;
         }
-        if (a.k <= SCORES_CLASS_MOST && (by_class || a.n >= 32)) {
+        if (a.k <= SCORES_CLASS_MOST && (by_class || a.k <= 32 || a.n >= 1024)) {
             const int apart = by_class ? 32 : 33;
             auto go = [&](auto kern, int groups, size_t own, int threads) {
                 const size_t smem = groups * (own + sizeof(float) * apart * a.k);
@@ -988,6 +1465,30 @@ void scores_sample(const SampleArgs &a, cudaStream_t stream) {
             if (a.k <= 32) go(k_sample_limited<T, 1>, 4, sizeof(ClassShared<1>) + sizeof(ListShared<1>), 128);
             else go(k_sample_limited<T, 8>, 1, sizeof(ClassShared<8>) + sizeof(ListShared<8>), 256);
             return;
+        }
+        if (a.in.cls == 1 || a.k == 1) {
+            const Scores<T> in = scores_of<T>(a.in);
+            const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T));
+            bool done = false;
+            // the smallest blocks that hold a row in a cluster of up to 8, and bigger ones before more than one where there are rows enough for every SM
+            auto go = [&](auto th, auto p, auto ev) {
+                constexpr bool EVEN = decltype(ev)::value;
+                constexpr int TH = decltype(th)::value, P = decltype(p)::value;
+                const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
+                if (done || c > LONG_CLUSTER) return;
+                launch_long(k_sample_long<T, TH, P, EVEN>, a.n, c, TH, stream, a, in);
+                done = true;
+            };
+            using std::integral_constant;
+            auto all = [&](auto ev) {
+                constexpr int S = decltype(ev)::value ? 4 / (int)sizeof(T) == 2 ? 1 : 2 : 8;   // 8 scores
+                if (a.k <= 2048) go(integral_constant<int, 256>{}, integral_constant<int, S>{}, ev);
+                go(integral_constant<int, 512>{}, integral_constant<int, S>{}, ev);
+                go(integral_constant<int, 512>{}, integral_constant<int, 2 * S>{}, ev);
+                go(integral_constant<int, 512>{}, integral_constant<int, 4 * S>{}, ev);
+            };
+            even ? all(std::true_type{}) : all(std::false_type{});
+            if (done) return;
         }
         k_sample_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, scores_of<T>(a.in));
     });

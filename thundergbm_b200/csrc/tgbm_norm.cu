@@ -9,6 +9,7 @@
 #include "../../include/thundergbm.h"
 #include "tgbm_scores.cuh"
 #include "tgbm_scores_check.h"
+#include "tgbm_scores_long.cuh"
 
 namespace tgbm {
 namespace {
@@ -184,12 +185,6 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : W == 16 ? 
 }
 
 // ---- by row, up to 1024 classes: L lanes have a row, E classes each, L apart -----------------------------------------
-template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v) {
-#pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-
 template <typename T, int L, int E>
 __global__ void __launch_bounds__(ROW_THREADS) k_norm_row(NormArgs a, Scores<T> in, Scores<T> out) {
     constexpr int R = ROW_THREADS / L;
@@ -234,60 +229,6 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_row(NormArgs a, Scores<T> 
         }
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// ---- long rows: a block, or a cluster of blocks, each with a part of the row in its registers -------------------------------
-// A thread's scores: packs of 16 bytes, TH packs apart (EVEN: rows, gains and results all begin on such boundaries), or single ones, TH apart.
-constexpr int LONG_CLUSTER = 8;
-
-template <typename T, int TH, int P, bool EVEN> struct Hold {
-    static constexpr int V = EVEN ? Pack<T>::V : 1, E = P * V;
-    static constexpr int CELLS = TH * E;   // of a block
-    static __device__ __forceinline__ int first(int u) { return (u * TH + (int)threadIdx.x) * V; }
-    Pack<T> w[EVEN ? P : 1];
-    T one[EVEN ? 1 : P];
-    __device__ __forceinline__ void read(const T *p, int cells) {   // cells: of the part (EVEN: whole packs)
-#pragma unroll
-        for (int u = 0; u < P; ++u)
-            if (cells == CELLS || first(u) < cells) {
-                if constexpr (EVEN) w[u].bits = __ldg(reinterpret_cast<const uint4 *>(p + first(u)));
-                else one[u] = p[first(u)];
-            }
-    }
-    __device__ __forceinline__ void get(int u, float (&v)[V]) const {
-        if constexpr (EVEN) w[u].unpack(v);
-        else v[0] = score_f32(one[u]);
-    }
-    // cells h to h + Q of pack u
-    template <int Q> __device__ __forceinline__ void get_some(int u, int h, float (&v)[Q]) const {
-        if constexpr (!EVEN) v[0] = score_f32(one[u]);
-        else if constexpr (Q == V) w[u].unpack(v);
-        else {
-            float all[V];
-            w[u].unpack(all);
-#pragma unroll
-            for (int i = 0; i < Q; ++i) v[i] = all[h + i];
-        }
-    }
-    template <int Q> __device__ __forceinline__ void set_some(int u, int h, const float (&v)[Q]) {
-        if constexpr (!EVEN) one[u] = score_from<T>(v[0]);
-        else if constexpr (Q == V) w[u].pack(v);
-        else {
-            Pack<T> some;
-            float all[V] = {};
-#pragma unroll
-            for (int i = 0; i < Q; ++i) all[i] = v[i];
-            some.pack(all);
-            if (h == 0) { w[u].bits.x = some.bits.x; w[u].bits.y = some.bits.y; }
-            else { w[u].bits.z = some.bits.x; w[u].bits.w = some.bits.y; }
-        }
-    }
-    __device__ __forceinline__ void write(T *p, int u) const {
-        if constexpr (EVEN) *reinterpret_cast<uint4 *>(p + first(u)) = w[u].bits;
-        else p[first(u)] = one[u];
-    }
-};
 template <int V> __device__ __forceinline__ void read_floats(const float *p, float none, float (&v)[V]) {
     if constexpr (V == 1) {
         v[0] = p ? __ldg(p) : none;
@@ -299,30 +240,8 @@ template <int V> __device__ __forceinline__ void read_floats(const float *p, flo
         }
     }
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    unsigned long long r, x = *reinterpret_cast<unsigned long long *>(&a), y = *reinterpret_cast<unsigned long long *>(&b), z = *reinterpret_cast<unsigned long long *>(&c);
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return *reinterpret_cast<float2 *>(&r);
-}
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 
-// Sums of M numbers over a warp (M a power of two up to 32): lanes exchange half of what they hold until each holds one.  Lane l has the sum
-// of number l / (32 / M).
-template <int M> __device__ __forceinline__ float sums_spread(float (&v)[M]) {
-    const int lane = threadIdx.x & 31;
-    int o = 16;
-#pragma unroll
-    for (int m = M; m > 1; m >>= 1, o >>= 1) {
-        const bool upper = lane & o;
-#pragma unroll
-        for (int i = 0; i < m / 2; ++i) {
-            const float give = upper ? v[i] : v[i + m / 2], keep = upper ? v[i + m / 2] : v[i];
-            v[i] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, o));
-        }
-    }
-    for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
-    return v[0];
-}
 // sums of M numbers over a block of TH threads, the same in all of them; all threads, with two barriers
 template <int TH, int M> struct LongSums {
     float part[TH / 32][M], sum[M];
@@ -576,19 +495,6 @@ template <typename F> void by_row_sizes(int k, F &&f) {
     else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
 constexpr int ROW_MOST = 1024;   // classes of a row that a warp's registers hold
-
-bool on_16(const void *p, long long row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
-
-template <typename... P, typename... A>
-void launch_long(void (*kernel)(P...), long long rows, int cluster, int threads, cudaStream_t stream, A &&...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(threads); cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = cluster; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr; cfg.numAttrs = cluster > 1 ? 1 : 0;
-    TGBM_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...));
-}
 
 void scores_norm(const NormArgs &a, cudaStream_t stream) {
     if (a.n == 0) return;
