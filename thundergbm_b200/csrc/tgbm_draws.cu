@@ -811,7 +811,7 @@ template <int W, int S> struct LongRow {
 };
 
 template <typename T, int TH, int P, bool EVEN>
-__global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) {
+__global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Scores<T> in) {
     typedef Hold<T, TH, P, EVEN> H;
     constexpr int V = H::V, W = TH / 32, S = P * W;
     __shared__ __align__(16) LongRow<W, S> sh;
@@ -892,9 +892,18 @@ __global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) 
     int count = 0;
     each([&](float x, int) {
         top = fmaxf(top, x);
-        low = fminf(low, x > minus_inf() ? x : low);
         count |= x != x;
     });
+    // Each group of lanes that holds a score has a largest one, and the least of these is reached by as many scores as there are groups: the first
+    // guess of a border.  Groups are as large as they may be to be top_k.
+    const int top_k = l.greedy ? 1 : l.top_k, groups = max(1, a.k / H::E);   // (threads that hold all their scores)
+    {
+        float its = top;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2)
+            if (groups / (2 * o) >= max(top_k < a.k ? top_k : 0, LONG_WANT / 4)) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
+        low = its > minus_inf() ? its : low;
+    }
     total(sum, low, top, count);
     const bool bad = l.broken || count || top == -minus_inf();
     if (bad || top == minus_inf()) {   // (the same for all blocks; none reads another's memory any more than it did before the last barrier)
@@ -906,9 +915,8 @@ __global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) 
     }
     const Exponent weight(l);
     auto weight_of = [&](float v) { return weight(sh.powers, v, top); };
-    const int top_k = l.greedy ? 1 : l.top_k;
     const bool by_count = top_k < a.k, by_mass = l.top_p < 1 && !l.greedy, by_share = l.min_p > 0 && !l.greedy;
-    const float lowest_of_all = low;
+    const float guess = low;
     double all = 0;
     // what is left: larger than `at`, or equal to it and a class up to `last`
     float at = minus_inf();
@@ -938,71 +946,95 @@ __global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) 
     double mass = 0;
     bool listed = false;
     if (by_count || by_mass || by_share) {
-        if (!by_count && !by_share) {
-            each([&](float x, int) { all += weight_of(x); });
-        } else {
-            const float c = (float)(l.inv_t * 1.4426950408889634);
-            float part = 0;
-#pragma unroll
-            for (int u = 0; u < P; ++u) {
-                float s = 0;
-                each_of(u, [&](float x, int) { s += exp2_fast(__fsub_rn(x, top) * c); });
-                part += s;
-            }
-            all = (double)part;
-        }
+        const float c = (float)(l.inv_t * 1.4426950408889634);
+        auto rough = [&](float x) { return exp2_fast(__fsub_rn(x, top) * c); };
         float f0 = 0, f1 = 0;
-        count = 0;
-        total(all, f0, f1, count);
-        if (l.greedy) all = 1.0;
+        const bool exact = !by_count && !by_share;   // top_p alone: a share of the whole mass
+        if (exact) {
+            each([&](float x, int) { all += weight_of(x); });
+            count = 0;
+            total(all, f0, f1, count);
+        }
         // the border, rounded down as in k_sample_limited; what lies 750 T below the largest score has no mass in any case
         const float t = (float)(1.0 / l.inv_t);
         float down = -750.f * t;
         if (by_share) down = logf((float)l.min_p) * t;
-        else if (by_mass && !by_count) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
+        else if (exact) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
         low = __fadd_rn(top, down) - (fabsf(down) + t + fabsf(top)) * 2e-6f;
         if (l.greedy) low = top;
-        if (!(low <= top)) low = lowest_of_all;
-        low = fmaxf(low, lowest_of_all);
-        count = 0;
-        each([&](float x, int) { count += x >= low; });
-        total(sum, f0, f1, count);
-        float high = top;
-        bool narrowing = count > LONG_WANT && (by_count ? top_k <= LONG_LIST : by_mass && !by_share);
-        const double enough = by_count ? (double)top_k : l.top_p * all * (1 + 1e-9);
-        const int want = max(LONG_WANT, by_count ? top_k : 0);
-        while (narrowing && count > want && low < high) {
-            const float mid = middle(low, high);
-            float up = -minus_inf(), below = minus_inf();
-            int reach = 0;
-            sum = 0;
+        if (!(low <= top)) low = minus_inf();
+        low = fmaxf(low, -FLT_MAX);
+        const float base = low;
+        if (by_count && guess <= top) low = fmaxf(low, guess);
+        unsigned reach = 0;   // bits of this thread's scores from the border on
+        auto mark = [&](float border) {
+            reach = 0;
+            int bit = 0;
             each([&](float x, int) {
-                if (x >= mid) {
-                    ++reach;
-                    up = fminf(up, x);
-                    if (!by_count) sum += weight_of(x);
-                } else if (x >= low) {
-                    below = fmaxf(below, x);
-                }
+                reach |= x >= border ? 1u << bit : 0u;
+                ++bit;
             });
-            total(sum, up, below, reach);
-            if ((by_count ? (double)reach : sum) >= enough) { low = up; count = reach; }
+        };
+        mark(low);
+        count = __popc(reach);
+        if (!exact) {
+            float part = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                float s = 0;
+                each_of(u, [&](float x, int) { s += rough(x); });
+                part += s;
+            }
+            all = (double)part;
+            total(all, f0, f1, count);
+        } else {
+            total(sum, f0, f1, count);
+        }
+        if (l.greedy) all = 1.0;
+        if (by_count && count < top_k && low > base) {   // (groups without a score: the guess was too high)
+            low = base;
+            mark(low);
+            count = __popc(reach);
+            total(sum, f0, f1, count);
+        }
+        float high = top;
+        const bool narrowing = count > LONG_WANT && (by_count ? top_k <= LONG_LIST : by_mass && !by_share);
+        // (masses by floats, off by less than 2^-18)
+        const double enough = by_count ? (double)top_k : l.top_p * all * (1 + 1e-5);
+        const int want = max(LONG_WANT, by_count ? top_k : 0);
+        bool first = !by_count && guess > low && guess < top, moved = false;
+        while (narrowing && count > want && low < high) {
+            const float mid = first ? guess : middle(low, high);
+            first = false;
+            float up = -minus_inf(), below = minus_inf();
+            int c = 0;
+            sum = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                if (!__any_sync(0xffffffffu, reach >> (u * V) & ((1ull << V) - 1))) continue;   // (nothing from the border on)
+                each_of(u, [&](float x, int) {
+                    if (x >= mid) {
+                        ++c;
+                        up = fminf(up, x);
+                        if (!by_count) sum += (double)rough(x);
+                    } else if (x >= low) {
+                        below = fmaxf(below, x);
+                    }
+                });
+            }
+            total(sum, up, below, c);
+            if ((by_count ? (double)c : sum) >= enough) { low = up; count = c; moved = true; }
             else high = below;
         }
         listed = count <= LONG_LIST;
         if (listed) {
             // into the first block's list, in class order
-            auto counted = [&](int u) {
-                int c = 0;
-                each_of(u, [&](float x, int) { c += x >= low; });
-                return c;
-            };
-            int mine = 0;
+            if (moved) mark(low);
+            auto bits = [&](int u) { return (unsigned)(reach >> (u * V) & ((1ull << V) - 1)); };
+            int mine = __popc(reach);
 #pragma unroll
             for (int u = 0; u < P; ++u) {
-                const int c = counted(u);
-                mine += c;
-                const int s = __reduce_add_sync(0xffffffffu, c);
+                const int s = __reduce_add_sync(0xffffffffu, __popc(bits(u)));
                 if (lane == 0) sh.segment_count[u * W + warp] = s;
             }
             total(sum, f0, f1, mine);
@@ -1010,7 +1042,7 @@ __global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) 
             LongRow<W, S> *to = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
 #pragma unroll
             for (int u = 0; u < P; ++u) {
-                const int c = counted(u);
+                const int c = __popc(bits(u));
                 if (!__any_sync(0xffffffffu, c)) continue;
                 int upto = c;
 #pragma unroll
@@ -1037,7 +1069,9 @@ __global__ void __launch_bounds__(TH) k_sample_long(SampleArgs a, Scores<T> in) 
                 total(sum, lightest, f1, count);
                 at = lightest;
             } else {
-                at = lowest_of_all;
+                each([&](float x, int) { at = fminf(x > minus_inf() ? x : -minus_inf(), at == minus_inf() ? -minus_inf() : at); });
+                count = 0;
+                total(sum, at, f1, count);
             }
             auto together = [&](double &s, float &up, float &below) {
                 int c = 0;
