@@ -1354,18 +1354,37 @@ __device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long lo
     return r;
 }
 
+// What lane l has of the draws l, l + 32, ...: read early where there is something else to wait for
+struct DrawsRead {
+    int cls[SCORES_MAX_TOP / 32];
+    float score[SCORES_MAX_TOP / 32];
+};
+template <typename T> __device__ __forceinline__ DrawsRead read_draws(const FeedbackArgs &a, const Scores<T> &in, long long n) {
+    DrawsRead r;
+#pragma unroll
+    for (int j = 0; j < SCORES_MAX_TOP / 32; ++j) {
+        const int e = (threadIdx.x & 31) + 32 * j;
+        if (e >= a.draws) break;
+        r.cls[j] = a.classes[n * a.draws + e];
+        r.score[j] = r.cls[j] >= 0 && r.cls[j] < a.k ? in(n, r.cls[j]) : minus_inf();
+    }
+    return r;
+}
 // One warp, for the row n: logs, the loss and what its gradients need.  cls[e], extra[e]: class of draw e and what is added there (-1: nothing;
-// of draws of one class the first has the sum).  score(i): the row's score of class i.
-template <typename F>
-__device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long long n, float top, float sum, float sum_d, int *cls, float *extra, bool writes, F &&score) {
+// of draws of one class the first has the sum).
+__device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long long n, float top, float sum, float sum_d, int *cls, float *extra, bool writes,
+                                                     const DrawsRead &draws) {
     const int lane = threadIdx.x & 31;
     const double log_sum = sum == 0.f ? 0.0 : fine_log(sum);
     double term = 0, to_log = 0, size = 0;
     int number = 0;
-    for (int e = lane; e < a.draws; e += 32) {
+#pragma unroll
+    for (int j = 0; j < SCORES_MAX_TOP / 32; ++j) {
+        const int e = lane + 32 * j;
+        if (e >= a.draws) break;
         const long long at = n * a.draws + e;
-        const int i = a.classes[at];
-        const float x = i >= 0 && i < a.k ? score(i) : minus_inf();
+        const int i = draws.cls[j];
+        const float x = draws.score[j];
         const bool counts = x > minus_inf() || x != x;
         const double lp = counts ? ((double)x - (double)top) * a.inv_t - log_sum : (double)minus_inf();
         if (a.logs && writes) a.logs[at] = (float)lp;
@@ -1450,7 +1469,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_any(FeedbackArgs a, Sc
     if (warp == 0) {
         s = warp_sum(lane < ROW_WARPS ? parts[1][lane] : 0.f);
         sd = warp_sum(lane < ROW_WARPS ? parts[2][lane] : 0.f);
-        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, [&](int i) { return in(n, i); });
+        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, read_draws(a, in, n));
         if (lane == 0) shared_row = r;
     }
     __syncthreads();
@@ -1637,7 +1656,7 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_row(FeedbackArgs a, Sc
             sd = __fmaf_rn(e, fmaxf(d, -1e30f), sd);
         }
         s = warp_sum(s); sd = warp_sum(sd);
-        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, [&](int i) { return in(n, i); });
+        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, read_draws(a, in, n));
         if (a.gives != GIVES_LOSS) {
             unsigned drawn = 0;
             for (int e = 0; e < a.draws; ++e) {
@@ -1674,6 +1693,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_feedback_long(FeedbackArgs a,
     const int lo = rank * H::CELLS, cells = min(a.k - lo, H::CELLS);
     H x;
     x.read(in.at(n, lo), cells);
+    __shared__ DrawsRead ahead[32];
+    if (warp == 0) ahead[lane] = read_draws(a, in, n);   // (kept in shared memory: the registers are the row's)
     auto each = [&](auto &&f) {
 #pragma unroll
         for (int u = 0; u < P; ++u)
@@ -1734,7 +1755,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_feedback_long(FeedbackArgs a,
             s = lane < C ? s * by : 0.f;
             s = warp_sum(s); sd = warp_sum(sd);   // (all lanes go on)
         }
-        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sd, cls, extra, rank == 0, [&](int i) { return in(n, i); });
+        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sd, cls, extra, rank == 0, ahead[lane]);
         if (lane == 0) shared_row = r;
     }
     if (C > 1) cluster_arrive();
@@ -1889,20 +1910,24 @@ void scores_feedback(const FeedbackArgs &given, cudaStream_t stream) {
         if (a.in.cls == 1 && (a.gives == GIVES_LOSS || a.out.cls == 1) && !a.maxbits) {
             const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T)) && (a.gives != GIVES_GRADIENT || on_16(a.out.data, a.out.row, sizeof(T)));
             bool done = false;
-            auto go = [&](auto p, auto ev) {
+            // the smallest blocks that hold a row in a cluster of up to 8, the largest ones where there are rows for several on every SM
+            auto go = [&](auto th, auto p, auto last, auto ev) {
                 constexpr bool EVEN = decltype(ev)::value;
-                constexpr int TH = 512, P = decltype(p)::value;
+                constexpr int TH = decltype(th)::value, P = decltype(p)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
-                if (done || c > LONG_CLUSTER) return;
+                if (done || c > LONG_CLUSTER || (!decltype(last)::value && c > 1 && (long long)a.n * c > 8 * 148)) return;
                 launch_long(k_feedback_long<T, TH, P, EVEN>, a.n, c, TH, stream, a, in);
                 done = true;
             };
             using std::integral_constant;
             auto all = [&](auto ev) {
-                constexpr int S = decltype(ev)::value ? sizeof(T) == 2 ? 1 : 2 : 8;   // 8 scores
-                go(integral_constant<int, S>{}, ev);
-                go(integral_constant<int, 2 * S>{}, ev);
-                go(integral_constant<int, 4 * S>{}, ev);
+                constexpr bool EVEN = decltype(ev)::value;
+                constexpr int S = EVEN ? sizeof(T) == 2 ? 1 : 2 : 8;   // 8 scores
+                go(integral_constant<int, 256>{}, integral_constant<int, S>{}, std::false_type{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, 2 * S>{}, std::false_type{}, ev);
+                constexpr bool more = EVEN && sizeof(T) == 2;
+                go(integral_constant<int, 256>{}, integral_constant<int, 4 * S>{}, integral_constant<bool, !more>{}, ev);
+                go(integral_constant<int, more ? 256 : 512>{}, integral_constant<int, more ? 8 * S : 4 * S>{}, std::true_type{}, ev);
             };
             even ? all(std::true_type{}) : all(std::false_type{});
             if (done) return;
