@@ -1322,14 +1322,14 @@ constexpr float MIN_HESSIAN = 1e-16f;   // the softmax objective's
 struct Draw {
     double term, to_log;   // loss of one draw, its derivative by the log-probability
 };
-__device__ __forceinline__ Draw draw_of(const FeedbackArgs &a, long long at, double lp) {
-    const double gain = (double)a.gains[at], r = a.old ? exp(lp - (double)a.old[at]) : 1.0;
+__device__ __forceinline__ Draw draw_of(const FeedbackArgs &a, double lp, float its_gain, float old, float reference) {
+    const double gain = (double)its_gain, r = a.old ? exp(lp - (double)old) : 1.0;
     const double held = fmin(fmax(r, (double)a.least), (double)a.most);
     Draw d;
     d.term = gain == 0 ? 0.0 : -fmin(r * gain, held * gain);   // (what weighs 0 counts for nothing, also where the ratio is infinite)
     d.to_log = gain != 0 && r * gain <= held * gain ? -r * gain : 0.0;
     if (a.kl != 0.f) {
-        const double x = (double)a.reference[at] - lp, e = exp(x);
+        const double x = (double)reference - lp, e = exp(x);
         d.term += (double)a.kl * (e - x - 1);
         d.to_log += (double)a.kl * (1 - e);
     }
@@ -1337,10 +1337,9 @@ __device__ __forceinline__ Draw draw_of(const FeedbackArgs &a, long long at, dou
 }
 
 // The row's loss, and what its gradients need; `by`: what a draw's derivative is multiplied by
-__device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long long n, float top, float sum, float sum_d, double log_sum, double term, double to_log,
-                                                  double size, int number, bool writes, double &by) {
+__device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long long n, float w, float top, float sum, float sum_d, double log_sum, double term,
+                                                  double to_log, double size, int number, bool writes, double &by) {
     const double inv_sum = sum == 0.f ? 0.0 : 1.0 / (double)sum, spread = log_sum - (double)sum_d * a.inv_t * inv_sum;   // (the entropy)
-    const float w = a.weights ? a.weights[n] : 1.f;
     FeedbackRow r;
     r.counts = number > 0 && w != 0.f;
     const double share = number == 1 ? 1.0 : number ? 1.0 / number : 0.0, scale = (double)w * a.inv_t;
@@ -1357,15 +1356,21 @@ __device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long lo
 // What lane l has of the draws l, l + 32, ...: read early where there is something else to wait for
 struct DrawsRead {
     int cls[SCORES_MAX_TOP / 32];
-    float score[SCORES_MAX_TOP / 32];
+    float score[SCORES_MAX_TOP / 32], gain[SCORES_MAX_TOP / 32], old[SCORES_MAX_TOP / 32], reference[SCORES_MAX_TOP / 32];
+    float weight;
 };
 template <typename T> __device__ __forceinline__ DrawsRead read_draws(const FeedbackArgs &a, const Scores<T> &in, long long n) {
     DrawsRead r;
+    r.weight = a.weights ? a.weights[n] : 1.f;
 #pragma unroll
     for (int j = 0; j < SCORES_MAX_TOP / 32; ++j) {
         const int e = (threadIdx.x & 31) + 32 * j;
         if (e >= a.draws) break;
-        r.cls[j] = a.classes[n * a.draws + e];
+        const long long at = n * a.draws + e;
+        r.cls[j] = a.classes[at];
+        r.gain[j] = a.gains[at];
+        r.old[j] = a.old ? a.old[at] : 0.f;
+        r.reference[j] = a.kl != 0.f ? a.reference[at] : 0.f;
         r.score[j] = r.cls[j] >= 0 && r.cls[j] < a.k ? in(n, r.cls[j]) : minus_inf();
     }
     return r;
@@ -1391,7 +1396,7 @@ __device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long 
         cls[e] = counts ? i : -1;
         extra[e] = 0.f;
         if (counts) {
-            const Draw d = draw_of(a, at, lp);
+            const Draw d = draw_of(a, lp, draws.gain[j], draws.old[j], draws.reference[j]);
             term += d.term; to_log += d.to_log; size += fabs(d.to_log);
             extra[e] = (float)d.to_log;
             ++number;
@@ -1401,7 +1406,7 @@ __device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long 
     term = warp_sum(term); to_log = warp_sum(to_log); size = warp_sum(size);
     __syncwarp();
     double by;
-    const FeedbackRow r = factors_of(a, n, top, sum, sum_d, log_sum, term, to_log, size, number, writes && lane == 0, by);
+    const FeedbackRow r = factors_of(a, n, draws.weight, top, sum, sum_d, log_sum, term, to_log, size, number, writes && lane == 0, by);
     if (a.gives != GIVES_LOSS) {   // of draws of one class the first takes the sum
         float total[SCORES_MAX_TOP / 32];
         bool first[SCORES_MAX_TOP / 32];
@@ -1564,7 +1569,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 3
             cls[e * 32 + lane] = counts ? i : -1;
             float more = 0;
             if (counts) {
-                const Draw d = draw_of(a, at, lp);
+                const Draw d = draw_of(a, lp, a.gains[at], a.old ? a.old[at] : 0.f, a.kl != 0.f ? a.reference[at] : 0.f);
                 term += d.term; to_log += d.to_log; size += fabs(d.to_log);
                 more = (float)d.to_log;
                 ++number;
@@ -1580,7 +1585,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 3
         int number = 0;
         for (int v = 0; v < busy; ++v) { term += sh.sums[0][v][lane]; to_log += sh.sums[1][v][lane]; size += sh.sums[2][v][lane]; number += sh.number[v][lane]; }
         double by;
-        sh.row[lane] = factors_of(a, n, top, s, sd, log_sum, term, to_log, size, number, n0 == n, by);
+        sh.row[lane] = factors_of(a, n, a.weights ? a.weights[n] : 1.f, top, s, sd, log_sum, term, to_log, size, number, n0 == n, by);
         sh.by[lane] = by;
     }
     if (a.gives == GIVES_LOSS) return;
@@ -1678,130 +1683,158 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_row(FeedbackArgs a, Sc
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
-// Long rows: a cluster of up to 8 blocks (or one) holds the row in registers.  Two exponentials per score and gradient.
-template <typename T, int TH, int P, bool EVEN>
-__global__ void __launch_bounds__(TH, 1024 / TH) k_feedback_long(FeedbackArgs a, Scores<T> in) {
+// Long rows: a cluster of up to 8 blocks (or one) holds the row in registers.  Two exponentials per score and gradient; a thread that has no
+// score of -inf needs no care for 0 times infinity.
+template <int TH> struct FeedbackShared {
+    float parts[3][TH / 32], moments[3];
+    int cls[SCORES_MAX_TOP];
+    float extra[SCORES_MAX_TOP];
+    FeedbackRow row;
+    DrawsRead ahead[32];   // (kept here: the registers are the row's)
+};
+// sums of exp((v - base) / T) and of that times (v - base), the second if asked for
+template <int V, bool MASKED>
+__device__ __forceinline__ void add_exps(const float (&v)[V], float base, float c, bool spread, float2 &s, float2 &sd) {
+    if constexpr (V == 1) {
+        const float d = __fsub_rn(v[0], base), e = exp2_fast(d * c);
+        s.x += e;
+        sd.x = __fmaf_rn(e, MASKED ? fmaxf(d, -1e30f) : d, sd.x);
+    } else {
+        const float2 mb = make_float2(-base, -base), c2 = make_float2(c, c);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            float2 d = add2(make_float2(v[i], v[i + 1]), mb);
+            const float2 y = mul2(d, c2), e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            s = add2(s, e);
+            if (spread) sd = fma2(e, MASKED ? make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)) : d, sd);
+        }
+    }
+}
+template <int V, bool MASKED> __device__ __forceinline__ void gradients(const FeedbackRow &r, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = feedback_gh(r, v[0], 0.f).x;
+    } else {
+        const float2 mb = make_float2(-r.top, -r.top), c2 = make_float2(r.c, r.c), p2 = make_float2(r.to_p, r.to_p);
+        const float2 by = make_float2(r.by_d, r.by_d), flat = make_float2(r.flat, r.flat);
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+            const float2 d = add2(make_float2(v[i], v[i + 1]), mb), y = mul2(d, c2);
+            const float2 p = mul2(make_float2(exp2_fast(y.x), exp2_fast(y.y)), p2);
+            const float2 g = mul2(p, fma2(by, MASKED ? make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)) : d, flat));
+            v[i] = g.x; v[i + 1] = g.y;
+        }
+    }
+}
+template <typename T, int TH, int P, bool EVEN, bool FULL>
+__device__ __forceinline__ void feedback_long(const FeedbackArgs &a, const Scores<T> &in, FeedbackShared<TH> &sh) {
     typedef Hold<T, TH, P, EVEN> H;
     constexpr int V = H::V, W = TH / 32;
-    __shared__ float parts[3][W], moments[3];
-    __shared__ int cls[SCORES_MAX_TOP];
-    __shared__ float extra[SCORES_MAX_TOP];
-    __shared__ FeedbackRow shared_row;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long n = blockIdx.x / C;
-    const int lo = rank * H::CELLS, cells = min(a.k - lo, H::CELLS);
+    const int lo = rank * H::CELLS, cells = FULL ? H::CELLS : min(a.k - lo, H::CELLS);
     H x;
     x.read(in.at(n, lo), cells);
-    __shared__ DrawsRead ahead[32];
-    if (warp == 0) ahead[lane] = read_draws(a, in, n);   // (kept in shared memory: the registers are the row's)
-    auto each = [&](auto &&f) {
-#pragma unroll
-        for (int u = 0; u < P; ++u)
-            if (H::first(u) < cells) {
-                float v[V];
-                x.get(u, v);
-                f(u, v);
-            }
-    };
-    float m = minus_inf();
-    each([&](int, const float (&v)[V]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, v[i]);
-    });
+    if (warp == 0) sh.ahead[lane] = read_draws(a, in, n);
+    float least, m;
+    x.range(cells, least, m);
+    const bool masked = least == minus_inf();
     m = warp_max(m);
-    if (lane == 0) parts[0][warp] = m;
+    if (lane == 0) sh.parts[0][warp] = m;
     __syncthreads();
-    m = lanes_max<W>(parts[0][lane & (W - 1)]);
+    m = lanes_max<W>(sh.parts[0][lane & (W - 1)]);
     const bool spread = a.entropy != 0.f;
-    float s = 0, sd = 0;
+    float s, sd;
     {
         const float base = row_top(m);
         float2 s2 = make_float2(0.f, 0.f), sd2 = s2;
-        const float2 mb = make_float2(-base, -base), c2 = make_float2(a.c, a.c);
-        each([&](int, const float (&v)[V]) {
-            if constexpr (V == 1) {
-                const float d = __fsub_rn(v[0], base), e = exp2_fast(d * a.c);
-                s2.x += e;
-                sd2.x = __fmaf_rn(e, fmaxf(d, -1e30f), sd2.x);
-            } else {
+        auto pass = [&](auto care) {
 #pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    float2 d = add2(make_float2(v[i], v[i + 1]), mb);
-                    const float2 y = mul2(d, c2), e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
-                    s2 = add2(s2, e);
-                    if (spread) sd2 = fma2(e, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), sd2);
+            for (int u = 0; u < P; ++u)
+                if (FULL || H::first(u) < cells) {
+                    float v[V];
+                    x.get(u, v);
+                    add_exps<V, decltype(care)::value>(v, base, a.c, spread, s2, sd2);
                 }
-            }
-        });
+        };
+        masked ? pass(std::true_type{}) : pass(std::false_type{});
         s = s2.x + s2.y; sd = sd2.x + sd2.y;
     }
     s = warp_sum(s); sd = warp_sum(sd);
-    if (lane == 0) { parts[1][warp] = s; parts[2][warp] = sd; }
+    if (lane == 0) { sh.parts[1][warp] = s; sh.parts[2][warp] = sd; }
     __syncthreads();
     if (warp == 0) {
-        s = lanes_sum<W>(parts[1][lane & (W - 1)]); sd = lanes_sum<W>(parts[2][lane & (W - 1)]);
-        if (C > 1 && lane == 0) { moments[0] = m; moments[1] = s; moments[2] = sd; }
+        s = lanes_sum<W>(sh.parts[1][lane & (W - 1)]); sd = lanes_sum<W>(sh.parts[2][lane & (W - 1)]);
+        if (C > 1 && lane == 0) { sh.moments[0] = m; sh.moments[1] = s; sh.moments[2] = sd; }
     }
     if (C > 1) cluster.sync();
     if (warp == 0) {
         if (C > 1) {
-            const float *o = cluster.map_shared_rank(moments, lane < C ? lane : 0);
+            const float *o = cluster.map_shared_rank(sh.moments, lane < C ? lane : 0);
             const float its = o[0], base = row_top(its);
             s = o[1]; sd = o[2];
             m = lanes_max<32>(its);
             const float low = __fsub_rn(base, row_top(m)), by = its == minus_inf() ? 0.f : exp2_fast(low * a.c);
-            sd = lane < C && its > minus_inf() ? __fmaf_rn(low, s, sd) * by : its != its ? its : 0.f;
+            sd = lane < C && its > minus_inf() ? __fmaf_rn(low, s, sd) * by : 0.f;
             s = lane < C ? s * by : 0.f;
             s = warp_sum(s); sd = warp_sum(sd);   // (all lanes go on)
         }
-        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sd, cls, extra, rank == 0, ahead[lane]);
-        if (lane == 0) shared_row = r;
+        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sd, sh.cls, sh.extra, rank == 0, sh.ahead[lane]);
+        if (lane == 0) sh.row = r;
     }
-    if (C > 1) cluster_arrive();
     __syncthreads();
+    if (C > 1) cluster_done();
     if (a.gives != GIVES_LOSS) {
-        const FeedbackRow r = shared_row;
+        const FeedbackRow r = sh.row;
         const long long at = n * a.out.row + lo;
         if (a.gives == GIVES_PAIRS) {
             float2 *to = static_cast<float2 *>(a.out.data) + at;
-            each([&](int u, const float (&v)[V]) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) to[H::first(u) + i] = feedback_gh(r, v[i], 0.f);
-            });
-        } else {
-            T *to = static_cast<T *>(a.out.data) + at;
-            const float2 mb = make_float2(-r.top, -r.top), c2 = make_float2(r.c, r.c), p2 = make_float2(r.to_p, r.to_p), by = make_float2(r.by_d, r.by_d), flat = make_float2(r.flat, r.flat);
 #pragma unroll
             for (int u = 0; u < P; ++u)
-                if (H::first(u) < cells) {
+                if (FULL || H::first(u) < cells) {
                     float v[V];
                     x.get(u, v);
-                    if constexpr (V == 1) {
-                        v[0] = feedback_gh(r, v[0], 0.f).x;
-                    } else if (!r.counts) {
 #pragma unroll
-                        for (int i = 0; i < V; ++i) v[i] = 0.f;
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < V; i += 2) {
-                            const float2 d = add2(make_float2(v[i], v[i + 1]), mb), y = mul2(d, c2);
-                            const float2 p = mul2(make_float2(exp2_fast(y.x), exp2_fast(y.y)), p2);
-                            const float2 g = mul2(p, fma2(by, make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)), flat));
-                            v[i] = g.x; v[i + 1] = g.y;
-                        }
-                    }
-                    x.template set_some<V>(u, 0, v);
-                    x.write(to, u);
+                    for (int i = 0; i < V; ++i) to[H::first(u) + i] = feedback_gh(r, v[i], 0.f);
                 }
+        } else {
+            T *to = static_cast<T *>(a.out.data) + at;
+            auto pass = [&](auto care) {
+#pragma unroll
+                for (int u = 0; u < P; ++u)
+                    if (FULL || H::first(u) < cells) {
+                        float v[V];
+                        x.get(u, v);
+                        gradients<V, decltype(care)::value>(r, v);
+                        x.template set_some<V>(u, 0, v);
+                        x.write(to, u);
+                    }
+            };
+            if (!r.counts) {
+#pragma unroll
+                for (int u = 0; u < P; ++u)
+                    if (FULL || H::first(u) < cells) {
+                        const float zero[V] = {};
+                        x.template set_some<V>(u, 0, zero);
+                        x.write(to, u);
+                    }
+            } else {
+                masked ? pass(std::true_type{}) : pass(std::false_type{});
+            }
         }
         __syncthreads();
         for (int e = threadIdx.x; e < a.draws; e += TH) {
-            const int i = cls[e];
-            if (i >= lo && i < lo + cells) put_gradient<T>(a, n, i, feedback_gh(r, in(n, i), extra[e]));
+            const int i = sh.cls[e];
+            if (i >= lo && i < lo + cells) put_gradient<T>(a, n, i, feedback_gh(r, in(n, i), sh.extra[e]));
         }
     }
     if (C > 1) cluster_wait();   // (no block leaves while another may still read its sums)
+}
+template <typename T, int TH, int P, bool EVEN>
+__global__ void __launch_bounds__(TH, 1024 / TH) k_feedback_long(FeedbackArgs a, Scores<T> in) {
+    __shared__ FeedbackShared<TH> sh;
+    if (a.k == (int)cg::this_cluster().num_blocks() * Hold<T, TH, P, EVEN>::CELLS) feedback_long<T, TH, P, EVEN, true>(a, in, sh);
+    else feedback_long<T, TH, P, EVEN, false>(a, in, sh);
 }
 }  // namespace
 

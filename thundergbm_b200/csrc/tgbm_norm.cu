@@ -384,8 +384,8 @@ __device__ __forceinline__ void norm_long(const NormArgs &a, const Scores<T> &in
                 }
             }
         }
-        if (C > 1) cluster_arrive();
         __syncthreads();
+        if (C > 1) cluster_done();
     }
     float rstd[R];
 #pragma unroll
@@ -524,9 +524,9 @@ void scores_norm(const NormArgs &a, cudaStream_t stream) {
             bool done = false;
             // Parts of a row that 512 threads hold, and several rows at a time where the rows are many: the smaller parts first, which need more blocks
             // for a row (at most LONG_CLUSTER) and hold more rows.
-            auto go = [&](auto p, auto rows, auto ev) {
+            auto go = [&](auto th, auto p, auto rows, auto ev) {
                 constexpr bool EVEN = decltype(ev)::value;
-                constexpr int TH = 512, P = decltype(p)::value, R = decltype(rows)::value;
+                constexpr int TH = decltype(th)::value, P = decltype(p)::value, R = decltype(rows)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
                 if (done || c > LONG_CLUSTER || (R > 1 && (long long)a.n * c < 2 * 148 * R)) return;
                 launch_long(k_norm_long<T, TH, P, R, EVEN>, (a.n + R - 1) / R, c, TH, stream, a, in, out);
@@ -535,11 +535,12 @@ void scores_norm(const NormArgs &a, cudaStream_t stream) {
             using std::integral_constant;
             auto all = [&](auto ev) {
                 constexpr int S = decltype(ev)::value ? 2 : 8;   // packs of a quarter of what a thread holds
-                go(integral_constant<int, S>{}, integral_constant<int, 4>{}, ev);
-                go(integral_constant<int, S>{}, integral_constant<int, 1>{}, ev);
-                go(integral_constant<int, 2 * S>{}, integral_constant<int, 2>{}, ev);
-                go(integral_constant<int, 2 * S>{}, integral_constant<int, 1>{}, ev);
-                go(integral_constant<int, 4 * S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, S>{}, integral_constant<int, 4>{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, 2 * S>{}, integral_constant<int, 2>{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, 2 * S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 256>{}, integral_constant<int, 4 * S>{}, integral_constant<int, 1>{}, ev);
+                go(integral_constant<int, 512>{}, integral_constant<int, 4 * S>{}, integral_constant<int, 1>{}, ev);
             };
             even ? all(std::true_type{}) : all(std::false_type{});
             if (done) return;

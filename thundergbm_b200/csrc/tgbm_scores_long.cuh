@@ -41,8 +41,10 @@ template <int M, typename F> __device__ __forceinline__ F sums_spread(F (&v)[M])
     for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
     return v[0];
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The last barrier of a kernel whose blocks have read one another's shared memory: none leaves before all have.  Nothing that was written is handed
+// over by it (relaxed: a release would wait for all that the block has stored).
+__device__ __forceinline__ void cluster_done() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 // ---- long rows: a block, or a cluster of blocks, each with a part of the row in its registers -------------------------------
 // A thread's scores: packs of 16 bytes, TH packs apart (EVEN: rows, gains and results all begin on such boundaries), or single ones, TH apart.
@@ -65,6 +67,40 @@ template <typename T, int TH, int P, bool EVEN> struct Hold {
     __device__ __forceinline__ void get(int u, float (&v)[V]) const {
         if constexpr (EVEN) w[u].unpack(v);
         else v[0] = score_f32(one[u]);
+    }
+    // least and largest of a thread's scores; NaN does not count
+    __device__ __forceinline__ void range(int cells, float &low, float &high) const {
+        low = -minus_inf(); high = minus_inf();
+        if constexpr (EVEN && sizeof(T) == 2) {
+            typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+            T2 lows, highs;
+            bool some = false;
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                if (cells == CELLS || first(u) < cells) {
+                    const unsigned words[4] = {w[u].bits.x, w[u].bits.y, w[u].bits.z, w[u].bits.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const T2 v = *reinterpret_cast<const T2 *>(&words[i]);
+                        lows = u + i == 0 ? v : __hmin2(lows, v);
+                        highs = u + i == 0 ? v : __hmax2(highs, v);
+                    }
+                    some = true;
+                }
+            if (some) {
+                low = fminf(fminf(low, score_f32(lows.x)), score_f32(lows.y));
+                high = fmaxf(fmaxf(high, score_f32(highs.x)), score_f32(highs.y));
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                if (cells == CELLS || first(u) < cells) {
+                    float v[V];
+                    get(u, v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) { low = fminf(low, v[i]); high = fmaxf(high, v[i]); }
+                }
+        }
     }
     // cells h to h + Q of pack u
     template <int Q> __device__ __forceinline__ void get_some(int u, int h, float (&v)[Q]) const {
