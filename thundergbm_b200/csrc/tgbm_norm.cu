@@ -432,10 +432,298 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_norm_long(NormArgs a, Scores<
     else norm_long<T, TH, P, R, EVEN, false>(a, in, out, sh);
 }
 
-// Gradients of gain and bias: a block sums a share of the rows for 32 classes, the shares are added in order afterwards.
-constexpr int SHARES = 296;
-inline int shares_of(int n, int k) { return (int)std::max(1ll, std::min<long long>({(long long)SHARES, (n + 31ll) / 32, (1ll << 23) / k + 1})); }
+// ---- the way back ------------------------------------------------------------------------------
+// Sums over the rows, for the gradients of gain and bias, are made by blocks that stay: each adds up what its rows give to a class in a
+// register of the thread that has the class and puts the sum down at the end; a second kernel adds the blocks' sums in order.
+constexpr int SHARES = 296, FEW_SHARES = 148 * 8;
+inline int shares_of(int n, int k) {
+    return (int)std::max(1ll, std::min<long long>({k <= 32 ? (long long)FEW_SHARES : (long long)SHARES, (n + 31ll) / 32, (1ll << 23) / k + 1}));
+}
 
+template <int W> struct BackShared {
+    float4 v[2][W > 1 ? W : 1][33];   // (padded: a warp reads a column)
+    float4 sum[2][32];
+};
+__device__ __forceinline__ float4 add4(float4 a, float4 b) { return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w); }
+// as over_warps, for three numbers
+template <int W> __device__ __forceinline__ float4 over_warps(BackShared<W> &sh, int turn, float4 v) {
+    if constexpr (W > 1) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        sh.v[turn][warp][lane] = v;
+        __syncthreads();
+        if constexpr (W <= 8) {
+            v = sh.v[turn][0][lane];
+#pragma unroll
+            for (int w = 1; w < W; ++w) v = add4(v, sh.v[turn][w][lane]);
+        } else {
+#pragma unroll
+            for (int r = warp; r < 32; r += W) {
+                float4 u = sh.v[turn][lane & (W - 1)][r];
+#pragma unroll
+                for (int o = W / 2; o > 0; o >>= 1)
+                    u = add4(u, make_float4(__shfl_xor_sync(0xffffffffu, u.x, o), __shfl_xor_sync(0xffffffffu, u.y, o), __shfl_xor_sync(0xffffffffu, u.z, o), 0.f));
+                if (lane == 0) sh.sum[turn][r] = u;
+            }
+            __syncthreads();
+            v = sh.sum[turn][lane];
+        }
+    }
+    return v;
+}
+
+// By class, up to 1024 classes: a lane has a row, W warps share its classes.  What 32 rows give to a class is added across the lanes, which hold 32 sums
+// then (16 of x g and of g each, or one kind after the other).
+template <typename T, int E, int W, bool WEIGHTS>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? (E == 32 ? 2 : 4) : W == 16 ? (E == 16 ? 2 : 1) : 1)
+    k_norm_backward_class(NormBackwardArgs a, Scores<T> grad, Scores<T> in, Scores<T> out) {
+    constexpr int G = W == 1 ? 4 : 1;
+    __shared__ BackShared<W> sh;
+    __shared__ float groups[WEIGHTS && W == 1 ? 4 : 1][2][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k0 = W == 1 ? 0 : warp * E, here = a.k - k0;
+    const long long tiles = (a.n + 32ll * G - 1) / (32 * G);
+    float acc[2] = {0.f, 0.f};
+    int turn = 0;
+    for (long long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+        const long long n0 = (W == 1 ? tile * 4 + warp : tile) * 32 + lane, n = min(n0, a.n - 1ll);
+        float x[E], g[E];
+        read_classes<E>(in.at(n, k0), (int)in.cls, here, minus_inf(), x);
+        read_classes<E>(grad.at(n, k0), (int)grad.cls, here, 0.f, g);
+        const float mean = a.mean[n], rstd = a.rstd[n];
+        const float *gain = a.gain ? a.gain + k0 : nullptr;
+        auto gain_of = [&](int j) { return gain ? (j < here ? __ldg(gain + j) : 0.f) : 1.f; };
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        unsigned gone = 0;   // classes that the row may not have
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool is = there(x[j]);
+            if (!is) gone |= 1u << j;
+            x[j] = is ? __fsub_rn(x[j], mean) * rstd : 0.f;
+            g[j] = is ? g[j] : 0.f;
+            const float b = g[j] * gain_of(j);
+            v.x += b;
+            v.y = __fmaf_rn(b, x[j], v.y);
+        }
+        v.z = (float)(E - __popc(gone));
+        v = over_warps(sh, turn, v);
+        turn ^= 1;
+        const float inv = 1.f / fmaxf(v.z, 1.f), c1 = v.x * inv, c2 = v.y * inv;
+        if (n0 == n)
+            write_classes<E>(out.at(n, k0), (int)out.cls, here, [&](int j) {
+                return gone >> j & 1 ? 0.f : rstd * __fsub_rn(__fsub_rn(g[j] * gain_of(j), c1), x[j] * c2);
+            });
+        if constexpr (WEIGHTS) {
+            if (n0 != n) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) g[j] = 0.f;   // (a row that was read for another lane)
+            }
+            if constexpr (E <= 16) {
+                float both[2 * E];
+#pragma unroll
+                for (int j = 0; j < E; ++j) { both[j] = g[j]; both[E + j] = g[j] * x[j]; }
+                acc[0] += sums_spread<2 * E>(both);
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; ++j) x[j] *= g[j];
+                acc[0] += sums_spread<E>(g);
+                acc[1] += sums_spread<E>(x);
+            }
+        }
+    }
+    if constexpr (WEIGHTS) {
+        float *to = a.work + blockIdx.x * 2ll * a.k;
+        constexpr int M = E <= 16 ? 2 * E : E, PER = 32 / M;
+        const int m = lane / PER, j = E <= 16 ? m % E : m, kind = E <= 16 ? m / E : 0;
+        if constexpr (W == 1) {
+            if (lane % PER == 0) {
+                groups[warp][kind][j] = acc[0];
+                if (E > 16) groups[warp][1][j] = acc[1];
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 2 * a.k; i += 128) {
+                const int which = i / a.k, c = i % a.k;
+                to[i] = (groups[0][which][c] + groups[1][which][c]) + (groups[2][which][c] + groups[3][which][c]);
+            }
+        } else if (lane % PER == 0 && j < here) {
+            to[kind * (long long)a.k + k0 + j] = acc[0];
+            if (E > 16) to[a.k + k0 + j] = acc[1];
+        }
+    }
+}
+
+// By row, up to 1024 classes: L lanes have a row, E classes each, L apart.
+template <typename T, int L, int E, bool WEIGHTS>
+__global__ void __launch_bounds__(ROW_THREADS) k_norm_backward_row(NormBackwardArgs a, Scores<T> grad, Scores<T> in, Scores<T> out) {
+    constexpr int R = ROW_THREADS / L;
+    __shared__ float sums[WEIGHTS ? 2 * L * E : 1];
+    const int l = threadIdx.x & (L - 1);
+    float to_bias[E], to_gain[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) to_bias[j] = to_gain[j] = 0.f;
+    for (long long first = blockIdx.x * (long long)R; first < a.n; first += gridDim.x * (long long)R) {
+        const long long n0 = first + threadIdx.x / L, n = min(n0, a.n - 1ll);
+        float x[E], g[E];
+        {
+            const T *xs = in.at(n, l), *gs = grad.at(n, l);
+            T rx[E], rg[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (l + j * L < a.k) { rx[j] = xs[(long long)j * L * in.cls]; rg[j] = gs[(long long)j * L * grad.cls]; }
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+                x[j] = l + j * L < a.k ? score_f32(rx[j]) : minus_inf();
+                g[j] = l + j * L < a.k ? score_f32(rg[j]) : 0.f;
+            }
+        }
+        const float mean = a.mean[n], rstd = a.rstd[n];
+        auto gain_of = [&](int j) { return a.gain && l + j * L < a.k ? __ldg(a.gain + l + j * L) : 1.f; };
+        unsigned gone = 0;
+        float s = 0, sx = 0;
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const bool is = there(x[j]);
+            if (!is) gone |= 1u << j;
+            x[j] = is ? __fsub_rn(x[j], mean) * rstd : 0.f;
+            g[j] = is ? g[j] : 0.f;
+            const float b = g[j] * gain_of(j);
+            s += b;
+            sx = __fmaf_rn(b, x[j], sx);
+        }
+        const float inv = 1.f / (float)max(1, lanes_sum<L>(E - __popc(gone))), c1 = lanes_sum<L>(s) * inv, c2 = lanes_sum<L>(sx) * inv;
+        if (n0 == n) {
+            T *to = out.at(n, l);
+#pragma unroll
+            for (int j = 0; j < E; ++j)
+                if (l + j * L < a.k) to[(long long)j * L * out.cls] = score_from<T>(gone >> j & 1 ? 0.f : rstd * __fsub_rn(__fsub_rn(g[j] * gain_of(j), c1), x[j] * c2));
+            if (WEIGHTS) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) { to_bias[j] += g[j]; to_gain[j] = __fmaf_rn(g[j], x[j], to_gain[j]); }
+            }
+        }
+    }
+    if constexpr (WEIGHTS) {
+        // lanes that have the same classes, then the warps one after the other
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+#pragma unroll
+            for (int o = L; o < 32; o <<= 1) {
+                to_bias[j] += __shfl_xor_sync(0xffffffffu, to_bias[j], o);
+                to_gain[j] += __shfl_xor_sync(0xffffffffu, to_gain[j], o);
+            }
+        for (int w = 0; w < ROW_WARPS; ++w) {
+            if ((int)(threadIdx.x >> 5) == w && (threadIdx.x & 31) < L) {
+#pragma unroll
+                for (int j = 0; j < E; ++j) {
+                    float *b = sums + l + j * L, *g = b + L * E;
+                    *b = w ? *b + to_bias[j] : to_bias[j];
+                    *g = w ? *g + to_gain[j] : to_gain[j];
+                }
+            }
+            __syncthreads();
+        }
+        for (int k = threadIdx.x; k < a.k; k += ROW_THREADS) {
+            a.work[blockIdx.x * 2ll * a.k + k] = sums[k];
+            a.work[(blockIdx.x * 2ll + 1) * a.k + k] = sums[L * E + k];
+        }
+    }
+}
+
+// Long rows: a cluster of up to 8 blocks (or one) takes row after row, each block the same part of every row; the next row is on its way while this one is
+// worked on.
+template <typename T, int TH, int P, bool EVEN, bool WEIGHTS>
+__global__ void __launch_bounds__(TH) k_norm_backward_long(NormBackwardArgs a, Scores<T> grad, Scores<T> in, Scores<T> out) {
+    typedef Hold<T, TH, P, EVEN> H;
+    constexpr int V = H::V, W = TH / 32;
+    __shared__ float4 parts[2][W], block[2];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lo = rank * H::CELLS, cells = min(a.k - lo, H::CELLS);
+    const long long step = gridDim.x / C;
+    float to_bias[WEIGHTS ? H::E : 1], to_gain[WEIGHTS ? H::E : 1];
+#pragma unroll
+    for (int j = 0; j < (WEIGHTS ? H::E : 1); ++j) to_bias[j] = to_gain[j] = 0.f;
+    H x, g, next_x, next_g;
+    long long n = blockIdx.x / C;
+    if (n < a.n) { next_x.read(in.at(n, lo), cells); next_g.read(grad.at(n, lo), cells); }
+    int turn = 0;
+    for (; n < a.n; n += step) {
+        x = next_x; g = next_g;
+        if (n + step < a.n) { next_x.read(in.at(n + step, lo), cells); next_g.read(grad.at(n + step, lo), cells); }
+        const float mean = a.mean[n], rstd = a.rstd[n];
+        // x hat, gradient of out and gain of pack u; 0 where the row may not have a class
+        auto each = [&](auto &&f) {
+#pragma unroll
+            for (int u = 0; u < P; ++u)
+                if (H::first(u) < cells) {
+                    float v[V], w[V], by[V];
+                    x.get(u, v);
+                    g.get(u, w);
+                    read_floats<V>(a.gain ? a.gain + lo + H::first(u) : nullptr, 1.f, by);
+                    f(u, v, w, by);
+                }
+        };
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        each([&](int u, const float (&v)[V], const float (&w)[V], const float (&by)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const bool is = there(v[i]);
+                const float hat = is ? __fsub_rn(v[i], mean) * rstd : 0.f, gy = is ? w[i] : 0.f, b = gy * by[i];
+                sum.x += b;
+                sum.y = __fmaf_rn(b, hat, sum.y);
+                sum.z += is ? 1.f : 0.f;
+                if constexpr (WEIGHTS) {
+                    to_bias[u * V + i] += gy;
+                    to_gain[u * V + i] = __fmaf_rn(gy, hat, to_gain[u * V + i]);
+                }
+            }
+        });
+        {
+            float v[4] = {sum.x, sum.y, sum.z, 0.f};
+            const float s = sums_spread<4>(v);
+            if ((lane & 7) == 0) reinterpret_cast<float *>(&parts[turn][warp])[lane >> 3] = s;
+        }
+        __syncthreads();
+        if (C > 1) {
+            if (warp == 0) {
+                const float4 p = parts[turn][lane & (W - 1)];
+                const float4 all = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
+                if (lane == 0) block[turn] = all;
+            }
+            cluster.sync();
+            const float4 p = lane < C ? *cluster.map_shared_rank(&block[turn], lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+            sum = make_float4(lanes_sum<32>(p.x), lanes_sum<32>(p.y), lanes_sum<32>(p.z), 0.f);
+        } else {
+            const float4 p = parts[turn][lane & (W - 1)];
+            sum = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
+        }
+        turn ^= 1;
+        const float inv = 1.f / fmaxf(sum.z, 1.f), c1 = sum.x * inv, c2 = sum.y * inv;
+        T *to = out.at(n, lo);
+        each([&](int u, float (&v)[V], const float (&w)[V], const float (&by)[V]) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float hat = __fsub_rn(v[i], mean) * rstd;
+                v[i] = there(v[i]) ? rstd * __fsub_rn(__fsub_rn(w[i] * by[i], c1), hat * c2) : 0.f;
+            }
+            x.template set_some<V>(u, 0, v);
+            x.write(to, u);
+        });
+    }
+    if constexpr (WEIGHTS) {
+        float *bias = a.work + (blockIdx.x / C) * 2ll * a.k + lo, *gain = bias + a.k;
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+            if (H::first(u) < cells) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) { bias[H::first(u) + i] = to_bias[u * V + i]; gain[H::first(u) + i] = to_gain[u * V + i]; }
+            }
+    }
+    if (C > 1) {   // (no block leaves while another may still read its sums)
+        cluster_done();
+        cluster_wait();
+    }
+}
+
+// Any strides: a block sums a share of the rows for 32 classes.
 template <typename T>
 __global__ void __launch_bounds__(ROW_THREADS) k_norm_weights_any(NormBackwardArgs a, Scores<T> grad, Scores<T> in, int shares) {
     __shared__ float sums[2][ROW_WARPS][32];
@@ -459,13 +747,24 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_weights_any(NormBackwardAr
         a.work[(share * 2 + warp) * a.k + k] = (float)t;
     }
 }
+// The sums of all blocks: a warp takes every eighth, what the warps have is added in order.
 __global__ void __launch_bounds__(ROW_THREADS) k_norm_weights_join(NormBackwardArgs a, int shares) {
-    const long long i = blockIdx.x * (long long)ROW_THREADS + threadIdx.x;
-    if (i >= 2ll * a.k) return;
+    __shared__ double sums[ROW_WARPS][32];
+    chain_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long i = blockIdx.x * 32ll + lane;
     double t = 0;
-    for (int s = 0; s < shares; ++s) t += (double)a.work[s * 2ll * a.k + i];
-    if (i < a.k) a.to_bias[i] = (float)t;
-    else a.to_gain[i - a.k] = (float)t;
+    if (i < 2ll * a.k) {
+#pragma unroll 8
+        for (int s = warp; s < shares; s += ROW_WARPS) t += (double)a.work[s * 2ll * a.k + i];
+    }
+    sums[warp][lane] = t;
+    __syncthreads();
+    if (warp == 0 && i < 2ll * a.k) {
+        for (int w = 1; w < ROW_WARPS; ++w) t += sums[w][lane];
+        if (i < a.k) a.to_bias[i] = (float)t;
+        else a.to_gain[i - a.k] = (float)t;
+    }
 }
 }  // namespace
 
@@ -560,16 +859,67 @@ void scores_norm_backward(const NormBackwardArgs &a, cudaStream_t stream) {
         }
         return;
     }
+    const int most = shares_of(a.n, a.k);
+    int shares = 0;   // blocks that have put sums down
     by_type(a.in.type, [&](auto t) {
         using T = decltype(t);
         const Scores<T> grad = scores_of<T>(a.grad), in = scores_of<T>(a.in), out = scores_of<T>(a.out);
-        k_norm_backward_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, grad, in, out);
-        if (a.to_gain) {
-            const int shares = shares_of(a.n, a.k);
+        const bool weights = a.to_gain != nullptr, by_class = (in.row < in.cls && grad.row < grad.cls && out.row < out.cls) || a.in.one_by_class;
+        using std::integral_constant;
+        if (by_class && a.k <= SCORES_CLASS_MOST && std::max({in.cls, grad.cls, out.cls}) <= INT_MAX) {
+            auto go = [&](auto e, auto w) {
+                constexpr int E = decltype(e)::value, W = decltype(w)::value;
+                const long long rows = W == 1 ? 128 : 32;
+                const int blocks = (int)std::min<long long>((a.n + rows - 1) / rows, most);
+                auto kern = weights ? k_norm_backward_class<T, E, W, true> : k_norm_backward_class<T, E, W, false>;
+                kern<<<blocks, W == 1 ? 128 : 32 * W, 0, stream>>>(a, grad, in, out);
+                shares = blocks;
+            };
+            if (a.k > 128 && a.k <= 256) go(integral_constant<int, 16>{}, integral_constant<int, 16>{});
+            else by_class_sizes(a.k, go);
+            return;
+        }
+        if (a.k <= ROW_MOST) {
+            by_row_sizes(a.k, [&](auto l, auto e) {
+                constexpr int L = decltype(l)::value, E = decltype(e)::value;
+                const long long rows = ROW_THREADS / L;
+                const int blocks = (int)std::min<long long>((a.n + rows - 1) / rows, most);
+                auto kern = weights ? k_norm_backward_row<T, L, E, true> : k_norm_backward_row<T, L, E, false>;
+                kern<<<blocks, ROW_THREADS, 0, stream>>>(a, grad, in, out);
+                shares = blocks;
+            });
+            return;
+        }
+        bool done = false, summed = false;
+        if (in.cls == 1 && grad.cls == 1 && out.cls == 1) {
+            const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T)) && on_16(grad.p, grad.row, sizeof(T)) && on_16(out.p, out.row, sizeof(T)) &&
+                              on_16(a.gain, 0, 4);
+            auto go = [&](auto p, auto ev, auto sums) {
+                constexpr bool EVEN = decltype(ev)::value, SUMS = decltype(sums)::value;
+                constexpr int TH = 512, P = decltype(p)::value;
+                const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
+                if (done || c > LONG_CLUSTER) return;
+                // as many clusters as the SMs hold at once, and as there is room for sums
+                const int rows = (int)std::min<long long>({(long long)a.n, std::max(1, 148 / c), (long long)most});
+                launch_long(k_norm_backward_long<T, TH, P, EVEN, SUMS>, rows, c, TH, stream, a, grad, in, out);
+                done = true;
+                if (SUMS) { summed = true; shares = rows; }
+            };
+            auto all = [&](auto ev) {
+                constexpr int S = decltype(ev)::value ? 16 / Pack<T>::V : 16;   // 16 scores
+                if (weights) go(integral_constant<int, S>{}, ev, std::true_type{});
+                go(integral_constant<int, S>{}, ev, std::false_type{});
+                go(integral_constant<int, 2 * S>{}, ev, std::false_type{});
+            };
+            even ? all(std::true_type{}) : all(std::false_type{});
+        }
+        if (!done) k_norm_backward_any<T><<<a.n, ROW_THREADS, 0, stream>>>(a, grad, in, out);
+        if (weights && !summed) {
+            shares = most;
             k_norm_weights_any<T><<<dim3((a.k + 31) / 32, shares), ROW_THREADS, 0, stream>>>(a, grad, in, shares);
-            k_norm_weights_join<<<(2 * a.k + ROW_THREADS - 1) / ROW_THREADS, ROW_THREADS, 0, stream>>>(a, shares);
         }
     });
+    if (a.to_gain) launch_after(k_norm_weights_join, dim3((2 * a.k + 31) / 32), dim3(ROW_THREADS), 0, stream, a, shares);
     TGBM_CUDA(cudaGetLastError());
 }
 
