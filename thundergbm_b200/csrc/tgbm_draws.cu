@@ -1885,7 +1885,7 @@ void scores_sample(const SampleArgs &a, cudaStream_t stream) {
                 constexpr int TH = decltype(th)::value, P = decltype(p)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
                 if (done || c > LONG_CLUSTER) return;
-                launch_long(k_sample_long<T, TH, P, EVEN>, a.n, c, TH, stream, a, in);
+                launch_long(k_sample_long<T, TH, P, EVEN>, a.n, c, TH, stream, 0, a, in);
                 done = true;
             };
             using std::integral_constant;
@@ -1949,7 +1949,7 @@ void scores_feedback(const FeedbackArgs &given, cudaStream_t stream) {
                 constexpr int TH = decltype(th)::value, P = decltype(p)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
                 if (done || c > LONG_CLUSTER || (!decltype(last)::value && c > 1 && (long long)a.n * c > 8 * 148)) return;
-                launch_long(k_feedback_long<T, TH, P, EVEN>, a.n, c, TH, stream, a, in);
+                launch_long(k_feedback_long<T, TH, P, EVEN>, a.n, c, TH, stream, 0, a, in);
                 done = true;
             };
             using std::integral_constant;

@@ -628,94 +628,254 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_backward_row(NormBackwardA
 }
 
 // Long rows: a cluster of up to 8 blocks (or one) takes row after row, each block the same part of every row; the next row is on its way while this one is
-// worked on.
+// worked on.  Two scores of a thread go through each instruction.  A score of -inf makes the row's second sum infinite or NaN; only then is
+// every score looked at whether it is there (and in the next row from the start).
+// Rows that begin anywhere come through shared memory, by asynchronous copies of 16 bytes and a few single scores, two rows ahead; the others
+// through registers, one row ahead.
+// What a thread has of scores and gradients: as it was read, or (single scores in 16 bits) both of a class in one register.
+template <typename T, int TH, int P, bool EVEN> struct Both {
+    typedef Hold<T, TH, P, EVEN> H;
+    static constexpr int V = H::V, E = H::E;
+    static constexpr bool JOINED = !EVEN && sizeof(T) == 2;
+    H x, g;
+    unsigned both[JOINED ? P : 1];
+    // single scores, from shared memory
+    __device__ __forceinline__ void take(const T *xs, const T *gs, int cells) {
+#pragma unroll
+        for (int u = 0; u < P; ++u) {
+            const int at = min(H::first(u), cells - 1);   // (behind the last class: another one, which counts for nothing)
+            if constexpr (JOINED) both[u] = (unsigned)*reinterpret_cast<const unsigned short *>(xs + at) | (unsigned)*reinterpret_cast<const unsigned short *>(gs + at) << 16;
+            else { x.one[u] = xs[at]; g.one[u] = gs[at]; }
+        }
+    }
+    __device__ __forceinline__ static float2 split(unsigned v) {
+        Pack<T> pack;
+        pack.bits = make_uint4(v, 0, 0, 0);
+        float f[Pack<T>::V];
+        pack.unpack(f);
+        return make_float2(f[0], f[1]);
+    }
+    // the thread's scores i and i + 1 (i even) and their gradients
+    __device__ __forceinline__ void pair(int i, float2 &v, float2 &w) const {
+        if constexpr (JOINED) {
+            const float2 a = split(both[i]), b = split(both[i + 1]);
+            v = make_float2(a.x, b.x); w = make_float2(a.y, b.y);
+        } else if constexpr (EVEN) {
+            float a[V], b[V];
+            x.get(i / V, a);
+            g.get(i / V, b);
+            v = make_float2(a[i % V], a[i % V + 1]); w = make_float2(b[i % V], b[i % V + 1]);
+        } else {
+            v = make_float2(score_f32(x.one[i]), score_f32(x.one[i + 1])); w = make_float2(score_f32(g.one[i]), score_f32(g.one[i + 1]));
+        }
+    }
+    static __device__ __forceinline__ int cell(int i) { return EVEN ? H::first(i / V) + i % V : H::first(i); }
+};
+
+__device__ __forceinline__ void copy_async16(void *to, const void *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// rows in shared memory at a time
+template <typename T, int CELLS> constexpr int LONG_STAGES = CELLS * (int)sizeof(T) <= 32768 ? 3 : 1;
+template <typename T, int CELLS> constexpr size_t LONG_RING = 2 * (size_t)LONG_STAGES<T, CELLS> * (CELLS * sizeof(T) + 16);
+
 template <typename T, int TH, int P, bool EVEN, bool WEIGHTS>
 __global__ void __launch_bounds__(TH) k_norm_backward_long(NormBackwardArgs a, Scores<T> grad, Scores<T> in, Scores<T> out) {
-    typedef Hold<T, TH, P, EVEN> H;
-    constexpr int V = H::V, W = TH / 32;
+    typedef Both<T, TH, P, EVEN> B;
+    typedef typename B::H H;
+    constexpr int V = B::V, E = B::E, W = TH / 32;
     __shared__ float4 parts[2][W], block[2];
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lo = rank * H::CELLS, cells = min(a.k - lo, H::CELLS);
     const long long step = gridDim.x / C;
-    float to_bias[WEIGHTS ? H::E : 1], to_gain[WEIGHTS ? H::E : 1];
+    float2 to_bias[WEIGHTS ? E / 2 : 1], to_gain[WEIGHTS ? E / 2 : 1], gain[E / 2];
 #pragma unroll
-    for (int j = 0; j < (WEIGHTS ? H::E : 1); ++j) to_bias[j] = to_gain[j] = 0.f;
-    H x, g, next_x, next_g;
-    long long n = blockIdx.x / C;
-    if (n < a.n) { next_x.read(in.at(n, lo), cells); next_g.read(grad.at(n, lo), cells); }
-    int turn = 0;
-    for (; n < a.n; n += step) {
-        x = next_x; g = next_g;
-        if (n + step < a.n) { next_x.read(in.at(n + step, lo), cells); next_g.read(grad.at(n + step, lo), cells); }
-        const float mean = a.mean[n], rstd = a.rstd[n];
-        // x hat, gradient of out and gain of pack u; 0 where the row may not have a class
-        auto each = [&](auto &&f) {
+    for (int j = 0; j < (WEIGHTS ? E / 2 : 1); ++j) to_bias[j] = to_gain[j] = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int u = 0; u < P; ++u)
-                if (H::first(u) < cells) {
-                    float v[V], w[V], by[V];
-                    x.get(u, v);
-                    g.get(u, w);
-                    read_floats<V>(a.gain ? a.gain + lo + H::first(u) : nullptr, 1.f, by);
-                    f(u, v, w, by);
-                }
-        };
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        each([&](int u, const float (&v)[V], const float (&w)[V], const float (&by)[V]) {
+    for (int i = 0; i < E; i += 2) {   // (0 behind the last class: what is read there adds nothing)
+        const int k0 = B::cell(i), k1 = B::cell(i + 1);
+        gain[i / 2] = make_float2(k0 < cells ? a.gain ? a.gain[lo + k0] : 1.f : 0.f, k1 < cells ? a.gain ? a.gain[lo + k1] : 1.f : 0.f);
+    }
+    B have;
+    H next_x, next_g;
+    constexpr int STAGES = LONG_STAGES<T, H::CELLS>;
+    extern __shared__ __align__(16) unsigned char room[];   // (not EVEN) per stage: a row's scores and gradients, placed as they lie to 16 bytes
+    T *const ring = reinterpret_cast<T *>(room);
+    constexpr int LINE = H::CELLS + 16 / (int)sizeof(T);
+    auto shift = [](const T *p) { return (int)(reinterpret_cast<uintptr_t>(p) % 16 / sizeof(T)); };
+    T single[2];                    // the few scores around the packs of the row asked for last, on their way
+    T *single_to[2] = {nullptr, nullptr};
+    auto settle_single = [&] {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const bool is = there(v[i]);
-                const float hat = is ? __fsub_rn(v[i], mean) * rstd : 0.f, gy = is ? w[i] : 0.f, b = gy * by[i];
-                sum.x += b;
-                sum.y = __fmaf_rn(b, hat, sum.y);
-                sum.z += is ? 1.f : 0.f;
-                if constexpr (WEIGHTS) {
-                    to_bias[u * V + i] += gy;
-                    to_gain[u * V + i] = __fmaf_rn(gy, hat, to_gain[u * V + i]);
+        for (int i = 0; i < 2; ++i)
+            if (single_to[i]) { *single_to[i] = single[i]; single_to[i] = nullptr; }
+    };
+    auto fetch = [&](long long n, int stage) {
+        const T *xs = in.at(n, lo), *gs = grad.at(n, lo);
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                const int at = min(H::first(u), cells - V);   // (behind the last class: another one, which counts for nothing)
+                next_x.w[u].bits = *reinterpret_cast<const uint4 *>(xs + at);
+                next_g.w[u].bits = *reinterpret_cast<const uint4 *>(gs + at);
+            }
+        } else {
+            settle_single();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const T *from = i ? gs : xs;
+                T *to = ring + (2 * stage + i) * LINE + shift(from);
+                const Part<T> part(from, 0, cells);
+                const uint4 *body = part.body();
+                for (int c = threadIdx.x; c < part.packs; c += TH) copy_async16(reinterpret_cast<uint4 *>(to + part.head) + c, body + c);
+                if ((int)threadIdx.x < part.head + part.tail) {
+                    const int at = part.single(threadIdx.x);
+                    single[i] = from[at];
+                    single_to[i] = to + at;
                 }
             }
-        });
-        {
-            float v[4] = {sum.x, sum.y, sum.z, 0.f};
+            copies_commit();
+        }
+    };
+    long long n = blockIdx.x / C;
+    if constexpr (EVEN) {
+        if (n < a.n) fetch(n, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (n + i * step < a.n) fetch(n + i * step, i);
+            else copies_commit();
+        }
+    }
+    int turn = 0, stage = 0;
+    bool care = false;
+    for (; n < a.n; n += step) {
+        if constexpr (EVEN) {
+#pragma unroll
+            for (int u = 0; u < P; ++u) { have.x.w[u] = next_x.w[u]; have.g.w[u] = next_g.w[u]; }
+            if (n + step < a.n) fetch(n + step, 0);
+        } else {
+            // the row that this block worked on last has left its place: all threads have passed the barrier of its sums
+            const long long ahead = n + (STAGES - 1) * step;
+            const int to = stage == 0 ? STAGES - 1 : stage - 1;
+            if (ahead < a.n) fetch(ahead, to);
+            else { settle_single(); copies_commit(); }
+            if (STAGES == 1) settle_single();
+            copies_wait<STAGES - 1>();
+            __syncthreads();
+            const T *xs = in.at(n, lo), *gs = grad.at(n, lo);
+            have.take(ring + 2 * stage * LINE + shift(xs), ring + (2 * stage + 1) * LINE + shift(gs), cells);
+            stage = stage == STAGES - 1 ? 0 : stage + 1;
+        }
+        const float mean = a.mean[n], rstd = a.rstd[n];
+        const float2 minus_mean = make_float2(-mean, -mean), by = make_float2(rstd, rstd);
+        auto total = [&](float (&v)[4]) {
             const float s = sums_spread<4>(v);
             if ((lane & 7) == 0) reinterpret_cast<float *>(&parts[turn][warp])[lane >> 3] = s;
-        }
-        __syncthreads();
-        if (C > 1) {
-            if (warp == 0) {
+            __syncthreads();
+            float4 sum;
+            if (C > 1) {
+                if (warp == 0) {
+                    const float4 p = parts[turn][lane & (W - 1)];
+                    const float4 all = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
+                    if (lane == 0) block[turn] = all;
+                }
+                cluster.sync();
+                const float4 p = lane < C ? *cluster.map_shared_rank(&block[turn], lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+                sum = make_float4(warp_sum(p.x), warp_sum(p.y), warp_sum(p.z), 0.f);
+            } else {
                 const float4 p = parts[turn][lane & (W - 1)];
-                const float4 all = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
-                if (lane == 0) block[turn] = all;
+                sum = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
             }
-            cluster.sync();
-            const float4 p = lane < C ? *cluster.map_shared_rank(&block[turn], lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-            sum = make_float4(lanes_sum<32>(p.x), lanes_sum<32>(p.y), lanes_sum<32>(p.z), 0.f);
-        } else {
-            const float4 p = parts[turn][lane & (W - 1)];
-            sum = make_float4(lanes_sum<W>(p.x), lanes_sum<W>(p.y), lanes_sum<W>(p.z), 0.f);
-        }
-        turn ^= 1;
-        const float inv = 1.f / fmaxf(sum.z, 1.f), c1 = sum.x * inv, c2 = sum.y * inv;
-        T *to = out.at(n, lo);
-        each([&](int u, float (&v)[V], const float (&w)[V], const float (&by)[V]) {
+            turn ^= 1;
+            return sum;
+        };
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (!care) {
+            float2 s = make_float2(0.f, 0.f), sx = s;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float hat = __fsub_rn(v[i], mean) * rstd;
-                v[i] = there(v[i]) ? rstd * __fsub_rn(__fsub_rn(w[i] * by[i], c1), hat * c2) : 0.f;
+            for (int i = 0; i < E; i += 2) {
+                float2 v, w;
+                have.pair(i, v, w);
+                const float2 hat = mul2(add2(v, minus_mean), by), b = mul2(w, gain[i / 2]);
+                s = add2(s, b);
+                sx = fma2(b, hat, sx);
             }
-            x.template set_some<V>(u, 0, v);
-            x.write(to, u);
-        });
+            float v[4] = {s.x + s.y, sx.x + sx.y, 0.f, 0.f};
+            sum = total(v);
+            sum.z = (float)a.k;
+        }
+        if (care || !finite(sum.y)) {   // (the same in all threads)
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                float2 x, w;
+                have.pair(i, x, w);
+                auto one = [&](float f, float g, float its, int k) {
+                    if (k < cells && there(f)) {
+                        const float b = g * its;
+                        v[0] += b;
+                        v[1] = __fmaf_rn(b, __fsub_rn(f, mean) * rstd, v[1]);
+                        v[2] += 1.f;
+                    }
+                };
+                one(x.x, w.x, gain[i / 2].x, B::cell(i));
+                one(x.y, w.y, gain[i / 2].y, B::cell(i + 1));
+            }
+            sum = total(v);
+            care = sum.z != (float)a.k;
+        }
+        // rstd (b - mean(b) - hat mean(b hat))
+        const float inv = rstd / fmaxf(sum.z, 1.f), c1 = -sum.x * inv, c2 = -sum.y * inv;
+        const float2 m1 = make_float2(c1, c1), m2 = make_float2(c2, c2);
+        T *to = out.at(n, lo);
+#pragma unroll
+        for (int u = 0; u < (EVEN ? P : P / 2); ++u) {
+            constexpr int N = EVEN ? V : 2;
+            float r[N];
+#pragma unroll
+            for (int i = u * N; i < u * N + N; i += 2) {
+                float2 v, w;
+                have.pair(i, v, w);
+                float2 hat = mul2(add2(v, minus_mean), by), g = w;
+                if (care) {
+                    if (!there(v.x)) hat.x = g.x = 0.f;
+                    if (!there(v.y)) hat.y = g.y = 0.f;
+                }
+                float2 f = fma2(hat, m2, fma2(mul2(g, gain[i / 2]), by, m1));
+                if (care) {
+                    if (!there(v.x)) f.x = 0.f;
+                    if (!there(v.y)) f.y = 0.f;
+                }
+                r[i - u * N] = f.x; r[i - u * N + 1] = f.y;
+                if constexpr (WEIGHTS) {
+                    to_bias[i / 2] = add2(to_bias[i / 2], g);
+                    to_gain[i / 2] = fma2(g, hat, to_gain[i / 2]);
+                }
+            }
+            if constexpr (EVEN) {
+                if (H::first(u) < cells) {
+                    Pack<T> pack;
+                    pack.pack(r);
+                    *reinterpret_cast<uint4 *>(to + H::first(u)) = pack.bits;
+                }
+            } else {
+                if (H::first(2 * u) < cells) to[H::first(2 * u)] = score_from<T>(r[0]);
+                if (H::first(2 * u + 1) < cells) to[H::first(2 * u + 1)] = score_from<T>(r[1]);
+            }
+        }
     }
     if constexpr (WEIGHTS) {
-        float *bias = a.work + (blockIdx.x / C) * 2ll * a.k + lo, *gain = bias + a.k;
+        float *bias = a.work + (blockIdx.x / C) * 2ll * a.k + lo, *gains = bias + a.k;
 #pragma unroll
-        for (int u = 0; u < P; ++u)
-            if (H::first(u) < cells) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) { bias[H::first(u) + i] = to_bias[u * V + i]; gain[H::first(u) + i] = to_gain[u * V + i]; }
-            }
+        for (int i = 0; i < E; i += 2) {
+            const int k0 = B::cell(i), k1 = B::cell(i + 1);
+            if (k0 < cells) { bias[k0] = to_bias[i / 2].x; gains[k0] = to_gain[i / 2].x; }
+            if (k1 < cells) { bias[k1] = to_bias[i / 2].y; gains[k1] = to_gain[i / 2].y; }
+        }
     }
     if (C > 1) {   // (no block leaves while another may still read its sums)
         cluster_done();
@@ -828,7 +988,7 @@ void scores_norm(const NormArgs &a, cudaStream_t stream) {
                 constexpr int TH = decltype(th)::value, P = decltype(p)::value, R = decltype(rows)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
                 if (done || c > LONG_CLUSTER || (R > 1 && (long long)a.n * c < 2 * 148 * R)) return;
-                launch_long(k_norm_long<T, TH, P, R, EVEN>, (a.n + R - 1) / R, c, TH, stream, a, in, out);
+                launch_long(k_norm_long<T, TH, P, R, EVEN>, (a.n + R - 1) / R, c, TH, stream, 0, a, in, out);
                 done = true;
             };
             using std::integral_constant;
@@ -901,7 +1061,9 @@ void scores_norm_backward(const NormBackwardArgs &a, cudaStream_t stream) {
                 if (done || c > LONG_CLUSTER) return;
                 // as many clusters as the SMs hold at once, and as there is room for sums
                 const int rows = (int)std::min<long long>({(long long)a.n, std::max(1, 148 / c), (long long)most});
-                launch_long(k_norm_backward_long<T, TH, P, EVEN, SUMS>, rows, c, TH, stream, a, grad, in, out);
+                constexpr size_t ring = EVEN ? 0 : LONG_RING<T, Hold<T, TH, P, EVEN>::CELLS>;
+                if (!EVEN) allow_shared(k_norm_backward_long<T, TH, P, EVEN, SUMS>, ring);
+                launch_long(k_norm_backward_long<T, TH, P, EVEN, SUMS>, rows, c, TH, stream, ring, a, grad, in, out);
                 done = true;
                 if (SUMS) { summed = true; shares = rows; }
             };

@@ -134,9 +134,9 @@ template <typename T, int TH, int P, bool EVEN> struct Hold {
 inline bool on_16(const void *p, long long row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
 
 template <typename... P, typename... A>
-void launch_long(void (*kernel)(P...), long long rows, int cluster, int threads, cudaStream_t stream, A &&...args) {
+void launch_long(void (*kernel)(P...), long long rows, int cluster, int threads, cudaStream_t stream, size_t smem, A &&...args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(threads); cfg.stream = stream;
+    cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = cluster; attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
