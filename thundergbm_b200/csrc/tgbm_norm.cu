@@ -831,42 +831,47 @@ __global__ void __launch_bounds__(TH) k_norm_backward_long(NormBackwardArgs a, S
         // rstd (b - mean(b) - hat mean(b hat))
         const float inv = rstd / fmaxf(sum.z, 1.f), c1 = -sum.x * inv, c2 = -sum.y * inv;
         const float2 m1 = make_float2(c1, c1), m2 = make_float2(c2, c2);
-        T *to = out.at(n, lo);
+        T *to = out.at(n, lo) + H::first(0);
+        const int behind = cells - H::first(0);   // cells from this thread's first one on
+        auto write = [&](auto with_care) {
+            constexpr bool CARE = decltype(with_care)::value;
 #pragma unroll
-        for (int u = 0; u < (EVEN ? P : P / 2); ++u) {
-            constexpr int N = EVEN ? V : 2;
-            float r[N];
+            for (int u = 0; u < (EVEN ? P : P / 2); ++u) {
+                constexpr int N = EVEN ? V : 2;
+                float r[N];
 #pragma unroll
-            for (int i = u * N; i < u * N + N; i += 2) {
-                float2 v, w;
-                have.pair(i, v, w);
-                float2 hat = mul2(add2(v, minus_mean), by), g = w;
-                if (care) {
-                    if (!there(v.x)) hat.x = g.x = 0.f;
-                    if (!there(v.y)) hat.y = g.y = 0.f;
+                for (int i = u * N; i < u * N + N; i += 2) {
+                    float2 v, w;
+                    have.pair(i, v, w);
+                    float2 hat = mul2(add2(v, minus_mean), by), g = w;
+                    if (CARE) {
+                        if (!there(v.x)) hat.x = g.x = 0.f;
+                        if (!there(v.y)) hat.y = g.y = 0.f;
+                    }
+                    float2 f = fma2(hat, m2, fma2(mul2(g, gain[i / 2]), by, m1));
+                    if (CARE) {
+                        if (!there(v.x)) f.x = 0.f;
+                        if (!there(v.y)) f.y = 0.f;
+                    }
+                    r[i - u * N] = f.x; r[i - u * N + 1] = f.y;
+                    if constexpr (WEIGHTS) {
+                        to_bias[i / 2] = add2(to_bias[i / 2], g);
+                        to_gain[i / 2] = fma2(g, hat, to_gain[i / 2]);
+                    }
                 }
-                float2 f = fma2(hat, m2, fma2(mul2(g, gain[i / 2]), by, m1));
-                if (care) {
-                    if (!there(v.x)) f.x = 0.f;
-                    if (!there(v.y)) f.y = 0.f;
-                }
-                r[i - u * N] = f.x; r[i - u * N + 1] = f.y;
-                if constexpr (WEIGHTS) {
-                    to_bias[i / 2] = add2(to_bias[i / 2], g);
-                    to_gain[i / 2] = fma2(g, hat, to_gain[i / 2]);
+                if constexpr (EVEN) {
+                    if (u * TH * V < behind) {
+                        Pack<T> pack;
+                        pack.pack(r);
+                        *reinterpret_cast<uint4 *>(to + u * TH * V) = pack.bits;
+                    }
+                } else {
+                    if (2 * u * TH < behind) to[2 * u * TH] = score_from<T>(r[0]);
+                    if ((2 * u + 1) * TH < behind) to[(2 * u + 1) * TH] = score_from<T>(r[1]);
                 }
             }
-            if constexpr (EVEN) {
-                if (H::first(u) < cells) {
-                    Pack<T> pack;
-                    pack.pack(r);
-                    *reinterpret_cast<uint4 *>(to + H::first(u)) = pack.bits;
-                }
-            } else {
-                if (H::first(2 * u) < cells) to[H::first(2 * u)] = score_from<T>(r[0]);
-                if (H::first(2 * u + 1) < cells) to[H::first(2 * u + 1)] = score_from<T>(r[1]);
-            }
-        }
+        };
+        care ? write(std::true_type{}) : write(std::false_type{});
     }
     if constexpr (WEIGHTS) {
         float *bias = a.work + (blockIdx.x / C) * 2ll * a.k + lo, *gains = bias + a.k;
@@ -1054,9 +1059,9 @@ void scores_norm_backward(const NormBackwardArgs &a, cudaStream_t stream) {
         if (in.cls == 1 && grad.cls == 1 && out.cls == 1) {
             const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T)) && on_16(grad.p, grad.row, sizeof(T)) && on_16(out.p, out.row, sizeof(T)) &&
                               on_16(a.gain, 0, 4);
-            auto go = [&](auto p, auto ev, auto sums) {
+            auto go = [&](auto th, auto p, auto ev, auto sums) {
                 constexpr bool EVEN = decltype(ev)::value, SUMS = decltype(sums)::value;
-                constexpr int TH = 512, P = decltype(p)::value;
+                constexpr int TH = decltype(th)::value, P = decltype(p)::value;
                 const int c = (a.k + Hold<T, TH, P, EVEN>::CELLS - 1) / Hold<T, TH, P, EVEN>::CELLS;
                 if (done || c > LONG_CLUSTER) return;
                 // as many clusters as the SMs hold at once, and as there is room for sums
@@ -1068,10 +1073,10 @@ void scores_norm_backward(const NormBackwardArgs &a, cudaStream_t stream) {
                 if (SUMS) { summed = true; shares = rows; }
             };
             auto all = [&](auto ev) {
-                constexpr int S = decltype(ev)::value ? 16 / Pack<T>::V : 16;   // 16 scores
-                if (weights) go(integral_constant<int, S>{}, ev, std::true_type{});
-                go(integral_constant<int, S>{}, ev, std::false_type{});
-                go(integral_constant<int, 2 * S>{}, ev, std::false_type{});
+                constexpr int S = decltype(ev)::value ? 16 / Pack<T>::V : 16, HALF = decltype(ev)::value || sizeof(T) == 4 ? 1 : 2;   // 16 scores
+                if (weights) go(integral_constant<int, 512 / HALF>{}, integral_constant<int, S * HALF>{}, ev, std::true_type{});
+                go(integral_constant<int, 512 / HALF>{}, integral_constant<int, S * HALF>{}, ev, std::false_type{});
+                go(integral_constant<int, 512>{}, integral_constant<int, 2 * S>{}, ev, std::false_type{});
             };
             even ? all(std::true_type{}) : all(std::false_type{});
         }
