@@ -792,10 +792,11 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
 // Classes stand in the order block, u, thread, place in the pack (Hold); a segment is what a warp has of one u, 32 packs side by side.
 //
 // Limits: as above the scores that can be left are those from a border on, which is raised by bisection over the registers while more than
-// LONG_WANT reach it.  They go into a list in the first block, in class order, and that block alone goes on: every entry counts the larger ones,
+// LONG_LIST reach it.  They go into a list in the first block, in class order, and that block alone goes on: every entry counts the larger ones,
 // which is its place in descending order; prefix sums in that order tell where top_p ends, prefix sums in class order which class a random number
-// falls on.  Rows where more than LONG_LIST are left, and rows without limits, take their draws from sums per segment.
-constexpr int LONG_LIST = 1024, LONG_WANT = 384;
+// falls on.  Where top_p alone leaves more, what is certainly left is told from what the end of it lies among, and only that goes into the list.
+// Rows with more than a list, and rows without limits, take their draws from sums per segment.
+constexpr int LONG_LIST = 1024;
 
 template <int W, int S> struct LongRow {
     Powers powers;
@@ -804,11 +805,115 @@ template <int W, int S> struct LongRow {
     int counts[W], slot_count[2], count, front_count;
     double segment[S];                                // of a segment, then of all in front of it
     int segment_count[S];
-    int tie;
-    float x[LONG_LIST];
+    int tie, last;
+    float tie_score, at;
+    __align__(16) unsigned key[LONG_LIST];
     int k[LONG_LIST];
     double w[LONG_LIST], upto[LONG_LIST];
 };
+
+// The list of a row, `size` entries in class order: what is left of it (w[i] > 0), prefix sums in class order (upto), its mass.  `base`: mass of what is
+// larger than all entries (only where `border`: then the last entry that is left is told, in at and last).  All threads of a block.
+template <int W, int S>
+__device__ __noinline__ double settle_list(LongRow<W, S> &sh, const Exponent &weight, float top, int size, double min_p, int top_k, bool by_mass, bool of_list, double top_p,
+                                           double all, double base, bool border) {
+    constexpr int TH = 32 * W, Q = LONG_LIST / TH;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // exclusive prefix of the threads' sums
+    auto scan = [&](double own, double &whole) {
+        double upto = own;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        __syncthreads();
+        if (lane == 31) sh.sums[warp] = upto;
+        __syncthreads();
+        double before = 0;
+        whole = 0;
+        for (int v = 0; v < W; ++v) {
+            if (v == warp) before = whole;
+            whole += sh.sums[v];
+        }
+        return before + (upto - own);
+    };
+    auto count = [&](int own) {
+        own = warp_sum(own);
+        __syncthreads();
+        if (lane == 0) sh.counts[warp] = own;
+        __syncthreads();
+        int s = 0;
+        for (int v = 0; v < W; ++v) s += sh.counts[v];
+        return s;
+    };
+    if (tid < 4 && size + tid < LONG_LIST) sh.key[size + tid] = 0;   // (read four at a time)
+    __syncthreads();
+    int place[Q], heavy = 0;
+    double mine[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int i = q * TH + tid;
+        place[q] = size;
+        mine[q] = 0;
+        if (i < size) {
+            const unsigned own = sh.key[i];
+            mine[q] = weight(sh.powers, key_score(own), top);
+            heavy += mine[q] >= min_p;
+            int larger = 0;   // entries in front of this one in descending order: of equal ones those of lower classes
+            for (int j = 0; j < size; j += 4) {
+                const uint4 o = *reinterpret_cast<const uint4 *>(&sh.key[j]);
+                const unsigned over = own + (j + 4 > i);
+                larger += (o.x >= over) + (o.y >= over) + (o.z >= over) + (o.w >= over);
+            }
+            for (int j = i & ~3; j < i; ++j) larger += sh.key[j] == own;
+            place[q] = larger;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (place[q] < size) sh.w[place[q]] = mine[q];
+    int keep = min(count(heavy), top_k);   // in descending order
+    if (by_mass) {
+        // entries tid Q + q in descending order: prefix sums
+        double s = 0, whole;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) s += tid * Q + q < keep ? sh.w[tid * Q + q] : 0.0;
+        double upto = base + scan(s, whole);
+        const double target = top_p * (of_list ? whole : all);
+        int before = 0;   // entries in front of which the target is not reached
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (tid * Q + q < keep) {
+                before += tid * Q + q == 0 || upto < target;
+                upto += sh.w[tid * Q + q];
+            }
+        keep = count(before);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int i = q * TH + tid;
+        if (i < size) {
+            sh.w[i] = place[q] < keep ? mine[q] : 0.0;   // in class order now
+            if (border && place[q] == keep - 1) { sh.at = key_score(sh.key[i]); sh.last = sh.k[i]; }
+        }
+    }
+    __syncthreads();
+    double s = 0, mass;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) s += tid * Q + q < size ? sh.w[tid * Q + q] : 0.0;
+    double upto = scan(s, mass);
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+        if (tid * Q + q < size) {
+            upto += sh.w[tid * Q + q];
+            sh.upto[tid * Q + q] = upto;
+        }
+    __syncthreads();
+    return sh.upto[size - 1];
+}
 
 template <typename T, int TH, int P, bool EVEN>
 __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Scores<T> in) {
@@ -901,7 +1006,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         float its = top;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2)
-            if (groups / (2 * o) >= max(top_k < a.k ? top_k : 0, LONG_WANT / 4)) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
+            if (groups / (2 * o) >= max(top_k < a.k ? top_k : 0, 96)) its = fmaxf(its, __shfl_xor_sync(0xffffffffu, its, o));
         low = its > minus_inf() ? its : low;
     }
     total(sum, low, top, count);
@@ -998,12 +1103,12 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
             total(sum, f0, f1, count);
         }
         float high = top;
-        const bool narrowing = count > LONG_WANT && (by_count ? top_k <= LONG_LIST : by_mass && !by_share);
-        // (masses by floats, off by less than 2^-18)
-        const double enough = by_count ? (double)top_k : l.top_p * all * (1 + 1e-5);
-        const int want = max(LONG_WANT, by_count ? top_k : 0);
+        const bool narrowing = by_count ? top_k <= LONG_LIST : by_mass && !by_share;
+        // top_p alone: masses by floats, off by less than 2^-18, tell what certainly reaches the target and what certainly does not
+        const double enough = l.top_p * all * (1 + 1e-5), short_of = l.top_p * all * (1 - 1e-5);
+        int above = 0;   // scores larger than `high`, which are left in any case
         bool first = !by_count && guess > low && guess < top, moved = false;
-        while (narrowing && count > want && low < high) {
+        while (narrowing && count - above > LONG_LIST && low < high) {
             const float mid = first ? guess : middle(low, high);
             first = false;
             float up = -minus_inf(), below = minus_inf();
@@ -1012,24 +1117,46 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
 #pragma unroll
             for (int u = 0; u < P; ++u) {
                 if (!__any_sync(0xffffffffu, reach >> (u * V) & ((1ull << V) - 1))) continue;   // (nothing from the border on)
+                float part = 0;
                 each_of(u, [&](float x, int) {
                     if (x >= mid) {
                         ++c;
                         up = fminf(up, x);
-                        if (!by_count) sum += (double)rough(x);
+                        if (!by_count) part += rough(x);
                     } else if (x >= low) {
                         below = fmaxf(below, x);
                     }
                 });
+                sum += (double)part;
             }
             total(sum, up, below, c);
-            if ((by_count ? (double)c : sum) >= enough) { low = up; count = c; moved = true; }
-            else high = below;
+            if (by_count ? c >= top_k : sum >= enough) { low = up; count = c; moved = true; }
+            else if (below > minus_inf() && (by_count || sum < short_of)) {
+                high = below;
+                if (!by_count) above = c;
+            } else break;
         }
-        listed = count <= LONG_LIST;
-        if (listed) {
+        // whole: all that can be left stands in the list; part: so does the border, and what is larger is left
+        const bool whole = count <= LONG_LIST, part = !whole && narrowing && !by_count && count - above <= LONG_LIST;
+        listed = whole;
+        if (whole) above = 0;
+        if (whole || part) {
+            double base = 0;
+            if (part) {
+                each([&](float x, int) { base += x > high ? weight_of(x) : 0.0; });
+            } else {
+                high = top;
+            }
+            auto inside = [&](float x) { return x >= low && x <= high; };
+            if (moved || part) {
+                reach = 0;
+                int bit = 0;
+                each([&](float x, int) {
+                    reach |= inside(x) ? 1u << bit : 0u;
+                    ++bit;
+                });
+            }
             // into the first block's list, in class order
-            if (moved) mark(low);
             auto bits = [&](int u) { return (unsigned)(reach >> (u * V) & ((1ull << V) - 1)); };
             int mine = __popc(reach);
 #pragma unroll
@@ -1037,7 +1164,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 const int s = __reduce_add_sync(0xffffffffu, __popc(bits(u)));
                 if (lane == 0) sh.segment_count[u * W + warp] = s;
             }
-            total(sum, f0, f1, mine);
+            total(base, f0, f1, mine);
             prefix(sh.segment_count);
             LongRow<W, S> *to = C > 1 ? cluster.map_shared_rank(&sh, 0) : &sh;
 #pragma unroll
@@ -1052,12 +1179,28 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 }
                 int place = front_count + sh.segment_count[u * W + warp] + upto - c;
                 each_of(u, [&](float x, int k) {
-                    if (x >= low) { to->x[place] = x; to->k[place] = lo + k; ++place; }
+                    if (inside(x)) { to->key[place] = plain_key(x); to->k[place] = lo + k; ++place; }
                 });
             }
             if (C > 1) cluster.sync();
             else __syncthreads();
-            if (rank != 0) return;
+            if (rank == 0) {
+                const int size = count - above;
+                mass = settle_list(sh, weight, top, size, l.min_p, top_k, by_mass, by_count || by_share, l.top_p, all, base, part);
+                if (part && tid < C) {   // the border, for all blocks
+                    LongRow<W, S> *o = C > 1 ? cluster.map_shared_rank(&sh, tid) : &sh;
+                    o->tie_score = sh.at; o->tie = sh.last;
+                }
+                count = size;
+            } else if (whole) {
+                return;
+            }
+            if (part) {
+                if (C > 1) cluster.sync();
+                else __syncthreads();
+                at = sh.tie_score; last = sh.tie;
+                mass = segments();
+            }
         } else {
             // over all scores
             if (by_share) {
@@ -1207,95 +1350,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         if (C > 1) cluster.sync();   // (others look at this block's sums)
         return;
     }
-    // ---- the list: `count` entries, in class order
-    constexpr int Q = LONG_LIST / TH;
     const int size = count;
-    // exclusive prefix of the threads' sums
-    auto scan = [&](double own, double &whole) {
-        double upto = own;
-#pragma unroll
-        for (int o = 1; o < 32; o *= 2) {
-            const double v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        __syncthreads();
-        if (lane == 31) sh.sums[warp] = upto;
-        __syncthreads();
-        double before = 0;
-        whole = 0;
-        for (int v = 0; v < W; ++v) {
-            if (v == warp) before = whole;
-            whole += sh.sums[v];
-        }
-        return before + (upto - own);
-    };
-    int place[Q], heavy = 0;
-    double mine[Q];
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-        const int i = q * TH + tid;
-        place[q] = size;
-        mine[q] = 0;
-        if (i < size) {
-            const float x = sh.x[i];
-            mine[q] = weight_of(x);
-            heavy += mine[q] >= l.min_p;
-            int larger = 0;
-            for (int j = 0; j < i; ++j) larger += sh.x[j] >= x;
-            for (int j = i + 1; j < size; ++j) larger += sh.x[j] > x;
-            place[q] = larger;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-        if (place[q] < size) sh.w[place[q]] = mine[q];
-    heavy = warp_sum(heavy);
-    if (lane == 0) sh.counts[warp] = heavy;
-    __syncthreads();
-    heavy = 0;
-    for (int v = 0; v < W; ++v) heavy += sh.counts[v];
-    int keep = min(heavy, top_k);   // in descending order
-    if (by_mass) {
-        // entry i Q + q in descending order: prefix sums
-        double s = 0, whole;
-#pragma unroll
-        for (int q = 0; q < Q; ++q) s += tid * Q + q < keep ? sh.w[tid * Q + q] : 0.0;
-        double upto = scan(s, whole);
-        const double target = l.top_p * (by_count || by_share ? whole : all);
-        int before = 0;   // entries in front of which the target is not reached
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-            if (tid * Q + q < keep) {
-                before += tid * Q + q == 0 || upto < target;
-                upto += sh.w[tid * Q + q];
-            }
-        before = warp_sum(before);
-        __syncthreads();
-        if (lane == 0) sh.counts[warp] = before;
-        __syncthreads();
-        keep = 0;
-        for (int v = 0; v < W; ++v) keep += sh.counts[v];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < Q; ++q)
-        if (q * TH + tid < size) sh.w[q * TH + tid] = place[q] < keep ? mine[q] : 0.0;   // in class order now
-    __syncthreads();
-    {
-        double s = 0;
-#pragma unroll
-        for (int q = 0; q < Q; ++q) s += tid * Q + q < size ? sh.w[tid * Q + q] : 0.0;
-        double upto = scan(s, mass);
-#pragma unroll
-        for (int q = 0; q < Q; ++q)
-            if (tid * Q + q < size) {
-                upto += sh.w[tid * Q + q];
-                sh.upto[tid * Q + q] = upto;
-            }
-    }
-    __syncthreads();
-    mass = sh.upto[size - 1];
     for (int d = tid; d < a.draws; d += TH) {
         const long long i = n * a.draws + d;
         const double target = uniform_of(a, i) * mass;
@@ -1306,7 +1361,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
             else from = mid + 1;
         }
         while (from > 0 && !(sh.w[from] > 0)) --from;   // (prefix sums by different threads are not rounded alike)
-        put(i, sh.k[from], sh.x[from], log(mass), log(all));
+        put(i, sh.k[from], key_score(sh.key[from]), log(mass), log(all));
     }
 }
 
