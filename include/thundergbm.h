@@ -128,6 +128,13 @@ int tgbm_booster_boost(TgbmBooster *b, int n_rounds);
  * (tgbm_booster_get_labels).  With a communicator every rank calls it, with the same temperature and alpha and all with lse or none; where
  * one rank's call is refused, all are, and what was set before stays.  Metrics stay those of the labels; model files do not change. */
 int tgbm_booster_set_teacher(TgbmBooster *b, int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
+/* The same from classes that were drawn for the rows and the gains that followed: trees are grown on the pairs of tgbm_scores_feedback (below,
+ * without a reference) instead of the labels'.  Host arrays n_rows x draws (old: or NULL), weights n_rows (or NULL); copied.  Not beside a teacher.
+ * Ranks call it together, as above, with the same temperature, clip and entropy and all with old and weights or none. */
+int tgbm_booster_set_feedback(TgbmBooster *b, int draws, const int *classes, const float *gains, const float *old, const float *weights, float temperature,
+                              float clip_low, float clip_high, float entropy);
+/* the mean over this rank's rows of that loss on the current scores */
+int tgbm_booster_feedback_loss(TgbmBooster *b, double *out);
 /* that loss on the current scores: its mean over this rank's rows (waits as tgbm_booster_sync does; with a communicator every rank calls it) */
 int tgbm_booster_teacher_loss(TgbmBooster *b, double *out);
 int tgbm_booster_sync(TgbmBooster *b);
@@ -340,6 +347,14 @@ int tgbm_predict_top(int row_size, float *val, int *row_ptr, int *col_ptr, Tree 
                      const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse);
 int tgbm_predict_top_dense(int row_size, int n_cols, void *x, int is_f64, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
                            const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse);
+/* The same scores through tgbm_scores_adjust and tgbm_scores_sample: `draws` classes for every row from the random numbers `uniform` (row_size x draws
+ * doubles), under the same limits for all rows.  classes, logs and all_logs (the last two or NULL): row_size x draws. */
+int tgbm_predict_sample(int row_size, float *val, int *row_ptr, int *col_ptr, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                        const TgbmTopRules *rules, int draws, const double *uniform, float temperature, int top_k, float top_p, float min_p, int *classes,
+                        float *logs, float *all_logs);
+int tgbm_predict_sample_dense(int row_size, int n_cols, void *x, int is_f64, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                              const TgbmTopRules *rules, int draws, const double *uniform, float temperature, int top_k, float top_p, float min_p,
+                              int *classes, float *logs, float *all_logs);
 
 #ifdef __cplusplus
 }

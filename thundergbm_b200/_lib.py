@@ -69,6 +69,11 @@ def load() -> C.CDLL:
     lib.tgbm_metric_score_noalloc.argtypes = [C.c_char_p, C.c_int, C.c_int, vp, vp, vp, vp]
     lib.tgbm_booster_set_teacher.argtypes = [vp, C.c_int, vp, vp, vp, C.c_float, C.c_float]
     lib.tgbm_booster_teacher_loss.argtypes = [vp, P(C.c_double)]
+    lib.tgbm_booster_set_feedback.argtypes = [vp, C.c_int, vp, vp, vp, vp] + [C.c_float] * 4
+    lib.tgbm_booster_feedback_loss.argtypes = [vp, P(C.c_double)]
+    draws = [vp, C.c_int, C.c_int, C.c_float, P(TgbmTopRules), C.c_int, vp, C.c_float, C.c_int, C.c_float, C.c_float, vp, vp, vp]   # from the model on
+    lib.tgbm_predict_sample.argtypes = [C.c_int, vp, vp, vp] + draws
+    lib.tgbm_predict_sample_dense.argtypes = [C.c_int, C.c_int, vp, C.c_int] + draws
     rules = [vp, C.c_int, C.c_int, C.c_float, P(TgbmTopRules), C.c_int, C.c_float, vp, vp, vp]   # from the model on
     lib.tgbm_predict_top.argtypes = [C.c_int, vp, vp, vp] + rules
     lib.tgbm_predict_top_dense.argtypes = [C.c_int, C.c_int, vp, C.c_int] + rules

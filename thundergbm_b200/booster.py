@@ -115,6 +115,38 @@ class Booster:
         _lib.check(self._lib.tgbm_booster_teacher_loss(self.handle, C.byref(o)))
         return o.value
 
+    def set_feedback(self, classes, gains, old=None, weights=None, temperature: float = 1.0, clip=None, entropy: float = 0.0):
+        """Grow trees from classes that were drawn for the rows (positions in labels(), -1: none) and the gains that followed
+        (multi:softmax, multi:softprob; before the first round, not beside a teacher): one per row, or rows x up to 128.  `old`: log-probabilities
+        at drawing time, by which gains weigh as much as a class has become likelier since, held within 1 - clip and 1 + clip (a pair: the
+        two distances) where that makes the loss larger; without it every round takes the classes as drawn from the present scores.
+        `weights`: one per row; `entropy`: what a row's entropy earns."""
+        n = self.info.n_rows
+        try:
+            classes, gains = class_numbers(classes), np.ascontiguousarray(gains, np.float32)
+            if classes.ndim not in (1, 2) or classes.shape != gains.shape or classes.shape[0] != n:
+                raise ValueError('classes and gains: one per row, or rows x draws')
+            old = None if old is None else np.ascontiguousarray(old, np.float32)
+            if old is not None and old.shape != classes.shape:
+                raise ValueError('old: one for every drawn class')
+            weights = None if weights is None else np.ascontiguousarray(weights, np.float32)
+            if weights is not None and weights.shape != (n,):
+                raise ValueError('weights: one per row')
+            low, high = (1.0, float('inf')) if clip is None else clip if isinstance(clip, (tuple, list)) else (clip, clip)
+            numbers = [float(v) for v in (temperature, low, high, entropy)]
+        except Exception:
+            # the other ranks of a communicator wait for this one to say that it has nothing to take
+            self._lib.tgbm_booster_set_feedback(self.handle, 0, None, None, None, None, 1.0, 1.0, 0.0, 0.0)
+            raise
+        draws = classes.shape[1] if classes.ndim == 2 else 1
+        _lib.check(self._lib.tgbm_booster_set_feedback(self.handle, draws, _ptr(classes), _ptr(gains), _ptr(old), _ptr(weights), *numbers))
+
+    def feedback_loss(self) -> float:
+        """Mean over the rows of the loss that set_feedback() describes, on the current scores."""
+        o = C.c_double(0)
+        _lib.check(self._lib.tgbm_booster_feedback_loss(self.handle, C.byref(o)))
+        return o.value
+
     def boost(self, n_rounds: int):
         _lib.check(self._lib.tgbm_booster_boost(self.handle, n_rounds))
 

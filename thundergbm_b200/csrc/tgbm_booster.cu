@@ -23,6 +23,7 @@
 #include "tgbm_exact.cuh"
 #include "tgbm_rank.cuh"
 #include "tgbm_scores.h"
+#include "tgbm_scores_check.h"
 
 namespace tgbm {
 
@@ -71,6 +72,16 @@ struct BoosterImpl {
         DevBuf<float> logits, lse;
     } teacher;
     DistillArgs distill_args() const;
+    // classes that were drawn for every row and what followed (draws = 0: none)
+    struct Feedback {
+        int draws = 0;
+        float temperature = 1, clip_low = 1, clip_high = 0, entropy = 0;
+        DevBuf<int> classes;
+        DevBuf<float> gains, old, weights;
+    } feedback;
+    FeedbackArgs feedback_args() const;
+    void agree_on(DevBuf<unsigned> &said, const float *same, int count, const char *what);
+    double mean_loss(const std::function<void(float *)> &losses);
     DevBuf<float2> gh;
     DevBuf<int2> ghq;
     DevBuf<unsigned> maxbits;
@@ -1155,6 +1166,14 @@ void BoosterImpl::gradient(int round) {
                     scores_distill(a, stream);
                     break;
                 }
+                if (feedback.draws) {
+                    FeedbackArgs a = feedback_args();
+                    a.gives = GIVES_PAIRS;
+                    a.out.data = gh.p; a.out.row = 1; a.out.cls = N;
+                    a.maxbits = maxbits.p;
+                    scores_feedback(a, stream);
+                    break;
+                }
                 launch_after(k_grad_softmax, gb, tb, 0, stream, y.p, ypred.p, N, K, gh.p, maxbits.p); break;
             case RANK_PAIRWISE: case RANK_NDCG:
                 rank.gradient(rstate.p, p.rank_seed, ypred.p, gh.p, maxbits.p, stream); break;
@@ -1201,16 +1220,81 @@ DistillArgs BoosterImpl::distill_args() const {
     return a;
 }
 
+FeedbackArgs BoosterImpl::feedback_args() const {
+    FeedbackArgs a;
+    a.n = N; a.k = K; a.draws = feedback.draws;
+    a.in.data = ypred.p; a.in.row = 1; a.in.cls = N; a.in.one_by_class = N == 1;
+    a.classes = feedback.classes.p; a.gains = feedback.gains.p; a.old = feedback.old.p; a.weights = feedback.weights.p;
+    a.temperature = feedback.temperature; a.clip_low = feedback.clip_low; a.clip_high = feedback.clip_high; a.entropy = feedback.entropy;
+    return a;
+}
+
+// Ranks with rows have to mean the same objective: of a number and of its complement the largest over the ranks are each other's
+// complement only if all of them said the same.  same[0] is not 0; said: 2 count words; throws on all ranks alike.
+void BoosterImpl::agree_on(DevBuf<unsigned> &said, const float *same, int count, const char *what) {
+    std::vector<unsigned> words(2 * count, 0u);
+    if (N)
+        for (int i = 0; i < count; ++i) {
+            memcpy(&words[2 * i], &same[i], sizeof(float));
+            words[2 * i + 1] = ~words[2 * i];
+        }
+    TGBM_CUDA(cudaMemcpyAsync(said.p, words.data(), said.bytes(), cudaMemcpyHostToDevice, stream));
+    comm->allreduce(said.p, words.size(), Comm::U32, Comm::MAX, stream);
+    TGBM_CUDA(cudaMemcpyAsync(words.data(), said.p, said.bytes(), cudaMemcpyDeviceToHost, stream));
+    comm->wait(stream);
+    for (int i = 0; i < count && words[0]; ++i)   // (0: no rank has rows)
+        TGBM_CHECK(words[2 * i] == ~words[2 * i + 1], what);
+}
+
+void Booster::set_feedback(int draws, const int *classes, const float *gains, const float *old, const float *weights, float temperature, float clip_low,
+                           float clip_high, float entropy) {
+    BoosterImpl &m = *impl_;
+    const bool multi = m.comm && m.comm->active();
+    BoosterImpl::Feedback next;
+    DevBuf<unsigned> said;
+    std::string local_err;   // see Booster::init: ranks take it together or not at all
+    try {
+        TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "feedback needs objective multi:softmax or multi:softprob");
+        TGBM_CHECK(m.rounds == 0, "feedback has to be there before the first round");
+        TGBM_CHECK(!m.teacher.top, "a booster learns from a teacher or from feedback, not from both");
+        check_draws(draws);
+        check_temperature(temperature);
+        check_feedback(clip_low, clip_high, 0.f, entropy);
+        TGBM_CHECK((classes && gains) || m.N == 0, "feedback: null pointer");
+        const size_t cells = (size_t)m.N * draws;
+        next.classes.alloc(cells); next.gains.alloc(cells); next.old.alloc(old ? cells : 0); next.weights.alloc(weights ? m.N : 0);
+        auto up = [&](auto &to, const auto *from) {
+            if (from && to.bytes()) upload_h2d(to.p, from, to.bytes(), m.stream, upload_threads());
+        };
+        up(next.classes, classes); up(next.gains, gains); up(next.old, old); up(next.weights, weights);
+        if (multi) said.alloc(12);
+        TGBM_CUDA(cudaStreamSynchronize(m.stream));
+        next.draws = draws; next.temperature = temperature; next.clip_low = clip_low; next.clip_high = clip_high; next.entropy = entropy;
+    } catch (const std::exception &e) {
+        local_err = e.what();
+    }
+    if (multi) {
+        m.comm->agree(local_err, "taking its feedback", m.stream);
+        const float same[6] = {temperature, clip_low, clip_high, entropy, old ? 1.f : 0.f, weights ? 1.f : 0.f};
+        m.agree_on(said, same, 6, "the ranks' feedback differs in temperature, clip, entropy or what is given");
+    } else if (!local_err.empty()) {
+        throw Error(local_err);
+    }
+    BoosterImpl::Feedback &f = m.feedback;
+    f.classes.take(next.classes); f.gains.take(next.gains); f.old.take(next.old); f.weights.take(next.weights);
+    f.draws = next.draws; f.temperature = next.temperature; f.clip_low = next.clip_low; f.clip_high = next.clip_high; f.entropy = next.entropy;
+}
+
 void Booster::set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha) {
     BoosterImpl &m = *impl_;
     const bool multi = m.comm && m.comm->active();
     BoosterImpl::Teacher next;
     DevBuf<unsigned> said;
-    unsigned words[6] = {};
     std::string local_err;   // see Booster::init: ranks take a teacher together or not at all
     try {
         TGBM_CHECK(m.objective == MULTI_SOFTMAX || m.objective == MULTI_SOFTPROB, "a teacher needs objective multi:softmax or multi:softprob");
         TGBM_CHECK(m.rounds == 0, "the teacher has to be there before the first round");
+        TGBM_CHECK(!m.feedback.draws, "a booster learns from a teacher or from feedback, not from both");
         TGBM_CHECK(top >= 1 && top <= SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(SCORES_MAX_TOP) + "]");
         TGBM_CHECK(temperature_fits(temperature), "the temperature has to be a positive number");
         TGBM_CHECK(alpha >= 0.f && alpha <= 1.f, "alpha outside [0, 1]");
@@ -1230,21 +1314,8 @@ void Booster::set_teacher(int top, const int *ids, const float *logits, const fl
     }
     if (multi) {
         m.comm->agree(local_err, "taking its teacher", m.stream);
-        // Ranks with rows have to mean the same objective: of a number and of its complement the largest over the ranks are each
-        // other's complement only if all of them said the same.
-        if (m.N) {
-            const float same[3] = {temperature, alpha, lse ? 1.f : 0.f};
-            for (int i = 0; i < 3; ++i) {
-                memcpy(&words[2 * i], &same[i], sizeof(float));
-                words[2 * i + 1] = ~words[2 * i];
-            }
-        }
-        TGBM_CUDA(cudaMemcpyAsync(said.p, words, sizeof(words), cudaMemcpyHostToDevice, m.stream));
-        m.comm->allreduce(said.p, 6, Comm::U32, Comm::MAX, m.stream);
-        TGBM_CUDA(cudaMemcpyAsync(words, said.p, sizeof(words), cudaMemcpyDeviceToHost, m.stream));
-        m.comm->wait(m.stream);
-        for (int i = 0; i < 3 && words[0]; ++i)   // (0: no rank has rows; a temperature is none)
-            TGBM_CHECK(words[2 * i] == ~words[2 * i + 1], "the ranks' teachers differ in temperature, alpha or whether the log-sum-exp is given");
+        const float same[3] = {temperature, alpha, lse ? 1.f : 0.f};
+        m.agree_on(said, same, 3, "the ranks' teachers differ in temperature, alpha or whether the log-sum-exp is given");
     } else if (!local_err.empty()) {
         throw Error(local_err);
     }
@@ -1253,26 +1324,44 @@ void Booster::set_teacher(int top, const int *ids, const float *logits, const fl
     t.top = next.top; t.temperature = next.temperature; t.alpha = next.alpha;
 }
 
+// the mean over this rank's rows of what `losses` writes, a float per row
+double BoosterImpl::mean_loss(const std::function<void(float *)> &losses) {
+    if (N == 0) return 0;
+    DevBuf<float> loss;
+    DevBuf<double> partial, sum;
+    loss.alloc(N);
+    const int blocks = std::max(1, std::min(ceil_div(N, 256), 1024));
+    partial.alloc(blocks); sum.alloc(1);
+    losses(loss.p);
+    k_partial_sums<<<blocks, 256, 0, stream>>>(loss.p, N, partial.p);
+    k_metric_sum<<<1, 32, 0, stream>>>(partial.p, blocks, sum.p);
+    TGBM_CUDA(cudaGetLastError());
+    double total = 0;
+    TGBM_CUDA(cudaMemcpyAsync(&total, sum.p, sizeof(total), cudaMemcpyDeviceToHost, stream));
+    TGBM_CUDA(cudaStreamSynchronize(stream));
+    return total / N;
+}
+
 double Booster::teacher_loss() {
     BoosterImpl &m = *impl_;
     TGBM_CHECK(m.teacher.top, "the booster has no teacher");
     sync();
-    if (m.N == 0) return 0;
-    DevBuf<float> loss;
-    DevBuf<double> partial, sum;
-    loss.alloc(m.N);
-    const int blocks = std::max(1, std::min(ceil_div(m.N, 256), 1024));
-    partial.alloc(blocks); sum.alloc(1);
-    DistillArgs a = m.distill_args();
-    a.loss = loss.p;
-    scores_distill(a, m.stream);
-    k_partial_sums<<<blocks, 256, 0, m.stream>>>(loss.p, m.N, partial.p);
-    k_metric_sum<<<1, 32, 0, m.stream>>>(partial.p, blocks, sum.p);
-    TGBM_CUDA(cudaGetLastError());
-    double total = 0;
-    TGBM_CUDA(cudaMemcpyAsync(&total, sum.p, sizeof(total), cudaMemcpyDeviceToHost, m.stream));
-    TGBM_CUDA(cudaStreamSynchronize(m.stream));
-    return total / m.N;
+    return m.mean_loss([&](float *loss) {
+        DistillArgs a = m.distill_args();
+        a.loss = loss;
+        scores_distill(a, m.stream);
+    });
+}
+
+double Booster::feedback_loss() {
+    BoosterImpl &m = *impl_;
+    TGBM_CHECK(m.feedback.draws, "the booster has no feedback");
+    sync();
+    return m.mean_loss([&](float *loss) {
+        FeedbackArgs a = m.feedback_args();
+        a.loss = loss;
+        scores_feedback(a, m.stream);
+    });
 }
 
 // Base score (include/thundergbm/objective/regression_obj.h:35-53 and :95-114): gradients at y_pred = 0,

@@ -48,6 +48,11 @@ public:
     // refuses, or says another temperature for, none takes: they throw and keep what they had.
     void set_teacher(int top, const int *ids, const float *logits, const float *lse, float temperature, float alpha);
     double teacher_loss();   // that loss on the current scores, the mean over this rank's rows; syncs
+    // The same from classes that were drawn for the rows and the gains that followed: n x draws, n x draws, n x draws (or null), n (or null).  Not beside
+    // a teacher.
+    void set_feedback(int draws, const int *classes, const float *gains, const float *old, const float *weights, float temperature, float clip_low,
+                      float clip_high, float entropy);
+    double feedback_loss();
 
     int rounds_done() const;
     int trees_per_round() const;

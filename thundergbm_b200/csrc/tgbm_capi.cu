@@ -15,6 +15,7 @@
 #include "tgbm_booster.h"
 #include "tgbm_device.cuh"
 #include "tgbm_scores.h"
+#include "tgbm_scores_check.h"
 
 // the opaque C handle is the C++ tree container
 struct Tree : tgbm::Tree {
@@ -307,20 +308,17 @@ void train_scikit(Load &&load, int depth, int n_trees, int n_device, float min_c
     });
 }
 
-// adjust and top on the raw scores of a prediction, from and to host arrays
-template <typename View>
-int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, float learning_rate, const TgbmTopRules *rules, int top, float temperature,
-                float *values, int *ids, float *lse) {
+// The raw scores of a prediction under the caller's rules, from and to host arrays: check(n, k) before anything is done, act(scores, stream) on what
+// adjust leaves.
+template <typename View, typename Check, typename Act>
+int predict_ruled(View &&view, ::Tree **model, int n_trees, int trees_per_iter, float learning_rate, const TgbmTopRules *rules, Check &&check, Act &&act) {
     return guard([&] {
         tgbm::DataSet ds;
         view(ds);
         TGBM_CHECK(model && *model, "model is null!");
-        TGBM_CHECK(trees_per_iter >= 2, "the largest scores of a row need a model of several classes (multi:softmax, multi:softprob)");
-        TGBM_CHECK(top >= 1 && top <= tgbm::SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(tgbm::SCORES_MAX_TOP) + "]");
-        TGBM_CHECK(tgbm::temperature_fits(temperature), "the temperature has to be a positive number");
         const int n = ds.n_rows, k = trees_per_iter, words = (k + 31) / 32;
+        check(n);
         if (n == 0) return;
-        TGBM_CHECK(values && ids, "values or ids: null pointer");
         static const TgbmTopRules none{nullptr, nullptr, 0, nullptr, nullptr, nullptr, 1.f, 0.f, 0.f};
         const TgbmTopRules &r = rules ? *rules : none;
         TGBM_CHECK(r.repetition > 0.f && std::isfinite(r.repetition) && std::isfinite(1.f / r.repetition) && std::isfinite(r.frequency) && std::isfinite(r.presence),
@@ -335,9 +333,9 @@ int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, fl
         }
         const tgbm::ScoreStep step = [&](float *scores, int rows, int classes, cudaStream_t st) {
             const int threads = tgbm::upload_threads();
-            tgbm::DevBuf<float> d_bias, d_values, d_lse;
+            tgbm::DevBuf<float> d_bias;
             tgbm::DevBuf<unsigned> d_allowed;
-            tgbm::DevBuf<int> d_row, d_history, d_ids;
+            tgbm::DevBuf<int> d_row, d_history;
             tgbm::DevBuf<long long> d_ptr;
             auto up = [&](auto &buf, const auto *src, size_t count) {
                 buf.alloc(count);
@@ -360,17 +358,65 @@ int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, fl
                 a.repetition = r.repetition; a.frequency = r.frequency; a.presence = r.presence;
             }
             if (a.bias || a.allowed || given) tgbm::scores_adjust(a, st);
-            tgbm::TopArgs t;
-            t.n = rows; t.k = classes; t.top = top; t.in = a.in; t.temperature = temperature;
-            d_values.alloc((size_t)rows * top); d_ids.alloc((size_t)rows * top);
-            t.values = d_values.p; t.ids = d_ids.p;
-            if (lse) { d_lse.alloc(rows); t.lse = d_lse.p; }
-            tgbm::scores_top(t, st);
-            tgbm::download_d2h(values, d_values.p, d_values.bytes(), st, threads);
-            tgbm::download_d2h(ids, d_ids.p, d_ids.bytes(), st, threads);
-            if (lse) tgbm::download_d2h(lse, d_lse.p, d_lse.bytes(), st, threads);
+            act(a.in, rows, classes, st);   // (waits: the buffers above go)
         };
         tgbm::predict(ds, *plan_of(*model, n_trees, trees_per_iter), learning_rate, 0.f, tgbm::OBJ_UNKNOWN, {}, nullptr, nullptr, &step);
+    });
+}
+
+template <typename View>
+int predict_top(View &&view, ::Tree **model, int n_trees, int trees_per_iter, float learning_rate, const TgbmTopRules *rules, int top, float temperature,
+                float *values, int *ids, float *lse) {
+    auto check = [&](int n) {
+        TGBM_CHECK(trees_per_iter >= 2, "the largest scores of a row need a model of several classes (multi:softmax, multi:softprob)");
+        TGBM_CHECK(top >= 1 && top <= tgbm::SCORES_MAX_TOP, "length of a row's list outside [1, " + std::to_string(tgbm::SCORES_MAX_TOP) + "]");
+        TGBM_CHECK(tgbm::temperature_fits(temperature), "the temperature has to be a positive number");
+        TGBM_CHECK(n == 0 || (values && ids), "values or ids: null pointer");
+    };
+    return predict_ruled(view, model, n_trees, trees_per_iter, learning_rate, rules, check, [&](const tgbm::ScoreView &scores, int rows, int classes, cudaStream_t st) {
+        const int threads = tgbm::upload_threads();
+        tgbm::DevBuf<float> d_values, d_lse;
+        tgbm::DevBuf<int> d_ids;
+        tgbm::TopArgs t;
+        t.n = rows; t.k = classes; t.top = top; t.in = scores; t.temperature = temperature;
+        d_values.alloc((size_t)rows * top); d_ids.alloc((size_t)rows * top);
+        t.values = d_values.p; t.ids = d_ids.p;
+        if (lse) { d_lse.alloc(rows); t.lse = d_lse.p; }
+        tgbm::scores_top(t, st);
+        tgbm::download_d2h(values, d_values.p, d_values.bytes(), st, threads);
+        tgbm::download_d2h(ids, d_ids.p, d_ids.bytes(), st, threads);
+        if (lse) tgbm::download_d2h(lse, d_lse.p, d_lse.bytes(), st, threads);
+    });
+}
+
+template <typename View>
+int predict_sample(View &&view, ::Tree **model, int n_trees, int trees_per_iter, float learning_rate, const TgbmTopRules *rules, int draws, const double *uniform,
+                   float temperature, int top_k, float top_p, float min_p, int *ids, float *logs, float *all_logs) {
+    auto check = [&](int n) {
+        TGBM_CHECK(trees_per_iter >= 2, "drawn classes need a model of several classes (multi:softmax, multi:softprob)");
+        tgbm::check_draws(draws);
+        tgbm::check_limits(temperature, top_k, top_p, min_p);
+        TGBM_CHECK(n == 0 || (uniform && ids), "random numbers or classes: null pointer");
+    };
+    return predict_ruled(view, model, n_trees, trees_per_iter, learning_rate, rules, check, [&](const tgbm::ScoreView &scores, int rows, int classes, cudaStream_t st) {
+        const int threads = tgbm::upload_threads();
+        tgbm::DevBuf<double> d_uniform;
+        tgbm::DevBuf<float> d_logs, d_all;
+        tgbm::DevBuf<int> d_ids;
+        const size_t cells = (size_t)rows * draws;
+        d_uniform.alloc(cells); d_ids.alloc(cells);
+        tgbm::upload_h2d(d_uniform.p, uniform, d_uniform.bytes(), st, threads);
+        tgbm::SampleArgs s;
+        s.n = rows; s.k = classes; s.draws = draws; s.in = scores;
+        s.uniform = d_uniform.p; s.uniform_f64 = true;
+        s.temperature = temperature; s.top_k = top_k; s.top_p = top_p; s.min_p = min_p;
+        s.classes = d_ids.p;
+        if (logs) { d_logs.alloc(cells); s.logs = d_logs.p; }
+        if (all_logs) { d_all.alloc(cells); s.all_logs = d_all.p; }
+        tgbm::scores_sample(s, st);
+        tgbm::download_d2h(ids, d_ids.p, d_ids.bytes(), st, threads);
+        if (logs) tgbm::download_d2h(logs, d_logs.p, d_logs.bytes(), st, threads);
+        if (all_logs) tgbm::download_d2h(all_logs, d_all.p, d_all.bytes(), st, threads);
     });
 }
 
@@ -467,6 +513,18 @@ int tgbm_predict_top_dense(int row_size, int n_cols, void *x, int is_f64, Tree *
                            const TgbmTopRules *rules, int top, float temperature, float *values, int *ids, float *lse) {
     return predict_top([&](tgbm::DataSet &ds) { ds.view_dense(row_size, n_cols, x, is_f64 != 0); }, model, n_trees, trees_per_iter, learning_rate,
                        rules, top, temperature, values, ids, lse);
+}
+int tgbm_predict_sample(int row_size, float *val, int *row_ptr, int *col_ptr, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                        const TgbmTopRules *rules, int draws, const double *uniform, float temperature, int top_k, float top_p, float min_p, int *classes,
+                        float *logs, float *all_logs) {
+    return predict_sample([&](tgbm::DataSet &ds) { ds.view_sparse(row_size, val, row_ptr, col_ptr); }, model, n_trees, trees_per_iter, learning_rate,
+                          rules, draws, uniform, temperature, top_k, top_p, min_p, classes, logs, all_logs);
+}
+int tgbm_predict_sample_dense(int row_size, int n_cols, void *x, int is_f64, Tree **model, int n_trees, int trees_per_iter, float learning_rate,
+                              const TgbmTopRules *rules, int draws, const double *uniform, float temperature, int top_k, float top_p, float min_p,
+                              int *classes, float *logs, float *all_logs) {
+    return predict_sample([&](tgbm::DataSet &ds) { ds.view_dense(row_size, n_cols, x, is_f64 != 0); }, model, n_trees, trees_per_iter, learning_rate,
+                          rules, draws, uniform, temperature, top_k, top_p, min_p, classes, logs, all_logs);
 }
 
 void save(char *model_path, char *objective, float learning_rate, int num_class, int n_trees, int trees_per_iter,
@@ -644,6 +702,19 @@ int tgbm_booster_teacher_loss(TgbmBooster *b, double *out) {
     return guard([&] {
         TGBM_CHECK(b && out, "null pointer");
         *out = b->b->teacher_loss();
+    });
+}
+int tgbm_booster_set_feedback(TgbmBooster *b, int draws, const int *classes, const float *gains, const float *old, const float *weights, float temperature,
+                              float clip_low, float clip_high, float entropy) {
+    return guard([&] {
+        TGBM_CHECK(b != nullptr, "null booster");
+        b->b->set_feedback(draws, classes, gains, old, weights, temperature, clip_low, clip_high, entropy);
+    });
+}
+int tgbm_booster_feedback_loss(TgbmBooster *b, double *out) {
+    return guard([&] {
+        TGBM_CHECK(b && out, "null pointer");
+        *out = b->b->feedback_loss();
     });
 }
 int tgbm_booster_boost(TgbmBooster *b, int n_rounds) { return guard([&] { b->b->boost(n_rounds); }); }

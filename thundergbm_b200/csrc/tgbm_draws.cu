@@ -254,7 +254,6 @@ struct Exponent {
         return __hiloint2double(__double2hiint(v) + ((n >> 5) << 20), __double2loint(v));
     }
 };
-__device__ __forceinline__ double not_a_number() { return __longlong_as_double(0x7ff8000000000000ll); }
 
 // ---- up to 1024 classes: a lane has a row, the W warps of a block (W = 1: each for itself) share its classes, E neighbours each ------
 // What a warp's lanes know of their rows is put together through shared memory; all warps come to the same numbers in the same order,
@@ -2040,10 +2039,7 @@ int tgbm_scores_sample(int n_rows, int n_classes, int type, const void *d_scores
         check_shape(n_rows, n_classes);
         check_draws(draws);
         TGBM_CHECK(uniform_type == TGBM_F32 || uniform_type == TGBM_F64, "random numbers: floats or doubles");
-        TGBM_CHECK(d_temperature || (temperature >= 0.f && temperature <= FLT_MAX), "the temperature has to be a number from 0 on");
-        TGBM_CHECK(d_top_k || top_k >= 0, "top_k: negative");
-        TGBM_CHECK(d_top_p || (top_p >= 0.f && top_p <= 1.f), "top_p outside [0, 1]");
-        TGBM_CHECK(d_min_p || (min_p >= 0.f && min_p <= 1.f), "min_p outside [0, 1]");
+        check_limits(d_temperature ? 1.f : temperature, d_top_k ? 0 : top_k, d_top_p ? 1.f : top_p, d_min_p ? 0.f : min_p);   // (numbers of rows stand in for those)
         if (n_rows == 0) return;
         SampleArgs a;
         a.n = n_rows; a.k = n_classes; a.draws = draws;

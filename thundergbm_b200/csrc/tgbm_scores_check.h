@@ -1,5 +1,6 @@
 // What the C entries of the operators on scores check before anything is queued.
 #pragma once
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -69,6 +70,12 @@ inline void check_list(int top) { TGBM_CHECK(top >= 1 && top <= TGBM_SCORES_MAX_
 
 inline void check_draws(int draws) {
     TGBM_CHECK(draws >= 1 && draws <= TGBM_SCORES_MAX_DRAWS, "draws of a row outside [1, " + std::to_string(TGBM_SCORES_MAX_DRAWS) + "]");
+}
+inline void check_limits(float temperature, int top_k, float top_p, float min_p) {
+    TGBM_CHECK(temperature >= 0.f && temperature <= FLT_MAX, "the temperature has to be a number from 0 on");
+    TGBM_CHECK(top_k >= 0, "top_k: negative");
+    TGBM_CHECK(top_p >= 0.f && top_p <= 1.f, "top_p outside [0, 1]");
+    TGBM_CHECK(min_p >= 0.f && min_p <= 1.f, "min_p outside [0, 1]");
 }
 inline void check_feedback(float clip_low, float clip_high, float kl, float entropy) {
     TGBM_CHECK(clip_low >= 0.f && clip_low <= 1.f && clip_high >= 0.f, "clip: the lower one outside [0, 1], or the upper one negative");

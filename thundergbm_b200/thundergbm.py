@@ -10,8 +10,8 @@ started from (src/thundergbm/scikit_tgbm.cpp:87-90).  A NumPy matrix goes to den
 as it is, and its CSR is made on the GPU: on the host the conversion took most of a call (260 ms of fit() and again of
 predict() for 400009 x 28 values, against 20 ms of training on the GPU).
 
-Beyond the reference: fit(teacher=) grows trees towards another model's largest scores (through Booster, from a CSR), and predict_top()
-gives the best classes of every row under rules.
+Beyond the reference: fit(teacher=) grows trees towards another model's largest scores and fit(feedback=) from drawn classes and the gains that
+followed (through Booster, from a CSR); predict_top() gives the best classes of every row under rules, predict_sample() draws classes.
 """
 from __future__ import annotations
 
@@ -100,12 +100,19 @@ class TGBMModel:
         return (C.c_float * max(len(self._group_label), self.num_class))(*self._group_label)
 
     # -- API ---------------------------------------------------------------------------------------
-    def fit(self, X, y, groups=None, teacher=None):
+    def fit(self, X, y, groups=None, teacher=None, feedback=None):
         """`teacher` (multi:softmax and multi:softprob, one GPU): the arguments of Booster.set_teacher as a dict -- ids, logits and, if
         wanted, lse, temperature, alpha; what predict_top() of another model returns is such a teacher's ids, logits and lse.
-        `groups` are those of ranking objectives; the others, and so training from a teacher, do not look at them."""
+        `feedback` (likewise): the arguments of Booster.set_feedback as a dict -- classes and gains and, if wanted, old, weights, temperature,
+        clip, entropy; what predict_sample() returns are such classes and their old.  `y` then only says which classes there are, and what
+        the metric of a round is measured by.
+        `groups` are those of ranking objectives; the others, and so training from a teacher or from feedback, do not look at them."""
+        if teacher is not None and feedback is not None:
+            raise ValueError('either a teacher or feedback')
         if teacher is not None:
-            return self._fit_teacher(X, y, teacher)
+            return self._fit_from(X, y, 'a teacher', lambda n, b=None: self._take_teacher(teacher, n, b))
+        if feedback is not None:
+            return self._fit_from(X, y, 'feedback', lambda n, b=None: self._take_feedback(feedback, n, b))
         self._free()
         dense = self._dense(X)
         if dense is not None:
@@ -144,21 +151,34 @@ class TGBMModel:
             self._group_label, self._n_labels = None, self._counted(n_labels)
         return self
 
-    def _fit_teacher(self, X, y, teacher):
+    @staticmethod
+    def _take_teacher(teacher, n, booster):
+        if np.shape(teacher['ids'])[0] != n:
+            raise ValueError('X and the teacher have different numbers of rows')
+        if booster:
+            booster.set_teacher(**teacher)
+
+    @staticmethod
+    def _take_feedback(feedback, n, booster):
+        if np.shape(feedback['classes'])[:1] != (n,):
+            raise ValueError('X and the drawn classes have different numbers of rows')
+        if booster:
+            booster.set_feedback(**feedback)
+
+    def _fit_from(self, X, y, what, take):
         from .booster import Booster
         from .synth import CsrData
         if self.objective not in ('multi:softmax', 'multi:softprob'):
-            raise ValueError('a teacher needs objective multi:softmax or multi:softprob')
+            raise ValueError(f'{what} needs objective multi:softmax or multi:softprob')
         if self.n_gpus != 1:
-            raise ValueError('training from a teacher runs on one GPU')
+            raise ValueError(f'training from {what} runs on one GPU')
         if self.tree_method not in ('auto', 'hist', 'exact'):
             raise ValueError('unknown tree_method ' + self.tree_method)
         val, indptr, indices, n = self._csr(X)
         y = np.ascontiguousarray(y, np.float32)
         if y.shape[0] != n:
             raise ValueError('X and y have different numbers of rows')
-        if np.shape(teacher['ids'])[0] != n:
-            raise ValueError('X and the teacher have different numbers of rows')
+        take(n)
         width = int(indices.max(initial=-1)) + 1
         exact = self.tree_method == 'exact' or (self.tree_method == 'auto' and width > 20000)   # src/thundergbm/trainer.cu:19-23
         b = Booster(CsrData(n, width, indptr, indices, val, y), depth=self.depth, n_trees=self.n_trees,
@@ -166,7 +186,7 @@ class TGBMModel:
                     verbose=self.verbose, column_sampling_rate=self.column_sampling_rate, bagging=int(self.bagging),
                     learning_rate=self.learning_rate, objective=self.objective, num_class=self.num_class, exact_builder=int(exact))
         try:
-            b.set_teacher(**teacher)
+            take(n, b)
             b.boost(self.n_trees)
             b.sync()
             model = C.c_void_p(None)
@@ -179,25 +199,19 @@ class TGBMModel:
         self.group_label = [float(v) for v in labels]
         return self
 
-    def predict_top(self, X, k=1, bias=None, allowed=None, allowed_row=None, history=None, repetition=1.0, frequency=0.0, presence=0.0,
-                    temperature=1.0):
-        """(classes, scores, lse) of the k best classes of every row, for models of several classes: classes are positions in `group_label`
-        (int32, rows x k; -1 where a row has no more), scores the model's raw ones under the rules given, best first, and
-        scores / temperature - lse the logs of their probabilities.
-
-        bias: one per class (log of the ratio of class priors, say).  allowed: truth values, rows x classes or masks x classes with
-        `allowed_row` naming every row's mask (-1: all classes).  history: per row a list of classes it was given before; one that
-        stands there c > 0 times has its score divided (above 0) or multiplied by `repetition`, less c * frequency + presence."""
+    def _ruled(self, X, bias, allowed, allowed_row, history, repetition, frequency, presence):
+        """(number of rows, the ending of the functions that take them, the rows as these do, TgbmTopRules, what all this points to)"""
         if self.model is None:
             raise ValueError('Please train the model first or load model from file!')
         dense = self._dense(X)
         if dense is not None:
-            n = X.shape[0]
+            n, keep = X.shape[0], [dense[0]]
+            data = (n, X.shape[1], _vp(dense[0]), dense[1])
         else:
-            val, indptr, indices, n = self._csr(X)
+            *keep, n = self._csr(X)
+            data = (n, *map(_vp, keep))
         classes = self.tree_per_iter
         rules = _lib.TgbmTopRules(repetition=repetition, frequency=frequency, presence=presence)
-        keep = []
 
         def field(name, a, dtype, shape, what):
             a = np.ascontiguousarray(a, dtype)
@@ -229,15 +243,43 @@ class TGBMModel:
             ids = class_numbers(np.concatenate([np.asarray(h).reshape(-1) for h in history if len(h)] or [np.zeros(0, np.int32)]))
             field('history_ptr', ptr, np.int64, (n + 1,), '')
             field('history', ids, np.int32, (int(ptr[-1]),), '')
+        return n, '' if dense is None else '_dense', data, rules, keep
+
+    def predict_top(self, X, k=1, bias=None, allowed=None, allowed_row=None, history=None, repetition=1.0, frequency=0.0, presence=0.0,
+                    temperature=1.0):
+        """(classes, scores, lse) of the k best classes of every row, for models of several classes: classes are positions in `group_label`
+        (int32, rows x k; -1 where a row has no more), scores the model's raw ones under the rules given, best first, and
+        scores / temperature - lse the logs of their probabilities.
+
+        bias: one per class (log of the ratio of class priors, say).  allowed: truth values, rows x classes or masks x classes with
+        `allowed_row` naming every row's mask (-1: all classes).  history: per row a list of classes it was given before; one that
+        stands there c > 0 times has its score divided (above 0) or multiplied by `repetition`, less c * frequency + presence."""
+        n, form, data, rules, _keep = self._ruled(X, bias, allowed, allowed_row, history, repetition, frequency, presence)
         if not 1 <= k <= 128:
             raise ValueError('k: 1 to 128')
         values, ids, lse = np.empty((n, k), np.float32), np.empty((n, k), np.int32), np.empty(n, np.float32)
         rest = (C.byref(self.model), self.n_trees, self.tree_per_iter, self.learning_rate, C.byref(rules), k, temperature, _vp(values), _vp(ids), _vp(lse))
-        if dense is not None:
-            _lib.check(self._lib.tgbm_predict_top_dense(n, X.shape[1], _vp(dense[0]), dense[1], *rest))
-        else:
-            _lib.check(self._lib.tgbm_predict_top(n, _vp(val), _vp(indptr), _vp(indices), *rest))
+        _lib.check(getattr(self._lib, 'tgbm_predict_top' + form)(*data, *rest))
         return ids, values, lse
+
+    def predict_sample(self, X, uniform, bias=None, allowed=None, allowed_row=None, history=None, repetition=1.0, frequency=0.0, presence=0.0,
+                       temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """(classes, logs, all_logs): classes drawn for every row from the random numbers `uniform` (in [0, 1); one per row, or rows x up to 128),
+        for models of several classes, with the logs of their probabilities among the classes that were left and among all: classes are positions in
+        `group_label` (int32; -1 where the rules leave none).  Rules as for predict_top; of what they leave, classes at least min_p times as
+        likely as the likeliest, of these the top_k likeliest (0: all), of these, likeliest first, as many as it takes for top_p of their
+        probability.  temperature 0: the likeliest."""
+        n, form, data, rules, _keep = self._ruled(X, bias, allowed, allowed_row, history, repetition, frequency, presence)
+        uniform = np.ascontiguousarray(uniform, np.float64)
+        if uniform.ndim not in (1, 2) or uniform.shape[0] != n or (uniform.ndim == 2 and not 1 <= uniform.shape[1] <= 128):
+            raise ValueError('uniform: one per row, or rows x up to 128')
+        classes = np.empty(uniform.shape, np.int32)
+        logs, all_logs = np.empty(uniform.shape, np.float32), np.empty(uniform.shape, np.float32)
+        rest = (C.byref(self.model), self.n_trees, self.tree_per_iter, self.learning_rate, C.byref(rules), uniform.shape[1] if uniform.ndim == 2 else 1,
+                _vp(uniform), temperature, top_k, top_p, min_p, _vp(classes), _vp(logs), _vp(all_logs))
+        _lib.check(getattr(self._lib, 'tgbm_predict_sample' + form)(*data, *rest))
+        return classes, logs, all_logs
+
 
     def predict(self, X, groups=None):
         if self.model is None:
