@@ -933,18 +933,6 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_weights_join(NormBackwardA
 }
 }  // namespace
 
-// f(E, W) for kernels by class: E classes of each of W warps
-template <typename F> void by_class_sizes(int k, F &&f) {
-    using std::integral_constant;
-    if (k <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    else if (k <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    else if (k <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    else if (k <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
-    else if (k <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
-    else if (k <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
-    else if (k <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
-    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
-}
 // f(L, E) for kernels by row: E classes of each of L lanes
 template <typename F> void by_row_sizes(int k, F &&f) {
     using std::integral_constant;

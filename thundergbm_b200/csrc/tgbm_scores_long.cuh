@@ -1,4 +1,5 @@
-// Long rows of scores, which a block or a cluster of blocks holds in its registers: what the kernels for them share.
+// What the kernels that draw, learn from draws and standardise share: sums over lanes, long rows that a block or a cluster of blocks holds in its
+// registers, sizes.
 #pragma once
 #include "tgbm_scores.cuh"
 
@@ -131,6 +132,19 @@ template <typename T, int TH, int P, bool EVEN> struct Hold {
         else p[first(u)] = one[u];
     }
 };
+// f(E, W) for kernels with a lane per row, up to 1024 classes: E classes of each of W warps
+template <typename F> inline void by_class_sizes(int k, F &&f) {
+    using std::integral_constant;
+    if (k <= 8) f(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    else if (k <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    else if (k <= 32) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    else if (k <= 64) f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+    else if (k <= 128) f(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    else if (k <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    else if (k <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 16>{});
+    else f(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+}
+
 inline bool on_16(const void *p, long long row, int size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row * size % 16 == 0; }
 
 template <typename... P, typename... A>
