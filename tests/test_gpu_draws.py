@@ -105,7 +105,7 @@ def test_sample_of_unusual_numbers(ops, kind, layout, n, k):
     z[9] = np.where(np.arange(k) == k - 1, -high, low)
     t = _tensor(torch, z, kind, layout)
     u = r.random((n, 3))
-    for limits in ({}, dict(top_k=2), dict(top_p=0.7), dict(min_p=0.5), dict(temperature=0), dict(temperature=1e-30), dict(temperature=1e30), dict(temperature=1e-45, top_p=0.5),
+    for limits in ({}, dict(top_k=2), dict(top_p=0.7), dict(min_p=0.5), dict(temperature=0), dict(temperature=1e-30), dict(temperature=1e30), dict(temperature=1e-45, top_p=0.5), dict(temperature=1e-45, top_k=3), dict(temperature=2e-40, min_p=0.5),
                    dict(temperature=np.array([np.nan, -1, np.inf, 0, 1e-45, 1, 1, 1, 1, 1, 0, -0.0], np.float32)),
                    dict(top_p=np.array([np.nan, -1, 2, 0] * 3, np.float32), min_p=np.array([-1, 5, np.nan] * 4, np.float32),
                         top_k=np.array([-1, 1 << 30, 1, 0] * 3, np.int32))):

@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
     if (__any_sync(0xffffffffu, live && !by_count && !by_share)) {
         each_score([&](float x, int) { all += live ? weight_of(x) : 0.0; });
     } else {
-        const float c = (float)(l.inv_t * 1.4426950408889634), base = live ? top : 0.f;
+        const float c = fminf((float)(l.inv_t * 1.4426950408889634), FLT_MAX), base = live ? top : 0.f;
         float part[4] = {0.f, 0.f, 0.f, 0.f};
         int i = 0;
         each_score([&](float x, int) {

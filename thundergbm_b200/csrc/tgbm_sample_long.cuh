@@ -219,10 +219,15 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
     float top = minus_inf(), low = -minus_inf(), none = 0;
     double sum = 0;
     int count = 0;
-    each([&](float x, int) {
-        top = fmaxf(top, x);
-        count |= x != x;
-    });
+    if constexpr (EVEN) {
+        top = hold.largest(cells);
+        if (top != top) { count = 1; top = minus_inf(); }
+    } else {
+        each([&](float x, int) {
+            top = fmaxf(top, x);
+            count |= x != x;
+        });
+    }
     // Each group of lanes that holds a score has a largest one, and the least of these is reached by as many scores as there are groups: the first
     // guess of a border.  Groups are as large as they may be to be top_k.
     const int top_k = l.greedy ? 1 : l.top_k, groups = max(1, a.k / H::E);   // (threads that hold all their scores)
@@ -275,27 +280,51 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
     double mass = 0;
     bool listed = false;
     if (by_count || by_mass || by_share) {
-        const float c = (float)(l.inv_t * 1.4426950408889634);
+        const float c = fminf((float)(l.inv_t * 1.4426950408889634), FLT_MAX);
         auto rough = [&](float x) { return exp2_fast(__fsub_rn(x, top) * c); };
         float f0 = 0, f1 = 0;
-        const bool exact = !by_count && !by_share;   // top_p alone: a share of the whole mass
+        int count_of_row = 0;   // (not looked at)
+        // sum of floats over this thread's scores; marks those from `border` on
+        unsigned reach = 0;
+        auto look = [&](float border) {
+            float2 part = make_float2(0.f, 0.f);
+            reach = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                if (H::first(u) >= cells) continue;
+                float v[V];
+                hold.get(u, v);
+                if constexpr (V == 1) {
+                    part.x += rough(v[0]);
+                    reach |= v[0] >= border ? 1u << u : 0u;
+                } else {
+                    const float2 mt = make_float2(-top, -top), c2 = make_float2(c, c);
+#pragma unroll
+                    for (int i = 0; i < V; i += 2) {
+                        part = add2(part, exp_pair(make_float2(v[i], v[i + 1]), mt, c2));
+                        reach |= (v[i] >= border ? 1u << (u * V + i) : 0u) | (v[i + 1] >= border ? 2u << (u * V + i) : 0u);
+                    }
+                }
+            }
+            return (double)__fadd_rn(part.x, part.y);
+        };
+        const bool exact = !by_count && !by_share;   // top_p alone: a share of the whole mass (by floats at first)
         if (exact) {
-            each([&](float x, int) { all += weight_of(x); });
+            all = look(-minus_inf());
             count = 0;
             total(all, f0, f1, count);
         }
-        // the border, rounded down as in k_sample_limited; what lies 750 T below the largest score has no mass in any case
+        // the border, rounded down as in k_sample_limited, and by what the sum of floats is off, less than 2^-18; what lies 750 T below the largest score has no mass in any case
         const float t = (float)(1.0 / l.inv_t);
         float down = -750.f * t;
         if (by_share) down = logf((float)l.min_p) * t;
         else if (exact) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
-        low = __fadd_rn(top, down) - (fabsf(down) + t + fabsf(top)) * 2e-6f;
+        low = __fadd_rn(top, down) - (fabsf(down) + 5.f * t + fabsf(top)) * 2e-6f;
         if (l.greedy) low = top;
         if (!(low <= top)) low = minus_inf();
         low = fmaxf(low, -FLT_MAX);
         const float base = low;
         if (by_count && guess <= top) low = fmaxf(low, guess);
-        unsigned reach = 0;   // bits of this thread's scores from the border on
         auto mark = [&](float border) {
             reach = 0;
             int bit = 0;
@@ -304,19 +333,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 ++bit;
             });
         };
-        mark(low);
-        count = __popc(reach);
         if (!exact) {
-            float part = 0;
-#pragma unroll
-            for (int u = 0; u < P; ++u) {
-                float s = 0;
-                each_of(u, [&](float x, int) { s += rough(x); });
-                part += s;
-            }
-            all = (double)part;
+            all = look(low);
+            count = __popc(reach);
             total(all, f0, f1, count);
         } else {
+            mark(low);
+            count = __popc(reach);
             total(sum, f0, f1, count);
         }
         if (l.greedy) all = 1.0;
@@ -328,11 +351,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         }
         float high = top;
         const bool narrowing = by_count ? top_k <= LONG_LIST : by_mass && !by_share;
-        // top_p alone: masses by floats, off by less than 2^-18, tell what certainly reaches the target and what certainly does not
-        const double enough = l.top_p * all * (1 + 1e-5), short_of = l.top_p * all * (1 - 1e-5);
+        // top_p alone: masses by floats, each off by less than 2^-18, tell what certainly reaches the target and what certainly does not
+        const double enough = l.top_p * all * (1 + 2e-5), short_of = l.top_p * all * (1 - 2e-5);
         int above = 0;   // scores larger than `high`, which are left in any case
         bool first = !by_count && guess > low && guess < top, moved = false;
-        while (narrowing && count - above > LONG_LIST && low < high) {
+        // An entry of the list is compared with all others: one block alone narrows on for less than that (1 x 1000: 17 us, 32 with 600 entries), a
+        // cluster, whose blocks wait for one another every time, not as far.
+        const int want = max(C == 1 ? 160 : 512, by_count ? top_k : 0);
+        while (narrowing && count - above > want && low < high) {
             const float mid = first ? guess : middle(low, high);
             first = false;
             float up = -minus_inf(), below = minus_inf();
@@ -366,10 +392,16 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         if (whole) above = 0;
         if (whole || part) {
             double base = 0;
-            if (part) {
-                each([&](float x, int) { base += x > high ? weight_of(x) : 0.0; });
-            } else {
-                high = top;
+            if (!part) high = top;
+            if (exact) {   // now by doubles: the whole mass, and that of what is larger
+                all = 0;
+                each([&](float x, int) {
+                    const double w = weight_of(x);
+                    all += w;
+                    if (x > high) base += w;
+                });
+                count_of_row = 0;
+                total(all, f0, f1, count_of_row);
             }
             auto inside = [&](float x) { return x >= low && x <= high; };
             if (moved || part) {
@@ -508,6 +540,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 measured(true)([&](float, double m) { sum += m; });
                 count = 0;
                 total(sum, f0, f1, count);
+                if (exact) all = sum;
                 settle(true, l.top_p * sum);
             }
             mass = segments();

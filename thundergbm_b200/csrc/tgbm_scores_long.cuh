@@ -69,6 +69,32 @@ template <typename T, int TH, int P, bool EVEN> struct Hold {
         if constexpr (EVEN) w[u].unpack(v);
         else v[0] = score_f32(one[u]);
     }
+    // largest of a thread's scores, NaN where one is
+    __device__ __forceinline__ float largest(int cells) const {
+        float high = minus_inf();
+        auto larger = [](float a, float b) {
+            float r;
+            asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+            return r;
+        };
+#pragma unroll
+        for (int u = 0; u < P; ++u)
+            if (cells == CELLS || first(u) < cells) {
+                if constexpr (EVEN && sizeof(T) == 2) {
+                    typedef typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type T2;
+                    const unsigned words[4] = {w[u].bits.x, w[u].bits.y, w[u].bits.z, w[u].bits.w};
+                    const T2 v = __hmax2_nan(__hmax2_nan(*reinterpret_cast<const T2 *>(&words[0]), *reinterpret_cast<const T2 *>(&words[1])),
+                                             __hmax2_nan(*reinterpret_cast<const T2 *>(&words[2]), *reinterpret_cast<const T2 *>(&words[3])));
+                    high = larger(high, larger(score_f32(v.x), score_f32(v.y)));
+                } else {
+                    float v[V];
+                    get(u, v);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) high = larger(high, v[i]);
+                }
+            }
+        return high;
+    }
     // least and largest of a thread's scores; NaN does not count
     __device__ __forceinline__ void range(int cells, float &low, float &high) const {
         low = -minus_inf(); high = minus_inf();
