@@ -149,6 +149,8 @@ template <int E, typename T, typename F> __device__ __forceinline__ void write_c
     }
 }
 
+// 50003 x 250: 26.7 us (floor 15.3), 22 instructions per score where a tenth is masked; addresses by 64-bit steps and a test of every class's number took 55, and
+// 43 us.
 template <typename T, int E, int W, bool WEIGHTS>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_norm_class(NormArgs a, Scores<T> in, Scores<T> out) {
     __shared__ Shared<W> sh;
@@ -263,6 +265,7 @@ template <int TH, int M> __device__ __forceinline__ void long_sums(LongSums<TH, 
 
 // R rows at a time: gains and biases are read once for all of them (for one row of 16-bit scores they are four times its bytes, from the L2 cache),
 // and barriers and exchanges are shared.  A row whose sum is finite holds no -inf, so only the others look at every score whether it is there.
+// 2048 x 65536 in 16 bits with gain and bias: 149 us (floor 82), bound by waiting for loads and for the cluster; one row at a time 168.
 template <int TH, int R> struct LongShared {
     LongSums<TH, R> sum, square;
     float part[TH / 32], moments[R][3], of_row[R][2];
@@ -471,7 +474,7 @@ template <int W> __device__ __forceinline__ float4 over_warps(BackShared<W> &sh,
     return v;
 }
 
-// By class, up to 1024 classes: a lane has a row, W warps share its classes.  What 32 rows give to a class is added across the lanes, which hold 32 sums
+// By class, up to 1024 classes: a lane has a row, W warps share its classes.  50003 x 250: 49 us (floor 23), 68 instructions per score.  What 32 rows give to a class is added across the lanes, which hold 32 sums
 // then (16 of x g and of g each, or one kind after the other).
 template <typename T, int E, int W, bool WEIGHTS>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? (E == 32 ? 2 : 4) : W == 16 ? (E == 16 ? 2 : 1) : 1)
@@ -629,7 +632,8 @@ __global__ void __launch_bounds__(ROW_THREADS) k_norm_backward_row(NormBackwardA
 
 // Long rows: a cluster of up to 8 blocks (or one) takes row after row, each block the same part of every row; the next row is on its way while this one is
 // worked on.  Two scores of a thread go through each instruction.  A score of -inf makes the row's second sum infinite or NaN; only then is
-// every score looked at whether it is there (and in the next row from the start).
+// every score looked at whether it is there (and in the next row from the start).  4096 x 8191 in 16 bits: 88 us (floor 31), 29 instructions per
+// score by 8 warps of 254 registers; 16 scores a thread of 512 took 100, the next row of single scores in registers 176.
 // Rows that begin anywhere come through shared memory, by asynchronous copies of 16 bytes and a few single scores, two rows ahead; the others
 // through registers, one row ahead.
 // What a thread has of scores and gradients: as it was read, or (single scores in 16 bits) both of a class in one register.

@@ -20,6 +20,10 @@ namespace cg = cooperative_groups;
 // which is its place in descending order; prefix sums in that order tell where top_p ends, prefix sums in class order which class a random number
 // falls on.  Where top_p alone leaves more, what is certainly left is told from what the end of it lies among, and only that goes into the list.
 // Rows with more than a list, and rows without limits, take their draws from sums per segment.
+//
+// Bound by instructions and by waiting for the cluster: 256 x 131072 in 16 bits under limits of all kinds 180 us (floor 10.2), 16 draws for each of
+// 333 x 50021 without limits, every exponential a double, 139 us (5.1).  64 registers, so that two blocks share an SM: with 128 and one block
+// 425 us and 233.
 constexpr int LONG_LIST = 1024;
 
 template <int W, int S> struct LongRow {
