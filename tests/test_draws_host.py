@@ -66,3 +66,12 @@ def test_work_of_the_weights_gradient(lib):
         for k in (1, 7, 250, 8191, 65536, 1 << 20):
             assert 8 * k <= lib.tgbm_scores_norm_work(n, k) <= 160 << 20
     assert lib.tgbm_scores_norm_work(0, 5) == lib.tgbm_scores_norm_work(5, 0) == 0
+
+
+@pytest.mark.parametrize('call,args', [(_sample, {}), (_feedback, dict(gives=0)), (_norm, dict(out=1 << 40, ors=131072))])
+@pytest.mark.parametrize('n', [1 << 28, (1 << 31) - 1])
+def test_more_blocks_than_a_launch_has_are_refused(lib, call, args, n):
+    """Rows that are all the same one (stride 0) take no memory, so there may be any number of them: 8 blocks for each would be more than a launch has,
+    and their number modulo 2^32 would leave rows out."""
+    assert call(lib, n=n, k=131072, rs=0, **args) == 1
+    assert 'rows' in lib.tgbm_last_error().decode()

@@ -175,6 +175,7 @@ inline bool on_16(const void *p, long long row, int size) { return reinterpret_c
 
 template <typename... P, typename... A>
 void launch_long(void (*kernel)(P...), long long rows, int cluster, int threads, cudaStream_t stream, size_t smem, A &&...args) {
+    TGBM_CHECK(rows * cluster < 1ll << 31, "too many rows of this length for one call");   // (rows that are all the same one take no memory)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster)); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = stream;
     cudaLaunchAttribute attr;
