@@ -218,7 +218,7 @@ def run(state):
             return (grad, gain, bias) if case['weights'] else (grad,)
         loss, logs, grad = scores.feedback(state['scores'], state['classes'], state['gains'], old=state['old'],
                                            reference=state['reference'], weights=state['weights'], temperature=case['temperature'],
-                                           clip=case['clip'] or None, kl=case['kl'], entropy=case['entropy'], gives=case['gives'])
+                                           clip=case['clip'] or None, kl=case['kl'] if case['reference'] else 0.0, entropy=case['entropy'], gives=case['gives'])
         return (loss, logs) if grad is None else (loss, logs, grad)
     return {'sample': _plain_sample, 'norm': _plain_norm, 'norm_backward': _plain_norm_backward,
             'feedback': _plain_feedback}[case['do']](state, case)
