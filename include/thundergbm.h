@@ -222,7 +222,8 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * Scores are a matrix of n_rows x n_classes in `type`, class k of row n at d_scores[n * row_stride + k * class_stride] (strides in
  * elements, none negative).  Row stride 1: by class, as tgbm_booster_get_ypred and tgbm_predict_raw lay them out; class stride 1:
  * by row, as networks do.  Where neither is 1 the operators work as well, more slowly, and so do top and distill by class above some 5000
- * classes (scores of 2000 x 10000 13 and 4 times as long as of 4000 x 5000). */
+ * classes (scores of 2000 x 10000 13 and 4 times as long as of 4000 x 5000), and sample, feedback, norm and norm_backward by class above 1024
+ * (4000 x 5000: up to 8 times as long as by row). */
 #define TGBM_F32 0
 #define TGBM_F16 1
 #define TGBM_BF16 2

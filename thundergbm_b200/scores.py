@@ -10,7 +10,8 @@ Scores are a tensor of rows x classes (float32, float16 or bfloat16, any strides
     feedback loss on drawn classes and the gains that followed, with its gradient
     norm     every row at mean 0 and variance 1, a gain and a bias per class; norm_backward: its gradient
 
-(top and distill take several times as long by class above some 5000 classes, or where neither rows nor classes lie side by side.)
+(top and distill take several times as long by class above some 5000 classes, the last four above 1024, all where neither rows nor classes lie
+side by side.)
 
 Results come on the stream that is torch's current one on the scores' device, in the layout of the scores; nothing waits.
 Autograd does not record them: results require no gradient, also where the scores do (distill, feedback and norm_backward return theirs).
