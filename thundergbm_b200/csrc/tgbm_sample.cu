@@ -385,6 +385,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
         for (int k = k0; k < k1; ++k, from += in.cls) tile[32 * k + lane] = score_f32(*from);
     }
     if (warp == 0) sh.powers.fill();
+    if (W == 1) __syncwarp();   // (W > 1: the first exchange is a barrier)
     float *const mine_x = tile + lane;
     auto each_score = [&](auto &&f) {
 #pragma unroll 8
