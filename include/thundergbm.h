@@ -279,7 +279,7 @@ int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_score
                         int gives, void *d_grad, long long grad_row_stride, long long grad_class_stride, void *cuda_stream);
 
 /* Classes drawn from the scores s of every row, one for each of `draws` given random numbers u (1 to TGBM_SCORES_MAX_DRAWS per row; d_uniform is
- * n_rows x draws of uniform_type TGBM_F32 or TGBM_F64, in [0, 1): numbers outside are taken as the nearest inside, NaN as 0).
+ * n_rows x draws of uniform_type TGBM_F32 or TGBM_F64, in [0, 1): numbers outside are taken as the nearest double inside, NaN as 0).
  *   w_k = exp((s_k - max s) / temperature) for every class whose score is above -infinity
  *   A: classes with w_k >= min_p that are among the top_k largest scores (of equal ones the lower class first; 0: all)
  *   B: the shortest beginning of A, largest first, whose mass is at least top_p of A's (never empty; top_p 1: all of A)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from test_gpu_draws import _check_sample, _dev, _masked
-from test_gpu_scores import _make, _tensor, ops  # noqa: F401
+from test_gpu_scores import _close, _make, _tensor, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -22,3 +22,28 @@ def test_limits_of_rows_that_a_warp_has(ops, layout, k):
         first = scores.sample(t, _dev(torch, u), **limits)
         for _ in range(20):
             assert all(torch.equal(a, b) for a, b in zip(first, scores.sample(t, _dev(torch, u), **limits)))
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('layout,n,k', [('class', 40, 5), ('class', 40, 200), ('class', 40, 600), ('class', 3, 1500), ('row', 1100, 300), ('row', 6, 300), ('row', 3, 3000),
+                                        ('row', 3, 20000), ('row+', 3, 20001), ('row', 3, 131072), ('any', 3, 300)])
+def test_numbers_that_are_not_below_one(ops, layout, n, k, kind):
+    """They are taken as the largest number below 1.  The likely classes have 1 each and the others e^-60, so that all sums of doubles are whole numbers
+    and nothing behind the last likely class counts."""
+    torch, scores = ops
+    likely = min(96, k // 2)
+    z = np.full((n, k), -60.0)
+    z[:, :likely] = 0
+    z[1, :] = -60
+    z[1, k - likely:] = 0
+    t = _tensor(torch, z, kind, layout)
+    u = np.tile([1.0, 1 - 2.0 ** -53, 7.0, np.inf], (n, 1))
+    for limits in ({}, dict(top_k=k - 1), dict(top_p=0.9999999), dict(min_p=1e-30), dict(top_k=likely), dict(top_k=np.resize([0, likely], n).astype(np.int32))):
+        given = {name: _dev(torch, v) if isinstance(v, np.ndarray) else v for name, v in limits.items()}
+        for at in (u, u[:, :1], u.astype(np.float32)):
+            ids, logs, every = scores.sample(t, _dev(torch, at), **given)
+            want = np.full(at.shape, likely - 1)
+            want[1] = k - 1
+            assert np.array_equal(ids.cpu().numpy(), want), limits
+            for got in (logs, every):
+                _close(got.cpu().numpy(), np.full(at.shape, -np.log(likely)), 2.0 ** -22, limits)

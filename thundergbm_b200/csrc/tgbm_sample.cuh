@@ -31,7 +31,8 @@ __device__ __forceinline__ Limits limits_of(const SampleArgs &a, long long n) {
 }
 __device__ __forceinline__ double uniform_of(const SampleArgs &a, long long i) {
     const double u = a.uniform_f64 ? static_cast<const double *>(a.uniform)[i] : (double)static_cast<const float *>(a.uniform)[i];
-    return u > 0 ? u : 0.0;   // (NaN: 0; what is not below 1 falls on the last class)
+    // (NaN: 0.)  Below 1: a share of a mass that is then below it, so that one of those who share the mass has the draw.
+    return u > 0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
 }
 __device__ __forceinline__ void put_draw(const SampleArgs &a, long long i, int cls, float log, float all_log) {
     a.classes[i] = cls;
