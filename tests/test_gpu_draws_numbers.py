@@ -3,10 +3,25 @@ tests/draws_ref.py, or stand beside the test."""
 import numpy as np
 import pytest
 
+import draws_ref as ref
+from scores_ref import HALF
 from test_gpu_draws import _check_sample, _dev, _masked
-from test_gpu_scores import _close, _make, _tensor, ops  # noqa: F401
+from test_gpu_scores import _close, _given, _make, _tensor, ops  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+
+def _check_far(ops, t, kind, classes, gains, gives, **more):
+    torch, scores = ops
+    want = ref.feedback(_given(t), classes, gains, **more)
+    loss, logs, grad = scores.feedback(t, _dev(torch, classes), _dev(torch, gains), gives=gives, **more)
+    _close(loss.cpu().numpy(), want['loss'], want['loss_off'], 'loss')
+    _close(logs.cpu().numpy(), want['logs'], want['logs_off'], 'logs')
+    if gives == 'gradient':
+        _close(_given(grad), want['g'], want['g_off'] + (HALF[kind] * np.abs(want['g']) * (1 + 2.0 ** -8) if kind != 'f32' else 0), 'gradient')
+    else:
+        _close(grad.cpu().numpy()[..., 0], want['g'], want['g_off'], 'g')
+        _close(grad.cpu().numpy()[..., 1], want['h'], want['h_off'], 'h')
 
 
 @pytest.mark.parametrize('layout', ['row', 'class'])
@@ -47,3 +62,17 @@ def test_numbers_that_are_not_below_one(ops, layout, n, k, kind):
             assert np.array_equal(ids.cpu().numpy(), want), limits
             for got in (logs, every):
                 _close(got.cpu().numpy(), np.full(at.shape, -np.log(likely)), 2.0 ** -22, limits)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('k', [40000, 40001])
+def test_feedback_where_a_block_has_only_masked_classes(ops, k, kind):
+    """Thousands of neighbouring classes at the type's lowest number: their part of the entropy's sum is 0, not 0 times infinity."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = np.full((3, k), float(torch.finfo(torch.float32 if kind == 'f32' else torch.bfloat16).min))
+    z[0, :3000], z[1, 30000:31000], z[2, ::4000] = r.standard_normal(3000), r.standard_normal(1000), 1.0
+    t = _tensor(torch, z, kind, 'row')
+    classes, gains = np.array([[0, 10], [30001, 30002], [4000, 8000]], np.int32), np.ones((3, 2), np.float32)
+    for gives in ('gradient', 'pairs'):
+        _check_far(ops, t, kind, classes, gains, gives, entropy=0.05)

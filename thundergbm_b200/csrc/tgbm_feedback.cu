@@ -487,7 +487,7 @@ __device__ __forceinline__ void feedback_long(const FeedbackArgs &a, const Score
             s = o[1]; sd = o[2];
             m = lanes_max<32>(its);
             const float low = __fsub_rn(base, row_top(m)), by = its == minus_inf() ? 0.f : exp2_fast(low * a.c);
-            sd = lane < C && its > minus_inf() ? __fmaf_rn(low, s, sd) * by : 0.f;
+            sd = lane < C && by != 0.f ? __fmaf_rn(low, s, sd) * by : 0.f;   // (a block of classes at the type's lowest number is infinitely far)
             s = lane < C ? s * by : 0.f;
             s = warp_sum(s); sd = warp_sum(sd);   // (all lanes go on)
         }
