@@ -76,3 +76,31 @@ def test_feedback_where_a_block_has_only_masked_classes(ops, k, kind):
     classes, gains = np.array([[0, 10], [30001, 30002], [4000, 8000]], np.int32), np.ones((3, 2), np.float32)
     for gives in ('gradient', 'pairs'):
         _check_far(ops, t, kind, classes, gains, gives, entropy=0.05)
+
+
+@pytest.mark.parametrize('gives', ['gradient', 'pairs'])
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('layout,n,k', [('class', 5, 5), ('class', 5, 200), ('row', 5, 5), ('row', 5, 200), ('row', 5, 2000), ('row', 5, 9000), ('row+', 5, 9000), ('any', 5, 40)])
+def test_feedback_of_classes_masked_by_the_lowest_number(ops, layout, n, k, kind, gives):
+    """A share of 0 times what a class so far away would earn for the row's entropy is 0."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = r.standard_normal((n, k))
+    low = float(torch.finfo(torch.float32 if kind == 'f32' else torch.bfloat16).min)
+    z[:, 1::2] = low
+    z[3, 2] = -np.inf
+    t = _tensor(torch, z, kind, layout)
+    classes, gains = np.array([[0, 2, -1]] * n, np.int32), r.standard_normal((n, 3)).astype(np.float32)
+    _check_far(ops, t, kind, classes, gains, gives, temperature=0.2, entropy=0.05)
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 5, 5), ('class', 5, 200), ('row', 5, 5), ('row', 5, 200), ('row', 5, 9000), ('row+', 5, 9000), ('any', 5, 40)])
+def test_feedback_at_small_temperatures(ops, layout, n, k):
+    """entropy / T^2 times a distance that stands for infinity must not be infinite."""
+    torch, _ = ops
+    r = np.random.default_rng(k)
+    z = _masked(r, r.standard_normal((n, k))) * 2.0 ** -17
+    t = _tensor(torch, z, 'f32', layout)
+    classes, gains = np.array([[0, 2, 1]] * n, np.int32), r.standard_normal((n, 3)).astype(np.float32)
+    for gives in ('gradient', 'pairs'):
+        _check_far(ops, t, 'f32', classes, gains, gives, temperature=2.0 ** -17, entropy=0.5)

@@ -21,13 +21,15 @@ template <int W> __device__ __forceinline__ void meet() {   // the warps that sh
     else __syncwarp();
 }
 
-// A row's sums, relative to its largest score: sum of e = exp((s - top) / T) and of e (s - top).  What follows from them and the draws:
-//   g_i = p_i (by_d (s_i - top) + flat) + [draws of i],  h_i = max(curve p_i (1 - p_i), 1e-16),  p_i = e_i to_p
+// A row's sums, with y = (s - top) log2(e) / T and top its largest score: sum of e = 2^y and of e y.  What follows from them and the draws:
+//   g_i = p_i (by_y y_i + flat) + [draws of i],  h_i = max(curve p_i (1 - p_i), 1e-16),  p_i = e_i to_p
 struct FeedbackRow {
-    float top, c, to_p, by_d, flat, curve;
+    float top, c, to_p, by_y, flat, curve;
     bool counts;   // without a draw that counts, or with a weight of 0, the row has no loss
 };
-constexpr float MIN_HESSIAN = 1e-16f;   // the softmax objective's
+// e is 0 from -126 on: y stops here, so that e y and p (by_y y + flat) are 0 where a score is -inf, or so low that y is (0 times infinity is none)
+constexpr float FAR = -200.f;
+constexpr double LN2 = 0.69314718055994530942;
 
 struct Draw {
     double term, to_log;   // loss of one draw, its derivative by the log-probability
@@ -47,16 +49,16 @@ __device__ __forceinline__ Draw draw_of(const FeedbackArgs &a, double lp, float 
 }
 
 // The row's loss, and what its gradients need; `by`: what a draw's derivative is multiplied by
-__device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long long n, float w, float top, float sum, float sum_d, double log_sum, double term,
+__device__ __forceinline__ FeedbackRow factors_of(const FeedbackArgs &a, long long n, float w, float top, float sum, float sum_y, double log_sum, double term,
                                                   double to_log, double size, int number, bool writes, double &by) {
-    const double inv_sum = sum == 0.f ? 0.0 : 1.0 / (double)sum, spread = log_sum - (double)sum_d * a.inv_t * inv_sum;   // (the entropy)
+    const double inv_sum = sum == 0.f ? 0.0 : 1.0 / (double)sum, spread = log_sum - (double)sum_y * LN2 * inv_sum;   // (the entropy)
     FeedbackRow r;
     r.counts = number > 0 && w != 0.f;
     const double share = number == 1 ? 1.0 : number ? 1.0 / number : 0.0, scale = (double)w * a.inv_t;
     if (a.loss && writes) a.loss[n] = r.counts ? (float)((double)w * (term * share - (a.entropy != 0.f ? (double)a.entropy * spread : 0.0))) : 0.f;
     r.top = top; r.c = a.c;
     r.to_p = (float)inv_sum;
-    r.by_d = (float)(scale * (double)a.entropy * a.inv_t);
+    r.by_y = (float)(scale * (double)a.entropy * LN2);
     r.flat = (float)(scale * ((a.entropy != 0.f ? (double)a.entropy * (spread - log_sum) : 0.0) - to_log * share));
     r.curve = (float)(2 * scale * a.inv_t * (size * share + (double)a.entropy));
     by = scale * share;
@@ -87,7 +89,7 @@ template <typename T> __device__ __forceinline__ DrawsRead read_draws(const Feed
 }
 // One warp, for the row n: logs, the loss and what its gradients need.  cls[e], extra[e]: class of draw e and what is added there (-1: nothing;
 // of draws of one class the first has the sum).
-__device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long long n, float top, float sum, float sum_d, int *cls, float *extra, bool writes,
+__device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long long n, float top, float sum, float sum_y, int *cls, float *extra, bool writes,
                                                      const DrawsRead &draws) {
     const int lane = threadIdx.x & 31;
     const double log_sum = sum == 0.f ? 0.0 : fine_log(sum);
@@ -116,7 +118,7 @@ __device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long 
     term = warp_sum(term); to_log = warp_sum(to_log); size = warp_sum(size);
     __syncwarp();
     double by;
-    const FeedbackRow r = factors_of(a, n, draws.weight, top, sum, sum_d, log_sum, term, to_log, size, number, writes && lane == 0, by);
+    const FeedbackRow r = factors_of(a, n, draws.weight, top, sum, sum_y, log_sum, term, to_log, size, number, writes && lane == 0, by);
     if (a.gives != GIVES_LOSS) {   // of draws of one class the first takes the sum
         float total[SCORES_MAX_TOP / 32];
         bool first[SCORES_MAX_TOP / 32];
@@ -145,11 +147,16 @@ __device__ __forceinline__ FeedbackRow feedback_row(const FeedbackArgs &a, long 
     }
     return r;
 }
+__device__ __forceinline__ void add_exp(float x, float top, float c, float &s, float &sy) {
+    const float y = __fsub_rn(x, top) * c, e = exp2_fast(y);
+    s += e;
+    sy = __fmaf_rn(e, fmaxf(y, FAR), sy);
+}
 __device__ __forceinline__ float2 feedback_gh(const FeedbackRow &r, float s, float extra) {
     if (!r.counts) return make_float2(0.f, MIN_HESSIAN);
-    const float d = __fsub_rn(s, r.top), p = exp2_fast(d * r.c) * r.to_p;
+    const float y = __fsub_rn(s, r.top) * r.c, p = exp2_fast(y) * r.to_p;
     const float cp = r.curve * p;
-    return make_float2(__fmaf_rn(p, __fmaf_rn(r.by_d, fmaxf(d, -1e30f), r.flat), extra), fmaxf(__fmaf_rn(-cp, p, cp), MIN_HESSIAN));   // (p = 0 for -inf)
+    return make_float2(__fmaf_rn(p, __fmaf_rn(r.by_y, fmaxf(y, FAR), r.flat), extra), fmaxf(__fmaf_rn(-cp, p, cp), MIN_HESSIAN));
 }
 template <typename T> __device__ __forceinline__ void put_gradient(const FeedbackArgs &a, long long n, long long k, float2 gh) {
     const long long at = n * a.out.row + k * a.out.cls;
@@ -172,19 +179,15 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_any(FeedbackArgs a, Sc
     if (lane == 0) parts[0][warp] = m;
     __syncthreads();
     const float top = row_top(warp_max(parts[0][lane & (ROW_WARPS - 1)]));
-    float s = 0, sd = 0;
-    for (int k = threadIdx.x; k < a.k; k += ROW_THREADS) {
-        const float d = __fsub_rn(in(n, k), top), e = exp2_fast(d * a.c);
-        s += e;
-        sd = __fmaf_rn(e, fmaxf(d, -1e30f), sd);
-    }
-    s = warp_sum(s); sd = warp_sum(sd);
-    if (lane == 0) { parts[1][warp] = s; parts[2][warp] = sd; }
+    float s = 0, sy = 0;
+    for (int k = threadIdx.x; k < a.k; k += ROW_THREADS) add_exp(in(n, k), top, a.c, s, sy);
+    s = warp_sum(s); sy = warp_sum(sy);
+    if (lane == 0) { parts[1][warp] = s; parts[2][warp] = sy; }
     __syncthreads();
     if (warp == 0) {
         s = warp_sum(lane < ROW_WARPS ? parts[1][lane] : 0.f);
-        sd = warp_sum(lane < ROW_WARPS ? parts[2][lane] : 0.f);
-        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, read_draws(a, in, n));
+        sy = warp_sum(lane < ROW_WARPS ? parts[2][lane] : 0.f);
+        const FeedbackRow r = feedback_row(a, n, top, s, sy, cls, extra, true, read_draws(a, in, n));
         if (lane == 0) shared_row = r;
     }
     __syncthreads();
@@ -248,20 +251,16 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 3
         for (int v = 0; v < W; ++v) top = fmaxf(top, sh.part[0][v][lane].x);
     }
     top = row_top(top);
-    float s = 0, sd = 0;
+    float s = 0, sy = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) {
-        const float d = __fsub_rn(x[j], top), e = exp2_fast(d * a.c);
-        s += e;
-        sd = __fmaf_rn(e, fmaxf(d, -1e30f), sd);
-    }
+    for (int j = 0; j < E; ++j) add_exp(x[j], top, a.c, s, sy);
     if constexpr (W > 1) {
-        sh.part[1][warp][lane] = make_float2(s, sd);
+        sh.part[1][warp][lane] = make_float2(s, sy);
         __syncthreads();
         float2 all = sh.part[1][0][lane];
 #pragma unroll
         for (int v = 1; v < W; ++v) all = add2(all, sh.part[1][v][lane]);
-        s = all.x; sd = all.y;
+        s = all.x; sy = all.y;
     } else {
         __syncwarp();
     }
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 3
         int number = 0;
         for (int v = 0; v < busy; ++v) { term += sh.sums[0][v][lane]; to_log += sh.sums[1][v][lane]; size += sh.sums[2][v][lane]; number += sh.number[v][lane]; }
         double by;
-        sh.row[lane] = factors_of(a, n, a.weights ? a.weights[n] : 1.f, top, s, sd, log_sum, term, to_log, size, number, n0 == n, by);
+        sh.row[lane] = factors_of(a, n, a.weights ? a.weights[n] : 1.f, top, s, sy, log_sum, term, to_log, size, number, n0 == n, by);
         sh.by[lane] = by;
     }
     if (a.gives == GIVES_LOSS) return;
@@ -364,15 +363,11 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_row(FeedbackArgs a, Sc
 #pragma unroll
         for (int j = 0; j < E; ++j) top = fmaxf(top, x[j]);
         top = row_top(warp_max(top));
-        float s = 0, sd = 0;
+        float s = 0, sy = 0;
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            const float d = __fsub_rn(x[j], top), e = exp2_fast(d * a.c);
-            s += e;
-            sd = __fmaf_rn(e, fmaxf(d, -1e30f), sd);
-        }
-        s = warp_sum(s); sd = warp_sum(sd);
-        const FeedbackRow r = feedback_row(a, n, top, s, sd, cls, extra, true, read_draws(a, in, n));
+        for (int j = 0; j < E; ++j) add_exp(x[j], top, a.c, s, sy);
+        s = warp_sum(s); sy = warp_sum(sy);
+        const FeedbackRow r = feedback_row(a, n, top, s, sy, cls, extra, true, read_draws(a, in, n));
         if (a.gives != GIVES_LOSS) {
             unsigned drawn = 0;
             for (int e = 0; e < a.draws; ++e) {
@@ -394,8 +389,8 @@ __global__ void __launch_bounds__(ROW_THREADS) k_feedback_row(FeedbackArgs a, Sc
     if (a.maxbits) track_max(mg, mh, a.maxbits);
 }
 
-// Long rows: a cluster of up to 8 blocks (or one) holds the row in registers.  Two exponentials per score and gradient; a thread that has no
-// score of -inf needs no care for 0 times infinity.  1024 x 131072 in 16 bits: 150 us (floor 82); the rest is waiting, for the cluster and for the
+// Long rows: a cluster of up to 8 blocks (or one) holds the row in registers.  Two exponentials per score and gradient; a thread whose
+// scores are not infinitely far from the largest needs no care for 0 times infinity.  1024 x 131072 in 16 bits: 150 us (floor 82); the rest is waiting, for the cluster and for the
 // warp that works out the draws.  Blocks of 512 threads, two per SM, took 255 us, of 256 with twice the scores a thread, four per SM, 158.
 template <int TH> struct FeedbackShared {
     float parts[3][TH / 32], moments[3];
@@ -404,35 +399,35 @@ template <int TH> struct FeedbackShared {
     FeedbackRow row;
     DrawsRead ahead[32];   // (kept here: the registers are the row's)
 };
-// sums of exp((v - base) / T) and of that times (v - base), the second if asked for
+// sums of e = 2^y, y = (v - base) log2(e) / T, and of e y, the second if asked for.  MASKED: y may be infinite
 template <int V, bool MASKED>
-__device__ __forceinline__ void add_exps(const float (&v)[V], float base, float c, bool spread, float2 &s, float2 &sd) {
+__device__ __forceinline__ void add_exps(const float (&v)[V], float base, float c, bool spread, float2 &s, float2 &sy) {
     if constexpr (V == 1) {
-        const float d = __fsub_rn(v[0], base), e = exp2_fast(d * c);
+        const float y = __fsub_rn(v[0], base) * c, e = exp2_fast(y);
         s.x += e;
-        sd.x = __fmaf_rn(e, MASKED ? fmaxf(d, -1e30f) : d, sd.x);
+        sy.x = __fmaf_rn(e, MASKED ? fmaxf(y, FAR) : y, sy.x);
     } else {
         const float2 mb = make_float2(-base, -base), c2 = make_float2(c, c);
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
-            float2 d = add2(make_float2(v[i], v[i + 1]), mb);
-            const float2 y = mul2(d, c2), e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
+            const float2 y = mul2(add2(make_float2(v[i], v[i + 1]), mb), c2), e = make_float2(exp2_fast(y.x), exp2_fast(y.y));
             s = add2(s, e);
-            if (spread) sd = fma2(e, MASKED ? make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)) : d, sd);
+            if (spread) sy = fma2(e, MASKED ? make_float2(fmaxf(y.x, FAR), fmaxf(y.y, FAR)) : y, sy);
         }
     }
 }
+// MASKED: by_y y may be infinite
 template <int V, bool MASKED> __device__ __forceinline__ void gradients(const FeedbackRow &r, float (&v)[V]) {
     if constexpr (V == 1) {
         v[0] = feedback_gh(r, v[0], 0.f).x;
     } else {
         const float2 mb = make_float2(-r.top, -r.top), c2 = make_float2(r.c, r.c), p2 = make_float2(r.to_p, r.to_p);
-        const float2 by = make_float2(r.by_d, r.by_d), flat = make_float2(r.flat, r.flat);
+        const float2 by = make_float2(r.by_y, r.by_y), flat = make_float2(r.flat, r.flat);
 #pragma unroll
         for (int i = 0; i < V; i += 2) {
-            const float2 d = add2(make_float2(v[i], v[i + 1]), mb), y = mul2(d, c2);
+            const float2 y = mul2(add2(make_float2(v[i], v[i + 1]), mb), c2);
             const float2 p = mul2(make_float2(exp2_fast(y.x), exp2_fast(y.y)), p2);
-            const float2 g = mul2(p, fma2(by, MASKED ? make_float2(fmaxf(d.x, -1e30f), fmaxf(d.y, -1e30f)) : d, flat));
+            const float2 g = mul2(p, fma2(by, MASKED ? make_float2(fmaxf(y.x, FAR), fmaxf(y.y, FAR)) : y, flat));
             v[i] = g.x; v[i + 1] = g.y;
         }
     }
@@ -450,48 +445,48 @@ __device__ __forceinline__ void feedback_long(const FeedbackArgs &a, const Score
     if (warp == 0) sh.ahead[lane] = read_draws(a, in, n);
     float least, m;
     x.range(cells, least, m);
-    const bool masked = least == minus_inf();
     m = warp_max(m);
     if (lane == 0) sh.parts[0][warp] = m;
     __syncthreads();
     m = lanes_max<W>(sh.parts[0][lane & (W - 1)]);
     const bool spread = a.entropy != 0.f;
-    float s, sd;
+    float s, sy;
     {
         const float base = row_top(m);
-        float2 s2 = make_float2(0.f, 0.f), sd2 = s2;
+        const bool masked = !finite(fminf(__fsub_rn(least, base), 0.f) * a.c);
+        float2 s2 = make_float2(0.f, 0.f), sy2 = s2;
         auto pass = [&](auto care) {
 #pragma unroll
             for (int u = 0; u < P; ++u)
                 if (FULL || H::first(u) < cells) {
                     float v[V];
                     x.get(u, v);
-                    add_exps<V, decltype(care)::value>(v, base, a.c, spread, s2, sd2);
+                    add_exps<V, decltype(care)::value>(v, base, a.c, spread, s2, sy2);
                 }
         };
         masked ? pass(std::true_type{}) : pass(std::false_type{});
-        s = s2.x + s2.y; sd = sd2.x + sd2.y;
+        s = s2.x + s2.y; sy = sy2.x + sy2.y;
     }
-    s = warp_sum(s); sd = warp_sum(sd);
-    if (lane == 0) { sh.parts[1][warp] = s; sh.parts[2][warp] = sd; }
+    s = warp_sum(s); sy = warp_sum(sy);
+    if (lane == 0) { sh.parts[1][warp] = s; sh.parts[2][warp] = sy; }
     __syncthreads();
     if (warp == 0) {
-        s = lanes_sum<W>(sh.parts[1][lane & (W - 1)]); sd = lanes_sum<W>(sh.parts[2][lane & (W - 1)]);
-        if (C > 1 && lane == 0) { sh.moments[0] = m; sh.moments[1] = s; sh.moments[2] = sd; }
+        s = lanes_sum<W>(sh.parts[1][lane & (W - 1)]); sy = lanes_sum<W>(sh.parts[2][lane & (W - 1)]);
+        if (C > 1 && lane == 0) { sh.moments[0] = m; sh.moments[1] = s; sh.moments[2] = sy; }
     }
     if (C > 1) cluster.sync();
     if (warp == 0) {
         if (C > 1) {
             const float *o = cluster.map_shared_rank(sh.moments, lane < C ? lane : 0);
             const float its = o[0], base = row_top(its);
-            s = o[1]; sd = o[2];
+            s = o[1]; sy = o[2];
             m = lanes_max<32>(its);
-            const float low = __fsub_rn(base, row_top(m)), by = its == minus_inf() ? 0.f : exp2_fast(low * a.c);
-            sd = lane < C && by != 0.f ? __fmaf_rn(low, s, sd) * by : 0.f;   // (a block of classes at the type's lowest number is infinitely far)
+            const float low = __fsub_rn(base, row_top(m)) * a.c, by = its == minus_inf() ? 0.f : exp2_fast(low);
+            sy = lane < C && by != 0.f ? __fmaf_rn(low, s, sy) * by : 0.f;   // (a block of classes at the type's lowest number is infinitely far)
             s = lane < C ? s * by : 0.f;
-            s = warp_sum(s); sd = warp_sum(sd);   // (all lanes go on)
+            s = warp_sum(s); sy = warp_sum(sy);   // (all lanes go on)
         }
-        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sd, sh.cls, sh.extra, rank == 0, sh.ahead[lane]);
+        const FeedbackRow r = feedback_row(a, n, row_top(m), s, sy, sh.cls, sh.extra, rank == 0, sh.ahead[lane]);
         if (lane == 0) sh.row = r;
     }
     __syncthreads();
@@ -531,6 +526,7 @@ __device__ __forceinline__ void feedback_long(const FeedbackArgs &a, const Score
                         x.write(to, u);
                     }
             } else {
+                const bool masked = !finite(fminf(__fsub_rn(least, r.top), 0.f) * r.c * r.by_y);
                 masked ? pass(std::true_type{}) : pass(std::false_type{});
             }
         }

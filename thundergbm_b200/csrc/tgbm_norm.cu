@@ -242,7 +242,6 @@ template <int V> __device__ __forceinline__ void read_floats(const float *p, flo
         }
     }
 }
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 
 // sums of M numbers over a block of TH threads, the same in all of them; all threads, with two barriers
 template <int TH, int M> struct LongSums {

@@ -1,10 +1,13 @@
 // What the kernels that draw, learn from draws and standardise share: sums over lanes, long rows that a block or a cluster of blocks holds in its
 // registers, sizes.
 #pragma once
+#include <cfloat>
+
 #include "tgbm_scores.cuh"
 
 namespace tgbm {
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 template <int L, typename V> __device__ __forceinline__ V lanes_sum(V v) {
 #pragma unroll
     for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
