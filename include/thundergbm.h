@@ -312,7 +312,8 @@ int tgbm_scores_feedback(int n_rows, int n_classes, int type, const void *d_scor
 
 /* Every row at mean 0 and variance 1 over its classes, then a gain and a bias per class:
  *   out_k = (s_k - mean) rstd gain_k + bias_k,  rstd = 1 / sqrt(variance + eps)
- * over the classes whose score is not -infinity; those stay -infinity.  A row without another class has mean 0 and rstd 0.  d_out: the type
+ * over the classes whose score is not -infinity; those stay -infinity.  A row without another class has mean 0 and rstd 0.  Sums are floats: where
+ * the squared deviations add up to more than one holds (scores some 1e19 apart) rstd is 0, where the scores do mean is not finite.  d_out: the type
  * of the scores, strides of its own; d_out = d_scores with the same strides works in place, otherwise the two must not share memory.
  * d_gain, d_bias: n_classes floats, NULL: 1, 0.  d_mean, d_rstd: n_rows floats, or NULL.  eps > 0. */
 int tgbm_scores_norm(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, void *d_out,

@@ -104,3 +104,23 @@ def test_feedback_at_small_temperatures(ops, layout, n, k):
     classes, gains = np.array([[0, 2, 1]] * n, np.int32), r.standard_normal((n, 3)).astype(np.float32)
     for gives in ('gradient', 'pairs'):
         _check_far(ops, t, 'f32', classes, gains, gives, temperature=2.0 ** -17, entropy=0.5)
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('layout,n,k', [('class', 40, 6), ('class', 40, 200), ('class', 9, 700), ('row', 9, 6), ('row', 9, 200), ('row', 9, 3000), ('row', 9, 3001), ('any', 9, 40), ('class', 9, 1500)])
+def test_norm_leaves_masked_classes_masked(ops, layout, n, k, kind):
+    """Also where the variance of the others is more than a float holds (their deviation counts as infinite, so they are 0), or their sum is."""
+    torch, scores = ops
+    z = np.random.default_rng(k).standard_normal((n, k))
+    low = float(torch.finfo(torch.float32 if kind == 'f32' else torch.bfloat16).min)
+    z[:, 3] = -np.inf
+    z[0, 0], z[0, 1] = 1e20, -1e20
+    z[1, 0] = low
+    z[2, 0] = z[2, 1] = low
+    t = _tensor(torch, z, kind, layout)
+    gone = _given(t) == -np.inf
+    for gain in (None, torch.ones(k, device='cuda')):
+        y, mean, rstd = scores.norm(t, gain)
+        y = _given(y)
+        assert (y[gone] == -np.inf).all()
+        assert (rstd[:2] == 0).all() and (y[:2][~gone[:2]] == 0).all() and np.isfinite(y[3:][~gone[3:]]).all()

@@ -184,6 +184,12 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : W == 16 ? 
         if (!WEIGHTS) return y;
         return there(x[j]) ? __fmaf_rn(y, gain ? __ldg(gain + j) : 1.f, bias ? __ldg(bias + j) : 0.f) : x[j];
     });
+    if (!WEIGHTS && !(by > 0.f && finite(mean))) {   // (and here, where (-inf - mean) by is NaN)
+        T *to = out.at(n, k0);
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (j < here && !there(x[j])) to[j * out.cls] = score_from<T>(x[j]);
+    }
 }
 
 // ---- by row, up to 1024 classes: L lanes have a row, E classes each, L apart -----------------------------------------
