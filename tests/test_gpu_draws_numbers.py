@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import draws_ref as ref
-from scores_ref import HALF
+from scores_ref import HALF, U
 from test_gpu_draws import _check_sample, _dev, _masked
 from test_gpu_scores import _close, _given, _make, _tensor, ops  # noqa: F401
 
@@ -124,3 +124,35 @@ def test_norm_leaves_masked_classes_masked(ops, layout, n, k, kind):
         y = _given(y)
         assert (y[gone] == -np.inf).all()
         assert (rstd[:2] == 0).all() and (y[:2][~gone[:2]] == 0).all() and np.isfinite(y[3:][~gone[3:]]).all()
+
+
+@pytest.mark.parametrize('kind', ['f32', 'bf16'])
+@pytest.mark.parametrize('layout,n,k', [('class', 70, 6), ('class', 70, 30), ('class', 70, 250), ('class', 70, 700), ('row', 70, 30), ('row', 1100, 250), ('row', 30, 250), ('row', 5, 9001),
+                                        ('row', 5, 70000), ('any', 9, 40)])
+def test_logs_among_all_classes(ops, layout, n, k, kind):
+    """Their mass is a sum of doubles under all limits: the logs are rounded once, no class is likelier among all than among those that are
+    left, and what a row gets does not depend on the limits of its neighbours."""
+    torch, scores = ops
+    r = np.random.default_rng(k)
+    z = _masked(r, _make(r, n, k))
+    z[3] = -30
+    z[3, k // 2] = 0      # nearly all of the mass
+    z[4] = np.where(np.arange(k) % 2, 0.0, -1.0)
+    t = _tensor(torch, z, kind, layout)
+    u = r.random((n, 3))
+    rows = dict(temperature=r.choice([0.5, 1.0, 2.0], n).astype(np.float32), top_k=r.choice([0, 1, 2, 20, 2 * k], n).astype(np.int32),
+                top_p=r.choice([1.0, 0.4, 0.9], n).astype(np.float32), min_p=r.choice([0.0, 0.01, 1.0], n).astype(np.float32))
+    for limits in ({}, dict(top_k=max(1, k // 3)), dict(min_p=0.001), dict(top_p=0.8), dict(top_k=5, top_p=0.9, min_p=1e-4, temperature=0.7), rows):
+        given = {name: _dev(torch, v) if isinstance(v, np.ndarray) else v for name, v in limits.items()}
+        ids, logs, every = scores.sample(t, _dev(torch, u), **given)
+        want = ref.sample(_given(t), u, **limits)
+        assert np.array_equal(ids.cpu().numpy(), want[0])
+        exact = want[2]
+        _close(every.cpu().numpy(), exact, 2.0 ** -32 + U * (1 + 2.0 ** -18) * np.abs(np.where(np.isfinite(exact), exact, 0)), limits)
+        assert bool(((every <= logs) | every.isnan()).all())
+        for i in (0, 3, 31, 32, n - 1):
+            if i >= n or layout == 'row' and n > 1000:   # (one row alone is another kernel's)
+                continue
+            one = slice(i, i + 1)
+            alone = scores.sample(t[one], _dev(torch, u)[one], **{name: v[one] if isinstance(v, torch.Tensor) else v for name, v in given.items()})
+            assert all(torch.equal(a.nan_to_num(nan=9.0), b[one].nan_to_num(nan=9.0)) for a, b in zip(alone, (ids, logs, every))), (i, limits)

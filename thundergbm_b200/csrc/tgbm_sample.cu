@@ -404,29 +404,11 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
     const int top_k = l.greedy ? 1 : l.top_k;
     const bool by_count = live && top_k < a.k, by_mass = live && l.top_p < 1 && !l.greedy, by_share = live && l.min_p > 0 && !l.greedy;
     const bool limited = by_count || by_mass || by_share;
-    // Borders are shares of the whole mass where nothing cuts it before: a sum of doubles.  Else it is only told of (all_logs): floats.
-    if (__any_sync(0xffffffffu, live && !by_count && !by_share)) {
-        each_score([&](float x, int) { all += live ? weight_of(x) : 0.0; });
-    } else {
-        const float c = fminf((float)(l.inv_t * 1.4426950408889634), FLT_MAX), base = live ? top : 0.f;
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
-        int i = 0;
-        each_score([&](float x, int) {
-            part[i & 3] += exp2_fast(__fsub_rn(x, base) * c);
-            ++i;
-        });
-        all = (double)__fadd_rn(__fadd_rn(part[0], part[1]), __fadd_rn(part[2], part[3]));
-    }
-    least = 0; count = 0;
-    {
-        float high = 0;
-        over.all(all, least, high, count);
-    }
-    if (l.greedy) all = 1.0;
-    // A border that all that is left reaches, rounded down by more than its floats can be off: 2^-19 of its distance from the largest score (logf: 2^-23,
-    // products 2^-24 each), of T (the share under the logarithm is rounded) and of that score.
+    // The whole mass, a sum of doubles, and the scores from a border on that all that is left reaches.  The border is rounded down by more than its floats
+    // can be off: 2^-19 of its distance from the largest score (logf: 2^-23, products 2^-24 each), of T (the share under the logarithm is
+    // rounded) and of that score.  Where it is a share of the whole mass, that comes first.
     float low = minus_inf(), high = top;
-    {
+    auto border = [&] {
         const float t = (float)(1.0 / l.inv_t);
         float down = -FLT_MAX;
         if (l.greedy) down = 0.f;
@@ -434,16 +416,34 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
         else if (by_mass && !by_count) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
         low = l.greedy ? top : __fadd_rn(top, down) - (fabsf(down) + t + fabsf(top)) * 2e-6f;
         if (!(low <= top)) low = down == -FLT_MAX ? minus_inf() : top;
-    }
+    };
     int own = 0;
-    least = -minus_inf();
     double sum = 0;
-    each_score([&](float x, int) {
+    least = -minus_inf();
+    auto look = [&](float x) {
         if (live && x >= low && x > minus_inf()) { ++own; least = fminf(least, x); }
-    });
+    };
+    const bool share_of_mass = __any_sync(0xffffffffu, by_mass && !by_count && !by_share);
+    if (share_of_mass) {
+        each_score([&](float x, int) { all += live ? weight_of(x) : 0.0; });
+        float none = 0, none_high = 0;
+        count = 0;
+        over.all(all, none, none_high, count);
+        border();
+        each_score([&](float x, int) { look(x); });
+    } else {
+        border();
+        each_score([&](float x, int) {
+            all += live ? weight_of(x) : 0.0;
+            look(x);
+        });
+        sum = all;
+    }
     count = (float)own;
     const int counted = over.turn;
     over.all(sum, least, high, count);
+    if (!share_of_mass) all = sum;
+    if (l.greedy) all = 1.0;
     low = least;
     high = top;
     bool again = false;   // what was counted above is not what the list takes

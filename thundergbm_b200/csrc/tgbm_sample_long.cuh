@@ -288,11 +288,10 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         auto rough = [&](float x) { return exp2_fast(__fsub_rn(x, top) * c); };
         float f0 = 0, f1 = 0;
         int count_of_row = 0;   // (not looked at)
-        // sum of floats over this thread's scores; marks those from `border` on
-        unsigned reach = 0;
-        auto look = [&](float border) {
+        unsigned reach = 0;   // scores from the border on
+        // sum of floats over this thread's scores
+        auto look = [&] {
             float2 part = make_float2(0.f, 0.f);
-            reach = 0;
 #pragma unroll
             for (int u = 0; u < P; ++u) {
                 if (H::first(u) >= cells) continue;
@@ -300,21 +299,17 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 hold.get(u, v);
                 if constexpr (V == 1) {
                     part.x += rough(v[0]);
-                    reach |= v[0] >= border ? 1u << u : 0u;
                 } else {
                     const float2 mt = make_float2(-top, -top), c2 = make_float2(c, c);
 #pragma unroll
-                    for (int i = 0; i < V; i += 2) {
-                        part = add2(part, exp_pair(make_float2(v[i], v[i + 1]), mt, c2));
-                        reach |= (v[i] >= border ? 1u << (u * V + i) : 0u) | (v[i + 1] >= border ? 2u << (u * V + i) : 0u);
-                    }
+                    for (int i = 0; i < V; i += 2) part = add2(part, exp_pair(make_float2(v[i], v[i + 1]), mt, c2));
                 }
             }
             return (double)__fadd_rn(part.x, part.y);
         };
         const bool exact = !by_count && !by_share;   // top_p alone: a share of the whole mass (by floats at first)
         if (exact) {
-            all = look(-minus_inf());
+            all = look();
             count = 0;
             total(all, f0, f1, count);
         }
@@ -337,14 +332,19 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 ++bit;
             });
         };
-        if (!exact) {
-            all = look(low);
-            count = __popc(reach);
-            total(all, f0, f1, count);
-        } else {
+        if (exact) {
             mark(low);
             count = __popc(reach);
             total(sum, f0, f1, count);
+        } else {
+            int bit = 0;
+            each([&](float x, int) {
+                reach |= x >= low ? 1u << bit : 0u;
+                ++bit;
+                all += weight_of(x);
+            });
+            count = __popc(reach);
+            total(all, f0, f1, count);
         }
         if (l.greedy) all = 1.0;
         if (by_count && count < top_k && low > base) {   // (groups without a score: the guess was too high)
