@@ -156,3 +156,20 @@ def test_logs_among_all_classes(ops, layout, n, k, kind):
             one = slice(i, i + 1)
             alone = scores.sample(t[one], _dev(torch, u)[one], **{name: v[one] if isinstance(v, torch.Tensor) else v for name, v in given.items()})
             assert all(torch.equal(a.nan_to_num(nan=9.0), b[one].nan_to_num(nan=9.0)) for a, b in zip(alone, (ids, logs, every))), (i, limits)
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 40, 5), ('class', 40, 200), ('class', 9, 700), ('row', 9, 5), ('row', 1100, 200), ('row', 9, 200), ('row', 5, 9001), ('row', 5, 70000),
+                                        ('any', 9, 40), ('class', 9, 1500)])
+def test_sample_at_the_largest_and_smallest_temperatures(ops, layout, n, k):
+    """Differences of scores above 3.4e38 and below 2^-126 at temperatures to match: e^-6 is e^-6."""
+    torch, _ = ops
+    r = np.random.default_rng(k)
+    unit = r.uniform(-1, 1, (n, k))
+    unit[0] = np.where(np.arange(k) % 3, 1, -1)
+    unit[1, 0], unit[1, 1] = 1, -1
+    u = r.random((n, 3))
+    for size, temperatures in ((3.3e38, (1e38, 3e37)), (3e-40, (1e-40, 3e-41))):
+        t = _tensor(torch, unit * size, 'f32', layout)
+        for limits in ({}, dict(top_k=max(1, k // 2)), dict(top_p=0.9), dict(top_p=0.2), dict(min_p=0.01), dict(min_p=0.01, top_p=0.7, top_k=k - 1)):
+            for T in temperatures:
+                _check_sample(ops, t, u, dict(limits, temperature=T), (layout, k, T, str(limits)))

@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
         if (l.greedy) down = 0.f;
         else if (by_share) down = logf((float)l.min_p) * t;
         else if (by_mass && !by_count) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
-        low = l.greedy ? top : __fadd_rn(top, down) - (fabsf(down) + t + fabsf(top)) * 2e-6f;
+        low = l.greedy ? top : __fadd_rn(top, down) - ((fabsf(down) + t + fabsf(top)) * 2e-6f + 1e-44f);   // (1e-44: products below 2^-126)
         if (!(low <= top)) low = down == -FLT_MAX ? minus_inf() : top;
     };
     int own = 0;
@@ -626,8 +626,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
             const double target = l.top_p * above;
             // by floats first, each sum off by less than 2^-18, as far as they tell on which side the border lies
             float up_to = top;
-            const float c = fminf((float)(l.inv_t * 1.4426950408889634), FLT_MAX);
-            bool told = part;
+            const float c = (float)(l.inv_t * 1.4426950408889634);
+            bool told = part && floats_tell(l);
             while (__any_sync(0xffffffffu, told && lowest < up_to)) {
                 const float mid = middle(lowest, up_to);
                 float mass = 0, up = -minus_inf(), below = minus_inf(), none = 0;

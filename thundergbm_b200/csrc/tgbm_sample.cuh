@@ -52,14 +52,12 @@ struct Powers {
     }
 };
 struct Exponent {
-    double by;      // 32 log2(e) / T
-    float about;    // the same
-    bool greedy;    // 1 for d = 0, else 0
-    __device__ __forceinline__ Exponent(const Limits &l) : by(l.inv_t * 46.166241308446828384), about((float)by), greedy(l.greedy) {}
+    double by;   // 32 log2(e) / T; temperature 0: so much that any distance counts for nothing
+    __device__ __forceinline__ Exponent(const Limits &l) : by(l.greedy ? 1e300 : l.inv_t * 46.166241308446828384) {}
     __device__ __forceinline__ double operator()(const Powers &t, float x, float top) const {
-        if (x == top) return 1.0;   // (also where `about` is infinite)
-        if (greedy || !(__fsub_rn(x, top) * about > -32000.f)) return 0.0;   // (2^-1000; -inf)
-        const double y = __dmul_rn(__dsub_rn((double)x, (double)top), by), shifted = __dadd_rn(y, 6755399441055744.0);   // 1.5 * 2^52: whole numbers
+        const double y = __dmul_rn(__dsub_rn((double)x, (double)top), by);
+        if ((unsigned)__double2hiint(y) > 0xc0df4000u) return 0.0;   // (y < -32000: 2^-1000; -inf.  y is at most 0: its sign, exponent and first digits tell)
+        const double shifted = __dadd_rn(y, 6755399441055744.0);   // 1.5 * 2^52: whole numbers
         const int n = __double2loint(shifted);
         const double r = __dsub_rn(y, __dsub_rn(shifted, 6755399441055744.0));
         constexpr double A1 = 0.6931471805599453094 / 32, A2 = A1 * A1 / 2, A3 = A1 * A1 * A1 / 6, A4 = A1 * A1 * A1 * A1 / 24;
@@ -68,6 +66,9 @@ struct Exponent {
         return __hiloint2double(__double2hiint(v) + ((n >> 5) << 20), __double2loint(v));
     }
 };
+
+// May masses be sums of 2^((x - top) c) by floats, c = log2(e) / T?  Not where c is none, nor where a difference that is none would still have a mass.
+__device__ __forceinline__ bool floats_tell(const Limits &l) { return l.inv_t >= 1e-30 && l.inv_t <= 2e38; }
 
 __device__ __forceinline__ float middle(float low, float high) {
     const float mid = 0.5f * low + 0.5f * high;

@@ -284,7 +284,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
     double mass = 0;
     bool listed = false;
     if (by_count || by_mass || by_share) {
-        const float c = fminf((float)(l.inv_t * 1.4426950408889634), FLT_MAX);
+        const float c = (float)(l.inv_t * 1.4426950408889634);
+        const bool told = floats_tell(l);
         auto rough = [&](float x) { return exp2_fast(__fsub_rn(x, top) * c); };
         float f0 = 0, f1 = 0;
         int count_of_row = 0;   // (not looked at)
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
             return (double)__fadd_rn(part.x, part.y);
         };
         const bool exact = !by_count && !by_share;   // top_p alone: a share of the whole mass (by floats at first)
-        if (exact) {
+        if (exact && told) {
             all = look();
             count = 0;
             total(all, f0, f1, count);
@@ -317,8 +318,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         const float t = (float)(1.0 / l.inv_t);
         float down = -750.f * t;
         if (by_share) down = logf((float)l.min_p) * t;
-        else if (exact) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
-        low = __fadd_rn(top, down) - (fabsf(down) + 5.f * t + fabsf(top)) * 2e-6f;
+        else if (exact && told) down = logf((float)((1 - l.top_p) * all / a.k)) * t;
+        low = __fadd_rn(top, down) - ((fabsf(down) + 5.f * t + fabsf(top)) * 2e-6f + 1e-44f);
         if (l.greedy) low = top;
         if (!(low <= top)) low = minus_inf();
         low = fmaxf(low, -FLT_MAX);
@@ -354,7 +355,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
             total(sum, f0, f1, count);
         }
         float high = top;
-        const bool narrowing = by_count ? top_k <= LONG_LIST : by_mass && !by_share;
+        const bool narrowing = by_count ? top_k <= LONG_LIST : by_mass && !by_share && told;
         // top_p alone: masses by floats, each off by less than 2^-18, tell what certainly reaches the target and what certainly does not
         const double enough = l.top_p * all * (1 + 2e-5), short_of = l.top_p * all * (1 - 2e-5);
         int above = 0;   // scores larger than `high`, which are left in any case
