@@ -173,3 +173,21 @@ def test_sample_at_the_largest_and_smallest_temperatures(ops, layout, n, k):
         for limits in ({}, dict(top_k=max(1, k // 2)), dict(top_p=0.9), dict(top_p=0.2), dict(min_p=0.01), dict(min_p=0.01, top_p=0.7, top_k=k - 1)):
             for T in temperatures:
                 _check_sample(ops, t, u, dict(limits, temperature=T), (layout, k, T, str(limits)))
+
+
+@pytest.mark.parametrize('layout,n,k', [('class', 5, 5), ('class', 5, 200), ('row', 5, 5), ('row', 5, 200), ('row', 5, 3000), ('any', 5, 40)])
+def test_feedback_of_gains_and_logs_that_are_none(ops, layout, n, k):
+    """A NaN among what a draw that counts came with is told by the row's loss and gradient, and by no other row's."""
+    torch, scores = ops
+    nan = float('nan')
+    z = _tensor(torch, np.random.default_rng(k).standard_normal((n, k)), 'f32', layout)
+    c = torch.tensor([[0, 1], [0, 1], [2, -1], [2, 3], [4, 4]], dtype=torch.int32, device='cuda')
+    gains = torch.tensor([[nan, 1.0], [1, 1], [1, nan], [1, 1], [1, 1]], device='cuda')
+    old = torch.tensor([[-1.0, -1], [-1, nan], [-1, nan], [-1, -1], [-1, nan]], device='cuda')
+    weights = torch.tensor([1.0, 1, 1, 1, 0], device='cuda')
+    for gives in ('gradient', 'pairs'):
+        loss, logs, grad = scores.feedback(z, c, gains, old=old, weights=weights, clip=0.2, gives=gives)
+        g = grad if gives == 'gradient' else grad[..., 0]
+        assert loss[:2].isnan().all() and g[:2].isnan().all()
+        assert loss[2:].isfinite().all() and g[2:].isfinite().all() and loss[4] == 0 and not g[4].any()
+        assert logs[:2].isfinite().all()

@@ -40,6 +40,7 @@ __device__ __forceinline__ Draw draw_of(const FeedbackArgs &a, double lp, float 
     Draw d;
     d.term = gain == 0 ? 0.0 : -fmin(r * gain, held * gain);   // (what weighs 0 counts for nothing, also where the ratio is infinite)
     d.to_log = gain != 0 && r * gain <= held * gain ? -r * gain : 0.0;
+    if (gain != 0 && r * gain != r * gain) d.term = d.to_log = r * gain;   // (NaN: neither bound holds it)
     if (a.kl != 0.f) {
         const double x = (double)reference - lp, e = exp(x);
         d.term += (double)a.kl * (e - x - 1);
