@@ -191,3 +191,18 @@ def test_feedback_of_gains_and_logs_that_are_none(ops, layout, n, k):
         assert loss[:2].isnan().all() and g[:2].isnan().all()
         assert loss[2:].isfinite().all() and g[2:].isfinite().all() and loss[4] == 0 and not g[4].any()
         assert logs[:2].isfinite().all()
+
+
+def test_counts_that_32_bits_do_not_hold_are_refused(ops):
+    """2^32 + 3 is not 3, and -2^32 does not mean all."""
+    torch, scores = ops
+    from thundergbm_b200.thundergbm import TGBMClassifier
+    z, u = torch.zeros(4, 9, device='cuda'), torch.rand(4, device='cuda')
+    x = np.random.default_rng(1).random((60, 3)).astype(np.float32)
+    model = TGBMClassifier(depth=2, n_trees=2, verbose=0).fit(x, np.arange(60) % 3)
+    for top_k in (2 ** 31, 2 ** 32 + 3, -2 ** 32, -2 ** 40, 2.5, float('inf'), float('nan')):
+        with pytest.raises(ValueError, match='whole number'):
+            scores.sample(z, u, top_k=top_k)
+        with pytest.raises(ValueError, match='whole number'):
+            model.predict_sample(x, np.zeros(60), top_k=top_k)
+    model.predict_sample(x, np.zeros(60), top_k=np.int64(2))

@@ -226,7 +226,7 @@ def sample(scores, uniform, *, temperature=1.0, top_k=None, top_p=None, min_p=No
     top, top_ptr = _limit(top_k, 0, torch.int32, n, device, 'top_k')
     p, p_ptr = _limit(top_p, 1.0, torch.float32, n, device, 'top_p')
     m, m_ptr = _limit(min_p, 0.0, torch.float32, n, device, 'min_p')
-    if top != int(top) or top >= 2 ** 31:
+    if not -2 ** 31 <= top < 2 ** 31 or top != int(top):   # (a C int would take the rest of the division by 2^32)
         _refuse('top_k: a whole number')
     classes = scores.new_empty(shape, dtype=torch.int32)
     logs = scores.new_empty(shape, dtype=torch.float32)

@@ -273,13 +273,14 @@ class TGBMModel:
         uniform = np.ascontiguousarray(uniform, np.float64)
         if uniform.ndim not in (1, 2) or uniform.shape[0] != n or (uniform.ndim == 2 and not 1 <= uniform.shape[1] <= 128):
             raise ValueError('uniform: one per row, or rows x up to 128')
+        if not -2 ** 31 <= top_k < 2 ** 31 or top_k != int(top_k):
+            raise ValueError('top_k: a whole number')
         classes = np.empty(uniform.shape, np.int32)
         logs, all_logs = np.empty(uniform.shape, np.float32), np.empty(uniform.shape, np.float32)
         rest = (C.byref(self.model), self.n_trees, self.tree_per_iter, self.learning_rate, C.byref(rules), uniform.shape[1] if uniform.ndim == 2 else 1,
-                _vp(uniform), temperature, top_k, top_p, min_p, _vp(classes), _vp(logs), _vp(all_logs))
+                _vp(uniform), temperature, int(top_k), top_p, min_p, _vp(classes), _vp(logs), _vp(all_logs))
         _lib.check(getattr(self._lib, 'tgbm_predict_sample' + form)(*data, *rest))
         return classes, logs, all_logs
-
 
     def predict(self, X, groups=None):
         if self.model is None:
