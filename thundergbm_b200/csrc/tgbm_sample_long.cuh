@@ -333,18 +333,12 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
                 ++bit;
             });
         };
+        mark(low);
+        count = __popc(reach);
         if (exact) {
-            mark(low);
-            count = __popc(reach);
             total(sum, f0, f1, count);
         } else {
-            int bit = 0;
-            each([&](float x, int) {
-                reach |= x >= low ? 1u << bit : 0u;
-                ++bit;
-                all += weight_of(x);
-            });
-            count = __popc(reach);
+            each([&](float x, int) { all += weight_of(x); });
             total(all, f0, f1, count);
         }
         if (l.greedy) all = 1.0;
