@@ -133,10 +133,9 @@ int tgbm_booster_set_teacher(TgbmBooster *b, int top, const int *ids, const floa
  * Ranks call it together, as above, with the same temperature, clip and entropy and all with old and weights or none. */
 int tgbm_booster_set_feedback(TgbmBooster *b, int draws, const int *classes, const float *gains, const float *old, const float *weights, float temperature,
                               float clip_low, float clip_high, float entropy);
-/* the mean over this rank's rows of that loss on the current scores */
-int tgbm_booster_feedback_loss(TgbmBooster *b, double *out);
-/* that loss on the current scores: its mean over this rank's rows (waits as tgbm_booster_sync does; with a communicator every rank calls it) */
+/* those losses on the current scores: their mean over this rank's rows (wait as tgbm_booster_sync does; with a communicator every rank calls them) */
 int tgbm_booster_teacher_loss(TgbmBooster *b, double *out);
+int tgbm_booster_feedback_loss(TgbmBooster *b, double *out);
 int tgbm_booster_sync(TgbmBooster *b);
 /* boost + sync, bracketed by CUDA events on the booster's stream: device time of the n_rounds in ms */
 int tgbm_booster_boost_timed(TgbmBooster *b, int n_rounds, float *elapsed_ms);
@@ -223,7 +222,8 @@ int tgbm_metric_score_noalloc(const char *objective, int n_rows, int trees_per_r
  * elements, none negative).  Row stride 1: by class, as tgbm_booster_get_ypred and tgbm_predict_raw lay them out; class stride 1:
  * by row, as networks do.  Where neither is 1 the operators work as well, more slowly, and so do top and distill by class above some 5000
  * classes (scores of 2000 x 10000 13 and 4 times as long as of 4000 x 5000), and sample, feedback, norm and norm_backward by class above 1024
- * (4000 x 5000: up to 8 times as long as by row). */
+ * (4000 x 5000: up to 9 times as long as by row).  How far a score lies below the largest of its row is a float (in sample a double): infinite beyond
+ * 3.4e38. */
 #define TGBM_F32 0
 #define TGBM_F16 1
 #define TGBM_BF16 2
@@ -289,7 +289,7 @@ int tgbm_scores_distill(int n_rows, int n_classes, int type, const void *d_score
  * logs of -infinity, one that holds NaN or +infinity class -1 and NaN.
  * Each of the four limits holds for all rows, or (where d_temperature, d_top_k, d_top_p, d_min_p is not NULL) is read per row: a temperature
  * that is negative or no finite number gives class -1 and NaN, top_k below 1, top_p above 1 or NaN and min_p below 0 or NaN limit
- * nothing.  Masses are sums of doubles. */
+ * nothing.  Masses are sums of doubles, of exponentials good to 2^-38. */
 #define TGBM_F64 3
 #define TGBM_SCORES_MAX_DRAWS 128
 int tgbm_scores_sample(int n_rows, int n_classes, int type, const void *d_scores, long long row_stride, long long class_stride, int draws,

@@ -149,7 +149,7 @@ template <int E, typename T, typename F> __device__ __forceinline__ void write_c
     }
 }
 
-// 50003 x 250: 26.7 us (floor 15.3), 22 instructions per score where a tenth is masked; addresses by 64-bit steps and a test of every class's number took 55, and
+// 50003 x 250: 24.9 us (floor 15.3), 23 instructions per score where a tenth is masked; addresses by 64-bit steps and a test of every class's number took 55, and
 // 43 us.
 template <typename T, int E, int W, bool WEIGHTS>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 8 ? 4 : W == 16 ? 2 : 1) k_norm_class(NormArgs a, Scores<T> in, Scores<T> out) {
@@ -1037,6 +1037,8 @@ void scores_norm_backward(const NormBackwardArgs &a, cudaStream_t stream) {
                 kern<<<blocks, W == 1 ? 128 : 32 * W, 0, stream>>>(a, grad, in, out);
                 shares = blocks;
             };
+            // 129 to 256 classes: 16 warps with 16 classes each rather than 8 with 32, whose scores and gradients leave room for two blocks on an SM.  16
+            // and 8 warps (us): 50003 x 130 40 and 41, 200 46 and 47, 250 50 and 53, in 16 bits 150 42 and 50, 250 44 and 51; with all of 256 classes 50 and 47.
             if (a.k > 128 && a.k <= 256) go(integral_constant<int, 16>{}, integral_constant<int, 16>{});
             else by_class_sizes(a.k, go);
             return;

@@ -197,8 +197,12 @@ __global__ void __launch_bounds__(ROW_THREADS) k_sample_any(SampleArgs a, Scores
 // walks its row's list there, without a barrier, as often as it takes.  Scores that can be are those from a border on: min_p gives one, and so does
 // top_p (classes with less than (1 - top_p) / classes of the mass each have less than 1 - top_p of it together); where more than LIST reach it, it is
 // raised by bisection over all scores as long as enough reach it.  Rows with more all the same (limits that leave that many, ties)
-// are settled by bisection over all scores, by floats as far as they tell: 20000 x 1000, top_p 0.9 of a normal distribution, 1283 us, 3146 by doubles from
+// are settled by bisection over all scores, by floats as far as they tell: 20000 x 1000, top_p 0.9 of a normal distribution, 1157 us, 3146 by doubles from
 // the start.
+// A longer list takes more rows, and leaves room for fewer blocks on an SM: with 56 entries three tiles of up to 250 classes share it.  Lists of 40, 56
+// and 80 entries (us): 50003 x 250 with some 40 likely classes, top_p 0.9: 130, 95, 126; min_p 0.02 beside it: 77, 77, 98; 50003 x 250 of a normal
+// distribution, top_k 50: 171, 190, 243; 20000 x 500, 100 likely classes, top_k 20: 152, 146, 217; 20000 x 1000 of a normal distribution, top_k 50,
+// where one block has an SM in any case: 546, 526, 446.
 constexpr int LIST = 56;
 template <int W> struct ClassShared {
     Powers powers;
@@ -279,7 +283,7 @@ template <int W> __device__ __forceinline__ void meet() {   // the warps that sh
     else __syncwarp();
 }
 
-// Nothing is cut off: exponentials stay in registers.  Bound by the call and by instructions: 581012 x 7 in 18.4 us (floor 4.3).
+// Nothing is cut off: exponentials stay in registers.  Bound by the call and by instructions: 581012 x 7 in 17.1 us (floor 4.3).
 template <typename T, int E, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 2 : 1) k_sample_class(SampleArgs a, Scores<T> in) {
     __shared__ ClassShared<W> shared[W == 1 ? 4 : 1];   // (W = 1: each warp has its own)
@@ -357,9 +361,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : W == 8 ? 2
 }
 
 // With limits: the scores lie in shared memory (row r and class k at k * apart + r), which leaves the registers to what is found out of them.  Bound by
-// instructions, 800 a row of 250 classes, half of them for the lists: 50003 x 250 with min_p and top_p in 83 us (floor 7.8).  Bisection over all
-// scores of a tile took 179 us, lists that one warp settles for all 32 rows 252; eight lanes a row, by all warps, 135, and with floats for the mass
-// that is only told 83.
+// instructions, 1040 a row of 250 classes, 240 of them for the mass of all classes in doubles: 50003 x 250 with min_p and top_p in 98 us (floor 7.8).
+// Bisection over all scores of a tile took 179 us, lists that one warp settles for all 32 rows 252, eight lanes a row, by all warps, 135.  With floats for the
+// mass where it is only told it was 83 us, but its log had no digits near 0 and could lie above that among the classes left.
 template <typename T, int W, int MOST>
 __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sample_limited(SampleArgs a, Scores<T> in, int apart) {
     extern __shared__ __align__(16) unsigned char room[];
@@ -624,7 +628,8 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W, W == 1 ? 4 : 3) k_sampl
         if (__any_sync(0xffffffffu, part)) {
             over_at(minus_inf(), true, above, ties, lowest);
             const double target = l.top_p * above;
-            // by floats first, each sum off by less than 2^-18, as far as they tell on which side the border lies
+            // by floats first, as far as they tell on which side the border lies: a warp adds up to 128 in a chain (127 roundings of 2^-24), each off by
+            // 2^-22 and by 3 roundings of its exponent, which is below 10 on the mean over the mass of 1024: 9.1e-6 in all
             float up_to = top;
             const float c = (float)(l.inv_t * 1.4426950408889634);
             bool told = part && floats_tell(l);

@@ -43,7 +43,7 @@ __device__ __forceinline__ void put_draw(const SampleArgs &a, long long i, int c
 // ---- exponentials in 64 bits ------------------------------------------------------------------
 // exp(d / T) for d <= 0, relative error below 2^-38: with y = 32 d log2(e) / T and n the whole number nearest to it, 2^(n / 32) is a power of two times one
 // of 32 numbers (a table in shared memory), and exp of the rest, |rest| <= ln 2 / 64, five terms of its series, the first left out
-// below 2^-39.  11 instructions of the fp64 units, which do half as many as the fp32 ones; the library's exp takes twice as many.
+// below 2^-39.  10 instructions of the fp64 units, which do half as many as the fp32 ones; the library's exp takes twice as many.
 struct Powers {
     double of[32];
     __device__ __forceinline__ void fill() {   // a warp; a barrier has to follow

@@ -21,9 +21,10 @@ namespace cg = cooperative_groups;
 // falls on.  Where top_p alone leaves more, what is certainly left is told from what the end of it lies among, and only that goes into the list.
 // Rows with more than a list, and rows without limits, take their draws from sums per segment.
 //
-// Bound by instructions and by waiting for the cluster: 256 x 131072 in 16 bits under limits of all kinds 180 us (floor 10.2), 16 draws for each of
-// 333 x 50021 without limits, every exponential a double, 139 us (5.1).  64 registers, so that two blocks share an SM: with 128 and one block
-// 425 us and 233.
+// Bound by instructions and by waiting for the cluster: 256 x 131072 in 16 bits, limits of their own for all rows, 211 to 264 us by what these are (floor
+// 10.2), 96 instructions a score, 14 of them of the fp64 units (every exponential that a mass takes is a double); 16 draws for each of 333 x 50021 without limits
+// 124 us (5.1), 116 instructions a score, 19 of them fp64: what is left of them is the cluster's exchanges and registers that the limits' code spills.
+// 64 registers, so that two blocks share an SM: with 128 and one block 425 us and 233 (before the lists were narrowed).
 constexpr int LONG_LIST = 1024;
 
 template <int W, int S> struct LongRow {
@@ -350,12 +351,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample_long(SampleArgs a, Sco
         }
         float high = top;
         const bool narrowing = by_count ? top_k <= LONG_LIST : by_mass && !by_share && told;
-        // top_p alone: masses by floats, each off by less than 2^-18, tell what certainly reaches the target and what certainly does not
+        // top_p alone: masses by floats, each off by less than 2^-18 (chains of up to 16), tell what certainly reaches the target and what certainly does not
         const double enough = l.top_p * all * (1 + 2e-5), short_of = l.top_p * all * (1 - 2e-5);
         int above = 0;   // scores larger than `high`, which are left in any case
         bool first = !by_count && guess > low && guess < top, moved = false;
-        // An entry of the list is compared with all others: one block alone narrows on for less than that (1 x 1000: 17 us, 32 with 600 entries), a
-        // cluster, whose blocks wait for one another every time, not as far.
+        // An entry of the list is compared with all others: one block alone narrows on for less than that, a cluster, whose blocks wait for one another
+        // every time, not as far.  At 160 and at 512 (us): one block, 1 x 2000 with top_p 0.9 29 and 38, 32 x 4000 42 and 40; clusters, 256 x 131072 with
+        // top_k 50 198 and 195, top_p 0.9 742 and 720, 333 x 50021 with top_p 0.95 634 and 606.
         const int want = max(C == 1 ? 160 : 512, by_count ? top_k : 0);
         while (narrowing && count - above > want && low < high) {
             const float mid = first ? guess : middle(low, high);
@@ -627,7 +629,7 @@ template <typename T> bool sample_long(const SampleArgs &a, cudaStream_t stream)
     const Scores<T> in = scores_of<T>(a.in);
     const bool even = a.k % Pack<T>::V == 0 && on_16(in.p, in.row, sizeof(T));
     bool done = false;
-    // the smallest blocks that hold a row in a cluster of up to 8, and bigger ones before more than one where there are rows enough for every SM
+    // the smallest blocks that hold a row in a cluster of up to 8
     auto go = [&](auto th, auto p, auto ev) {
         constexpr bool EVEN = decltype(ev)::value;
         constexpr int TH = decltype(th)::value, P = decltype(p)::value;
